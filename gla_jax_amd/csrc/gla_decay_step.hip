@@ -1,0 +1,274 @@
+// Linear attention with one decay a head, one token for each row of a batch: the states lie in a pool and are updated where
+// they lie.  Bound by reading and writing every state once.
+//
+// A wave takes 32 value columns of one state: a lane holds a piece of 16 bytes of each of DKP / (rows side by side) rows, all
+// of them requested before the first is used.  A lane's rows follow each other, so that it reads its keys and queries in
+// whole pieces; the lanes that hold the same columns are summed at the end.  Nothing goes through LDS.
+#include "gla_common.hpp"
+
+namespace gla {
+namespace {
+
+// Indices of 4 or 8 bytes.
+struct Indices {
+    const void *p;
+    int wide;
+    __device__ __forceinline__ int64_t at(int64_t i) const
+    {
+        return wide ? static_cast<const int64_t *>(p)[i] : (int64_t) static_cast<const int32_t *>(p)[i];
+    }
+};
+
+struct StepArgs {
+    int64_t pool, B, H, HK, DK, DV, beams;
+    void *states;
+    const float *log_decay;
+    int64_t gates_b, gates_h;
+    const void *value, *key, *query;
+    int64_t value_b, value_h, key_b, key_h, query_b, query_h;
+    Indices slots, parents;
+    void *out;
+};
+
+// The pool's row of batch row i: i itself, or what `slots` says; -1 where that is none.
+__device__ __forceinline__ int64_t slot_of(const StepArgs &a, int64_t i)
+{
+    const int64_t s = a.slots.p ? a.slots.at(i) : i;
+    return s >= 0 && s < a.pool ? s : -1;
+}
+
+template <typename T, typename HT, int DKP> struct StepState {
+    static constexpr int VEC = 16 / sizeof(HT), LPR = 32 / VEC, SIDE = 64 / LPR, PER = DKP / SIDE;
+    typedef HT Piece __attribute__((ext_vector_type(VEC)));
+    Piece x[PER];
+    __device__ __forceinline__ void load(const HT *state, int DK, int DV, int row0, int col)
+    {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            x[i] = Piece{};
+            if (row0 + i < DK && col < DV) x[i] = *reinterpret_cast<const Piece *>(state + (int64_t)(row0 + i) * DV + col);
+        }
+    }
+    // The token's update, and its output for the lane's columns (zeros outside): the sum runs over the key features in 32 bits
+    // from the state before it is rounded.
+    __device__ __forceinline__ void step(HT *state, float decay, const T *k, const T *q, const T *v, T *out, int DK, int DV, int row0, int col)
+    {
+        float kv[PER], qv[PER], vv[VEC], o[VEC];
+#pragma unroll
+        for (int i = 0; i < PER; ++i) kv[i] = qv[i] = 0.f;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) vv[e] = o[e] = 0.f;
+        if (row0 < DK) {                          // 16 divides DK: a lane's rows exist or do not, in pieces of PER <= 16
+#pragma unroll
+            for (int i = 0; i < PER; i += 4) {
+                if (row0 + i < DK) {
+                    float t[4];
+                    load_vec<T, 4>(k + row0 + i, t);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) kv[i + e] = t[e];
+                    load_vec<T, 4>(q + row0 + i, t);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) qv[i + e] = t[e];
+                }
+            }
+        }
+        if (col < DV) load_vec<T, VEC>(v + col, vv);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            float s[VEC];
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                s[e] = decay * (float)x[i][e] + kv[i] * vv[e];
+                o[e] += qv[i] * s[e];
+            }
+            if (row0 + i < DK && col < DV) store_vec<HT, VEC>(state + (int64_t)(row0 + i) * DV + col, s);
+        }
+#pragma unroll
+        for (int m = LPR; m < 64; m *= 2)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) o[e] += shfl_xor_f32(o[e], m);
+        if ((threadIdx.x & 63) < LPR && col < DV) store_vec<T, VEC>(out + col, o);
+    }
+};
+
+template <typename T, typename HT, int DKP>
+__global__ __launch_bounds__(256) void decay_step_kernel(const StepArgs a)
+{
+    typedef StepState<T, HT, DKP> State;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, waves = blockDim.x >> 6;
+    const int64_t b = blockIdx.x / a.H, h = blockIdx.x % a.H, hk = h / (a.H / a.HK);
+    const int DK = (int)a.DK, DV = (int)a.DV, col = 32 * (blockIdx.y * waves + w) + State::VEC * (lane % State::LPR),
+              row0 = State::PER * (lane / State::LPR);
+    const int64_t slot = slot_of(a, b);
+    T *out = static_cast<T *>(a.out) + (b * a.H + h) * DV;
+    if (slot < 0) {                               // a row without a state
+        const float zero[State::VEC] = {};
+        if (lane < State::LPR && col < DV) store_vec<T, State::VEC>(out + col, zero);
+        return;
+    }
+    HT *state = static_cast<HT *>(a.states) + (slot * a.H + h) * DK * DV;
+    State s;
+    s.load(state, DK, DV, row0, col);
+    s.step(state, expf(a.log_decay[b * a.gates_b + h * a.gates_h]), static_cast<const T *>(a.key) + b * a.key_b + hk * a.key_h,
+           static_cast<const T *>(a.query) + b * a.query_b + hk * a.query_h,
+           static_cast<const T *>(a.value) + b * a.value_b + h * a.value_h, out, DK, DV, row0, col);
+}
+
+// The waves that hold their part of a state in registers: 16 of 128 registers, 8 of 256.
+constexpr int waves_of_beams(int DK) { return DK <= 128 ? 16 : 8; }
+
+// The same for a group of beams, each from the state of the beam that it continues: a wave a beam, all of a group in one
+// workgroup, which has read every state (of these columns) before it writes the first.
+template <typename T, typename HT, int DKP>
+__global__ __launch_bounds__(64 * waves_of_beams(DKP)) void decay_step_beams_kernel(const StepArgs a)
+{
+    typedef StepState<T, HT, DKP> State;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int64_t group = blockIdx.x / a.H, h = blockIdx.x % a.H, hk = h / (a.H / a.HK), b = group * a.beams + w;
+    const int DK = (int)a.DK, DV = (int)a.DV, col = 32 * blockIdx.y + State::VEC * (lane % State::LPR),
+              row0 = State::PER * (lane / State::LPR);
+    const int64_t parent = a.parents.at(b), source = parent >= 0 && parent < a.beams ? group * a.beams + parent : b;
+    const int64_t slot = slot_of(a, b);
+    int64_t from = slot_of(a, source);
+    if (from < 0) from = slot;
+    T *out = static_cast<T *>(a.out) + (b * a.H + h) * DV;
+    State s;
+    if (slot >= 0) s.load(static_cast<const HT *>(a.states) + (from * a.H + h) * DK * DV, DK, DV, row0, col);
+    // the loads have to be back, not only issued, before another wave's stores may follow
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (slot < 0) {
+        const float zero[State::VEC] = {};
+        if (lane < State::LPR && col < DV) store_vec<T, State::VEC>(out + col, zero);
+        return;
+    }
+    s.step(static_cast<HT *>(a.states) + (slot * a.H + h) * DK * DV, expf(a.log_decay[b * a.gates_b + h * a.gates_h]),
+           static_cast<const T *>(a.key) + b * a.key_b + hk * a.key_h, static_cast<const T *>(a.query) + b * a.query_b + hk * a.query_h,
+           static_cast<const T *>(a.value) + b * a.value_b + h * a.value_h, out, DK, DV, row0, col);
+}
+
+template <typename T, typename HT, int DKP> int launch_step(hipStream_t stream, const StepArgs &a)
+{
+    const int64_t cols = (a.DV + 31) / 32;
+    if (a.beams) {
+        decay_step_beams_kernel<T, HT, DKP><<<dim3(a.B / a.beams * a.H, cols), a.beams * 64, 0, stream>>>(a);
+    } else {
+        // four waves side by side share the lines of a row; where there are few, each has a compute unit of its own
+        const int waves = a.B * a.H * cols >= 1024 ? (cols < 4 ? (int)cols : 4) : 1;
+        decay_step_kernel<T, HT, DKP><<<dim3(a.B * a.H, (cols + waves - 1) / waves), waves * 64, 0, stream>>>(a);
+    }
+    return launch_status();
+}
+template <typename T, typename HT> int dispatch_step(hipStream_t stream, const StepArgs &a)
+{
+    return a.DK <= 64 ? launch_step<T, HT, 64>(stream, a) : a.DK <= 128 ? launch_step<T, HT, 128>(stream, a) : launch_step<T, HT, 256>(stream, a);
+}
+
+// ---- states in another order ------------------------------------------------------------------
+// states[w] <- states[parents[w]] in place, for every group of `beams` rows.  A thread takes one piece of a row's bytes of all
+// the group's rows: it has read them all before it writes the first, and no other thread touches them.  A beam that continues
+// itself moves nothing.
+struct ReorderArgs {
+    int64_t pool, beams, pieces, blocks;       // pieces of a row; workgroups that share a row
+    void *states;
+    Indices parents, slots;
+};
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+template <typename P, int WMAX> __global__ __launch_bounds__(256) void reorder_states_kernel(const ReorderArgs a)
+{
+    const int64_t group = blockIdx.x / a.blocks, at = blockIdx.x % a.blocks * 256 + threadIdx.x, first = group * a.beams;
+    if (at >= a.pieces) return;
+    P *states = static_cast<P *>(a.states) + at;
+    auto row = [&](int64_t i) {
+        const int64_t s = a.slots.p ? a.slots.at(i) : i;
+        return s >= 0 && s < a.pool ? s : -1;
+    };
+    P x[WMAX];
+    int64_t to[WMAX];
+#pragma unroll
+    for (int w = 0; w < WMAX; ++w) {
+        to[w] = -1;
+        if (w < a.beams) {
+            const int64_t parent = a.parents.at(first + w);
+            if (parent >= 0 && parent < a.beams && parent != w) {
+                const int64_t from = row(first + parent);
+                if (from >= 0 && (to[w] = row(first + w)) >= 0) x[w] = states[from * a.pieces];
+            }
+        }
+    }
+#pragma unroll
+    for (int w = 0; w < WMAX; ++w)
+        if (to[w] >= 0) states[to[w] * a.pieces] = x[w];
+}
+template <typename P> int launch_reorder(hipStream_t stream, const ReorderArgs &a, int64_t groups)
+{
+    const dim3 grid(a.blocks * groups);
+    if (a.beams <= 4) reorder_states_kernel<P, 4><<<grid, 256, 0, stream>>>(a);
+    else if (a.beams <= 16) reorder_states_kernel<P, 16><<<grid, 256, 0, stream>>>(a);
+    else reorder_states_kernel<P, 64><<<grid, 256, 0, stream>>>(a);
+    return launch_status();
+}
+
+int64_t bytes_of(gla_dtype d) { return d == GLA_BF16 ? 2 : 4; }
+bool dtype_ok(gla_dtype d) { return d == GLA_F32 || d == GLA_BF16; }
+
+}  // namespace
+}  // namespace gla
+
+using namespace gla;
+
+extern "C" int gla_reorder_states(void *stream, int64_t pool, int64_t groups, int64_t beams, int64_t row_bytes, int wide_indices,
+                                  const void *parents, const void *slots, void *states)
+{
+    if (!parents || !states) return GLA_ERR_NULL;
+    if (pool < 1 || groups < 1 || beams < 1 || beams > GLA_MOST_BEAMS || row_bytes < 1) return GLA_ERR_SHAPE;
+    if (!slots && groups * beams > pool) return GLA_ERR_SHAPE;
+    const uintptr_t index = wide_indices ? 7 : 3;
+    if ((reinterpret_cast<uintptr_t>(parents) & index) || (reinterpret_cast<uintptr_t>(slots) & index)) return GLA_ERR_ALIGN;
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    const uintptr_t place = reinterpret_cast<uintptr_t>(states) | (uintptr_t)row_bytes;
+    ReorderArgs a{pool, beams, 0, 0, states, {parents, wide_indices}, {slots, wide_indices}};
+    // 16 bytes of up to 16 rows in a thread's registers, 4 bytes of more
+    const int64_t piece = place % 16 == 0 && beams <= 16 ? 16 : place % 4 == 0 ? 4 : 1;
+    a.pieces = row_bytes / piece;
+    a.blocks = (a.pieces + 255) / 256;
+    if (a.blocks >= ((int64_t)1 << 31) || groups >= ((int64_t)1 << 31) || a.blocks * groups >= ((int64_t)1 << 31)) return GLA_ERR_SHAPE;
+    return piece == 16 ? launch_reorder<u32x4>(s, a, groups) : piece == 4 ? launch_reorder<uint32_t>(s, a, groups) : launch_reorder<uint8_t>(s, a, groups);
+}
+
+extern "C" int gla_decay_step(void *stream, int64_t pool, int64_t B, int64_t H, int64_t HK, int64_t DK, int64_t DV, int64_t beams,
+                              gla_dtype dtype, gla_dtype state_dtype, int wide_indices, const int64_t *strides, const float *log_decay,
+                              const void *value, const void *key, const void *query, const void *slots, const void *parents,
+                              void *states, void *out)
+{
+    if (!log_decay || !value || !key || !query || !states || !out || (beams > 0 && !parents)) return GLA_ERR_NULL;
+    if (pool < 1 || B < 1 || H < 1 || HK < 1 || DK < 1 || DV < 1 || beams < 0 || H % HK || DK % 16 || DV % 16 || DK > 256 || DV > 256)
+        return GLA_ERR_SHAPE;
+    if (B * H >= ((int64_t)1 << 31) || (!slots && B > pool) || (beams > 0 && (B % beams || beams > GLA_MOST_BEAMS))) return GLA_ERR_SHAPE;
+    if (!dtype_ok(dtype) || !dtype_ok(state_dtype)) return GLA_ERR_DTYPE;
+    StepArgs a{pool, B, H, HK, DK, DV, beams, states, log_decay, H, 1, value, key, query,
+               H * DV, DV, HK * DK, DK, HK * DK, DK, {slots, wide_indices}, {parents, wide_indices}, out};
+    if (strides) {
+        int64_t *all[8] = {&a.gates_b, &a.gates_h, &a.value_b, &a.value_h, &a.key_b, &a.key_h, &a.query_b, &a.query_h};
+        for (int i = 0; i < 8; ++i) *all[i] = strides[i];
+    }
+    const int64_t piece = 16 / bytes_of(dtype);
+    for (int64_t x : {a.value_b, a.value_h, a.key_b, a.key_h, a.query_b, a.query_h})
+        if (x % piece) return GLA_ERR_ALIGN;
+    for (const void *x : {value, key, query, static_cast<const void *>(states), static_cast<const void *>(out)})
+        if (!aligned16(x)) return GLA_ERR_ALIGN;
+    const uintptr_t index = wide_indices ? 7 : 3;
+    if ((reinterpret_cast<uintptr_t>(slots) & index) || (reinterpret_cast<uintptr_t>(parents) & index) ||
+        (reinterpret_cast<uintptr_t>(log_decay) & 3))
+        return GLA_ERR_ALIGN;
+    if (beams > waves_of_beams((int)DK)) {
+        // more beams than a workgroup has waves for take the reordering as a pass of its own
+        const int rc = gla_reorder_states(stream, pool, B / beams, beams, H * DK * DV * bytes_of(state_dtype), wide_indices, parents,
+                                          slots, states);
+        if (rc) return rc;
+        a.beams = 0;
+    }
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    if (dtype == GLA_BF16) return state_dtype == GLA_BF16 ? dispatch_step<__bf16, __bf16>(s, a) : dispatch_step<__bf16, float>(s, a);
+    return state_dtype == GLA_BF16 ? dispatch_step<float, __bf16>(s, a) : dispatch_step<float, float>(s, a);
+}

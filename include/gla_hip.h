@@ -247,6 +247,73 @@ int gla_chunk_bwd_stages(void *stream, int stages, int64_t B, int64_t T, int64_t
                          void *dhidden_init, float *dlog_fgate, void *dvalue, void *dkey, void *dquery,
                          void *workspace, size_t workspace_bytes);
 
+/* ---- linear attention with one decay a head ------------------------------------------------------ */
+
+/* S_t = exp(a_t) S_{t-1} + k_t v_t^T,  o_t = S_t^T q_t  with one number a_t for each head and token: chunk_gla's recurrence where all
+ * features of a head share their gate.  No counterpart in the reference, which gates every feature.
+ *   log_decay [B,T,H] float32 (any strides, 0 among them: one constant a head has batch and token stride 0); -inf forgets all
+ *   value [B,T,H,DV];  key, query [B,T,HK,DK], HK divides H: heads h*H/HK .. share key head h
+ *   hidden_* [B,H,DK,DV];  out [B,T,H,DV]
+ * T >= 0, DK and DV multiples of 16 up to 256.  `strides` (host memory, read during the call) holds batch, token and head
+ * strides in elements of log_decay, value, key and query, in this order: 12 numbers; NULL: dense arrays.  Features lie side by
+ * side, rows begin on 16 bytes.  `lengths` (B int32 on the GPU, or NULL) ends every sequence early: what lies behind it is not
+ * read, out is zero there, and hidden_final is the state at the end; a length outside 0..T counts as the nearer of the two.
+ * The states are summed in 32 bits; an operand of the matrix products is rounded to `dtype` where a 16-bit result takes it in. */
+
+/* Bytes of the `states` that gla_decay_fwd leaves for gla_decay_bwd: the state before every chunk (of 64 tokens, float32 data:
+ * 32) in float32. */
+size_t gla_decay_states_bytes(int64_t B, int64_t T, int64_t H, int64_t HK, int64_t DK, int64_t DV, gla_dtype dtype);
+/* Bytes of scratch (0: none is needed and it may be NULL). */
+size_t gla_decay_fwd_workspace_bytes(int64_t B, int64_t T, int64_t H, int64_t HK, int64_t DK, int64_t DV, gla_dtype dtype);
+size_t gla_decay_bwd_workspace_bytes(int64_t B, int64_t T, int64_t H, int64_t HK, int64_t DK, int64_t DV, gla_dtype dtype,
+                                     int constant_decay);
+/* `states` may be NULL when no gradient will be taken. */
+int gla_decay_fwd(void *stream, int64_t B, int64_t T, int64_t H, int64_t HK, int64_t DK, int64_t DV, gla_dtype dtype,
+                  gla_dtype hidden_dtype, const int64_t *strides, const void *hidden_init, const float *log_decay,
+                  const void *value, const void *key, const void *query, const int32_t *lengths, void *hidden_final, void *out,
+                  void *states, void *workspace, size_t workspace_bytes);
+/* Gradients, dense, in the types of their arrays; dlog_decay is [B,T,H], or with constant_decay != 0 [H]: the sum over batch
+ * and tokens (log_decay then has strides 0 there).  dout is dense. */
+int gla_decay_bwd(void *stream, int64_t B, int64_t T, int64_t H, int64_t HK, int64_t DK, int64_t DV, gla_dtype dtype,
+                  gla_dtype hidden_dtype, int constant_decay, const int64_t *strides, const float *log_decay, const void *value,
+                  const void *key, const void *query, const int32_t *lengths, const void *states, const void *dhidden_final,
+                  const void *dout, void *dhidden_init, float *dlog_decay, void *dvalue, void *dkey, void *dquery, void *workspace,
+                  size_t workspace_bytes);
+
+#define GLA_MOST_BEAMS 64
+#define GLA_MOST_CANDIDATES 64
+
+/* One token for each of B rows, on a pool of states [pool,H,DK,DV] that is updated in place:
+ *   log_decay [B,H] float32, value [B,H,DV], key and query [B,HK,DK], out [B,H,DV].
+ * `strides` (host memory, or NULL: dense) holds the batch and head strides of log_decay, value, key and query: 8 numbers.
+ * `slots` (B indices, or NULL: row b is pool row b) says where each row's state lies; one outside the pool marks a row without a
+ * state: its out is zero.  No two rows may name the same slot.  `beams` > 0 takes the rows in groups of so many (at most 64): row w of
+ * a group continues from the state that row parents[group][w] of its group had before the call; a parent outside 0..beams-1, or
+ * one without a state, counts as w.  Indices are int32, or int64 with wide_indices != 0. */
+int gla_decay_step(void *stream, int64_t pool, int64_t B, int64_t H, int64_t HK, int64_t DK, int64_t DV, int64_t beams,
+                   gla_dtype dtype, gla_dtype state_dtype, int wide_indices, const int64_t *strides, const float *log_decay,
+                   const void *value, const void *key, const void *query, const void *slots, const void *parents, void *states,
+                   void *out);
+
+/* ---- beam search --------------------------------------------------------------------------------- */
+
+/* The `num` (at most 64) best continuations of every group's beams: logits [groups,beams,vocab] with `row` elements from one
+ * beam to the next, scores [groups,beams] float32, out_* [groups,num].  A candidate scores its beam's score plus the log softmax of its logit; a beam
+ * offers its `num` largest logits, the lower token first where two are equal, and equal scores come in the order of (beam, token).
+ * A logit that is not a number counts as -inf, and so does a score that comes out as none (a beam whose logits are all -inf).
+ * `finished` (a byte for each beam, or NULL): a beam for which it is not zero offers token `eos` at the score that it has and
+ * nothing else (its logits are not read).  groups * beams <= 65535, beams <= 64, beams * vocab < 2^31. */
+size_t gla_beam_select_workspace_bytes(int64_t groups, int64_t beams, int64_t vocab, int64_t num);
+int gla_beam_select(void *stream, int64_t groups, int64_t beams, int64_t vocab, int64_t num, gla_dtype dtype, int64_t row,
+                    const void *logits, const float *scores, const void *finished, int64_t eos, float *out_scores,
+                    int64_t *out_parents, int64_t *out_tokens, void *workspace, size_t workspace_bytes);
+
+/* states[group][w] <- states[group][parents[group][w]] in place, for rows of row_bytes each in a pool of `pool` rows: the
+ * states of a beam search follow its beams.  `slots` [groups,beams] (or NULL: the rows lie in order) says where they are; one outside
+ * the pool marks a row without a state.  A parent outside 0..beams-1 counts as w. */
+int gla_reorder_states(void *stream, int64_t pool, int64_t groups, int64_t beams, int64_t row_bytes, int wide_indices,
+                       const void *parents, const void *slots, void *states);
+
 #ifdef __cplusplus
 }
 #endif
