@@ -6,7 +6,7 @@ import torch
 
 from . import _lib
 from .decay import _check, _indices, _same_width
-from .gla import _DT, _ptr, _stream
+from .gla import _DT, _native, _ptr, _stream
 
 
 def beam_select(logits, scores, num=None, finished=None, eos=0):
@@ -20,6 +20,9 @@ def beam_select(logits, scores, num=None, finished=None, eos=0):
 
     Returns (scores [..,num] float32, parents [..,num] int64, tokens [..,num] int64): candidate i is tokens[i] behind beam
     parents[i].  Nothing here is differentiable."""
+    done = _native("beam_select", (logits, scores), num, finished, eos)
+    if done is not None:
+        return tuple(done)
     _check((("logits", logits), ("scores", scores)), logits.device if isinstance(logits, torch.Tensor) else None)
     if logits.ndim < 2:
         raise AssertionError("logits must be [..., W, V]")
@@ -70,6 +73,8 @@ def reorder_states(states, parents, slots=None):
     `beam_select` keeps.  `states` [N, ..] is dense, of any element type and shape behind its first axis (the states of chunk_decay and decay_step as
     those of recurrent_gla); `slots` [G,W] says where a beam's state lies when they do not lie in order, one outside 0..N-1 marks a
     beam without one.  A parent outside 0..W-1 counts as w.  W is at most 64.  Returns `states`."""
+    if _native("reorder", (states, parents), slots):
+        return states
     _check((("states", states), ("parents", parents)), states.device if isinstance(states, torch.Tensor) else None)
     if parents.ndim != 2:
         raise AssertionError("parents must be [G, W]")

@@ -14,6 +14,7 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <array>
 #include <optional>
 
 #include "../../include/gla_hip.h"
@@ -174,10 +175,10 @@ Tensor cotangent(const Tensor &d, at::IntArrayRef sizes, at::ScalarType type, co
     return d.scalar_type() == type && d.is_contiguous() ? d : d.to(type).contiguous();
 }
 
-template <typename... Args> variable_list python_rule(const char *name, Args &&...args)
+template <typename... Args> variable_list python_rule(const char *module, const char *name, Args &&...args)
 {
     const py::gil_scoped_acquire gil;
-    const py::object r = py::module_::import("gla_jax_amd.gla").attr(name).attr("apply")(std::forward<Args>(args)...);
+    const py::object r = py::module_::import(module).attr(name).attr("apply")(std::forward<Args>(args)...);
     return r.cast<variable_list>();
 }
 
@@ -212,7 +213,7 @@ struct Chunk : torch::autograd::Function<Chunk> {      // gla.py:483-550, 552-62
         check_saved(holds(s[0], gla_chunk_states_bytes(n.B, n.T, n.H, n.D, n.D, chunk, code(s[2])), s[3]));
         const Tensor dhT = cotangent(d[0], state_sizes(s[3]), (at::ScalarType)ctx->saved_data["hidden"].toInt(), s[3]);
         const Tensor dout = cotangent(d[1], s[2].sizes(), s[2].scalar_type(), s[2]);
-        variable_list r = transforms_active() ? python_rule("_ChunkGLABwd", s[0], s[1], s[2], s[3], s[4], dhT, dout, chunk)
+        variable_list r = transforms_active() ? python_rule("gla_jax_amd.gla", "_ChunkGLABwd", s[0], s[1], s[2], s[3], s[4], dhT, dout, chunk)
                           : at::GradMode::is_enabled() ? ChunkBackward::apply(s[0], s[1], s[2], s[3], s[4], dhT, dout, chunk)
                                                        : chunk_backward(s[0], s[1], s[2], s[3], s[4], dhT, dout, chunk);
         r.emplace_back();
@@ -294,11 +295,153 @@ struct Recurrent : torch::autograd::Function<Recurrent> {      // gla.py:99-170,
         const Tensor dhT = cotangent(d[0], s[0].sizes(), s[0].scalar_type(), s[0]);
         const Tensor dout = cotangent(d[1], s[2].sizes(), out_fp32 ? at::kFloat : s[2].scalar_type(), s[2]);
         variable_list r = transforms_active()
-                              ? python_rule("_RecurrentGLABwd", s[0], s[1], s[2], s[3], s[4], s[5], dhT, dout, reverse, out_fp32)
+                              ? python_rule("gla_jax_amd.gla", "_RecurrentGLABwd", s[0], s[1], s[2], s[3], s[4], s[5], dhT, dout, reverse, out_fp32)
                           : at::GradMode::is_enabled()
                               ? RecurrentBackward::apply(s[0], s[1], s[2], s[3], s[4], s[5], std::optional<Tensor>(s[6]), dhT, dout, reverse, out_fp32)
                               : recurrent_backward(s[0], s[1], s[2], s[3], s[4], s[5], s[6], dhT, dout, reverse, out_fp32);
         r.resize(7);
+        return r;
+    }
+};
+
+// ---- linear attention with one decay a head -------------------------------------------------------
+// Rows [B,T,heads,features] (or [T,heads,features]) that the kernels take where they lie: see decay.py's _rows.
+bool rows_on_gpu(const Tensor &t)
+{
+    if (!t.defined() || !t.is_cuda() || t.layout() != at::kStrided || t.dim() < 3 || t.dim() > 4 || t.stride(-1) != 1) return false;
+    const int64_t piece = 16 / (int64_t)t.element_size();
+    for (int64_t i = 0; i + 1 < t.dim(); ++i)
+        if (t.size(i) > 1 && t.stride(i) % piece) return false;
+    return t.numel() == 0 || reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+}
+struct DecayDims {
+    int64_t B, T, H, HK, DK, DV;
+};
+DecayDims decay_dims(const Tensor &v, const Tensor &k)
+{
+    return {v.dim() == 4 ? v.size(0) : 1, v.size(-3), v.size(-2), k.size(-2), k.size(-1), v.size(-1)};
+}
+bool decay_rows(const Tensor &a, const Tensor &v, const Tensor &k, const Tensor &q, const std::optional<Tensor> &lengths)
+{
+    if (!rows_on_gpu(v) || !rows_on_gpu(k) || !rows_on_gpu(q) || !a.defined() || !a.is_cuda() || a.layout() != at::kStrided) return false;
+    const DecayDims n = decay_dims(v, k);
+    if (k.dim() != v.dim() || q.sizes() != k.sizes() || k.size(-3) != n.T || (v.dim() == 4 && k.size(0) != n.B)) return false;
+    if (n.B < 1 || n.H < 1 || n.HK < 1 || n.H % n.HK || n.DK % 16 || n.DV % 16 || n.DK < 16 || n.DV < 16 || n.DK > 256 || n.DV > 256) return false;
+    if (!known(v.scalar_type()) || k.scalar_type() != v.scalar_type() || q.scalar_type() != v.scalar_type()) return false;
+    if (a.scalar_type() != at::kFloat || a.size(-1) != n.H) return false;
+    if (a.dim() != 1 && (a.dim() != v.dim() - 1 || a.size(-2) != n.T || (v.dim() == 4 && a.size(0) != n.B))) return false;
+    for (const Tensor *t : {&a, &k, &q})
+        if (t->device() != v.device()) return false;
+    if (lengths && (!dense_on_gpu(*lengths) || lengths->scalar_type() != at::kInt || lengths->dim() != v.dim() - 3 ||
+                    lengths->numel() != n.B || lengths->device() != v.device()))
+        return false;
+    return true;
+}
+std::vector<int64_t> decay_state_sizes(const Tensor &v, const Tensor &k)
+{
+    const DecayDims n = decay_dims(v, k);
+    return v.dim() == 4 ? std::vector<int64_t>{n.B, n.H, n.DK, n.DV} : std::vector<int64_t>{n.H, n.DK, n.DV};
+}
+std::array<int64_t, 12> decay_strides(const Tensor &a, const Tensor &v, const Tensor &k, const Tensor &q)
+{
+    std::array<int64_t, 12> s{};
+    int64_t i = 0;
+    const bool batch = v.dim() == 4;
+    s[i++] = a.dim() == 3 ? a.stride(0) : 0;
+    s[i++] = a.dim() == 1 ? 0 : a.stride(-2);
+    s[i++] = a.stride(-1);
+    for (const Tensor *t : {&v, &k, &q}) {
+        s[i++] = batch && t->size(0) > 1 ? t->stride(0) : 0;
+        s[i++] = t->size(-3) > 1 ? t->stride(-3) : 0;
+        s[i++] = t->size(-2) > 1 ? t->stride(-2) : 0;
+    }
+    return s;
+}
+const int32_t *lengths_of(const std::optional<Tensor> &lengths)
+{
+    return lengths ? (const int32_t *)lengths->data_ptr() : nullptr;
+}
+// a new dense array like `t`
+Tensor dense_like(const Tensor &t) { return at::empty(t.sizes(), t.options()); }
+
+ChunkOut decay_forward(const Tensor &h0, const Tensor &a, const Tensor &v, const Tensor &k, const Tensor &q,
+                       const std::optional<Tensor> &lengths, bool residual)
+{
+    const c10::DeviceGuard guard(v.device());
+    const DecayDims n = decay_dims(v, k);
+    const gla_dtype dt = code(v);
+    const size_t nws = gla_decay_fwd_workspace_bytes(n.B, n.T, n.H, n.HK, n.DK, n.DV, dt);
+    const size_t nst = residual ? gla_decay_states_bytes(n.B, n.T, n.H, n.HK, n.DK, n.DV, dt) : 0;
+    ChunkOut r{at::empty_like(h0), dense_like(v), Tensor()};
+    if (residual) r.states = at::empty({n.B, (int64_t)nst / n.B}, v.options().dtype(at::kByte));
+    Tensor ws;
+    if (nws) ws = bytes_like(nws, v);
+    const auto strides = decay_strides(a, v, k, q);
+    check("gla_decay_fwd",
+          gla_decay_fwd(stream_of(v), n.B, n.T, n.H, n.HK, n.DK, n.DV, dt, code(h0), strides.data(), h0.data_ptr(),
+                        (const float *)a.data_ptr(), v.data_ptr(), k.data_ptr(), q.data_ptr(), lengths_of(lengths), r.hT.data_ptr(),
+                        r.out.data_ptr(), nst ? r.states.data_ptr() : nullptr, nws ? ws.data_ptr() : nullptr, nws));
+    return r;
+}
+
+variable_list decay_backward(const Tensor &states, const Tensor &a, const Tensor &v, const Tensor &k, const Tensor &q,
+                             const std::optional<Tensor> &lengths, const Tensor &dhT, const Tensor &dout)
+{
+    const c10::DeviceGuard guard(v.device());
+    const DecayDims n = decay_dims(v, k);
+    const gla_dtype dt = code(v);
+    const bool constant = a.dim() == 1;
+    const size_t nws = gla_decay_bwd_workspace_bytes(n.B, n.T, n.H, n.HK, n.DK, n.DV, dt, constant);
+    Tensor ws;
+    if (nws) ws = bytes_like(nws, v);
+    Tensor dh0 = at::empty_like(dhT), da = dense_like(a), dv = dense_like(v), dk = dense_like(k), dq = dense_like(q);
+    const auto strides = decay_strides(a, v, k, q);
+    check("gla_decay_bwd",
+          gla_decay_bwd(stream_of(v), n.B, n.T, n.H, n.HK, n.DK, n.DV, dt, code(dhT), constant, strides.data(), (const float *)a.data_ptr(),
+                        v.data_ptr(), k.data_ptr(), q.data_ptr(), lengths_of(lengths), states.data_ptr(), dhT.data_ptr(),
+                        dout.data_ptr(), dh0.data_ptr(), (float *)da.data_ptr(), dv.data_ptr(), dk.data_ptr(), dq.data_ptr(),
+                        nws ? ws.data_ptr() : nullptr, nws));
+    return {dh0, da, dv, dk, dq};
+}
+
+struct DecayBackward : torch::autograd::Function<DecayBackward> {
+    static variable_list forward(AutogradContext *, const Tensor &states, const Tensor &a, const Tensor &v, const Tensor &k,
+                                 const Tensor &q, const std::optional<Tensor> &lengths, const Tensor &dhT, const Tensor &dout)
+    {
+        return decay_backward(states, a, v, k, q, lengths, dhT, dout);
+    }
+    static variable_list backward(AutogradContext *, variable_list) { no_double_backward("chunk_decay"); }
+};
+
+struct Decay : torch::autograd::Function<Decay> {
+    static variable_list forward(AutogradContext *ctx, const Tensor &h0, const Tensor &a, const Tensor &v, const Tensor &k,
+                                 const Tensor &q, const std::optional<Tensor> &lengths)
+    {
+        ChunkOut r = decay_forward(h0, a, v, k, q, lengths, true);
+        ctx->save_for_backward({r.states, a, v, k, q, lengths.value_or(Tensor())});
+        ctx->saved_data["hidden"] = (int64_t)h0.scalar_type();
+        ctx->set_materialize_grads(false);
+        return {r.hT, r.out};
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list d)
+    {
+        variable_list s = ctx->get_saved_variables();
+        // rows keep their strides; what a saved-tensor hook hands back in a layout that the kernels do not take is copied
+        for (size_t i = 2; i < 5; ++i)
+            if (s[i].defined() && !rows_on_gpu(s[i])) s[i] = s[i].contiguous();
+        if (!s[0].is_contiguous()) s[0] = s[0].contiguous();
+        if (s[5].defined() && !s[5].is_contiguous()) s[5] = s[5].contiguous();
+        const std::optional<Tensor> lengths = s[5].defined() ? std::optional<Tensor>(s[5]) : std::nullopt;
+        check_saved(decay_rows(s[1], s[2], s[3], s[4], lengths));
+        const DecayDims n = decay_dims(s[2], s[3]);
+        check_saved(holds(s[0], gla_decay_states_bytes(n.B, n.T, n.H, n.HK, n.DK, n.DV, code(s[2])), s[2]));
+        const Tensor dhT = cotangent(d[0], decay_state_sizes(s[2], s[3]), (at::ScalarType)ctx->saved_data["hidden"].toInt(), s[2]);
+        const Tensor dout = cotangent(d[1], s[2].sizes(), s[2].scalar_type(), s[2]);
+        variable_list r =
+            transforms_active() ? python_rule("gla_jax_amd.decay", "_ChunkDecayBwd", s[0], s[1], s[2], s[3], s[4], lengths, dhT, dout)
+            : at::GradMode::is_enabled() ? DecayBackward::apply(s[0], s[1], s[2], s[3], s[4], lengths, dhT, dout)
+                                         : decay_backward(s[0], s[1], s[2], s[3], s[4], lengths, dhT, dout);
+        r.emplace_back();
         return r;
     }
 };
@@ -374,6 +517,119 @@ std::optional<std::pair<Tensor, Tensor>> rnn(const Tensor &a, const Tensor &b, c
     return std::make_pair(oa, ox);
 }
 
+// [B,T,..] rows, or [T,..] as those of one sequence
+Result decay(const Tensor &h0, const Tensor &a, const Tensor &v, const Tensor &k, const Tensor &q, const std::optional<Tensor> &lengths)
+{
+    if (traced() || !decay_rows(a, v, k, q, lengths) || !dense_on_gpu(h0) || h0.device() != v.device() || !known(h0.scalar_type()) ||
+        h0.sizes() != at::IntArrayRef(decay_state_sizes(v, k)))
+        return std::nullopt;
+    if (wants_grad(h0, a, v, k, q)) return Decay::apply(h0, a, v, k, q, lengths);
+    ChunkOut r = decay_forward(h0, a, v, k, q, lengths, false);
+    return std::vector<Tensor>{r.hT, r.out};
+}
+
+bool index_array(const std::optional<Tensor> &t, at::IntArrayRef sizes, const Tensor &like, at::ScalarType type)
+{
+    return !t || (dense_on_gpu(*t) && t->sizes() == sizes && t->device() == like.device() && t->scalar_type() == type);
+}
+at::ScalarType index_type(const std::optional<Tensor> &x, const std::optional<Tensor> &y)
+{
+    const at::ScalarType t = x ? x->scalar_type() : y ? y->scalar_type() : at::kLong;
+    return t == at::kInt ? at::kInt : at::kLong;
+}
+bool takes_gradient(at::ArrayRef<Tensor> arrays)
+{
+    for (const Tensor &t : arrays)
+        if ((at::GradMode::is_enabled() && t.requires_grad()) || t._fw_grad(/*level=*/0).defined()) return true;
+    return false;
+}
+
+std::optional<Tensor> decay_step(const Tensor &states, const Tensor &a, const Tensor &v, const Tensor &k, const Tensor &q,
+                                 const std::optional<Tensor> &slots, const std::optional<Tensor> &parents)
+{
+    if (traced() || !dense_on_gpu(states) || states.dim() != 4 || !known(states.scalar_type()) || takes_gradient({states, a, v, k, q}))
+        return std::nullopt;
+    if (!rows_on_gpu(v) || !rows_on_gpu(k) || !rows_on_gpu(q) || v.dim() != 3 || k.dim() != 3 || q.sizes() != k.sizes()) return std::nullopt;
+    const int64_t B = v.size(0), H = v.size(1), DV = v.size(2), HK = k.size(1), DK = k.size(2), N = states.size(0);
+    if (B < 1 || H < 1 || N < 1 || HK < 1 || H % HK || k.size(0) != B || states.size(1) != H || states.size(2) != DK || states.size(3) != DV)
+        return std::nullopt;
+    if (!known(v.scalar_type()) || k.scalar_type() != v.scalar_type() || q.scalar_type() != v.scalar_type()) return std::nullopt;
+    if (!a.is_cuda() || a.layout() != at::kStrided || a.scalar_type() != at::kFloat || a.size(-1) != H || a.dim() > 2 || (a.dim() == 2 && a.size(0) != B))
+        return std::nullopt;
+    for (const Tensor *t : {&a, &v, &k, &q})
+        if (t->device() != states.device()) return std::nullopt;
+    const at::ScalarType type = index_type(slots, parents);
+    const int64_t W = parents && parents->dim() == 2 ? parents->size(1) : 0;
+    if (!index_array(slots, {B}, states, type) || (parents && (W < 1 || !index_array(parents, {B / W, W}, states, type) || B % W)) ||
+        (!slots && N < B))
+        return std::nullopt;
+    const c10::DeviceGuard guard(states.device());
+    Tensor out = dense_like(v);
+    const int64_t strides[8] = {a.dim() == 2 ? a.stride(0) : 0, a.stride(-1), B > 1 ? v.stride(0) : 0, H > 1 ? v.stride(1) : 0,
+                                B > 1 ? k.stride(0) : 0, HK > 1 ? k.stride(1) : 0, B > 1 ? q.stride(0) : 0, HK > 1 ? q.stride(1) : 0};
+    const int rc = gla_decay_step(stream_of(states), N, B, H, HK, DK, DV, W, code(v), code(states), type == at::kLong, strides,
+                                  (const float *)a.data_ptr(), v.data_ptr(), k.data_ptr(), q.data_ptr(), slots ? slots->data_ptr() : nullptr,
+                                  parents ? parents->data_ptr() : nullptr, states.data_ptr(), out.data_ptr());
+    if (rc == GLA_ERR_SHAPE || rc == GLA_ERR_ALIGN) return std::nullopt;       // decay.py says what is wrong
+    check("gla_decay_step", rc);
+    return out;
+}
+
+// ---- beam search ----------------------------------------------------------------------------------
+Result beam_select(const Tensor &logits, const Tensor &scores, const std::optional<int64_t> &wanted, const std::optional<Tensor> &finished, int64_t eos)
+{
+    const int64_t n = logits.dim();
+    if (traced() || n < 2 || !logits.is_cuda() || logits.layout() != at::kStrided || logits.stride(-1) != 1 || !known(logits.scalar_type()) ||
+        !plain_f32(scores) || scores.dim() != n - 1 || scores.device() != logits.device())
+        return std::nullopt;
+    const int64_t W = logits.size(-2), V = logits.size(-1), row = W > 1 ? logits.stride(-2) : V;
+    int64_t G = 1;
+    std::vector<int64_t> sizes;
+    // rows one distance apart from each other, whatever axes lie in front
+    int64_t step = W * row;
+    for (int64_t i = n - 3; i >= 0; --i) {
+        if (logits.size(i) > 1 && logits.stride(i) != step) return std::nullopt;
+        step *= logits.size(i);
+        G *= logits.size(i);
+    }
+    for (int64_t i = 0; i + 2 < n; ++i) sizes.push_back(logits.size(i));
+    for (int64_t i = 0; i + 1 < n; ++i)
+        if (scores.size(i) != logits.size(i)) return std::nullopt;
+    if (finished && (!dense_on_gpu(*finished) || finished->scalar_type() != at::kBool || finished->sizes() != scores.sizes() ||
+                     finished->device() != logits.device()))
+        return std::nullopt;
+    const int64_t num = wanted.value_or(W);
+    const size_t nws = row < V ? 0 : gla_beam_select_workspace_bytes(G, W, V, num);
+    if (nws == 0) return std::nullopt;
+    const c10::DeviceGuard guard(logits.device());
+    sizes.push_back(num);
+    Tensor best = at::empty(sizes, scores.options()), parents = at::empty(sizes, scores.options().dtype(at::kLong)),
+           tokens = at::empty(sizes, scores.options().dtype(at::kLong)), ws = bytes_like(nws, logits);
+    const int rc = gla_beam_select(stream_of(logits), G, W, V, num, code(logits), row, logits.data_ptr(), (const float *)scores.data_ptr(),
+                                   finished ? finished->data_ptr() : nullptr, eos, (float *)best.data_ptr(), (int64_t *)parents.data_ptr(),
+                                   (int64_t *)tokens.data_ptr(), ws.data_ptr(), nws);
+    if (rc == GLA_ERR_SHAPE) return std::nullopt;
+    check("gla_beam_select", rc);
+    return std::vector<Tensor>{best, parents, tokens};
+}
+
+bool reorder(const Tensor &states, const Tensor &parents, const std::optional<Tensor> &slots)
+{
+    if (traced() || !dense_on_gpu(states) || states.dim() < 1 || states.numel() == 0 || takes_gradient({states}) || parents.dim() != 2)
+        return false;
+    const at::ScalarType type = index_type(slots, parents);
+    const int64_t G = parents.size(0), W = parents.size(1), N = states.size(0);
+    if (!index_array(parents, parents.sizes(), states, type) || !index_array(slots, parents.sizes(), states, type) || G * W == 0 ||
+        (!slots && N < G * W))
+        return false;
+    const c10::DeviceGuard guard(states.device());
+    const int rc = gla_reorder_states(stream_of(states), N, G, W, states.numel() / N * (int64_t)states.element_size(), type == at::kLong,
+                                      parents.data_ptr(), slots ? slots->data_ptr() : nullptr, states.data_ptr());
+    if (rc == GLA_ERR_SHAPE) return false;
+    check("gla_reorder_states", rc);
+    return true;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_gla_torch, m)
@@ -384,4 +640,8 @@ PYBIND11_MODULE(_gla_torch, m)
     m.def("recurrent", &recurrent, NoGil());
     m.def("cumsum", &cumsum, NoGil());
     m.def("rnn", &rnn, NoGil());
+    m.def("decay", &decay, NoGil());
+    m.def("decay_step", &decay_step, NoGil());
+    m.def("beam_select", &beam_select, NoGil());
+    m.def("reorder", &reorder, NoGil());
 }

@@ -15,7 +15,8 @@ import ctypes
 import torch
 
 from . import _lib
-from .gla import _DT, _apply, _as, _merge_mapped, _no_double_backward, _ptr, _split_mapped, _stream, _transforms_active, _twin
+from .gla import (_DT, _apply, _as, _merge_mapped, _native, _no_double_backward, _plain_call, _ptr, _split_mapped, _stream,
+                  _transforms_active, _twin)
 
 
 def _rows(t, dtype):
@@ -29,8 +30,8 @@ def _rows(t, dtype):
 
 
 def _strides(*rows):
-    """The host array of strides that the C ABI takes: all axes but the features'."""
-    s = [x for t, n in rows for x in t.stride()[:n]]
+    """The host array of strides that the C ABI takes: all axes but the features' (of an axis of one, any will do)."""
+    s = [x if m > 1 else 0 for t, n in rows for x, m in zip(t.stride()[:n], t.shape)]
     return (ctypes.c_int64 * len(s))(*s)
 
 
@@ -163,6 +164,9 @@ def chunk_decay(hidden_init, log_decay, value, key, query, lengths=None):
 
     Returns (hidden_final [..,H,DK,DV] in hidden_init.dtype, out [..,T,H,DV] in value.dtype).  Differentiable in all five arrays;
     heads that share a key head add up to its gradient, tokens to that of a constant decay."""
+    done = _native("decay", (hidden_init, log_decay, value, key, query), lengths)
+    if done is not None:
+        return tuple(done)
     arrays = (("hidden_init", hidden_init), ("log_decay", log_decay), ("value", value), ("key", key), ("query", query))
     _check(arrays, hidden_init.device if isinstance(hidden_init, torch.Tensor) else None)
     if value.ndim < 3:
@@ -199,10 +203,9 @@ def chunk_decay(hidden_init, log_decay, value, key, query, lengths=None):
         # The kernels take 16 features at a time.  A zero feature adds nothing to a score or to the rest of the state.
         F = torch.nn.functional
         h0, v, k, q = F.pad(h0, (0, pv, 0, pk)), F.pad(v, (0, pv)), F.pad(k, (0, pk)), F.pad(q, (0, pk))
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (h0, a, v, k, q)) or _transforms_active():
-        hT, out = _apply(_ChunkDecay, h0, a, v, k, q, lengths)[:2]
-    else:
-        hT, out, _ = _decay_forward(h0, a, v, k, q, lengths, False)
+    v, k, q = (_rows(t, t.dtype) for t in (v, k, q))
+    hT, out = (_native("decay", (h0, a, v, k, q), lengths) if _plain_call()
+               else _apply(_ChunkDecay, h0, a, v, k, q, lengths)[:2])
     if pk or pv:
         hT, out = hT[..., :DK, :DV], out[..., :DV]
     return _as(hT, lead + (H, DK, DV), hidden_init.dtype), _as(out, lead + (T, H, DV), out.dtype)
@@ -235,6 +238,9 @@ def decay_step(states, log_decay, value, key, query, slots=None, parents=None):
     0..W-1 counts as w.  W is at most 64.
 
     States are updated in place: nothing here is differentiable, and arrays that require a gradient are refused."""
+    done = _native("decay_step", (states, log_decay, value, key, query), slots, parents)
+    if done is not None:
+        return done
     arrays = (("states", states), ("log_decay", log_decay), ("value", value), ("key", key), ("query", query))
     _check(arrays, states.device if isinstance(states, torch.Tensor) else None)
     if torch.is_grad_enabled() and any(t.requires_grad for _, t in arrays):
