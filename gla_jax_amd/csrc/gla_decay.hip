@@ -5,6 +5,7 @@ namespace gla {
 namespace {
 
 constexpr int64_t kMostFeatures = 256;
+constexpr int64_t kMostRow = (int64_t)1 << 23;      // elements from one token to the next: a chunk's places are 32-bit numbers
 
 int64_t pad256(int64_t x) { return (x + 255) & ~(int64_t)255; }
 
@@ -93,6 +94,8 @@ Places place(const DecaySizes &n, const int64_t *strides, const void *log_decay,
 }
 bool dtype_ok(gla_dtype d) { return d == GLA_F32 || d == GLA_BF16; }
 
+bool rows_near(const DecayRows &r) { return r.st >= 0 && r.st < kMostRow; }
+
 // Rows are read 16 bytes at a time.
 bool rows_aligned(const DecayRows &r, gla_dtype dtype)
 {
@@ -102,10 +105,11 @@ bool rows_aligned(const DecayRows &r, gla_dtype dtype)
 
 int check_sizes(const DecaySizes &n)
 {
-    const int64_t limit = (int64_t)1 << 31;
+    const int64_t limit = (int64_t)1 << 30;
     if (n.B < 1 || n.T < 0 || n.H < 1 || n.HK < 1 || n.DK < 1 || n.DV < 1) return GLA_ERR_SHAPE;
     if (n.H % n.HK || n.DK % 16 || n.DV % 16 || n.DK > kMostFeatures || n.DV > kMostFeatures) return GLA_ERR_SHAPE;
     if (n.B >= limit || n.H >= limit || n.T >= limit || n.B * n.H >= limit) return GLA_ERR_SHAPE;
+    if (n.H * n.DV >= kMostRow || n.HK * n.DK >= kMostRow) return GLA_ERR_SHAPE;
     return GLA_OK;
 }
 int64_t kept_bytes(const DecaySizes &n, gla_dtype dtype)
@@ -157,6 +161,7 @@ extern "C" int gla_decay_fwd(void *stream, int64_t B, int64_t T, int64_t H, int6
         !rows_aligned(p.values, dtype) || !rows_aligned(p.keys, dtype) || !rows_aligned(p.queries, dtype) ||
         (reinterpret_cast<uintptr_t>(log_decay) & 3) || (reinterpret_cast<uintptr_t>(lengths) & 3))
         return GLA_ERR_ALIGN;
+    if (!rows_near(p.values) || !rows_near(p.keys) || !rows_near(p.queries)) return GLA_ERR_SHAPE;
     const DecayPlan plan = forward_plan(n, dtype);
     const int64_t need = entering_bytes(n, plan);
     if (need && (!workspace || (int64_t)workspace_bytes < need)) return GLA_ERR_WORKSPACE;
@@ -187,6 +192,7 @@ extern "C" int gla_decay_bwd(void *stream, int64_t B, int64_t T, int64_t H, int6
     if (!rows_aligned(p.values, dtype) || !rows_aligned(p.keys, dtype) || !rows_aligned(p.queries, dtype) ||
         !aligned16(dlog_decay) || (reinterpret_cast<uintptr_t>(log_decay) & 3) || (reinterpret_cast<uintptr_t>(lengths) & 3))
         return GLA_ERR_ALIGN;
+    if (!rows_near(p.values) || !rows_near(p.keys) || !rows_near(p.queries)) return GLA_ERR_SHAPE;
     const DecayPlan plan = backward_plan(n, dtype);
     DecayParts parts = plan_parts(n);
     const int64_t first = entering_bytes(n, plan), need = first + place_parts(n, plan, constant_decay != 0, parts, nullptr);

@@ -28,46 +28,92 @@ struct DecayRows {
     int64_t sb, st, sh;
 };
 
-// LDS rows carry 32 bytes of padding: 16 rows' 16-byte reads fall into different banks eight by eight, and the four rows of
-// a transposing read as well.
-template <typename T> constexpr int lds_stride(int features) { return features + 32 / (int)sizeof(T); }
-
-// Per-lane offsets into an LDS tile of rows.
-template <typename T> struct DecayLane {
-    int row;        // row r, contraction over features in order:            r*S + 8c
-    int row2;       // the same in two halves:                               r*S + 4c   (and 16 further)
-    int col;        // feature r of a group of 16, contraction over rows in order
-    __device__ __forceinline__ DecayLane(int stride)
+// A tile of rows in LDS, F features each, and the three ways in which a product takes it as an operand.
+//
+// 16-bit data lie without padding, the 16-byte pieces of a row permuted by the row's number: piece p of row i is at p ^ f(i).  No read has
+// two lanes at a bank, as the counters say (256 bytes a cycle): 8-byte reads go by 32 lanes, i.e. 16 rows at one piece (halves) or 8 rows at
+// a pair of pieces (columns); 16-byte reads by 16 lanes, of rows 0-3 and 12-15 at one piece and rows 4-11 at its neighbour.  So f takes
+// every value once, neighbours of 8 rows get different pairs, and the values of rows 4-11 are whole pairs.  With rows padded by
+// 16 or 32 bytes instead, one of the three had two lanes to a bank, and half of the forward pass's LDS cycles were conflicts.
+// An exclusive or with the tile's or step's number and a constant number of rows makes every address from three numbers a
+// lane.  `here` gives a copy whose addresses are formed where they are used: kept for a whole loop, they took 30 registers of the
+// forward pass and 100 more were spilled.  float data keep rows padded by 32 bytes.
+template <typename T, int F> struct LdsTile;
+template <int F> struct LdsTile<__bf16, F> {
+    static constexpr int kRow = F;
+    int at_rows, at_halves, at_columns;
+    static __device__ __forceinline__ int permuted(int row)
+    {
+        const int upper = (row >> 3) & 1;
+        return F >= 128 ? (((row & 7) ^ (upper << 2)) << 1) | upper : ((((row >> 1) & 3) ^ (upper << 1)) << 1) | upper;
+    }
+    __device__ __forceinline__ LdsTile()
+    {
+        const int lane = threadIdx.x & 63, r = lane & 15, c = lane >> 4, row = 4 * c + (r >> 2);
+        at_rows = r * F + ((c ^ permuted(r)) << 3);
+        at_halves = r * F + (((c >> 1) ^ permuted(r)) << 3) + 4 * (c & 1);
+        at_columns = row * F + ((((r & 3) >> 1) ^ permuted(row)) << 3) + 4 * (r & 1);
+    }
+    __device__ __forceinline__ LdsTile here() const
+    {
+        LdsTile t = *this;
+        asm volatile("" : "+v"(t.at_rows), "+v"(t.at_halves), "+v"(t.at_columns));
+        return t;
+    }
+    static __device__ __forceinline__ int piece(int row, int col) { return row * F + (((col >> 3) ^ permuted(row)) << 3); }
+    // Volatile, or else the compiler joins the loads of one half for two tiles and moves every register of the operands to its place.
+    static __device__ __forceinline__ bf16x4 half(const __bf16 *p)
+    {
+        return *(const volatile __attribute__((address_space(3))) bf16x4 *)p;
+    }
+    // rows 16 * t + r as the operand's rows, features 32 * ks .. as the contracted index, in order
+    __device__ __forceinline__ bf16x8 rows(const __bf16 *p, int t, int ks) const { return ld8(p + 16 * t * F + (at_rows ^ (32 * ks))); }
+    // the same in two halves
+    __device__ __forceinline__ bf16x8 halves(const __bf16 *p, int t, int ks) const
+    {
+        return __builtin_shufflevector(half(p + 16 * t * F + (at_halves ^ (32 * ks))), half(p + 16 * t * F + (at_halves ^ (32 * ks + 16))),
+                                       0, 1, 2, 3, 4, 5, 6, 7);
+    }
+    // features 16 * t + r as the operand's rows, rows 32 * ks .. as the contracted index, in two halves
+    __device__ __forceinline__ bf16x8 columns(const __bf16 *p, int ks, int t) const
+    {
+        return lds_tr4x2(p + 32 * ks * F + (at_columns ^ (16 * t)), 16 * F);
+    }
+    // the place of features 16 * u + 4c .. of row 16 * t + r
+    __device__ __forceinline__ int four(int t, int u) const { return 16 * t * F + (at_halves ^ (16 * u)); }
+};
+template <int F> struct LdsTile<float, F> {
+    static constexpr int kRow = F + 8;
+    int at_rows, at_halves, at_columns;
+    __device__ __forceinline__ LdsTile()
     {
         const int lane = threadIdx.x & 63, r = lane & 15, c = lane >> 4;
-        row = r * stride + 8 * c;
-        row2 = r * stride + 4 * c;
-        if constexpr (sizeof(T) == 2) col = (8 * c + (r >> 2)) * stride + 4 * (r & 3);
-        else col = 8 * c * stride + r;
+        at_rows = r * kRow + 8 * c;
+        at_halves = r * kRow + 4 * c;
+        at_columns = 4 * c * kRow + r;
     }
+    __device__ __forceinline__ LdsTile here() const { return *this; }
+    static __device__ __forceinline__ int piece(int row, int col) { return row * kRow + col; }
+    __device__ __forceinline__ f32x8 rows(const float *p, int t, int ks) const { return ld8(p + 16 * t * kRow + at_rows + 32 * ks); }
+    __device__ __forceinline__ f32x8 halves(const float *p, int t, int ks) const
+    {
+        p += 16 * t * kRow + at_halves + 32 * ks;
+        const f32x4 a = *reinterpret_cast<const f32x4 *>(p), b = *reinterpret_cast<const f32x4 *>(p + 16);
+        f32x8 r;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) { r.v[e] = a[e]; r.v[4 + e] = b[e]; }
+        return r;
+    }
+    __device__ __forceinline__ f32x8 columns(const float *p, int ks, int t) const
+    {
+        p += 32 * ks * kRow + at_columns + 16 * t;
+        f32x8 r;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) r.v[e] = p[((e & 3) + 16 * (e >> 2)) * kRow];
+        return r;
+    }
+    __device__ __forceinline__ int four(int t, int u) const { return 16 * t * kRow + at_halves + 16 * u; }
 };
-__device__ __forceinline__ bf16x8 lds_two_halves(const __bf16 *p)
-{
-    return __builtin_shufflevector(*reinterpret_cast<const bf16x4 *>(p), *reinterpret_cast<const bf16x4 *>(p + 16), 0, 1, 2, 3,
-                                   4, 5, 6, 7);
-}
-__device__ __forceinline__ f32x8 lds_two_halves(const float *p)
-{
-    const f32x4 a = *reinterpret_cast<const f32x4 *>(p), b = *reinterpret_cast<const f32x4 *>(p + 16);
-    f32x8 r;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) { r.v[e] = a[e]; r.v[4 + e] = b[e]; }
-    return r;
-}
-// 32 rows of 16 features, the features as the operand's rows
-__device__ __forceinline__ bf16x8 lds_columns(const __bf16 *p, int stride) { return lds_tr4x2(p, 4 * stride); }
-__device__ __forceinline__ f32x8 lds_columns(const float *p, int stride)
-{
-    f32x8 r;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) r.v[e] = p[e * stride];
-    return r;
-}
 
 // A float operand as N bf16 ones whose sum it is: 1 rounds it (2^-9 of a value), 2 leaves 2^-17, 3 leaves 2^-25, which is
 // what a float holds.  float data take it as it is.
@@ -76,60 +122,83 @@ template <int N> struct Split<__bf16, N> {
     bf16x8 part[N];
     __device__ __forceinline__ explicit Split(const float (&x)[8])
     {
-        float rest[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) rest[e] = x[e];
+        for (int e = 0; e < 8; e += 2) {
+            f32x2 rest = {x[e], x[e + 1]};
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                part[i][e] = (__bf16)rest[e];
-                if (i + 1 < N) rest[e] -= (float)part[i][e];
+            for (int i = 0; i < N; ++i) {
+                const bf16x2 p = __builtin_convertvector(rest, bf16x2);       // two at a time
+                part[i][e] = p[0];
+                part[i][e + 1] = p[1];
+                if (i + 1 < N) {
+                    const uint32_t bits = __builtin_bit_cast(uint32_t, p);
+                    rest[0] -= __uint_as_float(bits << 16);
+                    rest[1] -= __uint_as_float(bits & 0xffff0000u);
+                }
             }
         }
     }
-    // the small parts first
-    __device__ __forceinline__ f32x4 left(bf16x8 b, f32x4 c) const
-    {
-#pragma unroll
-        for (int i = N - 1; i >= 0; --i) c = mma_d(part[i], b, c);
-        return c;
-    }
-    __device__ __forceinline__ f32x4 right(bf16x8 a, f32x4 c) const
-    {
-#pragma unroll
-        for (int i = N - 1; i >= 0; --i) c = mma_d(a, part[i], c);
-        return c;
-    }
 };
 template <int N> struct Split<float, N> {
-    f32x8 whole;
+    f32x8 part[1];
     __device__ __forceinline__ explicit Split(const float (&x)[8])
     {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) whole.v[e] = x[e];
+        for (int e = 0; e < 8; ++e) part[0].v[e] = x[e];
     }
-    __device__ __forceinline__ f32x4 left(const f32x8 &b, f32x4 c) const { return mma_d(whole, b, c); }
-    __device__ __forceinline__ f32x4 right(const f32x8 &a, f32x4 c) const { return mma_d(a, whole, c); }
 };
+// M products with the split operand on the left (right), the small parts first; products of one sum do not follow each other.
+template <typename T, int N, typename D8, int M>
+__device__ __forceinline__ void mma_left(const Split<T, N> &a, const D8 (&b)[M], f32x4 *c)
+{
+    constexpr int kParts = sizeof(a.part) / sizeof(a.part[0]);
+#pragma unroll
+    for (int i = kParts - 1; i >= 0; --i)
+#pragma unroll
+        for (int m = 0; m < M; ++m) c[m] = mma_d(a.part[i], b[m], c[m]);
+}
+template <typename T, int N, typename D8, int M>
+__device__ __forceinline__ void mma_right(const D8 (&a)[M], const Split<T, N> &b, f32x4 *c)
+{
+    constexpr int kParts = sizeof(b.part) / sizeof(b.part[0]);
+#pragma unroll
+    for (int i = kParts - 1; i >= 0; --i)
+#pragma unroll
+        for (int m = 0; m < M; ++m) c[m] = mma_d(a[m], b.part[i], c[m]);
+}
 __device__ __forceinline__ void two_tiles(f32x4 a, f32x4 b, float (&x)[8])
 {
 #pragma unroll
     for (int e = 0; e < 4; ++e) { x[e] = a[e]; x[4 + e] = b[e]; }
 }
 
-__device__ __forceinline__ double shfl_up_f64(double x, int by)
+// Sums of a wave's 64-bit numbers up to each lane's, by moves inside rows of 16 lanes and from the rows before.
+template <int CTRL, int ROWS> __device__ __forceinline__ double dpp_f64(double x)
 {
-    return __hiloint2double(__shfl_up(__double2hiint(x), by, 64), __shfl_up(__double2loint(x), by, 64));
+    return __hiloint2double(__builtin_amdgcn_update_dpp(0, __double2hiint(x), CTRL, ROWS, 0xf, false),
+                            __builtin_amdgcn_update_dpp(0, __double2loint(x), CTRL, ROWS, 0xf, false));
+}
+__device__ __forceinline__ double prefix_sum_wave(double x)
+{
+    x += dpp_f64<0x111, 0xf>(x);      // row_shr:1
+    x += dpp_f64<0x112, 0xf>(x);
+    x += dpp_f64<0x114, 0xf>(x);
+    x += dpp_f64<0x118, 0xf>(x);
+    x += dpp_f64<0x142, 0xa>(x);      // row_bcast:15 into rows 1 and 3
+    x += dpp_f64<0x143, 0xc>(x);      // row_bcast:31 into rows 2 and 3
+    return x;
 }
 
-// The chunk's gates, by one wave: lane i holds token i's log decay (0 past the end).  Sums in powers of two.
+// The chunk's gates, by one wave, which has token i's log decay in lane i (0 past the end).  Sums in powers of two, formed in 64 bits
+// and kept as a float and what it leaves, so that the difference of two is as exact as a float holds it.
 // A gate below 2^-100000 counts as that (so -inf - (-inf) does not arise); a NaN stays one.
 template <int C> struct ChunkGates {
-    double sum[C];          // L_i
+    float sum[C], rest[C];  // L_i
     float from_start[C];    // 2^{L_i}
     float to_end[C];        // 2^{L_C - L_i}
-    float whole;            // 2^{L_C}
+    float whole, pad[3];    // 2^{L_C}
+    // 2^{L_i - L_j}
+    static __device__ __forceinline__ float weight(float si, float ri, float sj, float rj) { return fast_exp2((si - sj) + (ri - rj)); }
 };
 template <int C> __device__ __forceinline__ double chunk_gates(ChunkGates<C> &g, float a)
 {
@@ -137,42 +206,84 @@ template <int C> __device__ __forceinline__ double chunk_gates(ChunkGates<C> &g,
     double x = (double)a * 1.4426950408889634074;
     x = x < -1e5 ? -1e5 : x;
     if (lane >= C) x = 0.0;
-#pragma unroll
-    for (int by = 1; by < C; by *= 2) {
-        const double other = shfl_up_f64(x, by);
-        if (lane >= by) x += other;
-    }
-    const double all = __hiloint2double(__shfl(__double2hiint(x), C - 1, 64), __shfl(__double2loint(x), C - 1, 64));
+    x = prefix_sum_wave(x);
+    const double all = __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(x), C - 1), __builtin_amdgcn_readlane(__double2loint(x), C - 1));
     if (lane < C) {
-        g.sum[lane] = x;
-        g.from_start[lane] = fast_exp2((float)x);
+        const float s = (float)x;
+        g.sum[lane] = s;
+        g.rest[lane] = (float)(x - (double)s);
+        g.from_start[lane] = fast_exp2(s);
         g.to_end[lane] = fast_exp2((float)(all - x));
         if (lane == 0) g.whole = fast_exp2((float)all);
     }
     return all;
 }
 
-// Rows of a chunk on their way from memory to LDS: `NT` threads hold C x F values in registers.
+// The same number, formed again from here on: what was derived from it before does not stay in registers.
+__device__ __forceinline__ unsigned again(unsigned x)
+{
+    asm volatile("" : "+v"(x));
+    return x;
+}
+
+__device__ __forceinline__ int again_uniform(int x)
+{
+    asm volatile("" : "+s"(x));
+    return x;
+}
+
+// A pointer that all lanes share and a lane's place behind it in bytes: one register of a lane, where a 64-bit sum takes two.
+template <typename P> __device__ __forceinline__ P *at_bytes(P *base, unsigned bytes)
+{
+    return reinterpret_cast<P *>(reinterpret_cast<std::conditional_t<std::is_const_v<P>, const char, char> *>(base) + bytes);
+}
+
+// Rows of a chunk on their way from memory to LDS: `NT` threads hold C x F values in registers.  A thread's pieces lie a fixed number of
+// rows apart; its place in a chunk is one number that stays, and a chunk is a pointer that all share.
 template <typename T, int C, int F, int NT> struct RowsInFlight {
     typedef typename FragTypes<T>::d8 d8;
-    static constexpr int kPieces = C * F / 8, kPer = (kPieces + NT - 1) / NT;
+    static constexpr int kPieces = C * F / 8, kPer = (kPieces + NT - 1) / NT, kStep = NT / (F / 8);
+    static_assert(NT % (F / 8) == 0, "");
     d8 x[kPer];
-    // rows t0 .. t0+C-1 of `rows` (at the pair's first row), zeros from token `len` and from feature `features` on
-    __device__ __forceinline__ void load(const T *rows, int64_t st, int64_t t0, int64_t len, int features)
+    int st, features;
+    __device__ __forceinline__ RowsInFlight(int64_t stride, int count, T *tile) : st((int)stride), features(count)
     {
+        const int row = threadIdx.x / (F / 8), col = 8 * (threadIdx.x % (F / 8));
+        if (col >= features) {                   // features past the end stay zeros
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            const int at = threadIdx.x + i * NT, row = at / (F / 8), col = 8 * (at % (F / 8));
-            x[i] = d8{};
-            if (at < kPieces && t0 + row < len && col < features) x[i] = ld8(rows + (t0 + row) * st + col);
+            for (int i = 0; i < kPer; ++i)
+                if (row + i * kStep < C) st8(tile + LdsTile<T, F>::piece(row + i * kStep, col), d8{});
         }
     }
-    __device__ __forceinline__ void store(T *tile, int stride) const
+    // the rows of a chunk that `rows` points at, `left` of which exist: zeros behind them
+    __device__ __forceinline__ void load(const T *rows, int left)
     {
+        // formed here each time: kept over the loop, a lane's place would take a register, and in 64 bits two
+        const unsigned tid = again(threadIdx.x);
+        const int row = tid / (F / 8), col = 8 * (tid % (F / 8));
+        const unsigned at = (unsigned)(row * st + col) * (unsigned)sizeof(T);
+        if (left >= C) {
+            if (col < features && (kPieces >= NT || row < C)) {
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            const int at = threadIdx.x + i * NT, row = at / (F / 8), col = 8 * (at % (F / 8));
-            if (at < kPieces) st8(tile + row * stride + col, x[i]);
+                for (int i = 0; i < kPer; ++i)
+                    if (kPieces % NT == 0 || row + i * kStep < C) x[i] = ld8(at_bytes(rows + (int64_t)(i * kStep) * st, at));
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                x[i] = d8{};
+                if (col < features && row + i * kStep < min(left, C)) x[i] = ld8(at_bytes(rows + (int64_t)(i * kStep) * st, at));
+            }
+        }
+    }
+    __device__ __forceinline__ void store(T *tile) const
+    {
+        const unsigned tid = again(threadIdx.x);
+        const int row = tid / (F / 8), col = 8 * (tid % (F / 8));
+        if (col < features) {
+#pragma unroll
+            for (int i = 0; i < kPer; ++i)
+                if (kPieces % NT == 0 || row + i * kStep < C) st8(tile + LdsTile<T, F>::piece(row + i * kStep, col), x[i]);
         }
     }
 };

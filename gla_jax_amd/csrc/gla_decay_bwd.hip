@@ -32,110 +32,122 @@ struct BackwardArgs {
     int row_parts, value_parts;                  // of dquery and dkey; of dvalue
 };
 
-// One workgroup: a segment of a (batch, head) pair, DKW key and DVW value features.  Wave w owns key features 16w .. 16w+15
-// for dq, dk and value features 16w .. 16w+15 for dv; dS is held twice, since it is contracted over either index: `by_value`
-// has the wave's value columns with key rows, `by_key` the wave's key columns with value rows, each an operand as it lies.
+// One workgroup: a segment of a (batch, head) pair, DKW key and DVW value features.  Its first waves make dq and dv: wave w of key
+// features 16w .. 16w+15, with its columns of S, and of value features 16w .. 16w+15.  The others make dk and carry dS: its columns of
+// key features lie in the accumulators with value features as rows, an operand of dk as they are; dv contracts dS over the other
+// index and takes it from LDS, rounded to `T` as any operand of a 16-bit result.  (A second copy of dS by value columns cost 32
+// registers and as many products as the first; all of it on 8 waves of twice the registers left a SIMD two waves, whose
+// matrix, vector and LDS phases then followed each other: 135 us against the %US% of 16 at B4 T4096 H6 D128.)
 // S and dS enter what the gates' gradient is formed from in three parts, i.e. as the 32-bit numbers that they are.
 template <typename T, int DKW, int DVW>
-__global__ __launch_bounds__((DKW > DVW ? DKW : DVW) * 4) void decay_gradient_kernel(const BackwardArgs a)
+__global__ __launch_bounds__(((DKW > DVW ? DKW : DVW) + DKW) * 4) void decay_gradient_kernel(const BackwardArgs a)
 {
-    constexpr int NW = (DKW > DVW ? DKW : DVW) / 16, NT = NW * 64, KT = DKW / 16, VT = DVW / 16, KK = DKW / 32, VK = DVW / 32;
+    constexpr int KT = DKW / 16, VT = DVW / 16, KK = DKW / 32, VK = DVW / 32, NA = KT > VT ? KT : VT, NW = NA + KT, NT = NW * 64;
     constexpr int C = DecayChunk<T>::C, CT = C / 16, CS = C / 32;
-    constexpr int SK = lds_stride<T>(DKW), SV = lds_stride<T>(DVW), SP = lds_stride<T>(C);
     typedef typename FragTypes<T>::d8 D8;
+    typedef LdsTile<T, DKW> TileK;
+    typedef LdsTile<T, DVW> TileV;
+    typedef LdsTile<T, C> TileP;
     extern __shared__ char smem[];
-    T *sQ = reinterpret_cast<T *>(smem), *sK = sQ + C * SK, *sV = sK + C * SK, *sO = sV + C * SV, *sP = sO + C * SV,
-      *sD = sP + C * SP;
-    ChunkGates<C> &gate = *reinterpret_cast<ChunkGates<C> *>(reinterpret_cast<char *>(sD + C * SP));
-    float *sRow = reinterpret_cast<float *>(&gate + 1);       // [CT][C] row sums of one column of tiles
-    float *sCol = sRow + CT * C;                              // [CT][C] column sums of one row of tiles
-    float *sU = sCol + CT * C, *sW = sU + KT * C, *sX = sW + KT * C;
+    T *sQ = reinterpret_cast<T *>(smem), *sK = sQ + C * TileK::kRow, *sV = sK + C * TileK::kRow, *sO = sV + C * TileV::kRow,
+      *sP = sO + C * TileV::kRow, *sD = sP + C * TileP::kRow, *sS = sD + C * TileP::kRow;
+    ChunkGates<C> *gates = reinterpret_cast<ChunkGates<C> *>(reinterpret_cast<char *>(sS + DKW * TileV::kRow));
+    // what the gates' gradient is formed from, of a chunk and of the one before
+    struct Sums {
+        float row[CT][C];                        // row sums of one column of tiles
+        float col[CT][C];                        // column sums of one row of tiles
+        float u[KT][C], w[KT][C];
+        float x[16];
+    };
+    Sums *sums = reinterpret_cast<Sums *>(gates + 2);
+    double *sGate = reinterpret_cast<double *>(sums + 2);     // the gates' gradients so far, by token of the chunk
 
-    const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63, r = lane & 15, c = lane >> 4;
+    const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, r = lane & 15, c = lane >> 4;
     const int64_t bh = blockIdx.x, b = bh / a.n.H, h = bh % a.n.H, group = a.n.H / a.n.HK, hk = h / group;
     const int DK = (int)a.n.DK, DV = (int)a.n.DV, vslabs = (DV + DVW - 1) / DVW;
     const int ks0 = blockIdx.y / vslabs, vs0 = blockIdx.y % vslabs, dk0 = ks0 * DKW, dv0 = vs0 * DVW;
     const int64_t order = blockIdx.z, seg = a.plan.segments - 1 - order;
-    const int64_t len = a.lengths ? min(max((int64_t)a.lengths[b], (int64_t)0), a.n.T) : a.n.T;
-    const int64_t first = seg * a.plan.per, last = min(first + a.plan.per, a.plan.chunks), live = min(last, (len + C - 1) / C);
+    const int T_ = (int)a.n.T, len = a.lengths ? min(max(a.lengths[b], 0), T_) : T_;
+    const int first = (int)(seg * a.plan.per), last = (int)min(first + a.plan.per, a.plan.chunks), live = min(last, (len + C - 1) / C);
     const T *K = static_cast<const T *>(a.keys.p) + b * a.keys.sb + hk * a.keys.sh + dk0;
     const T *Q = static_cast<const T *>(a.queries.p) + b * a.queries.sb + hk * a.queries.sh + dk0;
     const T *V = static_cast<const T *>(a.values.p) + b * a.values.sb + h * a.values.sh + dv0;
     const T *O = static_cast<const T *>(a.dout.p) + b * a.dout.sb + h * a.dout.sh + dv0;
     const float *G = static_cast<const float *>(a.gates.p) + b * a.gates.sb + h * a.gates.sh;
-    const bool key_wave = w < KT && dk0 + 16 * w < DK, value_wave = w < VT && dv0 + 16 * w < DV;
-    const DecayLane<T> LK(SK), LV(SV), LP(SP);
-    const int64_t part_qk = vs0 * group + h % group;
-    const int64_t row_qk = hk * DK + dk0 + 16 * w + 4 * c, rows_qk = a.n.HK * DK;       // within a token's row
-    const int64_t row_v = h * DV + dv0 + 16 * w + 4 * c, rows_v = a.n.H * DV;
+    const bool second = w >= NA;                 // dk and dS, or else dq and dv
+    const int wk = second ? w - NA : w;          // the wave's key features are 16 wk ..
+    const bool has_keys = wk < KT, key_wave = has_keys && dk0 + 16 * wk < DK, value_wave = !second && w < VT && dv0 + 16 * w < DV;
+    const TileK tk;
+    const TileV tv;
+    const TileP tp;
+    const int64_t part_qk = (vs0 * group + h % group) * a.n.B * a.n.T, part_v = ks0 * a.n.B * a.n.T;      // in rows
+    const int rows_qk = (int)(a.n.HK * DK), rows_v = (int)(a.n.H * DV);                                   // a token's row
+    const int row_qk = (int)(hk * DK) + dk0 + 16 * wk, row_v = (int)(h * DV) + dv0 + 16 * w;
 
-    auto put = [&](void *to, bool parts, int64_t part, int64_t t, int64_t width, int64_t at, const float (&x)[4]) {
-        const int64_t i = (b * a.n.T + t) * width + at;
-        if (parts) store_vec<float, 4>(static_cast<float *>(to) + part * a.n.B * a.n.T * width + i, x);
-        else store_vec<T, 4>(static_cast<T *>(to) + i, x);
+    // four values of token t + r, the features from `at`: 4c .. 4c+3
+    auto put = [&](void *to, bool parts, int64_t part, int t, int width, int at, unsigned lane_at, const float (&x)[4]) {
+        const int64_t row = b * a.n.T + t;
+        if (parts) store_vec<float, 4>(at_bytes(static_cast<float *>(to) + ((part + row) * width + at), 4 * lane_at), x);
+        else store_vec<T, 4>(at_bytes(static_cast<T *>(to) + (row * width + at), (unsigned)sizeof(T) * lane_at), x);
     };
 
-    // ---- the cotangent that enters, in both forms ----
-    f32x4 by_value[KT], by_key[VT];
+    // ---- the cotangent that enters: key feature r of the wave's, value features 16t + 4c .. ----
+    f32x4 state[VT];                             // dS, which stays; of the first waves S, a chunk's after the other
 #pragma unroll
-    for (int t = 0; t < KT; ++t) by_value[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int t = 0; t < VT; ++t) by_key[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int t = 0; t < VT; ++t) state[t] = f32x4{0.f, 0.f, 0.f, 0.f};
     if (order == 0) {
-        const int64_t base = bh * DK * DV;
-#pragma unroll
-        for (int t = 0; t < KT; ++t)
-            if (value_wave && dk0 + 16 * t < DK) {
-                float x[4];
-                load_hidden<4>(a.dhidden_final, a.hidden_dtype,
-                               base + (int64_t)(dk0 + 16 * t + 4 * c + (r & 3)) * DV + dv0 + 16 * w + (r & ~3), x);
-                quad_transpose(x);
-                by_value[t] = f32x4{x[0], x[1], x[2], x[3]};
-            }
 #pragma unroll
         for (int t = 0; t < VT; ++t)
-            if (key_wave && dv0 + 16 * t < DV) {
+            if (second && key_wave && dv0 + 16 * t < DV) {
                 float x[4];
-                load_hidden<4>(a.dhidden_final, a.hidden_dtype, base + (int64_t)(dk0 + 16 * w + r) * DV + dv0 + 16 * t + 4 * c, x);
-                by_key[t] = f32x4{x[0], x[1], x[2], x[3]};
+                load_hidden<4>(a.dhidden_final, a.hidden_dtype, (bh * DK + dk0 + 16 * wk + r) * DV + dv0 + 16 * t + 4 * c, x);
+                state[t] = f32x4{x[0], x[1], x[2], x[3]};
             }
     } else {
         const int tiles = (int)decay_key_width(DK) / 16;
         const float *from = a.entering + ((bh * a.plan.segments + order - 1) * vslabs + vs0) * (int64_t)(tiles * 16 * DVW);
 #pragma unroll
-        for (int t = 0; t < KT; ++t)
-            if (w < VT) by_value[t] = reinterpret_cast<const f32x4 *>(from)[(w * tiles + dk0 / 16 + t) * 64 + lane];
-#pragma unroll
         for (int t = 0; t < VT; ++t)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                if (w < KT) by_key[t][e] = from[((t * tiles + dk0 / 16 + w) * 64 + (r >> 2) * 16 + 4 * c + e) * 4 + (r & 3)];
+                if (second) state[t][e] = from[((t * tiles + dk0 / 16 + wk) * 64 + (r >> 2) * 16 + 4 * c + e) * 4 + (r & 3)];
     }
 
-    RowsInFlight<T, C, DKW, NT> fk, fq;
-    RowsInFlight<T, C, DVW, NT> fv, fo;
+    RowsInFlight<T, C, DKW, NT> fk(a.keys.st, DK - dk0, sK), fq(a.queries.st, DK - dk0, sQ);
+    RowsInFlight<T, C, DVW, NT> fv(a.values.st, DV - dv0, sV), fo(a.dout.st, DV - dv0, sO);
     float g = 0.f;
-    auto fetch = [&](int64_t n) {
-        fk.load(K, a.keys.st, n * C, len, DK - dk0);
-        fq.load(Q, a.queries.st, n * C, len, DK - dk0);
-        fv.load(V, a.values.st, n * C, len, DV - dv0);
-        fo.load(O, a.dout.st, n * C, len, DV - dv0);
-        g = w == 0 && lane < C && n * C + lane < len ? G[(n * C + lane) * a.gates.st] : 0.f;
+    auto fetch_gates = [&](int n) {              // by the wave that makes the chunk's gates
+        g = w == NW - 1 && lane < C && n * C + lane < len ? G[(int64_t)(n * C + lane) * a.gates.st] : 0.f;
+    };
+    auto fetch = [&](int n) {                    // the rows that the pointers have come to
+        const int left = len - n * C;
+        fk.load(K, left);
+        fq.load(Q, left);
+        fv.load(V, left);
+        fo.load(O, left);
+        K -= C * a.keys.st;
+        Q -= C * a.queries.st;
+        V -= C * a.values.st;
+        O -= C * a.dout.st;
     };
 
-    double gate_sum = 0.0;
+    if (tid < 64) sGate[tid] = 0.0;
     // The gates' gradient of chunk n, by one wave, from the sums that the others left.
-    auto gates_gradient = [&](int64_t n) {
+    auto gates_gradient = [&](int n, const Sums &s) {
+        const int lane = (int)again(tid) & 63;
         float u = 0.f, ww = 0.f;
         if (lane < C) {
 #pragma unroll
-            for (int i = 0; i < KT; ++i) { u += sU[i * C + lane]; ww += sW[i * C + lane]; }
-            for (int i = 0; i <= lane / 16; ++i) u += sRow[i * C + lane];
-            for (int i = lane / 16; i < CT; ++i) u -= sCol[i * C + lane];
+            for (int i = 0; i < KT; ++i) { u += s.u[i][lane]; ww += s.w[i][lane]; }
+#pragma unroll
+            for (int i = 0; i < CT; ++i) {
+                u += i <= lane / 16 ? s.row[i][lane] : 0.f;
+                u -= i >= lane / 16 ? s.col[i][lane] : 0.f;
+            }
         }
         float x = 0.f;
 #pragma unroll
-        for (int i = 0; i < KT; ++i) x += sX[i];
+        for (int i = 0; i < KT; ++i) x += s.x[i];
         float before = __shfl_up(ww, 1, 64);
         if (lane == 0) before = 0.f;
 #pragma unroll
@@ -144,242 +156,286 @@ __global__ __launch_bounds__((DKW > DVW ? DKW : DVW) * 4) void decay_gradient_ke
             if (lane >= by) before += lower;
             if (lane + by < 64) u += upper;
         }
-        const int64_t t = n * C + lane;
+        const int t = n * C + lane;
         const float d = t < len ? x + before + u : 0.f;
-        if (lane < C && t < a.n.T) {
-            if (a.dgate) a.dgate[(((int64_t)blockIdx.y * a.n.B + b) * a.n.T + t) * a.n.H + h] = d;
-            gate_sum += d;
+        if (lane < C && t < T_) {
+            if (a.dgate) a.dgate[((blockIdx.y * a.n.B + b) * a.n.T + t) * a.n.H + h] = d;
+            sGate[lane] += d;
         }
     };
 
-    for (int i = tid; i < C * SP; i += NT) sP[i] = sD[i] = (T)0.f;      // the tiles above the diagonal that products take along
-    const int gates_wave = NW - 1;
-    const int64_t count = max(live - first, (int64_t)0);
-    if (count > 0) fetch(live - 1);
-    for (int64_t i = 0; i < count; ++i) {
-        const int64_t n = live - 1 - i;
+    for (int i = tid; i < C * TileP::kRow; i += NT) sP[i] = sD[i] = (T)0.f;      // the tiles above the diagonal that products take along
+    const int sums_wave = NW - 2;
+    const int count = max(live - first, 0);
+    int n = live - 1;
+    if (count > 0) {
+        K += (int64_t)n * C * a.keys.st;
+        Q += (int64_t)n * C * a.queries.st;
+        V += (int64_t)n * C * a.values.st;
+        O += (int64_t)n * C * a.dout.st;
+        fetch_gates(n);
+        fetch(n);
+        if (w == NW - 1) chunk_gates<C>(gates[0], g);
+        if (count > 1) fetch_gates(n - 1);
+    }
+    for (int i = 0; i < count; ++i, --n) {
+        const ChunkGates<C> &gate = gates[i & 1];
+        Sums &sum = sums[i & 1];
         lds_barrier();                            // the last chunk's tiles are read, its sums written
-        fk.store(sK, SK);
-        fq.store(sQ, SK);
-        fv.store(sV, SV);
-        fo.store(sO, SV);
-        if (w == 0) chunk_gates<C>(gate, g);
-        if (w == gates_wave && i > 0) gates_gradient(n + 1);
+        fk.store(sK);
+        fq.store(sQ);
+        fv.store(sV);
+        fo.store(sO);
+        if (second) {                             // dS as the operand of dv
+            const TileV LV = tv.here();
+#pragma unroll
+            for (int t = 0; t < VT; ++t) {
+                const float x[4] = {state[t][0], state[t][1], state[t][2], state[t][3]};
+                store_vec<T, 4>(sS + LV.four(wk, t), x);
+            }
+        }
         lds_barrier();
         // the state before the chunk: key feature r of the wave's, value features in halves
-        f32x4 S[VT];
+        const float *kept = a.kept + ((bh * a.plan.chunks + n) * DK + dk0 + 16 * wk) * DV + dv0;
+        if (!second) {
+            const unsigned at = (again(r) * DV + 4 * c) * 4;
+            const int dv = again_uniform(key_wave ? DV - dv0 : 0);
 #pragma unroll
-        for (int t = 0; t < VT; ++t) {
-            S[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-            if (key_wave && dv0 + 16 * t < DV)
-                S[t] = *reinterpret_cast<const f32x4 *>(a.kept + ((bh * a.plan.chunks + n) * DK + dk0 + 16 * w + r) * DV + dv0 +
-                                                        16 * t + 4 * c);
+            for (int t = 0; t < VT; ++t) {
+                state[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+                if (16 * t < dv) state[t] = *reinterpret_cast<const f32x4 *>(at_bytes(kept + 16 * t, at));
+            }
         }
         if (i + 1 < count) fetch(n - 1);
 
         // ---- scores, transposed: lane (r, c) has keys 4c .. 4c+3 of tile tj for query r of tile ti ----
-        for (int n16 = w; n16 < CT * (CT + 1) / 2; n16 += NW) {
-            int ti, tj;
-            triangle(n16, ti, tj);
-            f32x4 s = {0.f, 0.f, 0.f, 0.f}, d = {0.f, 0.f, 0.f, 0.f};
+        {
+            const TileK LK = tk.here();
+            const TileV LV = tv.here();
+            const TileP LP = tp.here();
+#pragma unroll 1
+            for (int n16 = w; n16 < CT * (CT + 1) / 2; n16 += NW) {
+                int ti, tj;
+                triangle(n16, ti, tj);
+                f32x4 s = {0.f, 0.f, 0.f, 0.f}, d = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int ks = 0; ks < KK; ++ks)
-                s = mma_d(ld8(sK + 16 * tj * SK + LK.row + 32 * ks), ld8(sQ + 16 * ti * SK + LK.row + 32 * ks), s);
+                for (int ks = 0; ks < KK; ++ks) s = mma_d(LK.rows(sK, tj, ks), LK.rows(sQ, ti, ks), s);
 #pragma unroll
-            for (int ks = 0; ks < VK; ++ks)
-                d = mma_d(ld8(sV + 16 * tj * SV + LV.row + 32 * ks), ld8(sO + 16 * ti * SV + LV.row + 32 * ks), d);
-            const int qi = 16 * ti + r, kj = 16 * tj + 4 * c;
-            const double at = gate.sum[qi];
-            float p[4], dd[4], row = 0.f, col[4];
+                for (int ks = 0; ks < VK; ++ks) d = mma_d(LV.rows(sV, tj, ks), LV.rows(sO, ti, ks), d);
+                const int qi = 16 * ti + r, kj = 16 * tj + 4 * c;
+                const float at = gate.sum[qi], at_rest = gate.rest[qi];
+                const f32x4 to = *reinterpret_cast<const f32x4 *>(gate.sum + kj), to_rest = *reinterpret_cast<const f32x4 *>(gate.rest + kj);
+                float p[4], dd[4], row = 0.f, col[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float weight = fast_exp2((float)(at - gate.sum[kj + e]));
-                p[e] = kj + e <= qi ? s[e] * weight : 0.f;
-                dd[e] = kj + e <= qi ? d[e] * weight : 0.f;
-                col[e] = p[e] * d[e];
-                if (!(kj + e <= qi)) col[e] = 0.f;
-                row += col[e];
+                for (int e = 0; e < 4; ++e) {
+                    const float weight = kj + e <= qi ? ChunkGates<C>::weight(at, at_rest, to[e], to_rest[e]) : 0.f;
+                    p[e] = kj + e <= qi ? s[e] * weight : 0.f;
+                    dd[e] = kj + e <= qi ? d[e] * weight : 0.f;
+                    col[e] = kj + e <= qi ? p[e] * d[e] : 0.f;
+                    row += col[e];
+                }
+                store_vec<T, 4>(sP + LP.four(ti, tj), p);
+                store_vec<T, 4>(sD + LP.four(ti, tj), dd);
+                row = reduce_over_cgroups(row);
+                if (c == 0) sum.row[tj][16 * ti + again(r)] = row;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float x = col[e];
+                    x += dpp_f32<kDppQuadXor1>(x);
+                    x += dpp_f32<kDppQuadXor2>(x);
+                    x += dpp_f32<kDppRowHalfMirror>(x);
+                    x += dpp_f32<kDppRowMirror>(x);
+                    col[e] = x;
+                }
+                if (r == 0) store_vec<float, 4>(sum.col[ti] + 16 * tj + 4 * again(c), col);
             }
-            store_vec<T, 4>(sP + qi * SP + kj, p);
-            store_vec<T, 4>(sD + qi * SP + kj, dd);
-            row = reduce_over_cgroups(row);
-            if (c == 0) sRow[tj * C + qi] = row;
+        }
+        // beside the scores, by waves that have a tile less than the first ones or none: the last chunk's gradient of the gates, and
+        // the next chunk's gates
+        if (w == sums_wave && i > 0) gates_gradient(n + 1, sums[(i + 1) & 1]);
+        if (w == NW - 1 && i + 1 < count) {
+            chunk_gates<C>(gates[(i + 1) & 1], g);
+            if (i + 2 < count) fetch_gates(n - 2);
+        }
+        const float whole = gate.whole;
+        if (second) {
+            float x = 0.f;
+            const unsigned at = (again(r) * DV + 4 * c) * 4;
+            const int dv = again_uniform(key_wave ? DV - dv0 : 0);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                float x = col[e];
-                x += dpp_f32<kDppQuadXor1>(x);
-                x += dpp_f32<kDppQuadXor2>(x);
-                x += dpp_f32<kDppRowHalfMirror>(x);
-                x += dpp_f32<kDppRowMirror>(x);
-                if (r == 0) sCol[ti * C + kj + e] = x;
-            }
+            for (int t = 0; t < VT; ++t)
+                if (16 * t < dv) {
+                    const f32x4 S = *reinterpret_cast<const f32x4 *>(at_bytes(kept + 16 * t, at));
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x += S[e] * state[t][e];
+                }
+#pragma unroll
+            for (int m = 1; m < 64; m *= 2) x += shfl_xor_f32(x, m);
+            if (lane == 0) sum.x[wk] = whole * x;
         }
         lds_barrier();
 
-        const float whole = gate.whole;
-        D8 qc[CS], kc[CS];
-        if (w < KT) {
+        const unsigned lane_qk = again(r) * rows_qk + 4 * c, lane_v = again(r) * rows_v + 4 * c;
+        f32x4 o[CT];
 #pragma unroll
-            for (int ks = 0; ks < CS; ++ks) {
-                qc[ks] = lds_columns(sQ + 32 * ks * SK + 16 * w + LK.col, SK);
-                kc[ks] = lds_columns(sK + 32 * ks * SK + 16 * w + LK.col, SK);
-            }
-            f32x4 o[CT];
+        for (int ti = 0; ti < CT; ++ti) o[ti] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (!second && has_keys) {
             // ---- dq ----
-            float x = 0.f;
+            {
+                const TileV LV = tv.here();
 #pragma unroll
-            for (int t = 0; t < VT; ++t)
+                for (int ks = 0; ks < VK; ++ks) {
+                    float s[8];
+                    two_tiles(state[2 * ks], state[2 * ks + 1], s);
+                    const Split<T, 3> op(s);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) x += S[t][e] * by_key[t][e];
-#pragma unroll
-            for (int m = 1; m < 64; m *= 2) x += shfl_xor_f32(x, m);
-            if (lane == 0) sX[w] = whole * x;
-#pragma unroll
-            for (int ti = 0; ti < CT; ++ti) o[ti] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int ks = 0; ks < VK; ++ks) {
-                float s[8];
-                two_tiles(S[2 * ks], S[2 * ks + 1], s);
-                const Split<T, 3> op(s);
-#pragma unroll
-                for (int ti = 0; ti < CT; ++ti) o[ti] = op.left(lds_two_halves(sO + 16 * ti * SV + LV.row2 + 32 * ks), o[ti]);
+                    for (int ti = 0; ti < CT; ti += 2) {
+                        const D8 x[2] = {LV.halves(sO, ti, ks), LV.halves(sO, ti + 1, ks)};
+                        mma_left(op, x, o + ti);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);      // a step's operands at a time
+                }
             }
+            const TileK LK = tk.here();
+            const TileP LP = tp.here();
+            D8 kc[CS];
+#pragma unroll
+            for (int ks = 0; ks < CS; ++ks) kc[ks] = LK.columns(sK, ks, w);
 #pragma unroll
             for (int ti = 0; ti < CT; ++ti) {
                 const float scale = gate.from_start[16 * ti + r];
                 float qv[4], u = 0.f;
-                load_vec<T, 4>(sQ + (16 * ti + r) * SK + 16 * w + 4 * c, qv);
+                load_vec<T, 4>(sQ + LK.four(ti, w), qv);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     o[ti][e] *= scale;
                     u += qv[e] * o[ti][e];
                 }
                 u = reduce_over_cgroups(u);
-                if (c == 0) sU[w * C + 16 * ti + r] = u;
+                if (c == 0) sum.u[w][16 * ti + r] = u;
 #pragma unroll
-                for (int ks = 0; ks <= ti / 2; ++ks) o[ti] = mma_d(kc[ks], ld8(sD + 16 * ti * SP + LP.row + 32 * ks), o[ti]);
-                const int64_t t = n * C + 16 * ti + r;
+                for (int ks = 0; ks <= ti / 2; ++ks) o[ti] = mma_d(kc[ks], LP.halves(sD, ti, ks), o[ti]);
                 const float v[4] = {o[ti][0], o[ti][1], o[ti][2], o[ti][3]};
-                if (key_wave && t < a.n.T) put(a.dquery, a.row_parts > 1, part_qk, t, rows_qk, row_qk, v);
-            }
-            // ---- dk ----
-#pragma unroll
-            for (int tj = 0; tj < CT; ++tj) o[tj] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int ks = 0; ks < VK; ++ks) {
-                float s[8];
-                two_tiles(by_key[2 * ks], by_key[2 * ks + 1], s);
-                const Split<T, 3> op(s);
-#pragma unroll
-                for (int tj = 0; tj < CT; ++tj) o[tj] = op.left(lds_two_halves(sV + 16 * tj * SV + LV.row2 + 32 * ks), o[tj]);
-            }
-#pragma unroll
-            for (int tj = 0; tj < CT; ++tj) {
-                const float scale = gate.to_end[16 * tj + r];
-                float kv[4], ww = 0.f;
-                load_vec<T, 4>(sK + (16 * tj + r) * SK + 16 * w + 4 * c, kv);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    o[tj][e] *= scale;
-                    ww += kv[e] * o[tj][e];
-                }
-                ww = reduce_over_cgroups(ww);
-                if (c == 0) sW[w * C + 16 * tj + r] = ww;
-#pragma unroll
-                for (int ks = tj / 2; ks < CS; ++ks) o[tj] = mma_d(qc[ks], lds_columns(sD + 32 * ks * SP + 16 * tj + LP.col, SP), o[tj]);
-                const int64_t t = n * C + 16 * tj + r;
-                const float v[4] = {o[tj][0], o[tj][1], o[tj][2], o[tj][3]};
-                if (key_wave && t < a.n.T) put(a.dkey, a.row_parts > 1, part_qk, t, rows_qk, row_qk, v);
+                if (key_wave && n * C + 16 * ti + r < T_) put(a.dquery, a.row_parts > 1, part_qk, n * C + 16 * ti, rows_qk, row_qk, lane_qk, v);
+                o[ti] = f32x4{0.f, 0.f, 0.f, 0.f};
             }
         }
-        if (w < VT) {
-            D8 oc[CS];
+        if (second) {
+            // ---- dk ----
+            {
+                const TileV LV = tv.here();
 #pragma unroll
-            for (int ks = 0; ks < CS; ++ks) oc[ks] = lds_columns(sO + 32 * ks * SV + 16 * w + LV.col, SV);
+                for (int ks = 0; ks < VK; ++ks) {
+                    float s[8];
+                    two_tiles(state[2 * ks], state[2 * ks + 1], s);
+                    const Split<T, 3> op(s);
+#pragma unroll
+                    for (int tj = 0; tj < CT; tj += 2) {
+                        const D8 x[2] = {LV.halves(sV, tj, ks), LV.halves(sV, tj + 1, ks)};
+                        mma_left(op, x, o + tj);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+            const TileK LK = tk.here();
+            D8 qc[CS];
+#pragma unroll
+            for (int ks = 0; ks < CS; ++ks) qc[ks] = LK.columns(sQ, ks, wk);
+            {
+                const TileP LP = tp.here();
+#pragma unroll
+                for (int tj = 0; tj < CT; ++tj) {
+                    const float scale = gate.to_end[16 * tj + r];
+                    float kv[4], ww = 0.f;
+                    load_vec<T, 4>(sK + LK.four(tj, wk), kv);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        o[tj][e] *= scale;
+                        ww += kv[e] * o[tj][e];
+                    }
+                    ww = reduce_over_cgroups(ww);
+                    if (c == 0) sum.w[wk][16 * tj + r] = ww;
+#pragma unroll
+                    for (int ks = tj / 2; ks < CS; ++ks) o[tj] = mma_d(qc[ks], LP.columns(sD, ks, tj), o[tj]);
+                    const float v[4] = {o[tj][0], o[tj][1], o[tj][2], o[tj][3]};
+                    if (key_wave && n * C + 16 * tj + r < T_) put(a.dkey, a.row_parts > 1, part_qk, n * C + 16 * tj, rows_qk, row_qk, lane_qk, v);
+                }
+            }
+            // ---- dS: dhidden_init and the gates' gradient come from it ----
+            const TileV LV = tv.here();
+#pragma unroll
+            for (int t = 0; t < VT; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) state[t][e] *= whole;
+#pragma unroll
+            for (int ks = 0; ks < CS; ++ks) {
+                float v[8], by[8];
+                unpack8(qc[ks], v);
+                two_tiles(*reinterpret_cast<const f32x4 *>(gate.from_start + 32 * ks + 4 * c),
+                          *reinterpret_cast<const f32x4 *>(gate.from_start + 32 * ks + 16 + 4 * c), by);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] *= by[e];
+                const Split<T, 3> op(v);
+#pragma unroll
+                for (int t = 0; t < VT; t += 2) {
+                    const D8 x[2] = {LV.columns(sO, ks, t), LV.columns(sO, ks, t + 1)};
+                    mma_right(x, op, state + t);
+                    if (t % 4 == 2) __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+        } else if (w < VT) {
             // ---- dv ----
-            f32x4 o[CT];
-#pragma unroll
-            for (int tj = 0; tj < CT; ++tj) o[tj] = f32x4{0.f, 0.f, 0.f, 0.f};
+            const TileV LV = tv.here();
+            const TileK LK = tk.here();
 #pragma unroll
             for (int ks = 0; ks < KK; ++ks) {
-                float s[8];
-                two_tiles(by_value[2 * ks], by_value[2 * ks + 1], s);
-                const Split<T, 1> op(s);
+                const D8 op = LV.columns(sS, ks, w);
 #pragma unroll
-                for (int tj = 0; tj < CT; ++tj) o[tj] = op.left(lds_two_halves(sK + 16 * tj * SK + LK.row2 + 32 * ks), o[tj]);
+                for (int tj = 0; tj < CT; ++tj) o[tj] = mma_d(op, LK.halves(sK, tj, ks), o[tj]);
             }
+            const TileP LP = tp.here();
+            D8 oc[CS];
+#pragma unroll
+            for (int ks = 0; ks < CS; ++ks) oc[ks] = LV.columns(sO, ks, w);
 #pragma unroll
             for (int tj = 0; tj < CT; ++tj) {
                 const float scale = gate.to_end[16 * tj + r];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) o[tj][e] *= scale;
 #pragma unroll
-                for (int ks = tj / 2; ks < CS; ++ks) o[tj] = mma_d(oc[ks], lds_columns(sP + 32 * ks * SP + 16 * tj + LP.col, SP), o[tj]);
-                const int64_t t = n * C + 16 * tj + r;
+                for (int ks = tj / 2; ks < CS; ++ks) o[tj] = mma_d(oc[ks], LP.columns(sP, ks, tj), o[tj]);
                 const float v[4] = {o[tj][0], o[tj][1], o[tj][2], o[tj][3]};
-                if (value_wave && t < a.n.T) put(a.dvalue, a.value_parts > 1, ks0, t, rows_v, row_v, v);
-            }
-            // ---- dS by value columns: two parts, as its only use is as an operand of dv ----
-#pragma unroll
-            for (int t = 0; t < KT; ++t)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) by_value[t][e] *= whole;
-#pragma unroll
-            for (int ks = 0; ks < CS; ++ks) {
-                float v[8];
-                unpack8(oc[ks], v);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] *= gate.from_start[32 * ks + 8 * c + e];
-                const Split<T, 2> op(v);
-#pragma unroll
-                for (int t = 0; t < KT; ++t) by_value[t] = op.right(lds_columns(sQ + 32 * ks * SK + 16 * t + LK.col, SK), by_value[t]);
-            }
-        }
-        if (w < KT) {
-            // ---- dS by key columns: dhidden_init and the gates' gradient come from it ----
-#pragma unroll
-            for (int t = 0; t < VT; ++t)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) by_key[t][e] *= whole;
-#pragma unroll
-            for (int ks = 0; ks < CS; ++ks) {
-                float v[8];
-                unpack8(qc[ks], v);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] *= gate.from_start[32 * ks + 8 * c + e];
-                const Split<T, 3> op(v);
-#pragma unroll
-                for (int t = 0; t < VT; ++t) by_key[t] = op.right(lds_columns(sO + 32 * ks * SV + 16 * t + LV.col, SV), by_key[t]);
+                if (value_wave && n * C + 16 * tj + r < T_) put(a.dvalue, a.value_parts > 1, part_v, n * C + 16 * tj, rows_v, row_v, lane_v, v);
             }
         }
     }
     lds_barrier();
-    if (w == gates_wave) {
-        if (count > 0) gates_gradient(first);
+    if (w == sums_wave) {
+        if (count > 0) gates_gradient(first, sums[(count - 1) & 1]);
         if (a.dgate_sums) {
-            double x = gate_sum;
+            double x = sGate[lane];
 #pragma unroll
             for (int m = 1; m < 64; m *= 2) x += __hiloint2double(__shfl_xor(__double2hiint(x), m, 64), __shfl_xor(__double2loint(x), m, 64));
             if (lane == 0) a.dgate_sums[((blockIdx.y * a.n.H + h) * a.n.B + b) * a.plan.segments + order] = x;
         }
     }
     // rows past the end of a shorter sequence
-    for (int64_t t = max(live, first) * C + tid / 16; t < min(last * C, a.n.T); t += NT / 16) {
+    for (int t = max(live, first) * C + tid / 16; t < min(last * C, T_); t += NT / 16) {
         const float zero[4] = {0.f, 0.f, 0.f, 0.f};
         for (int col = 4 * (tid % 16); col < DKW && dk0 + col < DK; col += 64) {
-            put(a.dquery, a.row_parts > 1, part_qk, t, rows_qk, hk * DK + dk0 + col, zero);
-            put(a.dkey, a.row_parts > 1, part_qk, t, rows_qk, hk * DK + dk0 + col, zero);
+            put(a.dquery, a.row_parts > 1, part_qk, t, rows_qk, (int)(hk * DK) + dk0, col, zero);
+            put(a.dkey, a.row_parts > 1, part_qk, t, rows_qk, (int)(hk * DK) + dk0, col, zero);
         }
         for (int col = 4 * (tid % 16); col < DVW && dv0 + col < DV; col += 64)
-            put(a.dvalue, a.value_parts > 1, ks0, t, rows_v, h * DV + dv0 + col, zero);
-        if (a.dgate && tid % 16 == 0) a.dgate[(((int64_t)blockIdx.y * a.n.B + b) * a.n.T + t) * a.n.H + h] = 0.f;
+            put(a.dvalue, a.value_parts > 1, part_v, t, rows_v, (int)(h * DV) + dv0, col, zero);
+        if (a.dgate && tid % 16 == 0) a.dgate[((blockIdx.y * a.n.B + b) * a.n.T + t) * a.n.H + h] = 0.f;
     }
     if (seg == 0) {
 #pragma unroll
         for (int t = 0; t < VT; ++t)
-            if (key_wave && dv0 + 16 * t < DV) {
-                const float x[4] = {by_key[t][0], by_key[t][1], by_key[t][2], by_key[t][3]};
-                store_hidden<4>(a.dhidden_init, a.hidden_dtype, (bh * DK + dk0 + 16 * w + r) * DV + dv0 + 16 * t + 4 * c, x);
+            if (second && key_wave && dv0 + 16 * t < DV) {
+                const float x[4] = {state[t][0], state[t][1], state[t][2], state[t][3]};
+                store_hidden<4>(a.dhidden_init, a.hidden_dtype, (bh * DK + dk0 + 16 * wk + r) * DV + dv0 + 16 * t + 4 * c, x);
             }
     }
 }
@@ -423,11 +479,12 @@ template <typename T, int DKW, int DVW> int launch_gradient(hipStream_t stream, 
 {
     static LdsGrant grant;
     constexpr int C = DecayChunk<T>::C, CT = C / 16, KT = DKW / 16;
-    constexpr size_t lds = sizeof(T) * (2 * C * lds_stride<T>(DKW) + 2 * C * lds_stride<T>(DVW) + 2 * C * lds_stride<T>(C)) +
-                           sizeof(ChunkGates<C>) + sizeof(float) * (2 * CT * C + 2 * KT * C + KT);
+    constexpr size_t lds = sizeof(T) * (2 * C * LdsTile<T, DKW>::kRow + 2 * C * LdsTile<T, DVW>::kRow + 2 * C * LdsTile<T, C>::kRow +
+                                        DKW * LdsTile<T, DVW>::kRow) +
+                           2 * sizeof(ChunkGates<C>) + sizeof(float) * 2 * (2 * CT * C + 2 * KT * C + 16) + sizeof(double) * 64;
     if (int e = allow_lds(grant, reinterpret_cast<const void *>(decay_gradient_kernel<T, DKW, DVW>), lds)) return e;
     const dim3 grid(a.n.B * a.n.H, ((a.n.DK + DKW - 1) / DKW) * ((a.n.DV + DVW - 1) / DVW), a.plan.segments);
-    decay_gradient_kernel<T, DKW, DVW><<<grid, (DKW > DVW ? DKW : DVW) * 4, lds, stream>>>(a);
+    decay_gradient_kernel<T, DKW, DVW><<<grid, ((DKW > DVW ? DKW : DVW) + DKW) * 4, lds, stream>>>(a);
     return launch_status();
 }
 template <typename T> int dispatch_gradient(hipStream_t stream, const BackwardArgs &a)

@@ -312,6 +312,7 @@ bool rows_on_gpu(const Tensor &t)
     const int64_t piece = 16 / (int64_t)t.element_size();
     for (int64_t i = 0; i + 1 < t.dim(); ++i)
         if (t.size(i) > 1 && t.stride(i) % piece) return false;
+    if (t.size(-3) > 1 && t.stride(-3) >= 1 << 23) return false;
     return t.numel() == 0 || reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
 }
 struct DecayDims {

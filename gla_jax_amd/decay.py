@@ -24,7 +24,8 @@ def _rows(t, dtype):
     as they are (a projection's output cut into its parts stays where it lies)."""
     t = t.to(dtype)
     piece = 16 // t.element_size()
-    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % piece == 0 for s, n in zip(t.stride()[:-1], t.shape) if n > 1):
+    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(
+            s % piece == 0 and s < 1 << 23 or n == 1 for s, n in zip(t.stride()[1:-1], t.shape[1:])) and t.stride(0) % piece == 0:
         return t
     return t.contiguous()
 
