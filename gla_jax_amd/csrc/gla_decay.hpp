@@ -245,48 +245,34 @@ template <typename T, int C, int F, int NT> struct RowsInFlight {
     static constexpr int kPieces = C * F / 8, kPer = (kPieces + NT - 1) / NT, kStep = NT / (F / 8);
     static_assert(NT % (F / 8) == 0, "");
     d8 x[kPer];
-    int st, features;
-    __device__ __forceinline__ RowsInFlight(int64_t stride, int count, T *tile) : st((int)stride), features(count)
-    {
-        const int row = threadIdx.x / (F / 8), col = 8 * (threadIdx.x % (F / 8));
-        if (col >= features) {                   // features past the end stay zeros
-#pragma unroll
-            for (int i = 0; i < kPer; ++i)
-                if (row + i * kStep < C) st8(tile + LdsTile<T, F>::piece(row + i * kStep, col), d8{});
-        }
-    }
-    // the rows of a chunk that `rows` points at, `left` of which exist: zeros behind them
-    __device__ __forceinline__ void load(const T *rows, int left)
+    int st, features, left;
+    __device__ __forceinline__ RowsInFlight(int64_t stride, int count) : st((int)stride), features(count), left(0) {}
+    // The rows of a chunk that `rows` points at, the first of which exists and `there` in all.  No load is under a branch (a thread without
+    // a piece reads one that exists, and `store` puts zeros in its place): with loads that may or may not have been issued the compiler
+    // waits for every access to memory where it needs one of them.
+    __device__ __forceinline__ void load(const T *rows, int there)
     {
         // formed here each time: kept over the loop, a lane's place would take a register, and in 64 bits two
         const unsigned tid = again(threadIdx.x);
         const int row = tid / (F / 8), col = 8 * (tid % (F / 8));
-        const unsigned at = (unsigned)(row * st + col) * (unsigned)sizeof(T);
-        if (left >= C) {
-            if (col < features && (kPieces >= NT || row < C)) {
+        left = there;
 #pragma unroll
-                for (int i = 0; i < kPer; ++i)
-                    if (kPieces % NT == 0 || row + i * kStep < C) x[i] = ld8(at_bytes(rows + (int64_t)(i * kStep) * st, at));
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < kPer; ++i) {
-                x[i] = d8{};
-                if (col < features && row + i * kStep < min(left, C)) x[i] = ld8(at_bytes(rows + (int64_t)(i * kStep) * st, at));
-            }
-        }
+        for (int i = 0; i < kPer; ++i)
+            x[i] = ld8(at_bytes(rows, (unsigned)(min(min(row + i * kStep, C - 1), there - 1) * st + (col < features ? col : 0)) * (unsigned)sizeof(T)));
     }
     __device__ __forceinline__ void store(T *tile) const
     {
         const unsigned tid = again(threadIdx.x);
         const int row = tid / (F / 8), col = 8 * (tid % (F / 8));
-        if (col < features) {
 #pragma unroll
-            for (int i = 0; i < kPer; ++i)
-                if (kPieces % NT == 0 || row + i * kStep < C) st8(tile + LdsTile<T, F>::piece(row + i * kStep, col), x[i]);
-        }
+        for (int i = 0; i < kPer; ++i)
+            if (kPieces % NT == 0 || row + i * kStep < C)
+                st8(tile + LdsTile<T, F>::piece(row + i * kStep, col), row + i * kStep < left && col < features ? x[i] : d8{});
     }
 };
+// Waits for the wave's own accesses to memory, stores among them.  Put before a chunk's stores: the rows on their way have arrived by
+// then, and the next chunk, which needs them, does not wait for the stores.
+__device__ __forceinline__ void wait_for_memory() { __builtin_amdgcn_s_waitcnt(0x0f70); }
 
 // Tile number n of the lower triangle of 16 x 16 tiles, counted by rows.
 __device__ __forceinline__ void triangle(int n, int &ti, int &tj)

@@ -80,16 +80,30 @@ __global__ __launch_bounds__(((DKW > DVW ? DKW : DVW) + DKW) * 4) void decay_gra
     const TileK tk;
     const TileV tv;
     const TileP tp;
-    const int64_t part_qk = (vs0 * group + h % group) * a.n.B * a.n.T, part_v = ks0 * a.n.B * a.n.T;      // in rows
-    const int rows_qk = (int)(a.n.HK * DK), rows_v = (int)(a.n.H * DV);                                   // a token's row
-    const int row_qk = (int)(hk * DK) + dk0 + 16 * wk, row_v = (int)(h * DV) + dv0 + 16 * w;
 
-    // four values of token t + r, the features from `at`: 4c .. 4c+3
-    auto put = [&](void *to, bool parts, int64_t part, int t, int width, int at, unsigned lane_at, const float (&x)[4]) {
-        const int64_t row = b * a.n.T + t;
-        if (parts) store_vec<float, 4>(at_bytes(static_cast<float *>(to) + ((part + row) * width + at), 4 * lane_at), x);
-        else store_vec<T, 4>(at_bytes(static_cast<T *>(to) + (row * width + at), (unsigned)sizeof(T) * lane_at), x);
+    // Results, at the first row of the chunk that is worked on: dq of the first waves or dk of the others, and dv.
+    struct Result {
+        char *p;
+        unsigned row;                            // bytes from one token to the next
+        bool parts;                              // floats, to be summed
+        // four values of row 16t + r, 4c features behind the pointer
+        __device__ __forceinline__ void put(int t, unsigned r, unsigned c, f32x4 v) const
+        {
+            const float x[4] = {v[0], v[1], v[2], v[3]};
+            char *to = p + (size_t)(16 * t * row);
+            if (parts) store_vec<float, 4>(reinterpret_cast<float *>(at_bytes(to, r * row + 16 * c)), x);
+            else store_vec<T, 4>(reinterpret_cast<T *>(at_bytes(to, r * row + 4 * (unsigned)sizeof(T) * c)), x);
+        }
     };
+    auto result = [&](void *array, int parts, int64_t part, int64_t heads_features, int64_t at) {
+        const unsigned size = parts > 1 ? 4 : sizeof(T);
+        const int64_t row = (part * a.n.B + b) * a.n.T + (int64_t)(live - 1) * C;
+        return Result{static_cast<char *>(array) + (row * heads_features + at) * size, (unsigned)heads_features * size, parts > 1};
+    };
+    Result qk = result(second ? a.dkey : a.dquery, a.row_parts, vs0 * group + h % group, a.n.HK * DK, hk * DK + dk0 + 16 * wk);
+    Result dv = result(a.dvalue, a.value_parts, ks0, a.n.H * DV, h * DV + dv0 + 16 * w);
+    const float *kept = a.kept + ((bh * a.plan.chunks + live - 1) * DK + dk0 + (key_wave ? 16 * wk : 0)) * DV + dv0;
+    const int64_t kept_step = (int64_t)DK * DV;
 
     // ---- the cotangent that enters: key feature r of the wave's, value features 16t + 4c .. ----
     f32x4 state[VT];                             // dS, which stays; of the first waves S, a chunk's after the other
@@ -113,8 +127,8 @@ __global__ __launch_bounds__(((DKW > DVW ? DKW : DVW) + DKW) * 4) void decay_gra
                 if (second) state[t][e] = from[((t * tiles + dk0 / 16 + wk) * 64 + (r >> 2) * 16 + 4 * c + e) * 4 + (r & 3)];
     }
 
-    RowsInFlight<T, C, DKW, NT> fk(a.keys.st, DK - dk0, sK), fq(a.queries.st, DK - dk0, sQ);
-    RowsInFlight<T, C, DVW, NT> fv(a.values.st, DV - dv0, sV), fo(a.dout.st, DV - dv0, sO);
+    RowsInFlight<T, C, DKW, NT> fk(a.keys.st, DK - dk0), fq(a.queries.st, DK - dk0);
+    RowsInFlight<T, C, DVW, NT> fv(a.values.st, DV - dv0), fo(a.dout.st, DV - dv0);
     float g = 0.f;
     auto fetch_gates = [&](int n) {              // by the wave that makes the chunk's gates
         g = w == NW - 1 && lane < C && n * C + lane < len ? G[(int64_t)(n * C + lane) * a.gates.st] : 0.f;
@@ -165,6 +179,11 @@ __global__ __launch_bounds__(((DKW > DVW ? DKW : DVW) + DKW) * 4) void decay_gra
     };
 
     for (int i = tid; i < C * TileP::kRow; i += NT) sP[i] = sD[i] = (T)0.f;      // the tiles above the diagonal that products take along
+    // key feature r of the wave's, value features 16 t + 4c .. of the state that `from` points at (or others, where these do not exist)
+    auto state_tile = [&](const float *from, int t) {
+        const unsigned at = (again(r) * DV + 4 * c) * 4;
+        return *reinterpret_cast<const f32x4 *>(at_bytes(from + (16 * t < DV - dv0 ? 16 * t : 0), at));
+    };
     const int sums_wave = NW - 2;
     const int count = max(live - first, 0);
     int n = live - 1;
@@ -175,6 +194,10 @@ __global__ __launch_bounds__(((DKW > DVW ? DKW : DVW) + DKW) * 4) void decay_gra
         O += (int64_t)n * C * a.dout.st;
         fetch_gates(n);
         fetch(n);
+        if (!second) {
+#pragma unroll
+            for (int t = 0; t < VT; ++t) state[t] = state_tile(kept, t);
+        }
         if (w == NW - 1) chunk_gates<C>(gates[0], g);
         if (count > 1) fetch_gates(n - 1);
     }
@@ -195,16 +218,19 @@ __global__ __launch_bounds__(((DKW > DVW ? DKW : DVW) + DKW) * 4) void decay_gra
             }
         }
         lds_barrier();
-        // the state before the chunk: key feature r of the wave's, value features in halves
-        const float *kept = a.kept + ((bh * a.plan.chunks + n) * DK + dk0 + 16 * wk) * DV + dv0;
-        if (!second) {
-            const unsigned at = (again(r) * DV + 4 * c) * 4;
-            const int dv = again_uniform(key_wave ? DV - dv0 : 0);
+        const float whole = gate.whole;
+        if (second) {                             // <S, dS>; the first waves have brought S into the cache
+            float x = 0.f;
+            f32x4 S[VT];
 #pragma unroll
-            for (int t = 0; t < VT; ++t) {
-                state[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-                if (16 * t < dv) state[t] = *reinterpret_cast<const f32x4 *>(at_bytes(kept + 16 * t, at));
-            }
+            for (int t = 0; t < VT; ++t) S[t] = state_tile(kept, t);
+#pragma unroll
+            for (int t = 0; t < VT; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x += key_wave && 16 * t < DV - dv0 ? S[t][e] * state[t][e] : 0.f;
+#pragma unroll
+            for (int m = 1; m < 64; m *= 2) x += shfl_xor_f32(x, m);
+            if (lane == 0) sum.x[wk] = whole * x;
         }
         if (i + 1 < count) fetch(n - 1);
 
@@ -257,25 +283,10 @@ __global__ __launch_bounds__(((DKW > DVW ? DKW : DVW) + DKW) * 4) void decay_gra
             chunk_gates<C>(gates[(i + 1) & 1], g);
             if (i + 2 < count) fetch_gates(n - 2);
         }
-        const float whole = gate.whole;
-        if (second) {
-            float x = 0.f;
-            const unsigned at = (again(r) * DV + 4 * c) * 4;
-            const int dv = again_uniform(key_wave ? DV - dv0 : 0);
-#pragma unroll
-            for (int t = 0; t < VT; ++t)
-                if (16 * t < dv) {
-                    const f32x4 S = *reinterpret_cast<const f32x4 *>(at_bytes(kept + 16 * t, at));
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) x += S[e] * state[t][e];
-                }
-#pragma unroll
-            for (int m = 1; m < 64; m *= 2) x += shfl_xor_f32(x, m);
-            if (lane == 0) sum.x[wk] = whole * x;
-        }
         lds_barrier();
 
-        const unsigned lane_qk = again(r) * rows_qk + 4 * c, lane_v = again(r) * rows_v + 4 * c;
+        const unsigned row = again(r), col = again(c);
+        const int left = T_ - n * C - r;             // rows 16 t that exist
         f32x4 o[CT];
 #pragma unroll
         for (int ti = 0; ti < CT; ++ti) o[ti] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -283,11 +294,17 @@ __global__ __launch_bounds__(((DKW > DVW ? DKW : DVW) + DKW) * 4) void decay_gra
             // ---- dq ----
             {
                 const TileV LV = tv.here();
+                const float *next = i + 1 < count ? kept - kept_step : kept;
 #pragma unroll
                 for (int ks = 0; ks < VK; ++ks) {
                     float s[8];
                     two_tiles(state[2 * ks], state[2 * ks + 1], s);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) s[e] = 32 * ks + 16 * (e / 4) < DV - dv0 ? s[e] : 0.f;
                     const Split<T, 3> op(s);
+                    // the next chunk's, as soon as these are used
+                    state[2 * ks] = state_tile(next, 2 * ks);
+                    state[2 * ks + 1] = state_tile(next, 2 * ks + 1);
 #pragma unroll
                     for (int ti = 0; ti < CT; ti += 2) {
                         const D8 x[2] = {LV.halves(sO, ti, ks), LV.halves(sO, ti + 1, ks)};
@@ -301,6 +318,7 @@ __global__ __launch_bounds__(((DKW > DVW ? DKW : DVW) + DKW) * 4) void decay_gra
             D8 kc[CS];
 #pragma unroll
             for (int ks = 0; ks < CS; ++ks) kc[ks] = LK.columns(sK, ks, w);
+            wait_for_memory();
 #pragma unroll
             for (int ti = 0; ti < CT; ++ti) {
                 const float scale = gate.from_start[16 * ti + r];
@@ -315,8 +333,7 @@ __global__ __launch_bounds__(((DKW > DVW ? DKW : DVW) + DKW) * 4) void decay_gra
                 if (c == 0) sum.u[w][16 * ti + r] = u;
 #pragma unroll
                 for (int ks = 0; ks <= ti / 2; ++ks) o[ti] = mma_d(kc[ks], LP.halves(sD, ti, ks), o[ti]);
-                const float v[4] = {o[ti][0], o[ti][1], o[ti][2], o[ti][3]};
-                if (key_wave && n * C + 16 * ti + r < T_) put(a.dquery, a.row_parts > 1, part_qk, n * C + 16 * ti, rows_qk, row_qk, lane_qk, v);
+                if (key_wave && 16 * ti < left) qk.put(ti, row, col, o[ti]);
                 o[ti] = f32x4{0.f, 0.f, 0.f, 0.f};
             }
         }
@@ -341,6 +358,7 @@ __global__ __launch_bounds__(((DKW > DVW ? DKW : DVW) + DKW) * 4) void decay_gra
             D8 qc[CS];
 #pragma unroll
             for (int ks = 0; ks < CS; ++ks) qc[ks] = LK.columns(sQ, ks, wk);
+            wait_for_memory();
             {
                 const TileP LP = tp.here();
 #pragma unroll
@@ -357,8 +375,7 @@ __global__ __launch_bounds__(((DKW > DVW ? DKW : DVW) + DKW) * 4) void decay_gra
                     if (c == 0) sum.w[wk][16 * tj + r] = ww;
 #pragma unroll
                     for (int ks = tj / 2; ks < CS; ++ks) o[tj] = mma_d(qc[ks], LP.columns(sD, ks, tj), o[tj]);
-                    const float v[4] = {o[tj][0], o[tj][1], o[tj][2], o[tj][3]};
-                    if (key_wave && n * C + 16 * tj + r < T_) put(a.dkey, a.row_parts > 1, part_qk, n * C + 16 * tj, rows_qk, row_qk, lane_qk, v);
+                    if (key_wave && 16 * tj < left) qk.put(tj, row, col, o[tj]);
                 }
             }
             // ---- dS: dhidden_init and the gates' gradient come from it ----
@@ -404,10 +421,12 @@ __global__ __launch_bounds__(((DKW > DVW ? DKW : DVW) + DKW) * 4) void decay_gra
                 for (int e = 0; e < 4; ++e) o[tj][e] *= scale;
 #pragma unroll
                 for (int ks = tj / 2; ks < CS; ++ks) o[tj] = mma_d(oc[ks], LP.columns(sP, ks, tj), o[tj]);
-                const float v[4] = {o[tj][0], o[tj][1], o[tj][2], o[tj][3]};
-                if (value_wave && n * C + 16 * tj + r < T_) put(a.dvalue, a.value_parts > 1, part_v, n * C + 16 * tj, rows_v, row_v, lane_v, v);
+                if (value_wave && 16 * tj < left) dv.put(tj, row, col, o[tj]);
             }
         }
+        qk.p -= (int64_t)C * qk.row;
+        dv.p -= (int64_t)C * dv.row;
+        kept -= kept_step;
     }
     lds_barrier();
     if (w == sums_wave) {
@@ -419,16 +438,24 @@ __global__ __launch_bounds__(((DKW > DVW ? DKW : DVW) + DKW) * 4) void decay_gra
             if (lane == 0) a.dgate_sums[((blockIdx.y * a.n.H + h) * a.n.B + b) * a.plan.segments + order] = x;
         }
     }
-    // rows past the end of a shorter sequence
-    for (int t = max(live, first) * C + tid / 16; t < min(last * C, T_); t += NT / 16) {
-        const float zero[4] = {0.f, 0.f, 0.f, 0.f};
-        for (int col = 4 * (tid % 16); col < DKW && dk0 + col < DK; col += 64) {
-            put(a.dquery, a.row_parts > 1, part_qk, t, rows_qk, (int)(hk * DK) + dk0, col, zero);
-            put(a.dkey, a.row_parts > 1, part_qk, t, rows_qk, (int)(hk * DK) + dk0, col, zero);
+    // rows past the end of a shorter sequence, each wave its features
+    if (live < last) {
+        const int from = max(live, first);
+        qk.p += (int64_t)(from - live + 1 + count) * C * qk.row;
+        dv.p += (int64_t)(from - live + 1 + count) * C * dv.row;
+        for (int m = from; m < last; ++m) {
+            const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int t = 0; t < CT; ++t) {
+                const bool there = m * C + 16 * t + r < T_;
+                if (key_wave && there) qk.put(t, r, c, zero);
+                if (value_wave && there) dv.put(t, r, c, zero);
+            }
+            if (a.dgate && w == 0 && lane < C && m * C + lane < T_)
+                a.dgate[((blockIdx.y * a.n.B + b) * a.n.T + m * C + lane) * a.n.H + h] = 0.f;
+            qk.p += (int64_t)C * qk.row;
+            dv.p += (int64_t)C * dv.row;
         }
-        for (int col = 4 * (tid % 16); col < DVW && dv0 + col < DV; col += 64)
-            put(a.dvalue, a.value_parts > 1, part_v, t, rows_v, (int)(h * DV) + dv0, col, zero);
-        if (a.dgate && tid % 16 == 0) a.dgate[((blockIdx.y * a.n.B + b) * a.n.T + t) * a.n.H + h] = 0.f;
     }
     if (seg == 0) {
 #pragma unroll

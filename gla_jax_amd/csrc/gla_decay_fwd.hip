@@ -72,8 +72,8 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DKP == 
         for (int t = 0; t < TILES; ++t) S[t] = from[t * 64];
     }
 
-    RowsInFlight<T, C, DKP, NT> x(a.keys.st, DK, sX), q(kOut ? a.queries.st : 0, kOut ? DK : DKP, sQ);
-    RowsInFlight<T, C, DVS, NT> y(a.values.st, DV - dv0, sY);
+    RowsInFlight<T, C, DKP, NT> x(a.keys.st, DK), q(kOut ? a.queries.st : 0, DK);
+    RowsInFlight<T, C, DVS, NT> y(a.values.st, DV - dv0);
     float g = 0.f;
     auto fetch_gates = [&](int n) {              // by the wave that makes the chunk's gates
         g = w == NW - 1 && lane < C && n * C + lane < len ? G[(int64_t)(n * C + lane) * a.gates.st] : 0.f;
@@ -112,18 +112,6 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DKP == 
         if constexpr (kOut) q.store(sQ);
         lds_barrier();
         if (i + 1 < count) fetch(n + step);
-
-        if (kOut && a.kept) {
-            // (four bytes a lane, 64 side by side: moving the values between lanes for wider stores costs more than it saves)
-            float *to = a.kept + ((bh * a.plan.chunks + n) * DK * DV + dv0 + 16 * w);
-            const unsigned at = (4 * c * DV + again(r)) * 4;
-            const int dk = again_uniform(mine ? DK : 0);
-#pragma unroll
-            for (int t = 0; t < TILES; ++t)
-                if (16 * t < dk)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) *at_bytes(to + (size_t)((16 * t + e) * DV), at) = S[t][e];
-        }
 
         if constexpr (kOut) {
             // scores, transposed: lane (r, c) has keys 4c .. 4c+3 of tile tj for query r of tile ti
@@ -188,11 +176,27 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DKP == 
             for (int ti = 0; ti < CT; ++ti) {
 #pragma unroll
                 for (int ks = 0; ks <= ti / 2; ++ks) o[ti] = mma_d(yc[ks], tp.halves(sP, ti, ks), o[ti]);
+            }
+            wait_for_memory();
+#pragma unroll
+            for (int ti = 0; ti < CT; ++ti) {
                 if (mine && n * C + 16 * ti + r < T_) {
                     const float v[4] = {o[ti][0], o[ti][1], o[ti][2], o[ti][3]};
                     store_vec<T, 4>(at_bytes(out + (size_t)(16 * ti * row), at), v);
                 }
             }
+        }
+
+        if (kOut && a.kept) {
+            // (four bytes a lane, 64 side by side: moving the values between lanes for wider stores costs more than it saves)
+            float *to = a.kept + ((bh * a.plan.chunks + n) * DK * DV + dv0 + 16 * w);
+            const unsigned at = (4 * c * DV + again(r)) * 4;
+            const int dk = again_uniform(mine ? DK : 0);
+#pragma unroll
+            for (int t = 0; t < TILES; ++t)
+                if (16 * t < dk)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) *at_bytes(to + (size_t)((16 * t + e) * DV), at) = S[t][e];
         }
 
         // ---- the chunk's own contribution ----
