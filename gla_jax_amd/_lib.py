@@ -44,8 +44,8 @@ SIGNATURES = {
     "gla_chunk_fwd_stages": (_int, [_vp, _int] + [_i64] * 6 + [_int, _int] + [_vp] * 9 + [_sz]),
     "gla_chunk_bwd_stages": (_int, [_vp, _int] + [_i64] * 6 + [_int, _int] + [_vp] * 13 + [_sz]),
     "gla_decay_states_bytes": (_sz, [_i64] * 6 + [_int]),
-    "gla_decay_fwd_workspace_bytes": (_sz, [_i64] * 6 + [_int]),
-    "gla_decay_bwd_workspace_bytes": (_sz, [_i64] * 6 + [_int, _int]),
+    "gla_decay_fwd_workspace_bytes": (_sz, [_i64] * 6 + [_int, _int]),
+    "gla_decay_bwd_workspace_bytes": (_sz, [_i64] * 6 + [_int] * 3),
     "gla_decay_fwd": (_int, [_vp] + [_i64] * 6 + [_int, _int] + [_vp] * 11 + [_sz]),
     "gla_decay_bwd": (_int, [_vp] + [_i64] * 6 + [_int] * 3 + [_vp] * 15 + [_sz]),
     "gla_decay_step": (_int, [_vp] + [_i64] * 7 + [_int] * 3 + [_vp] * 9),

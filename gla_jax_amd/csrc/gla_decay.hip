@@ -9,26 +9,42 @@ constexpr int64_t kMostRow = (int64_t)1 << 23;      // elements from one token t
 
 int64_t pad256(int64_t x) { return (x + 255) & ~(int64_t)255; }
 
-// Sequences run as segments side by side where there are fewer workgroups than `wanted`: one workgroup walks a segment's
-// chunks in order, so B1 T32768 H8 D128 as whole sequences would use 8 of 256 compute units.  A segment has two chunks at
-// least: the pass that finds the states entering the segments reads half of the rows again, and hands on a state each.
-DecayPlan plan_segments(const DecaySizes &n, gla_dtype dtype, int64_t workgroups, int64_t wanted)
+// Sequences run as segments side by side where that fills the GPU better: one workgroup walks a segment's chunks in order, so B1
+// T32768 H8 D128 as whole sequences would use 8 of 256 compute units.  `slots` workgroups run at a time; weighed are, in the
+// time of a chunk, the rounds that they take, a workgroup's start, and what segments cost besides: the pass that finds the
+// states entering them (`pass` of the work, on half of the rows) and a state for each to write, scan and read.  A whole number of
+// rounds leaves no compute unit idle, so only the counts that just fill some are looked at; a segment has two chunks at least.  Ragged
+// sequences count as half full: there the longest segment is what the others wait for.
+DecayPlan plan_segments(const DecaySizes &n, gla_dtype dtype, int64_t workgroups, int64_t slots, double pass, bool ragged)
 {
     const int64_t C = dtype == GLA_BF16 ? DecayChunk<__bf16>::C : DecayChunk<float>::C;
-    DecayPlan p;
-    p.chunks = (n.T + C - 1) / C;
-    int64_t most = wanted / workgroups;
-    if (most > p.chunks / 2) most = p.chunks / 2;
-    if (most < 1) most = 1;
-    p.per = (p.chunks + most - 1) / most;
-    if (p.per < 1) p.per = 1;
-    p.segments = p.chunks ? (p.chunks + p.per - 1) / p.per : 1;
-    return p;
+    DecayPlan best{(n.T + C - 1) / C, 1};
+    const double work = (double)workgroups * best.chunks / slots;
+    double least = 0.0;
+    for (int64_t rounds = 0; rounds <= 4; ++rounds) {
+        int64_t segments = rounds ? rounds * slots / workgroups : 1;
+        if (segments > best.chunks / 2) segments = best.chunks / 2;
+        if (rounds && segments < 2) continue;
+        if (segments < 1) segments = 1;
+        const int64_t longest = (best.chunks + segments - 1) / segments, taken = (workgroups * segments + slots - 1) / slots;
+        // a state is written, scanned and read, the rows of a chunk are read: DK / 32 of them move as much
+        const double states = 0.012 * n.DK;
+        double cost = ragged ? 0.5 * work + longest + taken : taken * (longest + 1.0);
+        if (segments > 1) cost += pass * (ragged ? 0.5 * work + longest : work) + taken + states * workgroups * segments / slots + 1.0;
+        if (rounds == 0 || cost < least) {
+            least = cost;
+            best.segments = segments;
+        }
+    }
+    return best;
 }
-DecayPlan forward_plan(const DecaySizes &n, gla_dtype dtype) { return plan_segments(n, dtype, n.B * n.H * decay_slabs(n.DV), 512); }
-DecayPlan backward_plan(const DecaySizes &n, gla_dtype dtype)
+DecayPlan forward_plan(const DecaySizes &n, gla_dtype dtype, bool ragged)
 {
-    return plan_segments(n, dtype, n.B * n.H * decay_slabs(n.DV) * (n.DK > 128 ? 2 : 1), 256);
+    return plan_segments(n, dtype, n.B * n.H * decay_slabs(n.DV), 512, 0.45, ragged);
+}
+DecayPlan backward_plan(const DecaySizes &n, gla_dtype dtype, bool ragged)
+{
+    return plan_segments(n, dtype, n.B * n.H * decay_slabs(n.DV) * (n.DK > 128 ? 2 : 1), 256, 0.2, ragged);
 }
 
 int64_t entering_bytes(const DecaySizes &n, const DecayPlan &p)
@@ -130,19 +146,20 @@ extern "C" size_t gla_decay_states_bytes(int64_t B, int64_t T, int64_t H, int64_
     return (size_t)kept_bytes(n, dtype);
 }
 
-extern "C" size_t gla_decay_fwd_workspace_bytes(int64_t B, int64_t T, int64_t H, int64_t HK, int64_t DK, int64_t DV, gla_dtype dtype)
+extern "C" size_t gla_decay_fwd_workspace_bytes(int64_t B, int64_t T, int64_t H, int64_t HK, int64_t DK, int64_t DV, gla_dtype dtype,
+                                                int ragged)
 {
     const DecaySizes n{B, T, H, HK, DK, DV};
     if (check_sizes(n) || !dtype_ok(dtype)) return 0;
-    return (size_t)entering_bytes(n, forward_plan(n, dtype));
+    return (size_t)entering_bytes(n, forward_plan(n, dtype, ragged != 0));
 }
 
 extern "C" size_t gla_decay_bwd_workspace_bytes(int64_t B, int64_t T, int64_t H, int64_t HK, int64_t DK, int64_t DV, gla_dtype dtype,
-                                                int constant_decay)
+                                                int constant_decay, int ragged)
 {
     const DecaySizes n{B, T, H, HK, DK, DV};
     if (check_sizes(n) || !dtype_ok(dtype)) return 0;
-    const DecayPlan plan = backward_plan(n, dtype);
+    const DecayPlan plan = backward_plan(n, dtype, ragged != 0);
     DecayParts parts = plan_parts(n);
     return (size_t)(entering_bytes(n, plan) + place_parts(n, plan, constant_decay != 0, parts, nullptr));
 }
@@ -162,7 +179,7 @@ extern "C" int gla_decay_fwd(void *stream, int64_t B, int64_t T, int64_t H, int6
         (reinterpret_cast<uintptr_t>(log_decay) & 3) || (reinterpret_cast<uintptr_t>(lengths) & 3))
         return GLA_ERR_ALIGN;
     if (!rows_near(p.values) || !rows_near(p.keys) || !rows_near(p.queries)) return GLA_ERR_SHAPE;
-    const DecayPlan plan = forward_plan(n, dtype);
+    const DecayPlan plan = forward_plan(n, dtype, lengths != nullptr);
     const int64_t need = entering_bytes(n, plan);
     if (need && (!workspace || (int64_t)workspace_bytes < need)) return GLA_ERR_WORKSPACE;
     if (need && !aligned16(workspace)) return GLA_ERR_ALIGN;
@@ -193,7 +210,7 @@ extern "C" int gla_decay_bwd(void *stream, int64_t B, int64_t T, int64_t H, int6
         !aligned16(dlog_decay) || (reinterpret_cast<uintptr_t>(log_decay) & 3) || (reinterpret_cast<uintptr_t>(lengths) & 3))
         return GLA_ERR_ALIGN;
     if (!rows_near(p.values) || !rows_near(p.keys) || !rows_near(p.queries)) return GLA_ERR_SHAPE;
-    const DecayPlan plan = backward_plan(n, dtype);
+    const DecayPlan plan = backward_plan(n, dtype, lengths != nullptr);
     DecayParts parts = plan_parts(n);
     const int64_t first = entering_bytes(n, plan), need = first + place_parts(n, plan, constant_decay != 0, parts, nullptr);
     if (need && (!workspace || (int64_t)workspace_bytes < need)) return GLA_ERR_WORKSPACE;

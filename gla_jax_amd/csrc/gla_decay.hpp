@@ -28,6 +28,25 @@ struct DecayRows {
     int64_t sb, st, sh;
 };
 
+// The same number, formed again from here on: what was derived from it before does not stay in registers.
+__device__ __forceinline__ unsigned again(unsigned x)
+{
+    asm volatile("" : "+v"(x));
+    return x;
+}
+
+__device__ __forceinline__ int again_uniform(int x)
+{
+    asm volatile("" : "+s"(x));
+    return x;
+}
+
+// A pointer that all lanes share and a lane's place behind it in bytes: one register of a lane, where a 64-bit sum takes two.
+template <typename P> __device__ __forceinline__ P *at_bytes(P *base, unsigned bytes)
+{
+    return reinterpret_cast<P *>(reinterpret_cast<std::conditional_t<std::is_const_v<P>, const char, char> *>(base) + bytes);
+}
+
 // A tile of rows in LDS, F features each, and the three ways in which a product takes it as an operand.
 //
 // 16-bit data lie without padding, the 16-byte pieces of a row permuted by the row's number: piece p of row i is at p ^ f(i).  No read has
@@ -41,7 +60,7 @@ struct DecayRows {
 template <typename T, int F> struct LdsTile;
 template <int F> struct LdsTile<__bf16, F> {
     static constexpr int kRow = F;
-    int at_rows, at_halves, at_columns;
+    unsigned at_rows, at_halves, at_columns;     // in bytes: what is left to add is a constant, which the instruction holds
     static __device__ __forceinline__ int permuted(int row)
     {
         const int upper = (row >> 3) & 1;
@@ -50,9 +69,9 @@ template <int F> struct LdsTile<__bf16, F> {
     __device__ __forceinline__ LdsTile()
     {
         const int lane = threadIdx.x & 63, r = lane & 15, c = lane >> 4, row = 4 * c + (r >> 2);
-        at_rows = r * F + ((c ^ permuted(r)) << 3);
-        at_halves = r * F + (((c >> 1) ^ permuted(r)) << 3) + 4 * (c & 1);
-        at_columns = row * F + ((((r & 3) >> 1) ^ permuted(row)) << 3) + 4 * (r & 1);
+        at_rows = 2 * r * F + ((c ^ permuted(r)) << 4);
+        at_halves = 2 * r * F + (((c >> 1) ^ permuted(r)) << 4) + 8 * (c & 1);
+        at_columns = 2 * row * F + ((((r & 3) >> 1) ^ permuted(row)) << 4) + 8 * (r & 1);
     }
     __device__ __forceinline__ LdsTile here() const
     {
@@ -67,20 +86,21 @@ template <int F> struct LdsTile<__bf16, F> {
         return *(const volatile __attribute__((address_space(3))) bf16x4 *)p;
     }
     // rows 16 * t + r as the operand's rows, features 32 * ks .. as the contracted index, in order
-    __device__ __forceinline__ bf16x8 rows(const __bf16 *p, int t, int ks) const { return ld8(p + 16 * t * F + (at_rows ^ (32 * ks))); }
+    __device__ __forceinline__ bf16x8 rows(const __bf16 *p, int t, int ks) const { return ld8(at_bytes(p + 16 * t * F, at_rows ^ (64 * ks))); }
     // the same in two halves
     __device__ __forceinline__ bf16x8 halves(const __bf16 *p, int t, int ks) const
     {
-        return __builtin_shufflevector(half(p + 16 * t * F + (at_halves ^ (32 * ks))), half(p + 16 * t * F + (at_halves ^ (32 * ks + 16))),
-                                       0, 1, 2, 3, 4, 5, 6, 7);
+        p += 16 * t * F;
+        return __builtin_shufflevector(half(at_bytes(p, at_halves ^ (64 * ks))), half(at_bytes(p, at_halves ^ (64 * ks + 32))), 0, 1, 2, 3,
+                                       4, 5, 6, 7);
     }
     // features 16 * t + r as the operand's rows, rows 32 * ks .. as the contracted index, in two halves
     __device__ __forceinline__ bf16x8 columns(const __bf16 *p, int ks, int t) const
     {
-        return lds_tr4x2(p + 32 * ks * F + (at_columns ^ (16 * t)), 16 * F);
+        return lds_tr4x2(at_bytes(p + 32 * ks * F, at_columns ^ (32 * t)), 16 * F);
     }
     // the place of features 16 * u + 4c .. of row 16 * t + r
-    __device__ __forceinline__ int four(int t, int u) const { return 16 * t * F + (at_halves ^ (16 * u)); }
+    template <typename P> __device__ __forceinline__ P *four(P *p, int t, int u) const { return at_bytes(p + 16 * t * F, at_halves ^ (32 * u)); }
 };
 template <int F> struct LdsTile<float, F> {
     static constexpr int kRow = F + 8;
@@ -112,7 +132,7 @@ template <int F> struct LdsTile<float, F> {
         for (int e = 0; e < 8; ++e) r.v[e] = p[((e & 3) + 16 * (e >> 2)) * kRow];
         return r;
     }
-    __device__ __forceinline__ int four(int t, int u) const { return 16 * t * kRow + at_halves + 16 * u; }
+    template <typename P> __device__ __forceinline__ P *four(P *p, int t, int u) const { return p + (16 * t * kRow + at_halves + 16 * u); }
 };
 
 // A float operand as N bf16 ones whose sum it is: 1 rounds it (2^-9 of a value), 2 leaves 2^-17, 3 leaves 2^-25, which is
@@ -172,6 +192,32 @@ __device__ __forceinline__ void two_tiles(f32x4 a, f32x4 b, float (&x)[8])
     for (int e = 0; e < 4; ++e) { x[e] = a[e]; x[4 + e] = b[e]; }
 }
 
+// Four results, rounded, until they are stored.
+template <typename T> struct Packed4;
+template <> struct Packed4<__bf16> { typedef bf16x4 t; };
+template <> struct Packed4<float> { typedef f32x4 t; };
+template <typename T> __device__ __forceinline__ typename Packed4<T>::t pack_results(f32x4 v)
+{
+    return __builtin_convertvector(v, typename Packed4<T>::t);
+}
+
+// The sum over the four lanes that have the same r, and over all lanes, without LDS.
+__device__ __forceinline__ float sum_over_c(float x)
+{
+    auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(a[0]) + __uint_as_float(a[1]);
+}
+__device__ __forceinline__ float sum_over_r(float x)
+{
+    x += dpp_f32<kDppQuadXor1>(x);
+    x += dpp_f32<kDppQuadXor2>(x);
+    x += dpp_f32<kDppRowHalfMirror>(x);
+    x += dpp_f32<kDppRowMirror>(x);
+    return x;
+}
+
 // Sums of a wave's 64-bit numbers up to each lane's, by moves inside rows of 16 lanes and from the rows before.
 template <int CTRL, int ROWS> __device__ __forceinline__ double dpp_f64(double x)
 {
@@ -202,7 +248,7 @@ template <int C> struct ChunkGates {
 };
 template <int C> __device__ __forceinline__ double chunk_gates(ChunkGates<C> &g, float a)
 {
-    const int lane = threadIdx.x & 63;
+    const int lane = again(threadIdx.x) & 63;
     double x = (double)a * 1.4426950408889634074;
     x = x < -1e5 ? -1e5 : x;
     if (lane >= C) x = 0.0;
@@ -219,25 +265,6 @@ template <int C> __device__ __forceinline__ double chunk_gates(ChunkGates<C> &g,
     return all;
 }
 
-// The same number, formed again from here on: what was derived from it before does not stay in registers.
-__device__ __forceinline__ unsigned again(unsigned x)
-{
-    asm volatile("" : "+v"(x));
-    return x;
-}
-
-__device__ __forceinline__ int again_uniform(int x)
-{
-    asm volatile("" : "+s"(x));
-    return x;
-}
-
-// A pointer that all lanes share and a lane's place behind it in bytes: one register of a lane, where a 64-bit sum takes two.
-template <typename P> __device__ __forceinline__ P *at_bytes(P *base, unsigned bytes)
-{
-    return reinterpret_cast<P *>(reinterpret_cast<std::conditional_t<std::is_const_v<P>, const char, char> *>(base) + bytes);
-}
-
 // Rows of a chunk on their way from memory to LDS: `NT` threads hold C x F values in registers.  A thread's pieces lie a fixed number of
 // rows apart; its place in a chunk is one number that stays, and a chunk is a pointer that all share.
 template <typename T, int C, int F, int NT> struct RowsInFlight {
@@ -245,29 +272,32 @@ template <typename T, int C, int F, int NT> struct RowsInFlight {
     static constexpr int kPieces = C * F / 8, kPer = (kPieces + NT - 1) / NT, kStep = NT / (F / 8);
     static_assert(NT % (F / 8) == 0, "");
     d8 x[kPer];
-    int st, features, left;
-    __device__ __forceinline__ RowsInFlight(int64_t stride, int count) : st((int)stride), features(count), left(0) {}
     // The rows of a chunk that `rows` points at, the first of which exists and `there` in all.  No load is under a branch (a thread without
     // a piece reads one that exists, and `store` puts zeros in its place): with loads that may or may not have been issued the compiler
     // waits for every access to memory where it needs one of them.
-    __device__ __forceinline__ void load(const T *rows, int there)
+    __device__ __forceinline__ void load(const T *rows, int st, int there, int features)
     {
         // formed here each time: kept over the loop, a lane's place would take a register, and in 64 bits two
         const unsigned tid = again(threadIdx.x);
         const int row = tid / (F / 8), col = 8 * (tid % (F / 8));
-        left = there;
 #pragma unroll
         for (int i = 0; i < kPer; ++i)
             x[i] = ld8(at_bytes(rows, (unsigned)(min(min(row + i * kStep, C - 1), there - 1) * st + (col < features ? col : 0)) * (unsigned)sizeof(T)));
     }
-    __device__ __forceinline__ void store(T *tile) const
+    __device__ __forceinline__ void store(T *tile, int there, int features) const
     {
         const unsigned tid = again(threadIdx.x);
         const int row = tid / (F / 8), col = 8 * (tid % (F / 8));
+        if (there >= C && features >= F) {
 #pragma unroll
-        for (int i = 0; i < kPer; ++i)
-            if (kPieces % NT == 0 || row + i * kStep < C)
-                st8(tile + LdsTile<T, F>::piece(row + i * kStep, col), row + i * kStep < left && col < features ? x[i] : d8{});
+            for (int i = 0; i < kPer; ++i)
+                if (kPieces % NT == 0 || row + i * kStep < C) st8(tile + LdsTile<T, F>::piece(row + i * kStep, col), x[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kPer; ++i)
+                if (kPieces % NT == 0 || row + i * kStep < C)
+                    st8(tile + LdsTile<T, F>::piece(row + i * kStep, col), row + i * kStep < there && col < features ? x[i] : d8{});
+        }
     }
 };
 // Waits for the wave's own accesses to memory, stores among them.  Put before a chunk's stores: the rows on their way have arrived by
@@ -281,16 +311,33 @@ __device__ __forceinline__ void triangle(int n, int &ti, int &tj)
     tj = n - ti * (ti + 1) / 2;
 }
 
-// The segments that sequences run as, when there are too few pairs to fill the GPU: `chunks` each but the last.
+// The segments that sequences run as, as even as whole chunks make them.
 struct DecayPlan {
-    int64_t chunks;     // chunks of a sequence
-    int64_t per;        // chunks of a segment
+    int64_t chunks;     // of a sequence
     int64_t segments;
+    __host__ __device__ int64_t first(int64_t segment) const { return segment * chunks / segments; }
 };
 
 struct DecaySizes {
     int64_t B, T, H, HK, DK, DV;
 };
+
+// The pair (batch, head), as b * H + h, of workgroup x: heads that share their keys go to the same one of the 8 dies, to which
+// workgroups are dealt in turn, so that its cache reads them once.
+__device__ __forceinline__ int64_t pair_of(unsigned x, const DecaySizes &n)
+{
+    const unsigned group = (unsigned)(n.H / n.HK), units = (unsigned)(n.B * n.HK), even = units / 8 * 8;
+    if (group == 1) return x;
+    unsigned unit, member;
+    if (x < even * group) {
+        unit = 8 * (x / 8 / group) + x % 8;
+        member = x / 8 % group;
+    } else {
+        unit = x / group;
+        member = x % group;
+    }
+    return (int64_t)unit * group + member;
+}
 
 // The states that enter the segments, from what every segment adds: `pass` says which way (see the kernels).  Launches the
 // pass and the scan over the segments; `states` receives [B*H, segments, slabs][a slab in accumulator order] floats.

@@ -32,6 +32,23 @@ struct BackwardArgs {
     int row_parts, value_parts;                  // of dquery and dkey; of dvalue
 };
 
+// Results, at the first row of the chunk that is worked on.
+struct Result {
+    char *p;
+    unsigned row;                                // bytes from one token to the next
+    bool parts;                                  // floats, to be summed
+    // four values of row 16t + r, 4c features behind the pointer
+    template <typename V> __device__ __forceinline__ void put(int t, unsigned r, unsigned c, V v) const
+    {
+        *reinterpret_cast<V *>(at_bytes(p + (size_t)(16 * t * row), r * row + (unsigned)sizeof(V) * c)) = v;
+    }
+    template <typename T> __device__ __forceinline__ void put_as(int t, unsigned r, unsigned c, f32x4 v) const
+    {
+        if (parts) put(t, r, c, v);
+        else put(t, r, c, pack_results<T>(v));
+    }
+};
+
 // One workgroup: a segment of a (batch, head) pair, DKW key and DVW value features.  Its first waves make dq and dv: wave w of key
 // features 16w .. 16w+15, with its columns of S, and of value features 16w .. 16w+15.  The others make dk and carry dS: its columns of
 // key features lie in the accumulators with value features as rows, an operand of dk as they are; dv contracts dS over the other
@@ -63,12 +80,12 @@ __global__ __launch_bounds__(((DKW > DVW ? DKW : DVW) + DKW) * 4) void decay_gra
     double *sGate = reinterpret_cast<double *>(sums + 2);     // the gates' gradients so far, by token of the chunk
 
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, r = lane & 15, c = lane >> 4;
-    const int64_t bh = blockIdx.x, b = bh / a.n.H, h = bh % a.n.H, group = a.n.H / a.n.HK, hk = h / group;
+    const int64_t bh = pair_of(blockIdx.x, a.n), b = bh / a.n.H, h = bh % a.n.H, group = a.n.H / a.n.HK, hk = h / group;
     const int DK = (int)a.n.DK, DV = (int)a.n.DV, vslabs = (DV + DVW - 1) / DVW;
     const int ks0 = blockIdx.y / vslabs, vs0 = blockIdx.y % vslabs, dk0 = ks0 * DKW, dv0 = vs0 * DVW;
     const int64_t order = blockIdx.z, seg = a.plan.segments - 1 - order;
     const int T_ = (int)a.n.T, len = a.lengths ? min(max(a.lengths[b], 0), T_) : T_;
-    const int first = (int)(seg * a.plan.per), last = (int)min(first + a.plan.per, a.plan.chunks), live = min(last, (len + C - 1) / C);
+    const int first = (int)a.plan.first(seg), last = (int)a.plan.first(seg + 1), live = min(last, (len + C - 1) / C);
     const T *K = static_cast<const T *>(a.keys.p) + b * a.keys.sb + hk * a.keys.sh + dk0;
     const T *Q = static_cast<const T *>(a.queries.p) + b * a.queries.sb + hk * a.queries.sh + dk0;
     const T *V = static_cast<const T *>(a.values.p) + b * a.values.sb + h * a.values.sh + dv0;
@@ -81,20 +98,7 @@ __global__ __launch_bounds__(((DKW > DVW ? DKW : DVW) + DKW) * 4) void decay_gra
     const TileV tv;
     const TileP tp;
 
-    // Results, at the first row of the chunk that is worked on: dq of the first waves or dk of the others, and dv.
-    struct Result {
-        char *p;
-        unsigned row;                            // bytes from one token to the next
-        bool parts;                              // floats, to be summed
-        // four values of row 16t + r, 4c features behind the pointer
-        __device__ __forceinline__ void put(int t, unsigned r, unsigned c, f32x4 v) const
-        {
-            const float x[4] = {v[0], v[1], v[2], v[3]};
-            char *to = p + (size_t)(16 * t * row);
-            if (parts) store_vec<float, 4>(reinterpret_cast<float *>(at_bytes(to, r * row + 16 * c)), x);
-            else store_vec<T, 4>(reinterpret_cast<T *>(at_bytes(to, r * row + 4 * (unsigned)sizeof(T) * c)), x);
-        }
-    };
+    // dq of the first waves or dk of the others, and dv
     auto result = [&](void *array, int parts, int64_t part, int64_t heads_features, int64_t at) {
         const unsigned size = parts > 1 ? 4 : sizeof(T);
         const int64_t row = (part * a.n.B + b) * a.n.T + (int64_t)(live - 1) * C;
@@ -127,22 +131,24 @@ __global__ __launch_bounds__(((DKW > DVW ? DKW : DVW) + DKW) * 4) void decay_gra
                 if (second) state[t][e] = from[((t * tiles + dk0 / 16 + wk) * 64 + (r >> 2) * 16 + 4 * c + e) * 4 + (r & 3)];
     }
 
-    RowsInFlight<T, C, DKW, NT> fk(a.keys.st, DK - dk0), fq(a.queries.st, DK - dk0);
-    RowsInFlight<T, C, DVW, NT> fv(a.values.st, DV - dv0), fo(a.dout.st, DV - dv0);
+    RowsInFlight<T, C, DKW, NT> fk, fq;
+    RowsInFlight<T, C, DVW, NT> fv, fo;
+    const int k_st = (int)a.keys.st, q_st = (int)a.queries.st, v_st = (int)a.values.st, o_st = (int)a.dout.st;
     float g = 0.f;
     auto fetch_gates = [&](int n) {              // by the wave that makes the chunk's gates
+        const int lane = again(tid) & 63;
         g = w == NW - 1 && lane < C && n * C + lane < len ? G[(int64_t)(n * C + lane) * a.gates.st] : 0.f;
     };
     auto fetch = [&](int n) {                    // the rows that the pointers have come to
         const int left = len - n * C;
-        fk.load(K, left);
-        fq.load(Q, left);
-        fv.load(V, left);
-        fo.load(O, left);
-        K -= C * a.keys.st;
-        Q -= C * a.queries.st;
-        V -= C * a.values.st;
-        O -= C * a.dout.st;
+        fk.load(K, k_st, left, DK - dk0);
+        fq.load(Q, q_st, left, DK - dk0);
+        fv.load(V, v_st, left, DV - dv0);
+        fo.load(O, o_st, left, DV - dv0);
+        K -= (int64_t)C * k_st;
+        Q -= (int64_t)C * q_st;
+        V -= (int64_t)C * v_st;
+        O -= (int64_t)C * o_st;
     };
 
     if (tid < 64) sGate[tid] = 0.0;
@@ -181,7 +187,7 @@ __global__ __launch_bounds__(((DKW > DVW ? DKW : DVW) + DKW) * 4) void decay_gra
     for (int i = tid; i < C * TileP::kRow; i += NT) sP[i] = sD[i] = (T)0.f;      // the tiles above the diagonal that products take along
     // key feature r of the wave's, value features 16 t + 4c .. of the state that `from` points at (or others, where these do not exist)
     auto state_tile = [&](const float *from, int t) {
-        const unsigned at = (again(r) * DV + 4 * c) * 4;
+        const unsigned lane = again(tid), at = ((lane & 15) * DV + ((lane >> 2) & 12)) * 4;
         return *reinterpret_cast<const f32x4 *>(at_bytes(from + (16 * t < DV - dv0 ? 16 * t : 0), at));
     };
     const int sums_wave = NW - 2;
@@ -205,16 +211,16 @@ __global__ __launch_bounds__(((DKW > DVW ? DKW : DVW) + DKW) * 4) void decay_gra
         const ChunkGates<C> &gate = gates[i & 1];
         Sums &sum = sums[i & 1];
         lds_barrier();                            // the last chunk's tiles are read, its sums written
-        fk.store(sK);
-        fq.store(sQ);
-        fv.store(sV);
-        fo.store(sO);
+        fk.store(sK, len - n * C, DK - dk0);
+        fq.store(sQ, len - n * C, DK - dk0);
+        fv.store(sV, len - n * C, DV - dv0);
+        fo.store(sO, len - n * C, DV - dv0);
         if (second) {                             // dS as the operand of dv
             const TileV LV = tv.here();
 #pragma unroll
             for (int t = 0; t < VT; ++t) {
                 const float x[4] = {state[t][0], state[t][1], state[t][2], state[t][3]};
-                store_vec<T, 4>(sS + LV.four(wk, t), x);
+                store_vec<T, 4>(LV.four(sS, wk, t), x);
             }
         }
         lds_barrier();
@@ -227,9 +233,8 @@ __global__ __launch_bounds__(((DKW > DVW ? DKW : DVW) + DKW) * 4) void decay_gra
 #pragma unroll
             for (int t = 0; t < VT; ++t)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) x += key_wave && 16 * t < DV - dv0 ? S[t][e] * state[t][e] : 0.f;
-#pragma unroll
-            for (int m = 1; m < 64; m *= 2) x += shfl_xor_f32(x, m);
+                for (int e = 0; e < 4; ++e) x += S[t][e] * state[t][e];      // (where S is another's, dS is zero)
+            x = sum_over_c(sum_over_r(x));
             if (lane == 0) sum.x[wk] = whole * x;
         }
         if (i + 1 < count) fetch(n - 1);
@@ -239,6 +244,8 @@ __global__ __launch_bounds__(((DKW > DVW ? DKW : DVW) + DKW) * 4) void decay_gra
             const TileK LK = tk.here();
             const TileV LV = tv.here();
             const TileP LP = tp.here();
+            // (a lane's place formed again in every phase: spilled, it would be read behind the rows that are on their way)
+            const int r = again(tid) & 15, c = (again(tid) >> 4) & 3;
 #pragma unroll 1
             for (int n16 = w; n16 < CT * (CT + 1) / 2; n16 += NW) {
                 int ti, tj;
@@ -254,26 +261,25 @@ __global__ __launch_bounds__(((DKW > DVW ? DKW : DVW) + DKW) * 4) void decay_gra
                 float p[4], dd[4], row = 0.f, col[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const float weight = kj + e <= qi ? ChunkGates<C>::weight(at, at_rest, to[e], to_rest[e]) : 0.f;
-                    p[e] = kj + e <= qi ? s[e] * weight : 0.f;
-                    dd[e] = kj + e <= qi ? d[e] * weight : 0.f;
-                    col[e] = kj + e <= qi ? p[e] * d[e] : 0.f;
-                    row += col[e];
+                    const float weight = ChunkGates<C>::weight(at, at_rest, to[e], to_rest[e]);
+                    p[e] = s[e] * weight;
+                    dd[e] = d[e] * weight;
+                    col[e] = p[e] * d[e];
                 }
-                store_vec<T, 4>(sP + LP.four(ti, tj), p);
-                store_vec<T, 4>(sD + LP.four(ti, tj), dd);
-                row = reduce_over_cgroups(row);
-                if (c == 0) sum.row[tj][16 * ti + again(r)] = row;
+                if (ti == tj)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (!(kj + e <= qi)) p[e] = dd[e] = col[e] = 0.f;
+                row = (col[0] + col[1]) + (col[2] + col[3]);
+                store_vec<T, 4>(LP.four(sP, ti, tj), p);
+                store_vec<T, 4>(LP.four(sD, ti, tj), dd);
+                row = sum_over_c(row);
+                if (c == 0) sum.row[tj][qi] = row;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    float x = col[e];
-                    x += dpp_f32<kDppQuadXor1>(x);
-                    x += dpp_f32<kDppQuadXor2>(x);
-                    x += dpp_f32<kDppRowHalfMirror>(x);
-                    x += dpp_f32<kDppRowMirror>(x);
-                    col[e] = x;
+                    col[e] = sum_over_r(col[e]);
                 }
-                if (r == 0) store_vec<float, 4>(sum.col[ti] + 16 * tj + 4 * again(c), col);
+                if (r == 0) store_vec<float, 4>(sum.col[ti] + kj, col);
             }
         }
         // beside the scores, by waves that have a tile less than the first ones or none: the last chunk's gradient of the gates, and
@@ -285,8 +291,8 @@ __global__ __launch_bounds__(((DKW > DVW ? DKW : DVW) + DKW) * 4) void decay_gra
         }
         lds_barrier();
 
-        const unsigned row = again(r), col = again(c);
-        const int left = T_ - n * C - r;             // rows 16 t that exist
+        const unsigned row = again(tid) & 15, col = (again(tid) >> 4) & 3;
+        const int left = T_ - n * C - (int)row;      // rows 16 t that exist
         f32x4 o[CT];
 #pragma unroll
         for (int ti = 0; ti < CT; ++ti) o[ti] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -299,8 +305,6 @@ __global__ __launch_bounds__(((DKW > DVW ? DKW : DVW) + DKW) * 4) void decay_gra
                 for (int ks = 0; ks < VK; ++ks) {
                     float s[8];
                     two_tiles(state[2 * ks], state[2 * ks + 1], s);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) s[e] = 32 * ks + 16 * (e / 4) < DV - dv0 ? s[e] : 0.f;
                     const Split<T, 3> op(s);
                     // the next chunk's, as soon as these are used
                     state[2 * ks] = state_tile(next, 2 * ks);
@@ -321,19 +325,19 @@ __global__ __launch_bounds__(((DKW > DVW ? DKW : DVW) + DKW) * 4) void decay_gra
             wait_for_memory();
 #pragma unroll
             for (int ti = 0; ti < CT; ++ti) {
-                const float scale = gate.from_start[16 * ti + r];
+                const float scale = gate.from_start[16 * ti + row];
                 float qv[4], u = 0.f;
-                load_vec<T, 4>(sQ + LK.four(ti, w), qv);
+                load_vec<T, 4>(LK.four(sQ, ti, w), qv);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     o[ti][e] *= scale;
                     u += qv[e] * o[ti][e];
                 }
-                u = reduce_over_cgroups(u);
-                if (c == 0) sum.u[w][16 * ti + r] = u;
+                u = sum_over_c(u);
+                if (col == 0) sum.u[w][16 * ti + row] = u;
 #pragma unroll
                 for (int ks = 0; ks <= ti / 2; ++ks) o[ti] = mma_d(kc[ks], LP.halves(sD, ti, ks), o[ti]);
-                if (key_wave && 16 * ti < left) qk.put(ti, row, col, o[ti]);
+                if (key_wave && 16 * ti < left) qk.put_as<T>(ti, row, col, o[ti]);
                 o[ti] = f32x4{0.f, 0.f, 0.f, 0.f};
             }
         }
@@ -363,19 +367,19 @@ __global__ __launch_bounds__(((DKW > DVW ? DKW : DVW) + DKW) * 4) void decay_gra
                 const TileP LP = tp.here();
 #pragma unroll
                 for (int tj = 0; tj < CT; ++tj) {
-                    const float scale = gate.to_end[16 * tj + r];
+                    const float scale = gate.to_end[16 * tj + row];
                     float kv[4], ww = 0.f;
-                    load_vec<T, 4>(sK + LK.four(tj, wk), kv);
+                    load_vec<T, 4>(LK.four(sK, tj, wk), kv);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         o[tj][e] *= scale;
                         ww += kv[e] * o[tj][e];
                     }
-                    ww = reduce_over_cgroups(ww);
-                    if (c == 0) sum.w[wk][16 * tj + r] = ww;
+                    ww = sum_over_c(ww);
+                    if (col == 0) sum.w[wk][16 * tj + row] = ww;
 #pragma unroll
                     for (int ks = tj / 2; ks < CS; ++ks) o[tj] = mma_d(qc[ks], LP.columns(sD, ks, tj), o[tj]);
-                    if (key_wave && 16 * tj < left) qk.put(tj, row, col, o[tj]);
+                    if (key_wave && 16 * tj < left) qk.put_as<T>(tj, row, col, o[tj]);
                 }
             }
             // ---- dS: dhidden_init and the gates' gradient come from it ----
@@ -388,8 +392,8 @@ __global__ __launch_bounds__(((DKW > DVW ? DKW : DVW) + DKW) * 4) void decay_gra
             for (int ks = 0; ks < CS; ++ks) {
                 float v[8], by[8];
                 unpack8(qc[ks], v);
-                two_tiles(*reinterpret_cast<const f32x4 *>(gate.from_start + 32 * ks + 4 * c),
-                          *reinterpret_cast<const f32x4 *>(gate.from_start + 32 * ks + 16 + 4 * c), by);
+                two_tiles(*reinterpret_cast<const f32x4 *>(gate.from_start + 32 * ks + 4 * col),
+                          *reinterpret_cast<const f32x4 *>(gate.from_start + 32 * ks + 16 + 4 * col), by);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) v[e] *= by[e];
                 const Split<T, 3> op(v);
@@ -416,12 +420,12 @@ __global__ __launch_bounds__(((DKW > DVW ? DKW : DVW) + DKW) * 4) void decay_gra
             for (int ks = 0; ks < CS; ++ks) oc[ks] = LV.columns(sO, ks, w);
 #pragma unroll
             for (int tj = 0; tj < CT; ++tj) {
-                const float scale = gate.to_end[16 * tj + r];
+                const float scale = gate.to_end[16 * tj + row];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) o[tj][e] *= scale;
 #pragma unroll
                 for (int ks = tj / 2; ks < CS; ++ks) o[tj] = mma_d(oc[ks], LP.columns(sP, ks, tj), o[tj]);
-                if (value_wave && 16 * tj < left) dv.put(tj, row, col, o[tj]);
+                if (value_wave && 16 * tj < left) dv.put_as<T>(tj, row, col, o[tj]);
             }
         }
         qk.p -= (int64_t)C * qk.row;
@@ -448,8 +452,8 @@ __global__ __launch_bounds__(((DKW > DVW ? DKW : DVW) + DKW) * 4) void decay_gra
 #pragma unroll
             for (int t = 0; t < CT; ++t) {
                 const bool there = m * C + 16 * t + r < T_;
-                if (key_wave && there) qk.put(t, r, c, zero);
-                if (value_wave && there) dv.put(t, r, c, zero);
+                if (key_wave && there) qk.put_as<T>(t, r, c, zero);
+                if (value_wave && there) dv.put_as<T>(t, r, c, zero);
             }
             if (a.dgate && w == 0 && lane < C && m * C + lane < T_)
                 a.dgate[((blockIdx.y * a.n.B + b) * a.n.T + m * C + lane) * a.n.H + h] = 0.f;

@@ -36,11 +36,11 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DKP == 
     ChunkGates<C> *gates = reinterpret_cast<ChunkGates<C> *>(reinterpret_cast<char *>(sP + (kOut ? C * TileP::kRow : 0)));
 
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, r = lane & 15, c = lane >> 4;
-    const int64_t bh = blockIdx.x, b = bh / a.n.H, h = bh % a.n.H, hk = h / (a.n.H / a.n.HK);
+    const int64_t bh = pair_of(blockIdx.x, a.n), b = bh / a.n.H, h = bh % a.n.H, hk = h / (a.n.H / a.n.HK);
     const int dv0 = blockIdx.y * DVS, DK = (int)a.n.DK, DV = (int)a.n.DV;
     const int64_t order = blockIdx.z, seg = kReverse ? a.plan.segments - 1 - order : order;
     const int T_ = (int)a.n.T, len = a.lengths ? min(max(a.lengths[b], 0), T_) : T_;
-    const int first = (int)(seg * a.plan.per), last = (int)min(first + a.plan.per, a.plan.chunks), live = min(last, (len + C - 1) / C);
+    const int first = (int)a.plan.first(seg), last = (int)a.plan.first(seg + 1), live = min(last, (len + C - 1) / C);
     const T *X = static_cast<const T *>(a.keys.p) + b * a.keys.sb + hk * a.keys.sh;
     const T *Y = static_cast<const T *>(a.values.p) + b * a.values.sb + h * a.values.sh + dv0;
     const T *Q = kOut ? static_cast<const T *>(a.queries.p) + b * a.queries.sb + hk * a.queries.sh : nullptr;
@@ -72,21 +72,21 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DKP == 
         for (int t = 0; t < TILES; ++t) S[t] = from[t * 64];
     }
 
-    RowsInFlight<T, C, DKP, NT> x(a.keys.st, DK), q(kOut ? a.queries.st : 0, DK);
-    RowsInFlight<T, C, DVS, NT> y(a.values.st, DV - dv0);
+    RowsInFlight<T, C, DKP, NT> x, q;
+    RowsInFlight<T, C, DVS, NT> y;
+    const int x_st = (int)a.keys.st, y_st = (int)a.values.st, q_st = kOut ? (int)a.queries.st : 0;
     float g = 0.f;
     auto fetch_gates = [&](int n) {              // by the wave that makes the chunk's gates
         g = w == NW - 1 && lane < C && n * C + lane < len ? G[(int64_t)(n * C + lane) * a.gates.st] : 0.f;
     };
-    const int64_t x_step = (kReverse ? -C : C) * a.keys.st, y_step = (kReverse ? -C : C) * a.values.st, q_step = kOut ? C * a.queries.st : 0;
     auto fetch = [&](int n) {                    // the rows that the pointers have come to
         const int left = len - n * C;
-        x.load(X, left);
-        y.load(Y, left);
-        if constexpr (kOut) q.load(Q, left);
-        X += x_step;
-        Y += y_step;
-        Q += q_step;
+        x.load(X, x_st, left, DK);
+        y.load(Y, y_st, left, DV - dv0);
+        if constexpr (kOut) q.load(Q, q_st, left, DK);
+        X += (int64_t)(kReverse ? -C : C) * x_st;
+        Y += (int64_t)(kReverse ? -C : C) * y_st;
+        if constexpr (kOut) Q += (int64_t)C * q_st;
     };
     if constexpr (kOut) {
         // the upper tiles that a step of 32 keys takes along with the diagonal's
@@ -107,9 +107,9 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DKP == 
     for (int i = 0; i < count; ++i, n += step) {
         const ChunkGates<C> &gate = gates[i & 1];
         lds_barrier();                            // the last chunk's tiles are read
-        x.store(sX);
-        y.store(sY);
-        if constexpr (kOut) q.store(sQ);
+        x.store(sX, len - n * C, DK);
+        y.store(sY, len - n * C, DV - dv0);
+        if constexpr (kOut) q.store(sQ, len - n * C, DK);
         lds_barrier();
         if (i + 1 < count) fetch(n + step);
 
@@ -133,7 +133,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DKP == 
                     const float weight = ChunkGates<C>::weight(at, at_rest, to[e], to_rest[e]);
                     p[e] = kj + e <= qi ? s[e] * weight : 0.f;
                 }
-                store_vec<T, 4>(sP + LP.four(ti, tj), p);
+                store_vec<T, 4>(LP.four(sP, ti, tj), p);
             }
         }
         // the next chunk's gates, by a wave that has one score tile less than the first ones
@@ -146,6 +146,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DKP == 
 #pragma unroll
         for (int ks = 0; ks < CS; ++ks) yc[ks] = ty.columns(sY, ks, w);
 
+        typename Packed4<T>::t result[CT];
         if constexpr (kOut) {
             // the state's part, while the other waves finish their scores
             const TileX LX = tx.here();
@@ -157,10 +158,11 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DKP == 
                 float s[8];
                 two_tiles(S[2 * ks], S[2 * ks + 1], s);
                 const Split<T, 1> op(s);
-                D8 x[CT];
 #pragma unroll
-                for (int ti = 0; ti < CT; ++ti) x[ti] = LX.halves(sQ, ti, ks);
-                mma_left(op, x, o);
+                for (int ti = 0; ti < CT; ti += 2) {
+                    const D8 x[2] = {LX.halves(sQ, ti, ks), LX.halves(sQ, ti + 1, ks)};
+                    mma_left(op, x, o + ti);
+                }
                 __builtin_amdgcn_sched_barrier(0);     // a step's operands at a time: all of them at once do not fit the registers
             }
 #pragma unroll
@@ -170,23 +172,13 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DKP == 
                 for (int e = 0; e < 4; ++e) o[ti][e] *= scale;
             }
             lds_barrier();                        // the scores are there
-            T *out = static_cast<T *>(a.out) + ((b * a.n.T + n * C) * a.n.H + h) * DV + dv0 + 16 * w;
-            const unsigned row = (unsigned)a.n.H * DV, at = (again(r) * row + 4 * c) * (unsigned)sizeof(T);
 #pragma unroll
             for (int ti = 0; ti < CT; ++ti) {
 #pragma unroll
                 for (int ks = 0; ks <= ti / 2; ++ks) o[ti] = mma_d(yc[ks], tp.halves(sP, ti, ks), o[ti]);
-            }
-            wait_for_memory();
-#pragma unroll
-            for (int ti = 0; ti < CT; ++ti) {
-                if (mine && n * C + 16 * ti + r < T_) {
-                    const float v[4] = {o[ti][0], o[ti][1], o[ti][2], o[ti][3]};
-                    store_vec<T, 4>(at_bytes(out + (size_t)(16 * ti * row), at), v);
-                }
+                result[ti] = pack_results<T>(o[ti]);
             }
         }
-
         if (kOut && a.kept) {
             // (four bytes a lane, 64 side by side: moving the values between lanes for wider stores costs more than it saves)
             float *to = a.kept + ((bh * a.plan.chunks + n) * DK * DV + dv0 + 16 * w);
@@ -216,13 +208,20 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DKP == 
             for (int e = 0; e < 8; ++e) v[e] *= by[e];
             const Split<T, 3> op(v);
 #pragma unroll
-            for (int t = 0; t < TILES; t += 4) {
-                D8 k[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) k[i] = LX.columns(sX, ks, t + i);
+            for (int t = 0; t < TILES; t += 2) {
+                const D8 k[2] = {LX.columns(sX, ks, t), LX.columns(sX, ks, t + 1)};
                 mma_right(k, op, S + t);
-                __builtin_amdgcn_sched_barrier(0);
+                if (t % 4 == 2) __builtin_amdgcn_sched_barrier(0);
             }
+        }
+        if constexpr (kOut) {
+            wait_for_memory();
+            T *out = static_cast<T *>(a.out) + ((b * a.n.T + n * C) * a.n.H + h) * DV + dv0 + 16 * w;
+            const unsigned row = (unsigned)a.n.H * DV, at = (again(r) * row + 4 * c) * (unsigned)sizeof(T);
+#pragma unroll
+            for (int ti = 0; ti < CT; ++ti)
+                if (mine && n * C + 16 * ti + r < T_)
+                    *reinterpret_cast<typename Packed4<T>::t *>(at_bytes(out + (size_t)(16 * ti * row), at)) = result[ti];
         }
     }
 

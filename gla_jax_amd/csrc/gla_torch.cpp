@@ -371,7 +371,7 @@ ChunkOut decay_forward(const Tensor &h0, const Tensor &a, const Tensor &v, const
     const c10::DeviceGuard guard(v.device());
     const DecayDims n = decay_dims(v, k);
     const gla_dtype dt = code(v);
-    const size_t nws = gla_decay_fwd_workspace_bytes(n.B, n.T, n.H, n.HK, n.DK, n.DV, dt);
+    const size_t nws = gla_decay_fwd_workspace_bytes(n.B, n.T, n.H, n.HK, n.DK, n.DV, dt, (bool)lengths);
     const size_t nst = residual ? gla_decay_states_bytes(n.B, n.T, n.H, n.HK, n.DK, n.DV, dt) : 0;
     ChunkOut r{at::empty_like(h0), dense_like(v), Tensor()};
     if (residual) r.states = at::empty({n.B, (int64_t)nst / n.B}, v.options().dtype(at::kByte));
@@ -392,7 +392,7 @@ variable_list decay_backward(const Tensor &states, const Tensor &a, const Tensor
     const DecayDims n = decay_dims(v, k);
     const gla_dtype dt = code(v);
     const bool constant = a.dim() == 1;
-    const size_t nws = gla_decay_bwd_workspace_bytes(n.B, n.T, n.H, n.HK, n.DK, n.DV, dt, constant);
+    const size_t nws = gla_decay_bwd_workspace_bytes(n.B, n.T, n.H, n.HK, n.DK, n.DV, dt, constant, (bool)lengths);
     Tensor ws;
     if (nws) ws = bytes_like(nws, v);
     Tensor dh0 = at::empty_like(dhT), da = dense_like(a), dv = dense_like(v), dk = dense_like(k), dq = dense_like(q);

@@ -44,7 +44,7 @@ def _decay_forward(h0, a, v, k, q, lengths, residual):
     at = a.expand(B, T, H)
     with torch.cuda.device(v.device):
         hT, out = torch.empty_like(h0), torch.empty(v.shape, dtype=v.dtype, device=v.device)
-        n = lib.gla_decay_fwd_workspace_bytes(B, T, H, HK, DK, DV, dt)
+        n = lib.gla_decay_fwd_workspace_bytes(B, T, H, HK, DK, DV, dt, int(lengths is not None))
         ws = torch.empty(n, dtype=torch.uint8, device=v.device) if n else None
         # cut into B rows of bytes it maps over the batch axis as arrays do
         kept = lib.gla_decay_states_bytes(B, T, H, HK, DK, DV, dt) if residual else 0
@@ -105,7 +105,7 @@ class _ChunkDecayBwd(torch.autograd.Function):
         with torch.cuda.device(v.device):
             new = lambda t: torch.empty(t.shape, dtype=t.dtype, device=t.device)  # noqa: E731
             dh0, da, dv, dk, dq = new(dhT), new(a), new(v), new(k), new(q)
-            n = lib.gla_decay_bwd_workspace_bytes(B, T, H, HK, DK, DV, dt, int(constant))
+            n = lib.gla_decay_bwd_workspace_bytes(B, T, H, HK, DK, DV, dt, int(constant), int(lengths is not None))
             ws = torch.empty(n, dtype=torch.uint8, device=v.device) if n else None
             rc = lib.gla_decay_bwd(_stream(), B, T, H, HK, DK, DV, dt, _DT[dhT.dtype], int(constant),
                                    _strides((at, 3), (v, 3), (k, 3), (q, 3)), _ptr(at), _ptr(v), _ptr(k), _ptr(q), _ptr(lengths),

@@ -263,10 +263,11 @@ int gla_chunk_bwd_stages(void *stream, int stages, int64_t B, int64_t T, int64_t
 /* Bytes of the `states` that gla_decay_fwd leaves for gla_decay_bwd: the state before every chunk (of 64 tokens, float32 data:
  * 32) in float32. */
 size_t gla_decay_states_bytes(int64_t B, int64_t T, int64_t H, int64_t HK, int64_t DK, int64_t DV, gla_dtype dtype);
-/* Bytes of scratch (0: none is needed and it may be NULL). */
-size_t gla_decay_fwd_workspace_bytes(int64_t B, int64_t T, int64_t H, int64_t HK, int64_t DK, int64_t DV, gla_dtype dtype);
+/* Bytes of scratch (0: none is needed and it may be NULL); `ragged` != 0: lengths will be given. */
+size_t gla_decay_fwd_workspace_bytes(int64_t B, int64_t T, int64_t H, int64_t HK, int64_t DK, int64_t DV, gla_dtype dtype,
+                                     int ragged);
 size_t gla_decay_bwd_workspace_bytes(int64_t B, int64_t T, int64_t H, int64_t HK, int64_t DK, int64_t DV, gla_dtype dtype,
-                                     int constant_decay);
+                                     int constant_decay, int ragged);
 /* `states` may be NULL when no gradient will be taken. */
 int gla_decay_fwd(void *stream, int64_t B, int64_t T, int64_t H, int64_t HK, int64_t DK, int64_t DV, gla_dtype dtype,
                   gla_dtype hidden_dtype, const int64_t *strides, const void *hidden_init, const float *log_decay,
