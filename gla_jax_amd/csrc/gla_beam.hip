@@ -26,21 +26,7 @@ __device__ __forceinline__ u64 key_of(float x, uint32_t place)
 {
     return ((u64)ordered(x + 0.f) << 32) | (uint32_t)~place;      // (-0 + 0 is 0: the two are equal)
 }
-__device__ __forceinline__ u64 shfl_xor_u64(u64 x, int m)
-{
-    return ((u64)(uint32_t)__shfl_xor((int)(x >> 32), m, 64) << 32) | (uint32_t)__shfl_xor((int)x, m, 64);
-}
-__device__ __forceinline__ u64 wave_max(u64 x)
-{
-#pragma unroll
-    for (int m = 1; m < 64; m *= 2) {
-        const u64 y = shfl_xor_u64(x, m);
-        x = x > y ? x : y;
-    }
-    return x;
-}
-
-constexpr int kThreads = 256, kWaves = kThreads / 64;
+constexpr int kThreads = 256, kJoinThreads = 1024;
 
 struct SelectArgs {
     int64_t groups, beams, vocab, row;           // row: elements from a beam's logits to the next one's
@@ -56,70 +42,99 @@ struct SelectArgs {
     int64_t *out_parents, *out_tokens;
 };
 
-// The block's largest key, in every thread; `slots` has kWaves places of LDS.
-__device__ __forceinline__ u64 block_max(u64 x, u64 *slots)
+// The largest `num` of a workgroup's keys, in order, without a round for each.  Every thread names its own largest; in a wave the
+// num-th of 64 such is a bound that num keys reach, and the highest of the waves' bounds still is one.  What reaches it is collected (of
+// N keys a thread at most N * num a wave, keys being unique) and ranked by counting.  Comparing all names costs 64 steps, the collected
+// ones a few more than num; taking the maximum num times took four times as long at num = 8.
+template <int WAVES> struct SelectLds {
+    u64 names[WAVES][64];
+    u64 bound[WAVES];
+    int count;
+};
+// The bound, in every thread; the largest key of all comes back in `top`.  Has the workgroup's threads meet twice.
+template <int WAVES> __device__ __forceinline__ u64 select_bound(SelectLds<WAVES> &l, u64 best, int num, u64 &top)
 {
-    x = wave_max(x);
+    const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    l.names[w][lane] = best;
+    if (threadIdx.x == 0) l.count = 0;
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) slots[threadIdx.x >> 6] = x;
+    int above = 0;
+#pragma unroll 16
+    for (int i = 0; i < 64; ++i) above += l.names[w][i] > best || (l.names[w][i] == best && i < lane);
+    if (above == (num < 64 ? num : 64) - 1) l.bound[w] = best;
+    if (above == 0) l.names[w][0] = best;        // (each wave has read its own names: its lanes are in step)
     __syncthreads();
-    u64 best = slots[0];
+    u64 bound = l.bound[0];
+    top = l.names[0][0];
 #pragma unroll
-    for (int i = 1; i < kWaves; ++i) best = slots[i] > best ? slots[i] : best;
-    return best;
+    for (int i = 1; i < WAVES; ++i) {
+        bound = l.bound[i] > bound ? l.bound[i] : bound;
+        top = l.names[i][0] > top ? l.names[i][0] : top;
+    }
+    return bound;
 }
 
 // EACH values a thread, in pieces of VEC side by side.  VEC = 1 takes rows that do not begin on 16 bytes.
 template <typename T, int EACH, int VEC>
 __global__ __launch_bounds__(kThreads) void beam_stretch_kernel(const SelectArgs a)
 {
-    __shared__ u64 slots[kWaves];
+    constexpr int kWaves = kThreads / 64;
+    __shared__ SelectLds<kWaves> lds;
     __shared__ float parts[kWaves];
+    extern __shared__ u64 collected[];           // EACH * per of each wave
     const int tid = threadIdx.x;
     const int64_t row = blockIdx.y, split = blockIdx.x, first = split * (kThreads * EACH);
     if (a.finished && a.finished[row]) return;   // its one candidate is made later
-    const T *x = static_cast<const T *>(a.logits) + row * a.row;
-    u64 key[EACH];
+    const T *x = static_cast<const T *>(a.logits) + row * a.row + first;
+    const int there = (int)min(a.vocab - first, (int64_t)(kThreads * EACH));
     float v[EACH];
 #pragma unroll
     for (int i = 0; i < EACH; i += VEC) {
-        const int64_t at = first + (int64_t)(i / VEC) * (kThreads * VEC) + tid * VEC;
+        const int at = (i / VEC) * (kThreads * VEC) + tid * VEC;      // VEC divides what is there where it is more than 1
         float t[VEC];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) t[e] = 0.f;
-        if (VEC > 1 ? at < a.vocab : at < a.vocab) load_vec<T, VEC>(x + at, t);
+        for (int e = 0; e < VEC; ++e) t[e] = -INFINITY;
+        if (at < there) load_vec<T, VEC>(x + at, t);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            v[i + e] = t[e] != t[e] ? -INFINITY : t[e];
-            key[i + e] = at < a.vocab ? key_of(v[i + e], (uint32_t)(at + e)) : 0;
-            if (at >= a.vocab) v[i + e] = -INFINITY;
-        }
+        for (int e = 0; e < VEC; ++e) v[i + e] = t[e] != t[e] ? -INFINITY : t[e] + 0.f;
     }
-    u64 best = 0;
+    auto place = [&](int i) { return (i / VEC) * (kThreads * VEC) + tid * VEC + i % VEC; };
+    // of equal values the first: a thread's places ascend
+    float most = v[0];
+    int which = place(0);
 #pragma unroll
-    for (int i = 0; i < EACH; ++i) best = key[i] > best ? key[i] : best;
-    u64 top = block_max(best, slots);
-    const float most = value_of((uint32_t)(top >> 32));
+    for (int i = 1; i < EACH; ++i)
+        if (v[i] > most) {
+            most = v[i];
+            which = place(i);
+        }
+    u64 top;
+    const u64 bound = select_bound<kWaves>(lds, tid * VEC < there ? key_of(most, (uint32_t)(first + which)) : 0, a.per, top);
+    const float least = value_of((uint32_t)(bound >> 32));
+    most = value_of((uint32_t)(top >> 32));
     // the sum in two levels: a thread's, then the threads' in a fixed order
     float sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < EACH; ++i) sum += most == -INFINITY ? 0.f : fast_exp2((v[i] - most) * kLog2e);
+    for (int i = 0; i < EACH; ++i) {
+        sum += most == -INFINITY ? 0.f : fast_exp2((v[i] - most) * kLog2e);
+        if (bound == 0 || v[i] >= least) {       // (few are, but where the stretch has fewer than `per`)
+            const u64 key = place(i) < there ? key_of(v[i], (uint32_t)(first + place(i))) : 0;
+            if (key && key >= bound) collected[atomicAdd(&lds.count, 1)] = key;
+        }
+    }
 #pragma unroll
     for (int m = 1; m < 64; m *= 2) sum += shfl_xor_f32(sum, m);
     if ((tid & 63) == 0) parts[tid >> 6] = sum;
-    u64 *kept = a.kept + (row * a.splits + split) * a.per;
-    for (int n = 0; n < a.per; ++n) {
-        if (tid == 0) kept[n] = top;
-        if (n + 1 == a.per) break;
-        if (best == top && top) {
-            u64 next = 0;
-#pragma unroll
-            for (int i = 0; i < EACH; ++i) next = key[i] < top && key[i] > next ? key[i] : next;
-            best = next;
-        }
-        top = block_max(best, slots);
-    }
     __syncthreads();
+    const int count = lds.count;
+    u64 *kept = a.kept + (row * a.splits + split) * a.per;
+    for (int i = tid; i < count; i += kThreads) {
+        const u64 key = collected[i];
+        int above = 0;
+        for (int j = 0; j < count; ++j) above += collected[j] > key;
+        if (above < a.per) kept[above] = key;
+    }
+    for (int i = count + tid; i < a.per; i += kThreads) kept[i] = 0;
     if (tid == 0) {
         float s = parts[0];
 #pragma unroll
@@ -130,21 +145,23 @@ __global__ __launch_bounds__(kThreads) void beam_stretch_kernel(const SelectArgs
 }
 
 // One workgroup a search.
-__global__ __launch_bounds__(kThreads) void beam_join_kernel(const SelectArgs a)
+__global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(const SelectArgs a)
 {
-    __shared__ u64 slots[kWaves];
+    constexpr int kWaves = kJoinThreads / 64, kRoom = 2048, kHeld = 4;
+    __shared__ SelectLds<kWaves> lds;
+    __shared__ u64 collected[kRoom];
     __shared__ float lse[GLA_MOST_BEAMS];
     const int tid = threadIdx.x, lane = tid & 63;
     const int64_t group = blockIdx.x;
-    for (int64_t w = tid >> 6; w < a.beams; w += kWaves) {
+    for (int w = tid >> 6; w < a.beams; w += kWaves) {
         const int64_t row = group * a.beams + w;
         if (a.finished && a.finished[row]) continue;
         float most = -INFINITY;
-        for (int64_t i = lane; i < a.splits; i += 64) most = fmaxf(most, a.most[row * a.splits + i]);
+        for (int i = lane; i < a.splits; i += 64) most = fmaxf(most, a.most[row * a.splits + i]);
 #pragma unroll
         for (int m = 1; m < 64; m *= 2) most = fmaxf(most, shfl_xor_f32(most, m));
         float sum = 0.f;
-        for (int64_t i = lane; i < a.splits; i += 64) {
+        for (int i = lane; i < a.splits; i += 64) {
             const float m = a.most[row * a.splits + i];
             if (m != -INFINITY) sum += a.sums[row * a.splits + i] * expf(m - most);
         }
@@ -153,15 +170,16 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(const SelectArgs a)
         if (lane == 0) lse[w] = most + logf(sum);
     }
     __syncthreads();
-    const int64_t of_beam = a.splits * a.per, total = a.beams * of_beam;
+    const unsigned of_beam = (unsigned)(a.splits * a.per), total = (unsigned)a.beams * of_beam;
     // candidate i as a key: its score above, its place among beams x vocabulary below
-    auto candidate = [&](int64_t i) -> u64 {
-        const int64_t w = i / of_beam, n = i % of_beam, row = group * a.beams + w;
+    auto candidate = [&](unsigned i) -> u64 {
+        const unsigned w = i / of_beam, n = i % of_beam;
+        const int64_t row = group * a.beams + w;
         float score;
         uint32_t token;
         if (a.finished && a.finished[row]) {
             // the end again at the score that it has, and the others without a chance, in order
-            if (n >= a.per) return 0;
+            if (n >= (unsigned)a.per) return 0;
             token = (uint32_t)(n == 0 ? a.eos : n <= a.eos ? n - 1 : n);
             score = n == 0 ? a.scores[row] : -INFINITY;
         } else {
@@ -173,27 +191,54 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(const SelectArgs a)
         if (score != score) score = -INFINITY;
         return key_of(score, (uint32_t)(w * a.vocab) + token);
     };
-    u64 best = 0;
-    for (int64_t i = tid; i < total; i += kThreads) {
+    auto put = [&](int n, u64 key) {
+        const uint32_t place = ~(uint32_t)key;
+        a.out_scores[group * a.num + n] = value_of((uint32_t)(key >> 32));
+        a.out_parents[group * a.num + n] = place / (uint32_t)a.vocab;
+        a.out_tokens[group * a.num + n] = place % (uint32_t)a.vocab;
+    };
+    u64 held[kHeld], best = 0;
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j) {
+        held[j] = tid + j * kJoinThreads < total ? candidate(tid + j * kJoinThreads) : 0;
+        best = held[j] > best ? held[j] : best;
+    }
+    for (unsigned i = tid + kHeld * kJoinThreads; i < total; i += kJoinThreads) {
         const u64 k = candidate(i);
         best = k > best ? k : best;
     }
+    u64 top;
+    u64 bound = select_bound<kWaves>(lds, best, a.num, top);
+    if (bound == 0) bound = 1;                   // fewer threads with candidates than are wanted: all of them
+    auto collect = [&](u64 k) {
+        if (k < bound) return;
+        const int at = atomicAdd(&lds.count, 1);
+        if (at < kRoom) collected[at] = k;
+    };
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j) collect(held[j]);
+    for (unsigned i = tid + kHeld * kJoinThreads; i < total; i += kJoinThreads) collect(candidate(i));
+    __syncthreads();
+    const int count = lds.count;
+    if (count <= kRoom) {
+        for (int i = tid; i < count; i += kJoinThreads) {
+            const u64 key = collected[i];
+            int above = 0;
+            for (int j = 0; j < count; ++j) above += collected[j] > key;
+            if (above < a.num) put(above, key);
+        }
+        return;
+    }
+    // more than there is room for (many candidates of few threads): one after the other
     for (int n = 0; n < a.num; ++n) {
-        const u64 top = block_max(best, slots);
-        if (tid == 0) {
-            const uint32_t place = ~(uint32_t)top;
-            a.out_scores[group * a.num + n] = value_of((uint32_t)(top >> 32));
-            a.out_parents[group * a.num + n] = place / a.vocab;
-            a.out_tokens[group * a.num + n] = place % a.vocab;
+        u64 next = 0;
+        for (unsigned i = tid; i < total; i += kJoinThreads) {
+            const u64 k = candidate(i);
+            next = (n == 0 || k < top) && k > next ? k : next;
         }
-        if (best == top) {
-            u64 next = 0;
-            for (int64_t i = tid; i < total; i += kThreads) {
-                const u64 k = candidate(i);
-                next = k < top && k > next ? k : next;
-            }
-            best = next;
-        }
+        __syncthreads();
+        select_bound<kWaves>(lds, next, 1, top);
+        if (tid == 0) put(n, top);
     }
 }
 
@@ -254,15 +299,16 @@ extern "C" int gla_beam_select(void *stream, int64_t groups, int64_t beams, int6
     a.out_tokens = out_tokens;
     const hipStream_t s = static_cast<hipStream_t>(stream);
     const dim3 grid(a.splits, groups * beams);
+    const size_t room = (size_t)kThreads / 64 * kEach * a.per * sizeof(u64);
     const bool pieces = aligned16(logits) && row * size % 16 == 0 && vocab * size % 16 == 0;
     if (dtype == GLA_BF16) {
-        if (pieces) beam_stretch_kernel<__bf16, kEach, 8><<<grid, kThreads, 0, s>>>(a);
-        else beam_stretch_kernel<__bf16, kEach, 1><<<grid, kThreads, 0, s>>>(a);
+        if (pieces) beam_stretch_kernel<__bf16, kEach, 8><<<grid, kThreads, room, s>>>(a);
+        else beam_stretch_kernel<__bf16, kEach, 1><<<grid, kThreads, room, s>>>(a);
     } else {
-        if (pieces) beam_stretch_kernel<float, kEach, 4><<<grid, kThreads, 0, s>>>(a);
-        else beam_stretch_kernel<float, kEach, 1><<<grid, kThreads, 0, s>>>(a);
+        if (pieces) beam_stretch_kernel<float, kEach, 4><<<grid, kThreads, room, s>>>(a);
+        else beam_stretch_kernel<float, kEach, 1><<<grid, kThreads, room, s>>>(a);
     }
     if (int e = launch_status()) return e;
-    beam_join_kernel<<<groups, kThreads, 0, s>>>(a);
+    beam_join_kernel<<<groups, kJoinThreads, 0, s>>>(a);
     return launch_status();
 }
