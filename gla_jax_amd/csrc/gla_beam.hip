@@ -51,17 +51,19 @@ template <int WAVES> struct SelectLds {
     u64 bound[WAVES];
     int count;
 };
-// The bound, in every thread; the largest key of all comes back in `top`.  Has the workgroup's threads meet twice.
+// The bound, in every thread (below 64: num keys are not there), and the largest key of all in `top`; num is at most 64.  Has the
+// workgroup's threads meet twice.
 template <int WAVES> __device__ __forceinline__ u64 select_bound(SelectLds<WAVES> &l, u64 best, int num, u64 &top)
 {
     const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    if (best == 0) best = 63 - lane;             // a thread without a key: a name below all keys, and no other thread's
     l.names[w][lane] = best;
     if (threadIdx.x == 0) l.count = 0;
     __syncthreads();
     int above = 0;
 #pragma unroll 16
-    for (int i = 0; i < 64; ++i) above += l.names[w][i] > best || (l.names[w][i] == best && i < lane);
-    if (above == (num < 64 ? num : 64) - 1) l.bound[w] = best;
+    for (int i = 0; i < 64; ++i) above += l.names[w][i] > best;
+    if (above == num - 1) l.bound[w] = best;
     if (above == 0) l.names[w][0] = best;        // (each wave has read its own names: its lanes are in step)
     __syncthreads();
     u64 bound = l.bound[0];
@@ -74,11 +76,11 @@ template <int WAVES> __device__ __forceinline__ u64 select_bound(SelectLds<WAVES
     return bound;
 }
 
-// EACH values a thread, in pieces of VEC side by side.  VEC = 1 takes rows that do not begin on 16 bytes.
-template <typename T, int EACH, int VEC>
+// EACH values a thread, in pieces of 16 bytes, which rows that do not begin on 16 bytes read one by one: the sums come out the same.
+template <typename T, int EACH, bool PIECES>
 __global__ __launch_bounds__(kThreads) void beam_stretch_kernel(const SelectArgs a)
 {
-    constexpr int kWaves = kThreads / 64;
+    constexpr int kWaves = kThreads / 64, VEC = 16 / sizeof(T);
     __shared__ SelectLds<kWaves> lds;
     __shared__ float parts[kWaves];
     extern __shared__ u64 collected[];           // EACH * per of each wave
@@ -90,13 +92,19 @@ __global__ __launch_bounds__(kThreads) void beam_stretch_kernel(const SelectArgs
     float v[EACH];
 #pragma unroll
     for (int i = 0; i < EACH; i += VEC) {
-        const int at = (i / VEC) * (kThreads * VEC) + tid * VEC;      // VEC divides what is there where it is more than 1
+        const int at = (i / VEC) * (kThreads * VEC) + tid * VEC;
         float t[VEC];
 #pragma unroll
         for (int e = 0; e < VEC; ++e) t[e] = -INFINITY;
-        if (at < there) load_vec<T, VEC>(x + at, t);
+        if constexpr (PIECES) {
+            if (at < there) load_vec<T, VEC>(x + at, t);              // VEC divides what is there
+        } else {
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) v[i + e] = t[e] != t[e] ? -INFINITY : t[e] + 0.f;
+            for (int e = 0; e < VEC; ++e)
+                if (at + e < there) t[e] = (float)x[at + e];
+        }
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) v[i + e] = t[e] != t[e] ? -INFINITY : t[e];
     }
     auto place = [&](int i) { return (i / VEC) * (kThreads * VEC) + tid * VEC + i % VEC; };
     // of equal values the first: a thread's places ascend
@@ -117,7 +125,7 @@ __global__ __launch_bounds__(kThreads) void beam_stretch_kernel(const SelectArgs
 #pragma unroll
     for (int i = 0; i < EACH; ++i) {
         sum += most == -INFINITY ? 0.f : fast_exp2((v[i] - most) * kLog2e);
-        if (bound == 0 || v[i] >= least) {       // (few are, but where the stretch has fewer than `per`)
+        if (bound < 64 || v[i] >= least) {       // (few are, but where the stretch has fewer than `per`)
             const u64 key = place(i) < there ? key_of(v[i], (uint32_t)(first + place(i))) : 0;
             if (key && key >= bound) collected[atomicAdd(&lds.count, 1)] = key;
         }
@@ -150,43 +158,54 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(const SelectArg
     constexpr int kWaves = kJoinThreads / 64, kRoom = 2048, kHeld = 4;
     __shared__ SelectLds<kWaves> lds;
     __shared__ u64 collected[kRoom];
-    __shared__ float lse[GLA_MOST_BEAMS];
+    __shared__ float lse[GLA_MOST_BEAMS], beam_score[GLA_MOST_BEAMS];
+    __shared__ int ended[GLA_MOST_BEAMS];
     const int tid = threadIdx.x, lane = tid & 63;
     const int64_t group = blockIdx.x;
-    for (int w = tid >> 6; w < a.beams; w += kWaves) {
-        const int64_t row = group * a.beams + w;
-        if (a.finished && a.finished[row]) continue;
-        float most = -INFINITY;
-        for (int i = lane; i < a.splits; i += 64) most = fmaxf(most, a.most[row * a.splits + i]);
+    // What is read does not wait for what was read: the first candidates, the beams and the stretches' sums are all on their way at once.
+    const unsigned of_beam = (unsigned)(a.splits * a.per), total = (unsigned)a.beams * of_beam;
+    const u64 *kept = a.kept + group * total;
+    u64 held[kHeld];
 #pragma unroll
-        for (int m = 1; m < 64; m *= 2) most = fmaxf(most, shfl_xor_f32(most, m));
-        float sum = 0.f;
+    for (int j = 0; j < kHeld; ++j) held[j] = tid + j * kJoinThreads < total ? kept[tid + j * kJoinThreads] : 0;
+    if (tid < a.beams) {
+        beam_score[tid] = a.scores[group * a.beams + tid];
+        ended[tid] = a.finished && a.finished[group * a.beams + tid];
+    }
+    for (int w = tid >> 6; w < a.beams; w += kWaves) {
+        const int64_t row = (group * a.beams + w) * a.splits;
+        float most = -INFINITY, sum = 0.f;       // (of a beam that has ended, whatever lies there: not used)
         for (int i = lane; i < a.splits; i += 64) {
-            const float m = a.most[row * a.splits + i];
-            if (m != -INFINITY) sum += a.sums[row * a.splits + i] * expf(m - most);
+            const float m = a.most[row + i], s = a.sums[row + i], higher = fmaxf(most, m);
+            if (higher != -INFINITY) {
+                sum = sum * expf(most - higher) + s * expf(m - higher);
+                most = higher;
+            }
+            if (m != m || s != s) sum = NAN;
         }
+        float all = most;
+#pragma unroll
+        for (int m = 1; m < 64; m *= 2) all = fmaxf(all, shfl_xor_f32(all, m));
+        sum = most == -INFINITY && sum == 0.f ? 0.f : sum * expf(most - all);
 #pragma unroll
         for (int m = 1; m < 64; m *= 2) sum += shfl_xor_f32(sum, m);
-        if (lane == 0) lse[w] = most + logf(sum);
+        if (lane == 0) lse[w] = all + logf(sum);
     }
     __syncthreads();
-    const unsigned of_beam = (unsigned)(a.splits * a.per), total = (unsigned)a.beams * of_beam;
     // candidate i as a key: its score above, its place among beams x vocabulary below
-    auto candidate = [&](unsigned i) -> u64 {
+    auto candidate = [&](unsigned i, u64 k) -> u64 {
         const unsigned w = i / of_beam, n = i % of_beam;
-        const int64_t row = group * a.beams + w;
         float score;
         uint32_t token;
-        if (a.finished && a.finished[row]) {
+        if (ended[w]) {
             // the end again at the score that it has, and the others without a chance, in order
             if (n >= (unsigned)a.per) return 0;
             token = (uint32_t)(n == 0 ? a.eos : n <= a.eos ? n - 1 : n);
-            score = n == 0 ? a.scores[row] : -INFINITY;
+            score = n == 0 ? beam_score[w] : -INFINITY;
         } else {
-            const u64 k = a.kept[row * of_beam + n];
             if (!k) return 0;
             token = ~(uint32_t)k;
-            score = a.scores[row] + (value_of((uint32_t)(k >> 32)) - lse[w]);
+            score = beam_score[w] + (value_of((uint32_t)(k >> 32)) - lse[w]);
         }
         if (score != score) score = -INFINITY;
         return key_of(score, (uint32_t)(w * a.vocab) + token);
@@ -197,27 +216,26 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(const SelectArg
         a.out_parents[group * a.num + n] = place / (uint32_t)a.vocab;
         a.out_tokens[group * a.num + n] = place % (uint32_t)a.vocab;
     };
-    u64 held[kHeld], best = 0;
+    u64 best = 0;
 #pragma unroll
     for (int j = 0; j < kHeld; ++j) {
-        held[j] = tid + j * kJoinThreads < total ? candidate(tid + j * kJoinThreads) : 0;
+        held[j] = tid + j * kJoinThreads < total ? candidate(tid + j * kJoinThreads, held[j]) : 0;
         best = held[j] > best ? held[j] : best;
     }
     for (unsigned i = tid + kHeld * kJoinThreads; i < total; i += kJoinThreads) {
-        const u64 k = candidate(i);
+        const u64 k = candidate(i, kept[i]);
         best = k > best ? k : best;
     }
     u64 top;
-    u64 bound = select_bound<kWaves>(lds, best, a.num, top);
-    if (bound == 0) bound = 1;                   // fewer threads with candidates than are wanted: all of them
+    const u64 bound = select_bound<kWaves>(lds, best, a.num, top);
     auto collect = [&](u64 k) {
-        if (k < bound) return;
+        if (k < bound || k == 0) return;
         const int at = atomicAdd(&lds.count, 1);
         if (at < kRoom) collected[at] = k;
     };
 #pragma unroll
     for (int j = 0; j < kHeld; ++j) collect(held[j]);
-    for (unsigned i = tid + kHeld * kJoinThreads; i < total; i += kJoinThreads) collect(candidate(i));
+    for (unsigned i = tid + kHeld * kJoinThreads; i < total; i += kJoinThreads) collect(candidate(i, kept[i]));
     __syncthreads();
     const int count = lds.count;
     if (count <= kRoom) {
@@ -233,7 +251,7 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(const SelectArg
     for (int n = 0; n < a.num; ++n) {
         u64 next = 0;
         for (unsigned i = tid; i < total; i += kJoinThreads) {
-            const u64 k = candidate(i);
+            const u64 k = candidate(i, kept[i]);
             next = (n == 0 || k < top) && k > next ? k : next;
         }
         __syncthreads();
@@ -242,8 +260,16 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(const SelectArg
     }
 }
 
-constexpr int kEach = 16;
-int64_t splits_of(int64_t vocab) { return (vocab + kThreads * kEach - 1) / (kThreads * kEach); }
+// Values a thread: 16, and 64 where that still makes enough workgroups.  Finding a stretch's bound takes as long as reading 50 values a
+// thread: 16 searches of 8 beams over 131072 tokens take 25 us with 16 and 18 with 64; one of 4 over 32000 would wait for
+// 8 workgroups instead of 32.
+constexpr int kFew = 16, kMany = 64;
+int each_of(int64_t rows, int64_t vocab) { return rows * vocab >= (int64_t)512 * kThreads * kMany ? kMany : kFew; }
+int64_t splits_of(int64_t rows, int64_t vocab)
+{
+    const int64_t stretch = (int64_t)kThreads * each_of(rows, vocab);
+    return (vocab + stretch - 1) / stretch;
+}
 int64_t per_of(int64_t vocab, int64_t num) { return num < vocab ? num : vocab; }
 
 bool sizes_ok(int64_t groups, int64_t beams, int64_t vocab, int64_t num)
@@ -260,7 +286,7 @@ using namespace gla;
 extern "C" size_t gla_beam_select_workspace_bytes(int64_t groups, int64_t beams, int64_t vocab, int64_t num)
 {
     if (!sizes_ok(groups, beams, vocab, num)) return 0;
-    const int64_t stretches = groups * beams * splits_of(vocab);
+    const int64_t stretches = groups * beams * splits_of(groups * beams, vocab);
     return (size_t)(stretches * (per_of(vocab, num) * 8 + 8));
 }
 
@@ -285,7 +311,7 @@ extern "C" int gla_beam_select(void *stream, int64_t groups, int64_t beams, int6
     a.row = row;
     a.num = (int)num;
     a.per = (int)per_of(vocab, num);
-    a.splits = splits_of(vocab);
+    a.splits = splits_of(groups * beams, vocab);
     a.logits = logits;
     a.scores = scores;
     a.finished = static_cast<const uint8_t *>(finished);
@@ -299,15 +325,17 @@ extern "C" int gla_beam_select(void *stream, int64_t groups, int64_t beams, int6
     a.out_tokens = out_tokens;
     const hipStream_t s = static_cast<hipStream_t>(stream);
     const dim3 grid(a.splits, groups * beams);
-    const size_t room = (size_t)kThreads / 64 * kEach * a.per * sizeof(u64);
     const bool pieces = aligned16(logits) && row * size % 16 == 0 && vocab * size % 16 == 0;
-    if (dtype == GLA_BF16) {
-        if (pieces) beam_stretch_kernel<__bf16, kEach, 8><<<grid, kThreads, room, s>>>(a);
-        else beam_stretch_kernel<__bf16, kEach, 1><<<grid, kThreads, room, s>>>(a);
-    } else {
-        if (pieces) beam_stretch_kernel<float, kEach, 4><<<grid, kThreads, room, s>>>(a);
-        else beam_stretch_kernel<float, kEach, 1><<<grid, kThreads, room, s>>>(a);
-    }
+    const bool many = each_of(groups * beams, vocab) == kMany;
+    const auto kernel = dtype == GLA_BF16 ? pieces ? many ? beam_stretch_kernel<__bf16, kMany, true> : beam_stretch_kernel<__bf16, kFew, true>
+                                                   : many ? beam_stretch_kernel<__bf16, kMany, false> : beam_stretch_kernel<__bf16, kFew, false>
+                                          : pieces ? many ? beam_stretch_kernel<float, kMany, true> : beam_stretch_kernel<float, kFew, true>
+                                                   : many ? beam_stretch_kernel<float, kMany, false> : beam_stretch_kernel<float, kFew, false>;
+    const size_t room = (size_t)kThreads / 64 * each_of(groups * beams, vocab) * a.per * sizeof(u64);
+    static LdsGrant grants[8];
+    const size_t most = many ? (size_t)kThreads / 64 * kMany * GLA_MOST_CANDIDATES * sizeof(u64) : room;      // granted once, for any num
+    if (int e = allow_lds(grants[(dtype == GLA_BF16) * 4 + pieces * 2 + many], reinterpret_cast<const void *>(kernel), most)) return e;
+    kernel<<<grid, kThreads, room, s>>>(a);
     if (int e = launch_status()) return e;
     beam_join_kernel<<<groups, kJoinThreads, 0, s>>>(a);
     return launch_status();

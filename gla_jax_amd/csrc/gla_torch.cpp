@@ -305,6 +305,7 @@ struct Recurrent : torch::autograd::Function<Recurrent> {      // gla.py:99-170,
 };
 
 // ---- linear attention with one decay a head -------------------------------------------------------
+bool on_16_bytes(const Tensor &t) { return t.numel() == 0 || reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
 // Rows [B,T,heads,features] (or [T,heads,features]) that the kernels take where they lie: see decay.py's _rows.
 bool rows_on_gpu(const Tensor &t)
 {
@@ -313,7 +314,7 @@ bool rows_on_gpu(const Tensor &t)
     for (int64_t i = 0; i + 1 < t.dim(); ++i)
         if (t.size(i) > 1 && t.stride(i) % piece) return false;
     if (t.size(-3) > 1 && t.stride(-3) >= 1 << 23) return false;
-    return t.numel() == 0 || reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+    return on_16_bytes(t);
 }
 struct DecayDims {
     int64_t B, T, H, HK, DK, DV;
@@ -429,15 +430,18 @@ struct Decay : torch::autograd::Function<Decay> {
         variable_list s = ctx->get_saved_variables();
         // rows keep their strides; what a saved-tensor hook hands back in a layout that the kernels do not take is copied
         for (size_t i = 2; i < 5; ++i)
-            if (s[i].defined() && !rows_on_gpu(s[i])) s[i] = s[i].contiguous();
-        if (!s[0].is_contiguous()) s[0] = s[0].contiguous();
+            if (s[i].defined() && !rows_on_gpu(s[i])) s[i] = s[i].clone(at::MemoryFormat::Contiguous);
+        if (!s[0].is_contiguous() || !on_16_bytes(s[0])) s[0] = s[0].clone(at::MemoryFormat::Contiguous);
         if (s[5].defined() && !s[5].is_contiguous()) s[5] = s[5].contiguous();
         const std::optional<Tensor> lengths = s[5].defined() ? std::optional<Tensor>(s[5]) : std::nullopt;
         check_saved(decay_rows(s[1], s[2], s[3], s[4], lengths));
         const DecayDims n = decay_dims(s[2], s[3]);
         check_saved(holds(s[0], gla_decay_states_bytes(n.B, n.T, n.H, n.HK, n.DK, n.DV, code(s[2])), s[2]));
-        const Tensor dhT = cotangent(d[0], decay_state_sizes(s[2], s[3]), (at::ScalarType)ctx->saved_data["hidden"].toInt(), s[2]);
-        const Tensor dout = cotangent(d[1], s[2].sizes(), s[2].scalar_type(), s[2]);
+        Tensor dhT = cotangent(d[0], decay_state_sizes(s[2], s[3]), (at::ScalarType)ctx->saved_data["hidden"].toInt(), s[2]);
+        Tensor dout = cotangent(d[1], s[2].sizes(), s[2].scalar_type(), s[2]);
+        if (!transforms_active())
+            for (Tensor *t : {&dhT, &dout})
+                if (!on_16_bytes(*t)) *t = t->clone();
         variable_list r =
             transforms_active() ? python_rule("gla_jax_amd.decay", "_ChunkDecayBwd", s[0], s[1], s[2], s[3], s[4], lengths, dhT, dout)
             : at::GradMode::is_enabled() ? DecayBackward::apply(s[0], s[1], s[2], s[3], s[4], lengths, dhT, dout)
@@ -521,7 +525,7 @@ std::optional<std::pair<Tensor, Tensor>> rnn(const Tensor &a, const Tensor &b, c
 // [B,T,..] rows, or [T,..] as those of one sequence
 Result decay(const Tensor &h0, const Tensor &a, const Tensor &v, const Tensor &k, const Tensor &q, const std::optional<Tensor> &lengths)
 {
-    if (traced() || !decay_rows(a, v, k, q, lengths) || !dense_on_gpu(h0) || h0.device() != v.device() || !known(h0.scalar_type()) ||
+    if (traced() || !decay_rows(a, v, k, q, lengths) || !dense_on_gpu(h0) || !on_16_bytes(h0) || h0.device() != v.device() || !known(h0.scalar_type()) ||
         h0.sizes() != at::IntArrayRef(decay_state_sizes(v, k)))
         return std::nullopt;
     if (wants_grad(h0, a, v, k, q)) return Decay::apply(h0, a, v, k, q, lengths);
@@ -562,7 +566,7 @@ std::optional<Tensor> decay_step(const Tensor &states, const Tensor &a, const Te
     const at::ScalarType type = index_type(slots, parents);
     const int64_t W = parents && parents->dim() == 2 ? parents->size(1) : 0;
     if (!index_array(slots, {B}, states, type) || (parents && (W < 1 || !index_array(parents, {B / W, W}, states, type) || B % W)) ||
-        (!slots && N < B))
+        (!slots && N < B) || W > GLA_MOST_BEAMS || DK % 16 || DV % 16 || DK > 256 || DV > 256 || !on_16_bytes(states))
         return std::nullopt;
     const c10::DeviceGuard guard(states.device());
     Tensor out = dense_like(v);
@@ -571,7 +575,6 @@ std::optional<Tensor> decay_step(const Tensor &states, const Tensor &a, const Te
     const int rc = gla_decay_step(stream_of(states), N, B, H, HK, DK, DV, W, code(v), code(states), type == at::kLong, strides,
                                   (const float *)a.data_ptr(), v.data_ptr(), k.data_ptr(), q.data_ptr(), slots ? slots->data_ptr() : nullptr,
                                   parents ? parents->data_ptr() : nullptr, states.data_ptr(), out.data_ptr());
-    if (rc == GLA_ERR_SHAPE || rc == GLA_ERR_ALIGN) return std::nullopt;       // decay.py says what is wrong
     check("gla_decay_step", rc);
     return out;
 }
@@ -600,6 +603,7 @@ Result beam_select(const Tensor &logits, const Tensor &scores, const std::option
                      finished->device() != logits.device()))
         return std::nullopt;
     const int64_t num = wanted.value_or(W);
+    if (finished && (eos < 0 || eos >= V)) return std::nullopt;
     const size_t nws = row < V ? 0 : gla_beam_select_workspace_bytes(G, W, V, num);
     if (nws == 0) return std::nullopt;
     const c10::DeviceGuard guard(logits.device());
@@ -609,7 +613,6 @@ Result beam_select(const Tensor &logits, const Tensor &scores, const std::option
     const int rc = gla_beam_select(stream_of(logits), G, W, V, num, code(logits), row, logits.data_ptr(), (const float *)scores.data_ptr(),
                                    finished ? finished->data_ptr() : nullptr, eos, (float *)best.data_ptr(), (int64_t *)parents.data_ptr(),
                                    (int64_t *)tokens.data_ptr(), ws.data_ptr(), nws);
-    if (rc == GLA_ERR_SHAPE) return std::nullopt;
     check("gla_beam_select", rc);
     return std::vector<Tensor>{best, parents, tokens};
 }
@@ -621,12 +624,11 @@ bool reorder(const Tensor &states, const Tensor &parents, const std::optional<Te
     const at::ScalarType type = index_type(slots, parents);
     const int64_t G = parents.size(0), W = parents.size(1), N = states.size(0);
     if (!index_array(parents, parents.sizes(), states, type) || !index_array(slots, parents.sizes(), states, type) || G * W == 0 ||
-        (!slots && N < G * W))
+        W > GLA_MOST_BEAMS || (!slots && N < G * W))
         return false;
     const c10::DeviceGuard guard(states.device());
     const int rc = gla_reorder_states(stream_of(states), N, G, W, states.numel() / N * (int64_t)states.element_size(), type == at::kLong,
                                       parents.data_ptr(), slots ? slots->data_ptr() : nullptr, states.data_ptr());
-    if (rc == GLA_ERR_SHAPE) return false;
     check("gla_reorder_states", rc);
     return true;
 }

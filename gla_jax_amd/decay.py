@@ -27,7 +27,13 @@ def _rows(t, dtype):
     if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(
             s % piece == 0 and s < 1 << 23 or n == 1 for s, n in zip(t.stride()[1:-1], t.shape[1:])) and t.stride(0) % piece == 0:
         return t
-    return t.contiguous()
+    return _dense(t)
+
+
+def _dense(t):
+    """`t` without gaps, on 16 bytes."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
 def _strides(*rows):
@@ -40,7 +46,7 @@ def _decay_forward(h0, a, v, k, q, lengths, residual):
     B, T, H, DV = v.shape
     HK, DK = k.shape[2:]
     lib, dt = _lib.load(), _DT[v.dtype]
-    h0, v, k, q = h0.contiguous(), _rows(v, v.dtype), _rows(k, k.dtype), _rows(q, q.dtype)
+    h0, v, k, q = _dense(h0), _rows(v, v.dtype), _rows(k, k.dtype), _rows(q, q.dtype)
     at = a.expand(B, T, H)
     with torch.cuda.device(v.device):
         hT, out = torch.empty_like(h0), torch.empty(v.shape, dtype=v.dtype, device=v.device)
@@ -99,7 +105,7 @@ class _ChunkDecayBwd(torch.autograd.Function):
         HK, DK = k.shape[2:]
         lib, dt = _lib.load(), _DT[v.dtype]
         states, v, k, q = states.contiguous(), _rows(v, v.dtype), _rows(k, k.dtype), _rows(q, q.dtype)
-        dhT, dout = dhT.to(dhT.dtype if dhT.dtype in _DT else torch.float32).contiguous(), dout.to(v.dtype).contiguous()
+        dhT, dout = _dense(dhT.to(dhT.dtype if dhT.dtype in _DT else torch.float32)), _dense(dout.to(v.dtype))
         constant = a.ndim == 1
         at = a.expand(B, T, H)
         with torch.cuda.device(v.device):
@@ -204,9 +210,10 @@ def chunk_decay(hidden_init, log_decay, value, key, query, lengths=None):
         # The kernels take 16 features at a time.  A zero feature adds nothing to a score or to the rest of the state.
         F = torch.nn.functional
         h0, v, k, q = F.pad(h0, (0, pv, 0, pk)), F.pad(v, (0, pv)), F.pad(k, (0, pk)), F.pad(q, (0, pk))
-    v, k, q = (_rows(t, t.dtype) for t in (v, k, q))
-    hT, out = (_native("decay", (h0, a, v, k, q), lengths) if _plain_call()
-               else _apply(_ChunkDecay, h0, a, v, k, q, lengths)[:2])
+    if _plain_call():
+        hT, out = _native("decay", (_dense(h0), a, *(_rows(t, t.dtype) for t in (v, k, q))), lengths)
+    else:
+        hT, out = _apply(_ChunkDecay, h0, a, v, k, q, lengths)[:2]
     if pk or pv:
         hT, out = hT[..., :DK, :DV], out[..., :DV]
     return _as(hT, lead + (H, DK, DV), hidden_init.dtype), _as(out, lead + (T, H, DV), out.dtype)
