@@ -40,11 +40,11 @@ DecayPlan plan_segments(const DecaySizes &n, gla_dtype dtype, int64_t workgroups
 }
 DecayPlan forward_plan(const DecaySizes &n, gla_dtype dtype, bool ragged)
 {
-    return plan_segments(n, dtype, n.B * n.H * decay_slabs(n.DV), 512, 0.45, ragged);
+    return plan_segments(n, dtype, n.B * n.H * decay_slabs(n.DV), kComputeUnits, 0.6, ragged);
 }
 DecayPlan backward_plan(const DecaySizes &n, gla_dtype dtype, bool ragged)
 {
-    return plan_segments(n, dtype, n.B * n.H * decay_slabs(n.DV) * (n.DK > 128 ? 2 : 1), 256, 0.2, ragged);
+    return plan_segments(n, dtype, n.B * n.H * decay_slabs(n.DV) * (n.DK > 128 ? 2 : 1), kComputeUnits, 0.2, ragged);
 }
 
 int64_t entering_bytes(const DecaySizes &n, const DecayPlan &p)

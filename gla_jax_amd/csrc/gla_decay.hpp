@@ -18,6 +18,8 @@
 
 namespace gla {
 
+constexpr int64_t kComputeUnits = 256;
+
 template <typename T> struct DecayChunk;                       // tokens of a chunk
 template <> struct DecayChunk<__bf16> { static constexpr int C = 64; };
 template <> struct DecayChunk<float> { static constexpr int C = 32; };
@@ -186,6 +188,44 @@ __device__ __forceinline__ void mma_right(const D8 (&a)[M], const Split<T, N> &b
 #pragma unroll
         for (int m = 0; m < M; ++m) c[m] = mma_d(a[m], b.part[i], c[m]);
 }
+// A tile of scores: rows 16 * ta + 4c .. of one array against rows 16 * tb + r of another, over KS * 32 features.  Four steps' operands are
+// read at a time, and two sums keep the products apart.
+template <int KS, typename Tile, typename T>
+__device__ __forceinline__ f32x4 tile_product(const Tile &l, const T *a, int ta, const T *b, int tb)
+{
+    typedef typename FragTypes<T>::d8 D8;
+    constexpr int kAhead = sizeof(T) == 2 ? (KS < 4 ? KS : 4) : 1;
+    f32x4 s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+    for (int k0 = 0; k0 < KS; k0 += kAhead) {
+        D8 x[kAhead], y[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            x[i] = l.rows(a, ta, k0 + i);
+            y[i] = l.rows(b, tb, k0 + i);
+        }
+        if constexpr (kAhead > 1) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) s[(k0 + i) & 1] = mma_d(x[i], y[i], s[(k0 + i) & 1]);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s[0][e] += s[1][e];
+    return s[0];
+}
+// Two tiles of scores behind each other as an operand, or (the second lies above the diagonal) one and zeros.
+__device__ __forceinline__ bf16x8 two_score_tiles(const __bf16 *p, bool both)
+{
+    const bf16x4 zero = {};
+    return __builtin_shufflevector(LdsTile<__bf16, 64>::half(p), both ? LdsTile<__bf16, 64>::half(p + 256) : zero, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+__device__ __forceinline__ f32x8 two_score_tiles(const float *p, bool both)
+{
+    const f32x4 zero = {0.f, 0.f, 0.f, 0.f}, a = *reinterpret_cast<const f32x4 *>(p), b = both ? *reinterpret_cast<const f32x4 *>(p + 256) : zero;
+    f32x8 r;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) { r.v[e] = a[e]; r.v[4 + e] = b[e]; }
+    return r;
+}
 __device__ __forceinline__ void two_tiles(f32x4 a, f32x4 b, float (&x)[8])
 {
 #pragma unroll
@@ -272,31 +312,32 @@ template <typename T, int C, int F, int NT> struct RowsInFlight {
     static constexpr int kPieces = C * F / 8, kPer = (kPieces + NT - 1) / NT, kStep = NT / (F / 8);
     static_assert(NT % (F / 8) == 0, "");
     d8 x[kPer];
+    // A thread's place: kept over a loop it would take registers, so it is formed again for every chunk, once for all arrays.
+    static __device__ __forceinline__ unsigned here() { return again(threadIdx.x); }
     // The rows of a chunk that `rows` points at, the first of which exists and `there` in all.  No load is under a branch (a thread without
     // a piece reads one that exists, and `store` puts zeros in its place): with loads that may or may not have been issued the compiler
     // waits for every access to memory where it needs one of them.
-    __device__ __forceinline__ void load(const T *rows, int st, int there, int features)
+    __device__ __forceinline__ void load(unsigned tid, const T *rows, int st, int there, int features)
     {
-        // formed here each time: kept over the loop, a lane's place would take a register, and in 64 bits two
-        const unsigned tid = again(threadIdx.x);
-        const int row = tid / (F / 8), col = 8 * (tid % (F / 8));
+        const int row = tid / (F / 8), col = 8 * (tid % (F / 8)), from = col < features ? col : 0;
 #pragma unroll
-        for (int i = 0; i < kPer; ++i)
-            x[i] = ld8(at_bytes(rows, (unsigned)(min(min(row + i * kStep, C - 1), there - 1) * st + (col < features ? col : 0)) * (unsigned)sizeof(T)));
+        for (int i = 0; i < kPer; ++i)      // (rows lie less than 2^23 elements apart: 24-bit products, which take a quarter of the time)
+            x[i] = ld8(at_bytes(rows, (__umul24(min(min(row + i * kStep, C - 1), there - 1), st) + from) * (unsigned)sizeof(T)));
     }
-    __device__ __forceinline__ void store(T *tile, int there, int features) const
+    __device__ __forceinline__ void store(unsigned tid, T *tile, int there, int features) const
     {
-        const unsigned tid = again(threadIdx.x);
-        const int row = tid / (F / 8), col = 8 * (tid % (F / 8));
+        const int row = tid / (F / 8), col = 8 * (tid % (F / 8)), first = LdsTile<T, F>::piece(row, col);
+        auto place = [&](int i) {           // 16 rows further the order of the pieces is the same
+            return tile + (kStep % 16 == 0 ? first + i * kStep * LdsTile<T, F>::kRow : LdsTile<T, F>::piece(row + i * kStep, col));
+        };
         if (there >= C && features >= F) {
 #pragma unroll
             for (int i = 0; i < kPer; ++i)
-                if (kPieces % NT == 0 || row + i * kStep < C) st8(tile + LdsTile<T, F>::piece(row + i * kStep, col), x[i]);
+                if (kPieces % NT == 0 || row + i * kStep < C) st8(place(i), x[i]);
         } else {
 #pragma unroll
             for (int i = 0; i < kPer; ++i)
-                if (kPieces % NT == 0 || row + i * kStep < C)
-                    st8(tile + LdsTile<T, F>::piece(row + i * kStep, col), row + i * kStep < there && col < features ? x[i] : d8{});
+                if (kPieces % NT == 0 || row + i * kStep < C) st8(place(i), row + i * kStep < there && col < features ? x[i] : d8{});
         }
     }
 };
@@ -316,6 +357,8 @@ struct DecayPlan {
     int64_t chunks;     // of a sequence
     int64_t segments;
     __host__ __device__ int64_t first(int64_t segment) const { return segment * chunks / segments; }
+    // the segment in which a sequence of so many chunks ends: behind it there is nothing to do
+    __host__ __device__ int64_t tail(int64_t live) const { return live > 0 ? (live * segments - 1) / chunks : 0; }
 };
 
 struct DecaySizes {
@@ -339,10 +382,9 @@ __device__ __forceinline__ int64_t pair_of(unsigned x, const DecaySizes &n)
     return (int64_t)unit * group + member;
 }
 
-// The states that enter the segments, from what every segment adds: `pass` says which way (see the kernels).  Launches the
+// The states that enter the segments, from what every segment adds, or (cotangents) the cotangents of those that leave them.  Launches the
 // pass and the scan over the segments; `states` receives [B*H, segments, slabs][a slab in accumulator order] floats.
-enum DecayPass { kDecayForward = 0, kDecayStates = 1, kDecayCotangents = 2 };
-int decay_entering_states(void *stream, DecayPass pass, const DecaySizes &n, const DecayPlan &plan, gla_dtype dtype,
+int decay_entering_states(void *stream, bool cotangents, const DecaySizes &n, const DecayPlan &plan, gla_dtype dtype,
                           gla_dtype hidden_dtype, const void *hidden, const DecayRows &gates, const DecayRows &keys,
                           const DecayRows &values, const int32_t *lengths, float *states, float *decays);
 __host__ __device__ inline int64_t decay_key_width(int64_t DK) { return DK <= 64 ? 64 : DK <= 128 ? 128 : 256; }     // features that a workgroup holds

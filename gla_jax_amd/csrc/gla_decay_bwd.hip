@@ -83,8 +83,10 @@ __global__ __launch_bounds__(((DKW > DVW ? DKW : DVW) + DKW) * 4) void decay_gra
     const int64_t bh = pair_of(blockIdx.x, a.n), b = bh / a.n.H, h = bh % a.n.H, group = a.n.H / a.n.HK, hk = h / group;
     const int DK = (int)a.n.DK, DV = (int)a.n.DV, vslabs = (DV + DVW - 1) / DVW;
     const int ks0 = blockIdx.y / vslabs, vs0 = blockIdx.y % vslabs, dk0 = ks0 * DKW, dv0 = vs0 * DVW;
-    const int64_t order = blockIdx.z, seg = a.plan.segments - 1 - order;
     const int T_ = (int)a.n.T, len = a.lengths ? min(max(a.lengths[b], 0), T_) : T_;
+    // from the segment in which the sequence ends down to the first; then those behind it, where only zeros are to be written
+    const int order = blockIdx.z, tail = (int)a.plan.tail((len + C - 1) / C),
+              seg = tail - order + (order <= tail ? 0 : (int)a.plan.segments);
     const int first = (int)a.plan.first(seg), last = (int)a.plan.first(seg + 1), live = min(last, (len + C - 1) / C);
     const T *K = static_cast<const T *>(a.keys.p) + b * a.keys.sb + hk * a.keys.sh + dk0;
     const T *Q = static_cast<const T *>(a.queries.p) + b * a.queries.sb + hk * a.queries.sh + dk0;
@@ -106,7 +108,7 @@ __global__ __launch_bounds__(((DKW > DVW ? DKW : DVW) + DKW) * 4) void decay_gra
     };
     Result qk = result(second ? a.dkey : a.dquery, a.row_parts, vs0 * group + h % group, a.n.HK * DK, hk * DK + dk0 + 16 * wk);
     Result dv = result(a.dvalue, a.value_parts, ks0, a.n.H * DV, h * DV + dv0 + 16 * w);
-    const float *kept = a.kept + ((bh * a.plan.chunks + live - 1) * DK + dk0 + (key_wave ? 16 * wk : 0)) * DV + dv0;
+    const float *kept = a.kept + (((bh * a.plan.chunks + live - 1) * (DK / 16) + (key_wave ? dk0 / 16 + wk : 0)) * (DV / 16) + dv0 / 16) * 256;
     const int64_t kept_step = (int64_t)DK * DV;
 
     // ---- the cotangent that enters: key feature r of the wave's, value features 16t + 4c .. ----
@@ -121,7 +123,7 @@ __global__ __launch_bounds__(((DKW > DVW ? DKW : DVW) + DKW) * 4) void decay_gra
                 load_hidden<4>(a.dhidden_final, a.hidden_dtype, (bh * DK + dk0 + 16 * wk + r) * DV + dv0 + 16 * t + 4 * c, x);
                 state[t] = f32x4{x[0], x[1], x[2], x[3]};
             }
-    } else {
+    } else if (seg <= tail) {
         const int tiles = (int)decay_key_width(DK) / 16;
         const float *from = a.entering + ((bh * a.plan.segments + order - 1) * vslabs + vs0) * (int64_t)(tiles * 16 * DVW);
 #pragma unroll
@@ -141,10 +143,11 @@ __global__ __launch_bounds__(((DKW > DVW ? DKW : DVW) + DKW) * 4) void decay_gra
     };
     auto fetch = [&](int n) {                    // the rows that the pointers have come to
         const int left = len - n * C;
-        fk.load(K, k_st, left, DK - dk0);
-        fq.load(Q, q_st, left, DK - dk0);
-        fv.load(V, v_st, left, DV - dv0);
-        fo.load(O, o_st, left, DV - dv0);
+        const unsigned at = fk.here();
+        fk.load(at, K, k_st, left, DK - dk0);
+        fq.load(at, Q, q_st, left, DK - dk0);
+        fv.load(at, V, v_st, left, DV - dv0);
+        fo.load(at, O, o_st, left, DV - dv0);
         K -= (int64_t)C * k_st;
         Q -= (int64_t)C * q_st;
         V -= (int64_t)C * v_st;
@@ -187,8 +190,7 @@ __global__ __launch_bounds__(((DKW > DVW ? DKW : DVW) + DKW) * 4) void decay_gra
     for (int i = tid; i < C * TileP::kRow; i += NT) sP[i] = sD[i] = (T)0.f;      // the tiles above the diagonal that products take along
     // key feature r of the wave's, value features 16 t + 4c .. of the state that `from` points at (or others, where these do not exist)
     auto state_tile = [&](const float *from, int t) {
-        const unsigned lane = again(tid), at = ((lane & 15) * DV + ((lane >> 2) & 12)) * 4;
-        return *reinterpret_cast<const f32x4 *>(at_bytes(from + (16 * t < DV - dv0 ? 16 * t : 0), at));
+        return *reinterpret_cast<const f32x4 *>(at_bytes(from + (16 * t < DV - dv0 ? 256 * t : 0), (again(tid) & 63) * 16));
     };
     const int sums_wave = NW - 2;
     const int count = max(live - first, 0);
@@ -211,10 +213,11 @@ __global__ __launch_bounds__(((DKW > DVW ? DKW : DVW) + DKW) * 4) void decay_gra
         const ChunkGates<C> &gate = gates[i & 1];
         Sums &sum = sums[i & 1];
         lds_barrier();                            // the last chunk's tiles are read, its sums written
-        fk.store(sK, len - n * C, DK - dk0);
-        fq.store(sQ, len - n * C, DK - dk0);
-        fv.store(sV, len - n * C, DV - dv0);
-        fo.store(sO, len - n * C, DV - dv0);
+        const unsigned at = fk.here();
+        fk.store(at, sK, len - n * C, DK - dk0);
+        fq.store(at, sQ, len - n * C, DK - dk0);
+        fv.store(at, sV, len - n * C, DV - dv0);
+        fo.store(at, sO, len - n * C, DV - dv0);
         if (second) {                             // dS as the operand of dv
             const TileV LV = tv.here();
 #pragma unroll
@@ -539,7 +542,7 @@ int decay_backward(void *stream, const DecaySizes &n, const DecayPlan &plan, gla
                    void *dhidden_init, float *dlog_decay, void *dvalue, void *dkey, void *dquery, float *entering, float *decays,
                    const DecayParts &parts)
 {
-    int e = decay_entering_states(stream, kDecayCotangents, n, plan, dtype, hidden_dtype, dhidden_final, gates, queries, dout,
+    int e = decay_entering_states(stream, true, n, plan, dtype, hidden_dtype, dhidden_final, gates, queries, dout,
                                   lengths, entering, decays);
     if (e) return e;
     const hipStream_t s = static_cast<hipStream_t>(stream);
