@@ -51,8 +51,8 @@ struct Result {
 
 // One workgroup: a segment of a (batch, head) pair, DKW key and DVW value features.  Its first waves make dq and dv: wave w of key
 // features 16w .. 16w+15, with its columns of S, and of value features 16w .. 16w+15.  The others make dk and carry dS: its columns of
-// key features lie in the accumulators with value features as rows, an operand of dk as they are; dv contracts dS over the other
-// index and takes it from LDS, rounded to `T` as any operand of a 16-bit result.  (A second copy of dS by value columns cost 32
+// key features lie in the accumulators with value features as rows, an operand of dk as they are; the first waves take dS from LDS, for
+// <S, dS> and for dv, which contracts it over the other index, rounded to `T` as any operand of a 16-bit result.  (A second copy of dS by value columns cost 32
 // registers and as many products as the first; all of it on 8 waves of twice the registers left a SIMD two waves, whose
 // matrix, vector and LDS phases then followed each other: 135 us against the %US% of 16 at B4 T4096 H6 D128.)
 // S and dS enter what the gates' gradient is formed from in three parts, i.e. as the 32-bit numbers that they are.
@@ -67,8 +67,9 @@ __global__ __launch_bounds__(((DKW > DVW ? DKW : DVW) + DKW) * 4) void decay_gra
     typedef LdsTile<T, C> TileP;
     extern __shared__ char smem[];
     T *sQ = reinterpret_cast<T *>(smem), *sK = sQ + C * TileK::kRow, *sV = sK + C * TileK::kRow, *sO = sV + C * TileV::kRow,
-      *sP = sO + C * TileV::kRow, *sD = sP + C * TileP::kRow, *sS = sD + C * TileP::kRow;
-    ChunkGates<C> *gates = reinterpret_cast<ChunkGates<C> *>(reinterpret_cast<char *>(sS + DKW * TileV::kRow));
+      *sP = sO + C * TileV::kRow, *sD = sP + C * TileP::kRow;
+    float *sS = reinterpret_cast<float *>(sD + C * TileP::kRow);
+    ChunkGates<C> *gates = reinterpret_cast<ChunkGates<C> *>(sS + DKW * DVW);
     // what the gates' gradient is formed from, of a chunk and of the one before
     struct Sums {
         float row[CT][C];                        // row sums of one column of tiles
@@ -192,6 +193,18 @@ __global__ __launch_bounds__(((DKW > DVW ? DKW : DVW) + DKW) * 4) void decay_gra
     auto state_tile = [&](const float *from, int t) {
         return *reinterpret_cast<const f32x4 *>(at_bytes(from + (16 * t < DV - dv0 ? 256 * t : 0), (again(tid) & 63) * 16));
     };
+    // dS in LDS, tiles of 16 key and 16 value features as the waves hold them.  The places of 16 lanes are permuted by the lanes' row, so that
+    // reads along key features, too, have no two lanes at a bank.
+    auto dS_tile = [&](int tk, int t) {
+        const unsigned lane = again(tid) & 63, c = lane >> 4;
+        return sS + (tk * VT + t) * 256 + (lane ^ c) * 4;
+    };
+    // key features 32 ks + 4c .. and 32 ks + 16 + 4c .. of value feature 16 t + r
+    auto dS_columns = [&](int ks, int t, float (&x)[8]) {
+        const unsigned lane = again(tid) & 63, r = lane & 15, c = lane >> 4, row = r >> 2;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = sS[((2 * ks + e / 4) * VT + t) * 256 + (16 * row + 4 * c + ((e & 3) ^ row)) * 4 + (r & 3)];
+    };
     const int sums_wave = NW - 2;
     const int count = max(live - first, 0);
     int n = live - 1;
@@ -218,25 +231,22 @@ __global__ __launch_bounds__(((DKW > DVW ? DKW : DVW) + DKW) * 4) void decay_gra
         fq.store(at, sQ, len - n * C, DK - dk0);
         fv.store(at, sV, len - n * C, DV - dv0);
         fo.store(at, sO, len - n * C, DV - dv0);
-        if (second) {                             // dS as the operand of dv
-            const TileV LV = tv.here();
+        if (second) {                             // dS for the first waves
+            float *p = dS_tile(wk, 0);
 #pragma unroll
-            for (int t = 0; t < VT; ++t) {
-                const float x[4] = {state[t][0], state[t][1], state[t][2], state[t][3]};
-                store_vec<T, 4>(LV.four(sS, wk, t), x);
-            }
+            for (int t = 0; t < VT; ++t) *reinterpret_cast<f32x4 *>(p + t * 256) = state[t];
         }
         lds_barrier();
         const float whole = gate.whole;
-        if (second) {                             // <S, dS>; the first waves have brought S into the cache
+        if (!second && has_keys) {                // <S, dS>
             float x = 0.f;
-            f32x4 S[VT];
+            const float *p = dS_tile(w, 0);
 #pragma unroll
-            for (int t = 0; t < VT; ++t) S[t] = state_tile(kept, t);
+            for (int t = 0; t < VT; ++t) {
+                const f32x4 d = *reinterpret_cast<const f32x4 *>(p + t * 256);
 #pragma unroll
-            for (int t = 0; t < VT; ++t)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) x += S[t][e] * state[t][e];      // (where S is another's, dS is zero)
+                for (int e = 0; e < 4; ++e) x += d[e] * state[t][e];         // (where S is another's, dS is zero)
+            }
             x = sum_over_c(sum_over_r(x));
             if (lane == 0) sum.x[wk] = whole * x;
         }
@@ -413,7 +423,9 @@ __global__ __launch_bounds__(((DKW > DVW ? DKW : DVW) + DKW) * 4) void decay_gra
             const TileK LK = tk.here();
 #pragma unroll
             for (int ks = 0; ks < KK; ++ks) {
-                const D8 op = LV.columns(sS, ks, w);
+                float d[8];
+                dS_columns(ks, w, d);
+                const D8 op = Split<T, 1>(d).part[0];
 #pragma unroll
                 for (int tj = 0; tj < CT; ++tj) o[tj] = mma_d(op, LK.halves(sK, tj, ks), o[tj]);
             }
@@ -513,9 +525,10 @@ template <typename T, int DKW, int DVW> int launch_gradient(hipStream_t stream, 
 {
     static LdsGrant grant;
     constexpr int C = DecayChunk<T>::C, CT = C / 16, KT = DKW / 16;
-    constexpr size_t lds = sizeof(T) * (2 * C * LdsTile<T, DKW>::kRow + 2 * C * LdsTile<T, DVW>::kRow + 2 * C * LdsTile<T, C>::kRow +
-                                        DKW * LdsTile<T, DVW>::kRow) +
+    constexpr size_t lds = sizeof(T) * (2 * C * LdsTile<T, DKW>::kRow + 2 * C * LdsTile<T, DVW>::kRow + 2 * C * LdsTile<T, C>::kRow) +
+                           sizeof(float) * DKW * DVW +
                            2 * sizeof(ChunkGates<C>) + sizeof(float) * 2 * (2 * CT * C + 2 * KT * C + 16) + sizeof(double) * 64;
+    static_assert(lds <= 160 * 1024, "");
     if (int e = allow_lds(grant, reinterpret_cast<const void *>(decay_gradient_kernel<T, DKW, DVW>), lds)) return e;
     const dim3 grid(a.n.B * a.n.H, ((a.n.DK + DKW - 1) / DKW) * ((a.n.DV + DVW - 1) / DVW), a.plan.segments);
     decay_gradient_kernel<T, DKW, DVW><<<grid, ((DKW > DVW ? DKW : DVW) + DKW) * 4, lds, stream>>>(a);
