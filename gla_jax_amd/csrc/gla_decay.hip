@@ -18,25 +18,26 @@ int64_t pad256(int64_t x) { return (x + 255) & ~(int64_t)255; }
 DecayPlan plan_segments(const DecaySizes &n, gla_dtype dtype, int64_t workgroups, int64_t slots, double pass, bool ragged)
 {
     const int64_t C = dtype == GLA_BF16 ? DecayChunk<__bf16>::C : DecayChunk<float>::C;
-    DecayPlan best{(n.T + C - 1) / C, 1};
-    const double work = (double)workgroups * best.chunks / slots;
+    const int64_t chunks = (n.T + C - 1) / C;
+    int64_t best = 1;
+    const double work = (double)workgroups * chunks / slots;
     double least = 0.0;
     for (int64_t rounds = 0; rounds <= 4; ++rounds) {
         int64_t segments = rounds ? rounds * slots / workgroups : 1;
-        if (segments > best.chunks / 2) segments = best.chunks / 2;
+        if (segments > chunks / 2) segments = chunks / 2;
         if (rounds && segments < 2) continue;
         if (segments < 1) segments = 1;
-        const int64_t longest = (best.chunks + segments - 1) / segments, taken = (workgroups * segments + slots - 1) / slots;
+        const int64_t longest = (chunks + segments - 1) / segments, taken = (workgroups * segments + slots - 1) / slots;
         // a state is written, scanned and read, the rows of a chunk are read: DK / 32 of them move as much
         const double states = 0.012 * n.DK;
         double cost = ragged ? 0.5 * work + longest + taken : taken * (longest + 1.0);
         if (segments > 1) cost += pass * (ragged ? 0.5 * work + longest : work) + taken + states * workgroups * segments / slots + 1.0;
         if (rounds == 0 || cost < least) {
             least = cost;
-            best.segments = segments;
+            best = segments;
         }
     }
-    return best;
+    return DecayPlan(chunks, best);
 }
 DecayPlan forward_plan(const DecaySizes &n, gla_dtype dtype, bool ragged)
 {

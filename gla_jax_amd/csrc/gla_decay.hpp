@@ -352,13 +352,21 @@ __device__ __forceinline__ void triangle(int n, int &ti, int &tj)
     tj = n - ti * (ti + 1) / 2;
 }
 
-// The segments that sequences run as, as even as whole chunks make them.
+// The segments that sequences run as: the first `longer` ones have a chunk more than the others, which have `each`.  (Divisions in 64 bits
+// took a microsecond of every kernel's beginning.)
 struct DecayPlan {
     int64_t chunks;     // of a sequence
     int64_t segments;
-    __host__ __device__ int64_t first(int64_t segment) const { return segment * chunks / segments; }
+    int each, longer;
+    DecayPlan() = default;
+    DecayPlan(int64_t chunks, int64_t segments) : chunks(chunks), segments(segments), each((int)(chunks / segments)), longer((int)(chunks % segments)) {}
+    __host__ __device__ int first(int segment) const { return segment * each + (segment < longer ? segment : longer); }
     // the segment in which a sequence of so many chunks ends: behind it there is nothing to do
-    __host__ __device__ int64_t tail(int64_t live) const { return live > 0 ? (live * segments - 1) / chunks : 0; }
+    __host__ __device__ int tail(int live) const
+    {
+        const unsigned last = live - 1, those = longer * (each + 1);
+        return live <= 0 ? 0 : last < those ? last / (unsigned)(each + 1) : longer + (last - those) / (unsigned)each;
+    }
 };
 
 struct DecaySizes {
@@ -367,9 +375,9 @@ struct DecaySizes {
 
 // The pair (batch, head), as b * H + h, of workgroup x: heads that share their keys go to the same one of the 8 dies, to which
 // workgroups are dealt in turn, so that its cache reads them once.
-__device__ __forceinline__ int64_t pair_of(unsigned x, const DecaySizes &n)
+__device__ __forceinline__ unsigned pair_of(unsigned x, const DecaySizes &n)
 {
-    const unsigned group = (unsigned)(n.H / n.HK), units = (unsigned)(n.B * n.HK), even = units / 8 * 8;
+    const unsigned group = (unsigned)n.H / (unsigned)n.HK, units = (unsigned)n.B * (unsigned)n.HK, even = units / 8 * 8;
     if (group == 1) return x;
     unsigned unit, member;
     if (x < even * group) {
@@ -379,7 +387,7 @@ __device__ __forceinline__ int64_t pair_of(unsigned x, const DecaySizes &n)
         unit = x / group;
         member = x % group;
     }
-    return (int64_t)unit * group + member;
+    return unit * group + member;
 }
 
 // The states that enter the segments, from what every segment adds, or (cotangents) the cotangents of those that leave them.  Launches the

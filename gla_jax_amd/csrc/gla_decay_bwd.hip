@@ -81,14 +81,15 @@ __global__ __launch_bounds__(((DKW > DVW ? DKW : DVW) + DKW) * 4) void decay_gra
     double *sGate = reinterpret_cast<double *>(sums + 2);     // the gates' gradients so far, by token of the chunk
 
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, r = lane & 15, c = lane >> 4;
-    const int64_t bh = pair_of(blockIdx.x, a.n), b = bh / a.n.H, h = bh % a.n.H, group = a.n.H / a.n.HK, hk = h / group;
+    const unsigned H = (unsigned)a.n.H, pair = pair_of(blockIdx.x, a.n);
+    const int64_t bh = pair, b = pair / H, h = pair % H, group = H / (unsigned)a.n.HK, hk = pair % H / (unsigned)group;
     const int DK = (int)a.n.DK, DV = (int)a.n.DV, vslabs = (DV + DVW - 1) / DVW;
     const int ks0 = blockIdx.y / vslabs, vs0 = blockIdx.y % vslabs, dk0 = ks0 * DKW, dv0 = vs0 * DVW;
     const int T_ = (int)a.n.T, len = a.lengths ? min(max(a.lengths[b], 0), T_) : T_;
     // from the segment in which the sequence ends down to the first; then those behind it, where only zeros are to be written
-    const int order = blockIdx.z, tail = (int)a.plan.tail((len + C - 1) / C),
+    const int order = blockIdx.z, tail = a.plan.tail((len + C - 1) / C),
               seg = tail - order + (order <= tail ? 0 : (int)a.plan.segments);
-    const int first = (int)a.plan.first(seg), last = (int)a.plan.first(seg + 1), live = min(last, (len + C - 1) / C);
+    const int first = a.plan.first(seg), last = a.plan.first(seg + 1), live = min(last, (len + C - 1) / C);
     const T *K = static_cast<const T *>(a.keys.p) + b * a.keys.sb + hk * a.keys.sh + dk0;
     const T *Q = static_cast<const T *>(a.queries.p) + b * a.queries.sb + hk * a.queries.sh + dk0;
     const T *V = static_cast<const T *>(a.values.p) + b * a.values.sb + h * a.values.sh + dv0;

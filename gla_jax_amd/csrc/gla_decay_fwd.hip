@@ -52,11 +52,12 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DKP == 
     ChunkGates<C> *gates = reinterpret_cast<ChunkGates<C> *>(reinterpret_cast<char *>(sP + C * TileP::kRow));
 
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, r = lane & 15, c = lane >> 4;
-    const int64_t bh = pair_of(blockIdx.x, a.n), b = bh / a.n.H, h = bh % a.n.H, hk = h / (a.n.H / a.n.HK);
+    const unsigned H = (unsigned)a.n.H, pair = pair_of(blockIdx.x, a.n);
+    const int64_t bh = pair, b = pair / H, h = pair % H, hk = pair % H / (H / (unsigned)a.n.HK);
     const int dv0 = blockIdx.y * DVS, DK = (int)a.n.DK, DV = (int)a.n.DV;
     const int T_ = (int)a.n.T, len = a.lengths ? min(max(a.lengths[b], 0), T_) : T_;
-    const int seg = blockIdx.z, tail = (int)a.plan.tail((len + C - 1) / C);
-    const int first = (int)a.plan.first(seg), last = (int)a.plan.first(seg + 1), live = min(last, (len + C - 1) / C);
+    const int seg = blockIdx.z, tail = a.plan.tail((len + C - 1) / C);
+    const int first = a.plan.first(seg), last = a.plan.first(seg + 1), live = min(last, (len + C - 1) / C);
     const T *X = static_cast<const T *>(a.keys.p) + b * a.keys.sb + hk * a.keys.sh;
     const T *Y = static_cast<const T *>(a.values.p) + b * a.values.sb + h * a.values.sh + dv0;
     const T *Q = static_cast<const T *>(a.queries.p) + b * a.queries.sb + hk * a.queries.sh;
@@ -260,11 +261,12 @@ __global__ __launch_bounds__(NW * 128) __attribute__((amdgpu_waves_per_eu(DKP ==
     ChunkGates<C> *gates = reinterpret_cast<ChunkGates<C> *>(sP + 2 * kScores);
 
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, r = lane & 15, c = lane >> 4;
-    const int64_t bh = pair_of(blockIdx.x, a.n), b = bh / a.n.H, h = bh % a.n.H, hk = h / (a.n.H / a.n.HK);
+    const unsigned H = (unsigned)a.n.H, pair = pair_of(blockIdx.x, a.n);
+    const int64_t bh = pair, b = pair / H, h = pair % H, hk = pair % H / (H / (unsigned)a.n.HK);
     const int dv0 = blockIdx.y * DVS, DK = (int)a.n.DK, DV = (int)a.n.DV;
     const int T_ = (int)a.n.T, len = a.lengths ? min(max(a.lengths[b], 0), T_) : T_;
-    const int seg = blockIdx.z, tail = (int)a.plan.tail((len + C - 1) / C);
-    const int first = (int)a.plan.first(seg), last = (int)a.plan.first(seg + 1), live = min(last, (len + C - 1) / C);
+    const int seg = blockIdx.z, tail = a.plan.tail((len + C - 1) / C);
+    const int first = a.plan.first(seg), last = a.plan.first(seg + 1), live = min(last, (len + C - 1) / C);
     const int count = max(live - first, 0);
     const TileX tx;
     const TileY ty;
@@ -455,9 +457,10 @@ __global__ __launch_bounds__(NW * 128) __attribute__((amdgpu_waves_per_eu(DKP ==
 
 // What a segment adds to the state that leaves it (cotangents: the chunks in reverse, queries for keys and cotangents of out for values),
 // and how much of the state that entered it is left.  Two chunks' rows in LDS, one barrier a chunk; rows are on their way for two
-// chunks, since a chunk takes less time than memory does.
+// chunks, since a chunk takes less time than memory does.  A wave of its own makes the gates: 600 of a chunk's 4400 cycles, for which the
+// others had to wait.
 template <typename T, int DKP, int NW, bool kReverse>
-__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DKP == 256 ? 2 : DKP == 128 && NW == 4 ? 3 : 4))) void decay_states_kernel(const ForwardArgs a)
+__global__ __launch_bounds__(NW * 64 + 64) __attribute__((amdgpu_waves_per_eu(DKP == 256 && NW == 4 ? 2 : 3))) void decay_states_kernel(const ForwardArgs a)
 {
     constexpr int C = DecayChunk<T>::C, NT = NW * 64, DVS = 16 * NW, TILES = DKP / 16, CS = C / 32;
     typedef typename FragTypes<T>::d8 D8;
@@ -469,18 +472,38 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DKP == 
     ChunkGates<C> *gates = reinterpret_cast<ChunkGates<C> *>(sX + 2 * kChunk);
 
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, r = lane & 15, c = lane >> 4;
-    const int64_t bh = pair_of(blockIdx.x, a.n), b = bh / a.n.H, h = bh % a.n.H, hk = h / (a.n.H / a.n.HK);
+    const unsigned H = (unsigned)a.n.H, pair = pair_of(blockIdx.x, a.n);
+    const int64_t bh = pair, b = pair / H, h = pair % H, hk = pair % H / (H / (unsigned)a.n.HK);
     const int dv0 = blockIdx.y * DVS, DK = (int)a.n.DK, DV = (int)a.n.DV;
     const int T_ = (int)a.n.T, len = a.lengths ? min(max(a.lengths[b], 0), T_) : T_;
-    const int order = blockIdx.z, tail = (int)a.plan.tail((len + C - 1) / C), seg = kReverse ? tail - order : order;
+    const int order = blockIdx.z, tail = a.plan.tail((len + C - 1) / C), seg = kReverse ? tail - order : order;
     if (kReverse ? seg <= 0 : seg >= tail) return;      // no segment that it would be handed to
-    const int first = (int)a.plan.first(seg), live = min((int)a.plan.first(seg + 1), (len + C - 1) / C);
+    const int first = a.plan.first(seg), live = min(a.plan.first(seg + 1), (len + C - 1) / C);
     const int count = live - first, step = kReverse ? -1 : 1, start = kReverse ? live - 1 : first;
     const T *X = static_cast<const T *>(a.keys.p) + b * a.keys.sb + hk * a.keys.sh + (int64_t)start * C * a.keys.st;
     const T *Y = static_cast<const T *>(a.values.p) + b * a.values.sb + h * a.values.sh + dv0 + (int64_t)start * C * a.values.st;
     const float *G = static_cast<const float *>(a.gates.p) + b * a.gates.sb + h * a.gates.sh;
     const TileX tx;
     const TileY ty;
+
+    if (w == NW) {
+        auto gate = [&](int i) {
+            const int n = start + i * step;
+            return i < count && lane < C && lane < len - n * C ? G[(int64_t)(n * C + lane) * a.gates.st] : 0.f;
+        };
+        float even = gate(0), odd = gate(1);
+        double total = chunk_gates<C>(gates[0], even);
+        even = gate(2);
+        lds_barrier();
+        for (int i = 0; i < count; ++i) {
+            if (i + 1 < count) total += chunk_gates<C>(gates[(i + 1) & 1], odd);
+            odd = even;
+            even = gate(i + 3);
+            lds_barrier();
+        }
+        if (blockIdx.y == 0 && lane == 0) a.decays[bh * a.plan.segments + order] = fast_exp2((float)total);
+        return;
+    }
 
     // key features 16t + 4c .., value feature 16w + r
     f32x4 S[TILES];
@@ -502,17 +525,14 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DKP == 
     struct Flight {
         RowsInFlight<T, C, DKP, NT> x;
         RowsInFlight<T, C, DVS, NT> y;
-        float g;
     } even, odd;
     const int x_st = (int)a.keys.st, y_st = (int)a.values.st;
-    double total = 0.0;
     auto fetch = [&](Flight &f, int i) {         // chunk i, which the pointers have come to
         if (i >= count) return;
         const int n = start + i * step, left = len - n * C;
         const unsigned at = f.x.here();
         f.x.load(at, X, x_st, left, DK);
         f.y.load(at, Y, y_st, left, DV - dv0);
-        f.g = w == NW - 1 && lane < C && lane < left ? G[(int64_t)(n * C + lane) * a.gates.st] : 0.f;
         X += (int64_t)(step * C) * x_st;
         Y += (int64_t)(step * C) * y_st;
     };
@@ -522,7 +542,6 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DKP == 
         const unsigned at = f.x.here();
         f.x.store(at, sX + chunk, left, DK);
         f.y.store(at, sY + chunk, left, DV - dv0);
-        if (w == NW - 1) total += chunk_gates<C>(gates[i & 1], f.g);
     };
     auto add = [&](int i) {
         const ChunkGates<C> &gate = gates[i & 1];
@@ -568,7 +587,6 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DKP == 
     f32x4 *to = reinterpret_cast<f32x4 *>(a.entering + ((bh * a.plan.segments + order) * gridDim.y + blockIdx.y) * (int64_t)(DKP * DVS)) + w * TILES * 64 + lane;
 #pragma unroll
     for (int t = 0; t < TILES; ++t) to[t * 64] = S[t];
-    if (blockIdx.y == 0 && tid == NT - 1) a.decays[bh * a.plan.segments + order] = fast_exp2((float)total);
 }
 
 // The states that enter segments 2, 3, ... from what each segment adds, in place: slot s holds the state after segment s (of cotangents,
@@ -580,7 +598,7 @@ __global__ __launch_bounds__(256) void decay_scan_kernel(float *__restrict__ ent
 {
     const int64_t at = blockIdx.x * (int64_t)256 + threadIdx.x, bh = blockIdx.y, segments = plan.segments;
     if (at >= count) return;
-    const int64_t len = lengths ? min(max((int64_t)lengths[bh / n.H], (int64_t)0), n.T) : n.T, tail = plan.tail((len + C - 1) / C);
+    const int T = (int)n.T, len = lengths ? min(max(lengths[blockIdx.y / (unsigned)n.H], 0), T) : T, tail = plan.tail((len + C - 1) / C);
     float *p = entering + bh * segments * count + at;
     const float *d = decays + bh * segments;
     float s = p[0];
@@ -598,7 +616,7 @@ template <typename T, int DKP, int NW, bool kReverse> int launch_states(hipStrea
     constexpr size_t lds = sizeof(T) * 2 * C * (LdsTile<T, DKP>::kRow + LdsTile<T, 16 * NW>::kRow) + 2 * sizeof(ChunkGates<C>);
     if (int e = allow_lds(grant, reinterpret_cast<const void *>(decay_states_kernel<T, DKP, NW, kReverse>), lds)) return e;
     const dim3 grid(a.n.B * a.n.H, decay_slabs(a.n.DV), a.plan.segments - 1);
-    decay_states_kernel<T, DKP, NW, kReverse><<<grid, NW * 64, lds, stream>>>(a);
+    decay_states_kernel<T, DKP, NW, kReverse><<<grid, NW * 64 + 64, lds, stream>>>(a);
     return launch_status();
 }
 template <typename T, bool kReverse> int dispatch_states(hipStream_t stream, const ForwardArgs &a)
