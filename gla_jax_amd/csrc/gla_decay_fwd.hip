@@ -18,7 +18,8 @@ struct ForwardArgs {
 };
 
 // The state before chunk n, which the gradients need: tiles of 16 x 16 as a wave of decay_gradient_kernel takes them, lane 16c + r key
-// feature r and value features 4c .. 4c+3.
+// feature r and value features 4c .. 4c+3.  (Four bytes a lane in the order of the rows, without the exchange between lanes, took 56 us of the
+// forward pass instead of 52 at B4 T4096 H6 D128, and 88 instead of 84 of the gradients.)
 template <int DKP, int TILES = DKP / 16>
 __device__ __forceinline__ void keep_states(const ForwardArgs &a, const f32x4 (&S)[TILES], int64_t bh, int64_t n, int column, bool mine)
 {
@@ -38,7 +39,8 @@ __device__ __forceinline__ void keep_states(const ForwardArgs &a, const f32x4 (&
 // state, TILES accumulators of 16 key features each.  Scores are formed transposed, so that a lane holds four neighbouring
 // keys of one query, and kept in `T`: their one rounding adds as much as that of out itself.  The state is an operand in `T`
 // too where it meets the queries; what it accumulates comes from values scaled in 32 bits and handed over in three parts,
-// since hidden_final is a 32-bit result.
+// since hidden_final is a 32-bit result.  Half of a chunk's cycles are the vector instructions' (a wave's 520, 16 of them conversions of S and
+// 120 the split of the values); two workgroups a compute unit fill the rest.
 template <typename T, int DKP, int NW>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DKP == 256 ? 2 : DKP == 128 && NW == 4 ? 3 : 4))) void decay_pass_kernel(const ForwardArgs a)
 {
@@ -246,7 +248,9 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DKP == 
 
 // The forward pass for up to 128 key features: the work of decay_pass_kernel, by two kinds of waves.  The first NW carry the state, 16
 // value columns each, and make out.  The others bring the chunk after the next one from memory to LDS and form the next one's scores
-// meanwhile: three chunks' rows and two chunks' scores in LDS, and one barrier a chunk.
+// meanwhile: three chunks' rows and two chunks' scores in LDS, and one barrier a chunk.  A chunk takes 6400 cycles so, where one kind of
+// waves with three barriers took 9800; of the 6400 a SIMD issues vector and matrix instructions in 3800.  B1 T32768 H8 D128: 67 us for
+// 268 MB, 4.0 TB/s, of the 5.2 that a copy reaches.
 template <typename T, int DKP, int NW>
 __global__ __launch_bounds__(NW * 128) __attribute__((amdgpu_waves_per_eu(DKP == 128 && NW == 4 ? 2 : 4))) void decay_forward_kernel(const ForwardArgs a)
 {
@@ -458,7 +462,7 @@ __global__ __launch_bounds__(NW * 128) __attribute__((amdgpu_waves_per_eu(DKP ==
 // What a segment adds to the state that leaves it (cotangents: the chunks in reverse, queries for keys and cotangents of out for values),
 // and how much of the state that entered it is left.  Two chunks' rows in LDS, one barrier a chunk; rows are on their way for two
 // chunks, since a chunk takes less time than memory does.  A wave of its own makes the gates: 600 of a chunk's 4400 cycles, for which the
-// others had to wait.
+// others had to wait.  B1 T32768 H8 D128: 41 us for 130 MB, 3.2 TB/s: two waves a SIMD, whose vector and matrix instructions overlap little.
 template <typename T, int DKP, int NW, bool kReverse>
 __global__ __launch_bounds__(NW * 64 + 64) __attribute__((amdgpu_waves_per_eu(DKP == 256 && NW == 4 ? 2 : 3))) void decay_states_kernel(const ForwardArgs a)
 {
@@ -591,7 +595,7 @@ __global__ __launch_bounds__(NW * 64 + 64) __attribute__((amdgpu_waves_per_eu(DK
 
 // The states that enter segments 2, 3, ... from what each segment adds, in place: slot s holds the state after segment s (of cotangents,
 // after the s-th from the sequence's end).
-// One value a thread: four would make wider accesses of it, but B1 T32768 H8 D128 then has 128 workgroups (20 us).
+// One value a thread: four would make wider accesses of it and a quarter of the workgroups (B1 T32768 H8 D128, 32 segments: 12.5 us).
 __global__ __launch_bounds__(256) void decay_scan_kernel(float *__restrict__ entering, const float *__restrict__ decays,
                                                          const int32_t *__restrict__ lengths, DecaySizes n, DecayPlan plan, int C,
                                                          int64_t count)
