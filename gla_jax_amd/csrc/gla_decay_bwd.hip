@@ -490,8 +490,19 @@ __global__ __launch_bounds__(((DKW > DVW ? DKW : DVW) + DKW) * 4) void decay_gra
     }
 }
 
-// dst = the sum of `parts` arrays of n floats behind each other, rounded once.
-template <typename T> __global__ __launch_bounds__(256) void decay_sum_parts_kernel(const float *__restrict__ src, int parts, int64_t n, T *__restrict__ dst)
+// An array as the sum of `parts` arrays of n floats behind each other, rounded once; all of a call's in one launch.
+struct PartSum {
+    const float *src;
+    void *dst;
+    int64_t n;
+    int parts;
+    bool floats;                                 // dst is float, else T
+};
+struct PartSums {
+    PartSum of[4];
+    int count;
+};
+template <typename T> __device__ void sum_parts_of(const float *__restrict__ src, int parts, int64_t n, T *__restrict__ dst)
 {
     for (int64_t i = 4 * (blockIdx.x * (int64_t)256 + threadIdx.x); i < n; i += 1024 * (int64_t)gridDim.x) {
         if (i + 4 <= n) {
@@ -511,6 +522,12 @@ template <typename T> __global__ __launch_bounds__(256) void decay_sum_parts_ker
             }
         }
     }
+}
+template <typename T> __global__ __launch_bounds__(256) void decay_sum_parts_kernel(const PartSums a)
+{
+    const PartSum &s = a.of[blockIdx.y];
+    if (s.floats) sum_parts_of(s.src, s.parts, s.n, static_cast<float *>(s.dst));
+    else sum_parts_of(s.src, s.parts, s.n, static_cast<T *>(s.dst));
 }
 
 // The gradient of one constant a head: the sum over parts, batch and segments, by one wave a head.
@@ -542,13 +559,6 @@ template <typename T> int dispatch_gradient(hipStream_t stream, const BackwardAr
 {
     if (a.n.DK <= 64) return a.n.DV <= 64 ? launch_gradient<T, 64, 64>(stream, a) : launch_gradient<T, 64, 128>(stream, a);
     return a.n.DV <= 64 ? launch_gradient<T, 128, 64>(stream, a) : launch_gradient<T, 128, 128>(stream, a);
-}
-
-template <typename T> int sum_parts(hipStream_t stream, const float *src, int parts, int64_t n, void *dst)
-{
-    const int64_t blocks = (n + 1023) / 1024;
-    decay_sum_parts_kernel<T><<<(unsigned)(blocks < 4096 ? blocks : 4096), 256, 0, stream>>>(src, parts, n, static_cast<T *>(dst));
-    return launch_status();
 }
 
 }  // namespace
@@ -586,15 +596,24 @@ int decay_backward(void *stream, const DecaySizes &n, const DecayPlan &plan, gla
     a.dgate_sums = constant_gates ? parts.gate_sums : nullptr;
     e = dtype == GLA_BF16 ? dispatch_gradient<__bf16>(s, a) : dispatch_gradient<float>(s, a);
     const int64_t nk = n.B * n.T * n.HK * n.DK, nv = n.B * n.T * n.H * n.DV;
-    auto sum = [&](const float *src, int count, int64_t m, void *dst) {
-        if (!e && m) e = dtype == GLA_BF16 ? sum_parts<__bf16>(s, src, count, m, dst) : sum_parts<float>(s, src, count, m, dst);
+    PartSums sums{};
+    int64_t most = 0;
+    auto sum = [&](const float *src, int count, int64_t m, void *dst, bool floats) {
+        if (count < 2 || m < 1) return;
+        sums.of[sums.count++] = PartSum{src, dst, m, count, floats};
+        most = most < m ? m : most;
     };
-    if (parts.rows > 1) {
-        sum(parts.dquery, parts.rows, nk, dquery);
-        sum(parts.dkey, parts.rows, nk, dkey);
+    sum(parts.dquery, parts.rows, nk, dquery, false);
+    sum(parts.dkey, parts.rows, nk, dkey, false);
+    sum(parts.dvalue, parts.values, nv, dvalue, false);
+    if (!constant_gates) sum(parts.dgate, parts.gates, n.B * n.T * n.H, dlog_decay, true);
+    if (!e && sums.count) {
+        const int64_t blocks = (most + 1023) / 1024;
+        const dim3 grid((unsigned)(blocks < 4096 ? blocks : 4096), sums.count);
+        if (dtype == GLA_BF16) decay_sum_parts_kernel<__bf16><<<grid, 256, 0, s>>>(sums);
+        else decay_sum_parts_kernel<float><<<grid, 256, 0, s>>>(sums);
+        e = launch_status();
     }
-    if (parts.values > 1) sum(parts.dvalue, parts.values, nv, dvalue);
-    if (!e && !constant_gates && parts.gates > 1 && n.T) e = sum_parts<float>(s, parts.dgate, parts.gates, n.B * n.T * n.H, dlog_decay);
     if (!e && constant_gates) {
         decay_sum_gates_kernel<<<n.H, 64, 0, s>>>(parts.gate_sums, parts.gates, n.H, n.B * plan.segments, dlog_decay);
         e = launch_status();
