@@ -168,4 +168,4 @@ def test_sizes_of_what_the_forward_leaves():
     assert lib.gla_decay_states_bytes(2, 0, 4, 2, 32, 48, BF16) == 0
     # sequences enough to fill the GPU run whole, few long ones as segments
     assert lib.gla_decay_fwd_workspace_bytes(64, 4096, 8, 8, 64, 64, BF16, 0) == 0
-    assert lib.gla_decay_fwd_workspace_bytes(1, 32768, 8, 8, 128, 128, BF16, 0) >= 8 * 64 * 128 * 128 * 4
+    assert lib.gla_decay_fwd_workspace_bytes(1, 32768, 8, 8, 128, 128, BF16, 0) >= 8 * 32 * 128 * 128 * 4
