@@ -79,7 +79,7 @@ template <int WAVES> __device__ __forceinline__ u64 select_bound(SelectLds<WAVES
 
 // EACH values a thread, in pieces of 16 bytes, which rows that do not begin on 16 bytes read one by one: the sums come out the same.
 template <typename T, int EACH, bool PIECES>
-__global__ __launch_bounds__(kThreads) void beam_stretch_kernel(const SelectArgs a)
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(PIECES ? 4 : 2))) void beam_stretch_kernel(const SelectArgs a)
 {
     constexpr int kWaves = kThreads / 64, VEC = 16 / sizeof(T);
     __shared__ SelectLds<kWaves> lds;
@@ -90,22 +90,27 @@ __global__ __launch_bounds__(kThreads) void beam_stretch_kernel(const SelectArgs
     if (a.finished && a.finished[row]) return;   // its one candidate is made later
     const T *x = static_cast<const T *>(a.logits) + row * a.row + first;
     const int there = (int)min(a.vocab - first, (int64_t)(kThreads * EACH));
-    float v[EACH];
+    // Every load is issued before the first is used, and none is under a condition (a wait for memory would follow each): what lies behind the
+    // row's end reads its last values and counts as -inf.
+    T raw[EACH];
 #pragma unroll
     for (int i = 0; i < EACH; i += VEC) {
         const int at = (i / VEC) * (kThreads * VEC) + tid * VEC;
-        float t[VEC];
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) t[e] = -INFINITY;
         if constexpr (PIECES) {
-            if (at < there) load_vec<T, VEC>(x + at, t);              // VEC divides what is there
+            typedef T Piece __attribute__((ext_vector_type(VEC)));
+            const Piece t = *reinterpret_cast<const Piece *>(x + min(at, there - VEC));      // (VEC divides what is there)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) raw[i + e] = t[e];
         } else {
 #pragma unroll
-            for (int e = 0; e < VEC; ++e)
-                if (at + e < there) t[e] = (float)x[at + e];
+            for (int e = 0; e < VEC; ++e) raw[i + e] = x[min(at + e, there - 1)];
         }
+    }
+    float v[EACH];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) v[i + e] = t[e] != t[e] ? -INFINITY : t[e];
+    for (int i = 0; i < EACH; ++i) {
+        const float t = (float)raw[i];
+        v[i] = t == t && (i / VEC) * (kThreads * VEC) + tid * VEC + i % VEC < there ? t : -INFINITY;
     }
     auto place = [&](int i) { return (i / VEC) * (kThreads * VEC) + tid * VEC + i % VEC; };
     // of equal values the first: a thread's places ascend

@@ -41,7 +41,24 @@ __device__ __forceinline__ int64_t slot_of(const StepArgs &a, int64_t i)
 template <typename T, typename HT, int DKP> struct StepState {
     static constexpr int VEC = 16 / sizeof(HT), LPR = 32 / VEC, SIDE = 64 / LPR, PER = DKP / SIDE;
     typedef HT Piece __attribute__((ext_vector_type(VEC)));
+    typedef T Four __attribute__((ext_vector_type(4)));
     Piece x[PER];
+    Four k[PER / 4], q[PER / 4], v[VEC / 4];
+    float log_decay;
+    // The token's rows, before the state: it takes longer, and in the beams' case it is not yet known where it lies.  No load is under a
+    // condition, after which memory would be waited for; what does not exist reads what does, and counts as zero later.
+    __device__ __forceinline__ void load_rows(const T *key, const T *query, const T *value, const float *gate, int DK, int DV, int row0, int col)
+    {
+#pragma unroll
+        for (int i = 0; i < PER; i += 4) {
+            const int at = row0 + i < DK ? row0 + i : 0;
+            k[i / 4] = *reinterpret_cast<const Four *>(key + at);
+            q[i / 4] = *reinterpret_cast<const Four *>(query + at);
+        }
+#pragma unroll
+        for (int e = 0; e < VEC; e += 4) v[e / 4] = *reinterpret_cast<const Four *>(value + (col < DV ? col : 0) + e);
+        log_decay = *gate;
+    }
     __device__ __forceinline__ void load(const HT *state, int DK, int DV, int row0, int col)
     {
 #pragma unroll
@@ -52,35 +69,24 @@ template <typename T, typename HT, int DKP> struct StepState {
     }
     // The token's update, and its output for the lane's columns (zeros outside): the sum runs over the key features in 32 bits
     // from the state before it is rounded.
-    __device__ __forceinline__ void step(HT *state, float decay, const T *k, const T *q, const T *v, T *out, int DK, int DV, int row0, int col)
+    __device__ __forceinline__ void step(HT *state, T *out, int DK, int DV, int row0, int col)
     {
-        float kv[PER], qv[PER], vv[VEC], o[VEC];
+        const float decay = expf(log_decay);
+        float vv[VEC], o[VEC];
 #pragma unroll
-        for (int i = 0; i < PER; ++i) kv[i] = qv[i] = 0.f;
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) vv[e] = o[e] = 0.f;
-        if (row0 < DK) {                          // 16 divides DK: a lane's rows exist or do not, in pieces of PER <= 16
-#pragma unroll
-            for (int i = 0; i < PER; i += 4) {
-                if (row0 + i < DK) {
-                    float t[4];
-                    load_vec<T, 4>(k + row0 + i, t);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) kv[i + e] = t[e];
-                    load_vec<T, 4>(q + row0 + i, t);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) qv[i + e] = t[e];
-                }
-            }
+        for (int e = 0; e < VEC; ++e) {
+            vv[e] = (float)v[e / 4][e % 4];
+            o[e] = 0.f;
         }
-        if (col < DV) load_vec<T, VEC>(v + col, vv);
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
+            // (4 divides DK: four rows exist or do not)
+            const float ki = row0 + i < DK ? (float)k[i / 4][i % 4] : 0.f, qi = row0 + i < DK ? (float)q[i / 4][i % 4] : 0.f;
             float s[VEC];
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
-                s[e] = decay * (float)x[i][e] + kv[i] * vv[e];
-                o[e] += qv[i] * s[e];
+                s[e] = decay * (float)x[i][e] + ki * vv[e];
+                o[e] += qi * s[e];
             }
             if (row0 + i < DK && col < DV) store_vec<HT, VEC>(state + (int64_t)(row0 + i) * DV + col, s);
         }
@@ -97,9 +103,13 @@ __global__ __launch_bounds__(256) void decay_step_kernel(const StepArgs a)
 {
     typedef StepState<T, HT, DKP> State;
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, waves = blockDim.x >> 6;
-    const int64_t b = blockIdx.x / a.H, h = blockIdx.x % a.H, hk = h / (a.H / a.HK);
+    const unsigned H = (unsigned)a.H;
+    const int64_t b = blockIdx.x / H, h = blockIdx.x % H, hk = blockIdx.x % H / (H / (unsigned)a.HK);
     const int DK = (int)a.DK, DV = (int)a.DV, col = 32 * (blockIdx.y * waves + w) + State::VEC * (lane % State::LPR),
               row0 = State::PER * (lane / State::LPR);
+    State s;
+    s.load_rows(static_cast<const T *>(a.key) + b * a.key_b + hk * a.key_h, static_cast<const T *>(a.query) + b * a.query_b + hk * a.query_h,
+                static_cast<const T *>(a.value) + b * a.value_b + h * a.value_h, a.log_decay + b * a.gates_b + h * a.gates_h, DK, DV, row0, col);
     const int64_t slot = slot_of(a, b);
     T *out = static_cast<T *>(a.out) + (b * a.H + h) * DV;
     if (slot < 0) {                               // a row without a state
@@ -108,11 +118,8 @@ __global__ __launch_bounds__(256) void decay_step_kernel(const StepArgs a)
         return;
     }
     HT *state = static_cast<HT *>(a.states) + (slot * a.H + h) * DK * DV;
-    State s;
     s.load(state, DK, DV, row0, col);
-    s.step(state, expf(a.log_decay[b * a.gates_b + h * a.gates_h]), static_cast<const T *>(a.key) + b * a.key_b + hk * a.key_h,
-           static_cast<const T *>(a.query) + b * a.query_b + hk * a.query_h,
-           static_cast<const T *>(a.value) + b * a.value_b + h * a.value_h, out, DK, DV, row0, col);
+    s.step(state, out, DK, DV, row0, col);
 }
 
 // The waves that hold their part of a state in registers: 16 of 128 registers, 8 of 256.
@@ -126,15 +133,18 @@ __global__ __launch_bounds__(64 * waves_of_beams(DKP)) void decay_step_beams_ker
 {
     typedef StepState<T, HT, DKP> State;
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const int64_t group = blockIdx.x / a.H, h = blockIdx.x % a.H, hk = h / (a.H / a.HK), b = group * a.beams + w;
+    const unsigned H = (unsigned)a.H;
+    const int64_t group = blockIdx.x / H, h = blockIdx.x % H, hk = blockIdx.x % H / (H / (unsigned)a.HK), b = group * a.beams + w;
     const int DK = (int)a.DK, DV = (int)a.DV, col = 32 * blockIdx.y + State::VEC * (lane % State::LPR),
               row0 = State::PER * (lane / State::LPR);
+    State s;
+    s.load_rows(static_cast<const T *>(a.key) + b * a.key_b + hk * a.key_h, static_cast<const T *>(a.query) + b * a.query_b + hk * a.query_h,
+                static_cast<const T *>(a.value) + b * a.value_b + h * a.value_h, a.log_decay + b * a.gates_b + h * a.gates_h, DK, DV, row0, col);
     const int64_t parent = a.parents.at(b), source = parent >= 0 && parent < a.beams ? group * a.beams + parent : b;
     const int64_t slot = slot_of(a, b);
     int64_t from = slot_of(a, source);
     if (from < 0) from = slot;
     T *out = static_cast<T *>(a.out) + (b * a.H + h) * DV;
-    State s;
     if (slot >= 0) s.load(static_cast<const HT *>(a.states) + (from * a.H + h) * DK * DV, DK, DV, row0, col);
     // the loads have to be back, not only issued, before another wave's stores may follow
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -144,9 +154,7 @@ __global__ __launch_bounds__(64 * waves_of_beams(DKP)) void decay_step_beams_ker
         if (lane < State::LPR && col < DV) store_vec<T, State::VEC>(out + col, zero);
         return;
     }
-    s.step(static_cast<HT *>(a.states) + (slot * a.H + h) * DK * DV, expf(a.log_decay[b * a.gates_b + h * a.gates_h]),
-           static_cast<const T *>(a.key) + b * a.key_b + hk * a.key_h, static_cast<const T *>(a.query) + b * a.query_b + hk * a.query_h,
-           static_cast<const T *>(a.value) + b * a.value_b + h * a.value_h, out, DK, DV, row0, col);
+    s.step(static_cast<HT *>(a.states) + (slot * a.H + h) * DK * DV, out, DK, DV, row0, col);
 }
 
 template <typename T, typename HT, int DKP> int launch_step(hipStream_t stream, const StepArgs &a)
