@@ -108,10 +108,11 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(PIECES
     }
     float v[EACH];
 #pragma unroll
-    for (int i = 0; i < EACH; ++i) {
-        const float t = (float)raw[i];
-        v[i] = t == t && (i / VEC) * (kThreads * VEC) + tid * VEC + i % VEC < there ? t : -INFINITY;
-    }
+    for (int i = 0; i < EACH; ++i) v[i] = fmaxf((float)raw[i], -INFINITY);      // (of a NaN and a number the number)
+    if (there < kThreads * EACH)
+#pragma unroll
+        for (int i = 0; i < EACH; ++i)
+            if ((i / VEC) * (kThreads * VEC) + tid * VEC + i % VEC >= there) v[i] = -INFINITY;
     auto place = [&](int i) { return (i / VEC) * (kThreads * VEC) + tid * VEC + i % VEC; };
     // of equal values the first: a thread's places ascend
     float most = v[0];
