@@ -187,36 +187,44 @@ struct ReorderArgs {
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 template <typename P, int WMAX> __global__ __launch_bounds__(256) void reorder_states_kernel(const ReorderArgs a)
 {
+    // lane w of every wave reads beam w's indices, all at once, and hands them round
     const int64_t group = blockIdx.x / a.blocks, at = blockIdx.x % a.blocks * 256 + threadIdx.x, first = group * a.beams;
-    if (at >= a.pieces) return;
-    P *states = static_cast<P *>(a.states) + at;
-    auto row = [&](int64_t i) {
-        const int64_t s = a.slots.p ? a.slots.at(i) : i;
-        return s >= 0 && s < a.pool ? s : -1;
+    const int lane = threadIdx.x & 63;
+    int64_t slot = -1, parent = lane;
+    if (lane < a.beams) {
+        parent = a.parents.at(first + lane);
+        slot = a.slots.p ? a.slots.at(first + lane) : first + lane;
+    }
+    if (slot < 0 || slot >= a.pool) slot = -1;
+    const int source = parent >= 0 && parent < a.beams ? (int)parent : lane, low = (int)slot, high = (int)(slot >> 32);
+    // (no thread leaves before: what a lane hands round it has to have formed)
+    const bool mine = at < a.pieces;
+    P *states = static_cast<P *>(a.states);
+    auto row = [&](int w) {
+        return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane(high, w) << 32 | (uint32_t)__builtin_amdgcn_readlane(low, w));
     };
+    // every load is issued before the first store; a beam that moves nothing has its wave read one piece of the pool's beginning
     P x[WMAX];
     int64_t to[WMAX];
 #pragma unroll
     for (int w = 0; w < WMAX; ++w) {
-        to[w] = -1;
-        if (w < a.beams) {
-            const int64_t parent = a.parents.at(first + w);
-            if (parent >= 0 && parent < a.beams && parent != w) {
-                const int64_t from = row(first + parent);
-                if (from >= 0 && (to[w] = row(first + w)) >= 0) x[w] = states[from * a.pieces];
-            }
-        }
+        const int from = __builtin_amdgcn_readlane(source, w);
+        const int64_t s = row(from), d = row(w);
+        const bool moves = w < a.beams && from != w && s >= 0 && d >= 0;
+        to[w] = moves ? d : -1;
+        x[w] = states[moves && mine ? s * a.pieces + at : 0];
     }
 #pragma unroll
     for (int w = 0; w < WMAX; ++w)
-        if (to[w] >= 0) states[to[w] * a.pieces] = x[w];
+        if (mine && to[w] >= 0) states[to[w] * a.pieces + at] = x[w];
 }
 template <typename P> int launch_reorder(hipStream_t stream, const ReorderArgs &a, int64_t groups)
 {
     const dim3 grid(a.blocks * groups);
     if (a.beams <= 4) reorder_states_kernel<P, 4><<<grid, 256, 0, stream>>>(a);
     else if (a.beams <= 16) reorder_states_kernel<P, 16><<<grid, 256, 0, stream>>>(a);
-    else reorder_states_kernel<P, 64><<<grid, 256, 0, stream>>>(a);
+    else if constexpr (sizeof(P) < 16) reorder_states_kernel<P, 64><<<grid, 256, 0, stream>>>(a);
+    else return GLA_ERR_SHAPE;                   // (64 pieces of 16 bytes a thread do not fit its registers: the caller takes smaller ones)
     return launch_status();
 }
 
