@@ -4,8 +4,8 @@
 // logits are read once: every workgroup takes a stretch of a row, leaves its largest value, its sum of exponentials and its
 // `num` largest logits; a workgroup a search then joins the sums, scores what is left and takes the best `num` of all beams.
 // Everything compared is one 64-bit key, the value above and the inverted place below: keys are unique and equal values come in
-// the order of their places.  16 searches of 8 beams over 131072 bfloat16 logits: 18 us for the stretches' 33.5 MB (all of them begin together: first
-// memory is waited for, then 64 exponentials a thread and the bound) and 6.5 for the join, a chain of dependent steps.
+// the order of their places.  16 searches of 8 beams over 131072 bfloat16 logits: 14.5 us for the stretches' 33.5 MB (all of them begin together: first
+// memory is waited for, then come 64 exponentials a thread and the bound) and 6.5 for the join, a chain of dependent steps.
 #include "gla_common.hpp"
 
 namespace gla {
@@ -173,7 +173,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(PIECES
 }
 
 // One workgroup a search.  1024 threads hold 4096 candidates; up to 1024 take a quarter of them, whose waves need not share a SIMD's time where all
-// compare names (1 search of 4 beams over 32000: 4.6 us instead of 6.0; 16 of 8 over 131072: 6.4 instead of 7.0).
+// compare names (1 search of 4 beams over 32000, both kernels: 8.9 us instead of 10.5; 32 of them 12.4 instead of 14.0; 8192 candidates with a quarter of them 38.8
+// instead of 19.2).
 template <int THREADS> __global__ __launch_bounds__(THREADS) void beam_join_kernel(const SelectArgs a)
 {
     constexpr int kWaves = THREADS / 64, kRoom = 2048;
@@ -281,17 +282,17 @@ template <int THREADS> __global__ __launch_bounds__(THREADS) void beam_join_kern
     }
 }
 
-// Values a thread: 16, and 64 where that still makes enough workgroups.  Finding a stretch's bound takes as long as reading 50 values a
-// thread: 16 searches of 8 beams over 131072 tokens take 25 us with 16 and 18 with 64; one of 4 over 32000 would wait for
-// 8 workgroups instead of 32.
-constexpr int kFew = 16, kMany = 64;
-int each_of(int64_t rows, int64_t vocab) { return rows * vocab >= (int64_t)512 * kThreads * kMany ? kMany : kFew; }
-int64_t splits_of(int64_t rows, int64_t vocab)
-{
-    const int64_t stretch = (int64_t)kThreads * each_of(rows, vocab);
-    return (vocab + stretch - 1) / stretch;
-}
 int64_t per_of(int64_t vocab, int64_t num) { return num < vocab ? num : vocab; }
+// Values a thread: 16, and 64 where that still makes enough workgroups, or where 16 left a search's join more than its threads hold.
+// Finding a stretch's bound takes as long as reading 50 values a thread: 16 searches of 8 beams over 131072 tokens take 25.6 us with 16 and 20.4 with 64,
+// and one of 16 beams 19.2 (8192 candidates for the join) and 15.8; one of 4 over 32000 has 32 workgroups with 16 and 8 with 64: 8.9 and 11.3.
+constexpr int kFew = 16, kMany = 64;
+int64_t stretches(int64_t vocab, int each) { return (vocab + (int64_t)kThreads * each - 1) / ((int64_t)kThreads * each); }
+int each_of(int64_t groups, int64_t beams, int64_t vocab, int64_t num)
+{
+    return groups * beams * vocab >= (int64_t)512 * kThreads * kMany || beams * stretches(vocab, kFew) * per_of(vocab, num) > kHeld * 1024 ? kMany : kFew;
+}
+int64_t splits_of(int64_t groups, int64_t beams, int64_t vocab, int64_t num) { return stretches(vocab, each_of(groups, beams, vocab, num)); }
 
 bool sizes_ok(int64_t groups, int64_t beams, int64_t vocab, int64_t num)
 {
@@ -307,7 +308,7 @@ using namespace gla;
 extern "C" size_t gla_beam_select_workspace_bytes(int64_t groups, int64_t beams, int64_t vocab, int64_t num)
 {
     if (!sizes_ok(groups, beams, vocab, num)) return 0;
-    const int64_t stretches = groups * beams * splits_of(groups * beams, vocab);
+    const int64_t stretches = groups * beams * splits_of(groups, beams, vocab, num);
     return (size_t)(stretches * (per_of(vocab, num) * 8 + 8));
 }
 
@@ -332,7 +333,7 @@ extern "C" int gla_beam_select(void *stream, int64_t groups, int64_t beams, int6
     a.row = row;
     a.num = (int)num;
     a.per = (int)per_of(vocab, num);
-    a.splits = splits_of(groups * beams, vocab);
+    a.splits = splits_of(groups, beams, vocab, num);
     a.logits = logits;
     a.scores = scores;
     a.finished = static_cast<const uint8_t *>(finished);
@@ -347,12 +348,12 @@ extern "C" int gla_beam_select(void *stream, int64_t groups, int64_t beams, int6
     const hipStream_t s = static_cast<hipStream_t>(stream);
     const dim3 grid(a.splits, groups * beams);
     const bool pieces = aligned16(logits) && row * size % 16 == 0 && vocab * size % 16 == 0;
-    const bool many = each_of(groups * beams, vocab) == kMany;
+    const bool many = each_of(groups, beams, vocab, num) == kMany;
     const auto kernel = dtype == GLA_BF16 ? pieces ? many ? beam_stretch_kernel<__bf16, kMany, true> : beam_stretch_kernel<__bf16, kFew, true>
                                                    : many ? beam_stretch_kernel<__bf16, kMany, false> : beam_stretch_kernel<__bf16, kFew, false>
                                           : pieces ? many ? beam_stretch_kernel<float, kMany, true> : beam_stretch_kernel<float, kFew, true>
                                                    : many ? beam_stretch_kernel<float, kMany, false> : beam_stretch_kernel<float, kFew, false>;
-    const size_t room = (size_t)kThreads / 64 * each_of(groups * beams, vocab) * a.per * sizeof(u64);
+    const size_t room = (size_t)kThreads / 64 * each_of(groups, beams, vocab, num) * a.per * sizeof(u64);
     static LdsGrant grants[8];
     const size_t most = many ? (size_t)kThreads / 64 * kMany * GLA_MOST_CANDIDATES * sizeof(u64) : room;      // granted once, for any num
     if (int e = allow_lds(grants[(dtype == GLA_BF16) * 4 + pieces * 2 + many], reinterpret_cast<const void *>(kernel), most)) return e;

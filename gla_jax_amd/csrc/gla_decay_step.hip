@@ -4,7 +4,7 @@
 // A wave takes 32 value columns of one state: a lane holds a piece of 16 bytes of each of DKP / (rows side by side) rows, all
 // of them requested before the first is used.  A lane's rows follow each other, so that it reads its keys and queries in
 // whole pieces; the lanes that hold the same columns are summed at the end.  Nothing goes through LDS.  128 rows of 16 heads of 128 x 128
-// float states: 55 us for 270 MB, 4.9 TB/s.
+// float states: 51 us for 270 MB, 5.3 TB/s.
 #include "gla_common.hpp"
 
 namespace gla {
@@ -127,7 +127,7 @@ constexpr int waves_of_beams(int DK) { return DK <= 128 ? 16 : 8; }
 
 // The same for a group of beams, each from the state of the beam that it continues: a wave a beam, all of a group in one
 // workgroup, which has read every state (of these columns) before it writes the first.  16 groups of 8 beams, 16 heads of 64 x 64 bfloat16:
-// 8.5 us for 35 MB, 4.1 TB/s.
+// 7.7 us for 35 MB, 4.5 TB/s.
 template <typename T, typename HT, int DKP>
 __global__ __launch_bounds__(64 * waves_of_beams(DKP)) void decay_step_beams_kernel(const StepArgs a)
 {
@@ -163,8 +163,8 @@ template <typename T, typename HT, int DKP> int launch_step(hipStream_t stream, 
     if (a.beams) {
         decay_step_beams_kernel<T, HT, DKP><<<dim3(a.B / a.beams * a.H, cols), a.beams * 64, 0, stream>>>(a);
     } else {
-        // Four waves side by side share the lines of a row (128 rows of 16 heads of 128 x 128: 57 us, each in a workgroup of its own 65); where there
-        // are few, each has a compute unit of its own (4 rows: 4.7 us against 4.9; 16 rows take 8.6 either way).
+        // Four waves side by side share the lines of a row (128 rows of 16 heads of 128 x 128: 51 us, each in a workgroup of its own 57); where there
+        // are few, each has a compute unit of its own (4 rows: 4.3 us against 4.5; 16 rows take 8.0 either way).
         const int waves = a.B * a.H * cols >= 1024 ? (cols < 4 ? (int)cols : 4) : 1;
         decay_step_kernel<T, HT, DKP><<<dim3(a.B * a.H, (cols + waves - 1) / waves), waves * 64, 0, stream>>>(a);
     }
