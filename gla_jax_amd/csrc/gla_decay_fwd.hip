@@ -400,7 +400,7 @@ __global__ __launch_bounds__(NW * 128) __attribute__((amdgpu_waves_per_eu(DKP ==
             Y += (int64_t)C * y_st;
             Q += (int64_t)C * q_st;
         };
-        // chunk i and its gates to their place, the next one on its way
+        // chunk i and its gates to their place
         auto stage = [&](int i, int place) {
             const int n = first + i, chunk = place * kChunk, left = len - n * C;
             const unsigned at = x.here() - NT;
@@ -408,10 +408,12 @@ __global__ __launch_bounds__(NW * 128) __attribute__((amdgpu_waves_per_eu(DKP ==
             x.store(at, sX + chunk, left, DK);
             q.store(at, sQ + chunk, left, DK);
             y.store(at, sY + chunk, left, DV - dv0);
-            if (i + 1 < count) {
-                fetch_gates(n + 1);
-                fetch(n + 1);
-            }
+        };
+        // chunk i on its way
+        auto bring = [&](int i) {
+            if (i >= count) return;
+            fetch_gates(first + i);
+            fetch(first + i);
         };
         auto scores = [&](int i, int place) {
             // transposed: lane (r, c) has keys 4c .. 4c+3 of tile tj for query r of tile ti
@@ -435,17 +437,20 @@ __global__ __launch_bounds__(NW * 128) __attribute__((amdgpu_waves_per_eu(DKP ==
                 store_vec<T, 4>(sP + (i & 1) * kScores + n16 * 256 + 4 * lane, p);
             }
         };
-        fetch_gates(first);
-        fetch(first);
+        bring(0);
         stage(0, 0);
+        bring(1);
         lds_barrier();
         scores(0, 0);
         if (count > 1) stage(1, 1);
+        bring(2);
         lds_barrier();
         int next = 1, after = 2;
         for (int i = 0; i < count; ++i) {
             if (i + 2 < count) stage(i + 2, after);
             if (i + 1 < count) scores(i + 1, next);
+            // (issuing these loads takes 2000 cycles, for which the scores would have to wait: B16 T1337 H16 DK64 DV128 64 us instead of 74)
+            bring(i + 3);
             lds_barrier();
             next = after;
             after = after == 2 ? 0 : after + 1;
