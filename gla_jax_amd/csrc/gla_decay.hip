@@ -10,12 +10,12 @@ constexpr int64_t kMostRow = (int64_t)1 << 23;      // elements from one token t
 int64_t pad256(int64_t x) { return (x + 255) & ~(int64_t)255; }
 
 // Sequences run as segments side by side where that fills the GPU better: one workgroup walks a segment's chunks in order, so B1
-// T32768 H8 D128 as whole sequences would use 8 of 256 compute units (16 segments: 178 us, 32: 119, 64: 133).  A compute unit takes one
+// T32768 H8 D128 as whole sequences would use 8 of 256 compute units (16 segments: 178 us, 32: 115, 64: 133).  A compute unit takes one
 // workgroup at a time here: two at once hardly do more together.  Weighed are, in the time of a chunk, the rounds that `slots` of them take, a
 // workgroup's start, and what segments cost besides: the pass that finds the states entering them (`pass` of the work, on half of the rows)
 // and a state for each to write, scan and read.  A whole number of rounds leaves no compute unit idle, so only the counts that just fill some are looked
 // at; a segment has two chunks at least.  Ragged sequences count as half full, their longest segment as what the others wait for: B16 T1337
-// H16 D128 of lengths 0 to 1337 takes 79 us whole, 111 in two segments and 121 in four.
+// H16 D128 of lengths 0 to 1337 takes 75 us whole, 111 in two segments and 121 in four.
 DecayPlan plan_segments(const DecaySizes &n, gla_dtype dtype, int64_t workgroups, int64_t slots, double pass, bool ragged)
 {
     const int64_t C = dtype == GLA_BF16 ? DecayChunk<__bf16>::C : DecayChunk<float>::C;

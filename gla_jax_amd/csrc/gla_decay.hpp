@@ -58,7 +58,8 @@ template <typename P> __device__ __forceinline__ P *at_bytes(P *base, unsigned b
 // 16 or 32 bytes instead, one of the three had two lanes to a bank, and half of the forward pass's LDS cycles were conflicts.
 // An exclusive or with the tile's or step's number and a constant number of rows makes every address from three numbers a
 // lane.  `here` gives a copy whose addresses are formed where they are used: kept for a whole loop, they took 30 registers of the
-// forward pass and 100 more were spilled.  float data keep rows padded by 32 bytes.
+// forward pass and 100 more were spilled.  float data keep rows padded by 16 bytes, with
+// which three chunks of 128 x 128 features fit (forward pass of B16 T512 H16: 101 us; padded by 32 bytes, two of a chunk at a time, 110).
 template <typename T, int F> struct LdsTile;
 template <int F> struct LdsTile<__bf16, F> {
     static constexpr int kRow = F;
@@ -105,7 +106,7 @@ template <int F> struct LdsTile<__bf16, F> {
     template <typename P> __device__ __forceinline__ P *four(P *p, int t, int u) const { return at_bytes(p + 16 * t * F, at_halves ^ (32 * u)); }
 };
 template <int F> struct LdsTile<float, F> {
-    static constexpr int kRow = F + 8;
+    static constexpr int kRow = F + 4;
     int at_rows, at_halves, at_columns;
     __device__ __forceinline__ LdsTile()
     {

@@ -249,8 +249,8 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DKP == 
 // The forward pass for up to 128 key features: the work of decay_pass_kernel, by two kinds of waves.  The first NW carry the state, 16
 // value columns each, and make out.  The others bring the chunk after the next one from memory to LDS and form the next one's scores
 // meanwhile: three chunks' rows and two chunks' scores in LDS, and one barrier a chunk.  A chunk takes 6400 cycles so, where one kind of
-// waves with three barriers took 9800; of the 6400 a SIMD issues vector and matrix instructions in 3800.  B1 T32768 H8 D128: 67 us for
-// 268 MB, 4.0 TB/s, of the 5.2 that a copy reaches.
+// waves with three barriers took 9800; of the 6400 a SIMD issues vector and matrix instructions in 3800.  B1 T32768 H8 D128: 64 us for
+// 268 MB, 4.2 TB/s, of the 5.2 that a copy reaches.
 template <typename T, int DKP, int NW>
 __global__ __launch_bounds__(NW * 128) __attribute__((amdgpu_waves_per_eu(DKP == 128 && NW == 4 ? 2 : 4))) void decay_forward_kernel(const ForwardArgs a)
 {
@@ -641,8 +641,8 @@ template <typename T, bool kReverse> int dispatch_states(hipStream_t stream, con
 }
 
 // One workgroup of decay_forward_kernel is the fastest that a compute unit can be kept busy with (B16 T1024 H16 D128, 256 workgroups:
-// 76 us, decay_pass_kernel 98), but its LDS and registers leave no room for a second one; where there are more workgroups than compute units,
-// two of decay_pass_kernel at a time do more (64 x 64 features, 512 workgroups: 72 us against 83; 128 x 128: 150 against 153).
+// 72 us, decay_pass_kernel 91), but its LDS and registers leave no room for a second one; where there are more workgroups than compute units,
+// two of decay_pass_kernel at a time do more (64 x 64 features, 512 workgroups: 72 us against 77; 128 x 128: 145 against 148).
 template <typename T, int DKP, int NW> int launch_forward(hipStream_t stream, const ForwardArgs &a)
 {
     constexpr int C = DecayChunk<T>::C;
