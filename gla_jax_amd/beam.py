@@ -72,7 +72,8 @@ def reorder_states(states, parents, slots=None):
     """states[g*W + w] <- states[g*W + parents[g,w]] in place, for every search g and its W beams: the states follow the beams that
     `beam_select` keeps.  `states` [N, ..] is dense, of any element type and shape behind its first axis (the states of chunk_decay and decay_step as
     those of recurrent_gla); `slots` [G,W] says where a beam's state lies when they do not lie in order, one outside 0..N-1 marks a
-    beam without one.  A parent outside 0..W-1 counts as w.  W is at most 64.  Returns `states`."""
+    beam without one.  A parent outside 0..W-1 counts as w.  W is at most 64.  Returns `states`, which count as a new version to autograd, as after
+    any operation in place."""
     if _native("reorder", (states, parents), slots):
         return states
     _check((("states", states), ("parents", parents)), states.device if isinstance(states, torch.Tensor) else None)
@@ -97,4 +98,5 @@ def reorder_states(states, parents, slots=None):
         rc = _lib.load().gla_reorder_states(_stream(), states.shape[0], G, W, states[0].numel() * states.element_size(), wide,
                                             _ptr(parents), _ptr(slots), _ptr(states))
     _lib.check("gla_reorder_states", rc)
+    torch.autograd.graph.increment_version(states)
     return states

@@ -549,6 +549,13 @@ bool takes_gradient(at::ArrayRef<Tensor> arrays)
     return false;
 }
 
+// States that a call has updated in place count as a new version: autograd then refuses to use what it saved of the old one.  (What
+// inference mode makes has no version.)
+void updated(const Tensor &states)
+{
+    if (!states.is_inference()) states.unsafeGetTensorImpl()->bump_version();
+}
+
 std::optional<Tensor> decay_step(const Tensor &states, const Tensor &a, const Tensor &v, const Tensor &k, const Tensor &q,
                                  const std::optional<Tensor> &slots, const std::optional<Tensor> &parents)
 {
@@ -576,6 +583,7 @@ std::optional<Tensor> decay_step(const Tensor &states, const Tensor &a, const Te
                                   (const float *)a.data_ptr(), v.data_ptr(), k.data_ptr(), q.data_ptr(), slots ? slots->data_ptr() : nullptr,
                                   parents ? parents->data_ptr() : nullptr, states.data_ptr(), out.data_ptr());
     check("gla_decay_step", rc);
+    updated(states);
     return out;
 }
 
@@ -630,6 +638,7 @@ bool reorder(const Tensor &states, const Tensor &parents, const std::optional<Te
     const int rc = gla_reorder_states(stream_of(states), N, G, W, states.numel() / N * (int64_t)states.element_size(), type == at::kLong,
                                       parents.data_ptr(), slots ? slots->data_ptr() : nullptr, states.data_ptr());
     check("gla_reorder_states", rc);
+    updated(states);
     return true;
 }
 

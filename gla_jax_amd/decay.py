@@ -245,7 +245,8 @@ def decay_step(states, log_decay, value, key, query, slots=None, parents=None):
     parents[g,w] had before the call (`beam_select` returns them), which saves `reorder_states` its pass.  A parent outside
     0..W-1 counts as w.  W is at most 64.
 
-    States are updated in place: nothing here is differentiable, and arrays that require a gradient are refused."""
+    States are updated in place: nothing here is differentiable, and arrays that require a gradient are refused.  The update counts as a
+    new version of `states`: a backward that has saved them raises instead of using them."""
     done = _native("decay_step", (states, log_decay, value, key, query), slots, parents)
     if done is not None:
         return done
@@ -289,6 +290,7 @@ def decay_step(states, log_decay, value, key, query, slots=None, parents=None):
                                         _strides((a, 2), (v, 2), (k, 2), (q, 2)), _ptr(a), _ptr(v), _ptr(k), _ptr(q), _ptr(slots),
                                         _ptr(parents), _ptr(states), _ptr(out))
     _lib.check("gla_decay_step", rc)
+    torch.autograd.graph.increment_version(states)
     return out
 
 
