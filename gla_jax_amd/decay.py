@@ -234,6 +234,71 @@ def _same_width(*indices):
     return int(wide), [t if t is None or not wide else t.to(torch.int64) for t in indices]
 
 
+def _no_gradient(name):
+    raise RuntimeError(f"{name} has no gradient: call it under torch.no_grad()")
+
+
+def _refuse_gradients(name, *arrays):
+    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in arrays):
+        _no_gradient(name)
+
+
+class _DecayStep(torch.autograd.Function):
+    """decay_step for arrays that are not as the native host side takes them, and under a tracer, which records a Function as a call of
+    it.  So all checks are here, where a recorded call makes them again.  There is no gradient."""
+
+    @staticmethod
+    def forward(states, log_decay, value, key, query, slots, parents):
+        arrays = (("states", states), ("log_decay", log_decay), ("value", value), ("key", key), ("query", query))
+        _check(arrays, states.device if isinstance(states, torch.Tensor) else None)
+        if value.ndim != 3 or key.ndim != 3 or query.shape != key.shape or key.shape[0] != value.shape[0]:
+            raise AssertionError("value must be [B, H, DV], key and query [B, HK, DK]")
+        B, H, DV = value.shape
+        HK, DK = key.shape[1:]
+        _check_heads(value, key, query, HK, H)
+        if states.ndim != 4 or tuple(states.shape[1:]) != (H, DK, DV):
+            raise AssertionError(f"states shape {tuple(states.shape)} != {('N', H, DK, DV)}")
+        if states.dtype not in _DT:
+            raise TypeError("states must be float32 or bfloat16")
+        if not states.is_contiguous() or states.data_ptr() % 16 or DK % 16 or DV % 16:
+            raise AssertionError("states are updated where they lie: dense, on 16 bytes, DK and DV multiples of 16")
+        if tuple(log_decay.shape) not in ((B, H), (H,)):
+            raise AssertionError(f"log_decay shape {tuple(log_decay.shape)} is neither {(B, H)} nor {(H,)}")
+        if slots is None and states.shape[0] < B:
+            raise AssertionError(f"{states.shape[0]} states for {B} rows")
+        if slots is not None:
+            slots = _indices("slots", slots, (B,), states.device)
+        W = 0
+        if parents is not None:
+            if parents.ndim != 2 or parents.shape[0] * parents.shape[1] != B:
+                raise AssertionError(f"parents shape {tuple(parents.shape)} does not hold {B} rows")
+            W = parents.shape[1]
+            if W > _lib.GLA_MOST_BEAMS:
+                raise AssertionError(f"{W} beams: at most {_lib.GLA_MOST_BEAMS} are built")
+            parents = _indices("parents", parents, tuple(parents.shape), states.device)
+        if B == 0 or H == 0 or states.shape[0] == 0:
+            return torch.zeros_like(value)
+        wide, (slots, parents) = _same_width(slots, parents)
+        v, k, q = (_rows(t, value.dtype) for t in (value, key, query))
+        a = log_decay.to(torch.float32).expand(B, H)
+        with torch.cuda.device(states.device):
+            out = torch.empty(B, H, DV, dtype=v.dtype, device=v.device)
+            rc = _lib.load().gla_decay_step(_stream(), states.shape[0], B, H, HK, DK, DV, W, _DT[v.dtype], _DT[states.dtype], wide,
+                                            _strides((a, 2), (v, 2), (k, 2), (q, 2)), _ptr(a), _ptr(v), _ptr(k), _ptr(q), _ptr(slots),
+                                            _ptr(parents), _ptr(states), _ptr(out))
+        _lib.check("gla_decay_step", rc)
+        torch.autograd.graph.increment_version(states)
+        return out
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        pass
+
+    @staticmethod
+    def backward(ctx, *grads):
+        _no_gradient("decay_step")
+
+
 def decay_step(states, log_decay, value, key, query, slots=None, parents=None):
     """One token for each row of a batch: the recurrent form for decoding.  `states` [N,H,DK,DV] (float32 or bfloat16, dense) is
     updated in place and is a pool: row b's state is states[slots[b]] (slots None: states[b]); a slot outside 0..N-1 (-1) marks a row without a
@@ -250,49 +315,9 @@ def decay_step(states, log_decay, value, key, query, slots=None, parents=None):
     done = _native("decay_step", (states, log_decay, value, key, query), slots, parents)
     if done is not None:
         return done
-    arrays = (("states", states), ("log_decay", log_decay), ("value", value), ("key", key), ("query", query))
-    _check(arrays, states.device if isinstance(states, torch.Tensor) else None)
-    if torch.is_grad_enabled() and any(t.requires_grad for _, t in arrays):
-        raise RuntimeError("decay_step updates its states in place and has no gradient: call it under torch.no_grad()")
-    if value.ndim != 3 or key.ndim != 3 or query.shape != key.shape or key.shape[0] != value.shape[0]:
-        raise AssertionError("value must be [B, H, DV], key and query [B, HK, DK]")
-    B, H, DV = value.shape
-    HK, DK = key.shape[1:]
-    _check_heads(value, key, query, HK, H)
-    if states.ndim != 4 or tuple(states.shape[1:]) != (H, DK, DV):
-        raise AssertionError(f"states shape {tuple(states.shape)} != {('N', H, DK, DV)}")
-    if states.dtype not in _DT:
-        raise TypeError("states must be float32 or bfloat16")
-    if not states.is_contiguous() or states.data_ptr() % 16 or DK % 16 or DV % 16:
-        raise AssertionError("states are updated where they lie: dense, on 16 bytes, DK and DV multiples of 16")
-    if tuple(log_decay.shape) not in ((B, H), (H,)):
-        raise AssertionError(f"log_decay shape {tuple(log_decay.shape)} is neither {(B, H)} nor {(H,)}")
-    if slots is None and states.shape[0] < B:
-        raise AssertionError(f"{states.shape[0]} states for {B} rows")
-    if slots is not None:
-        slots = _indices("slots", slots, (B,), states.device)
-    W = 0
-    if parents is not None:
-        if parents.ndim != 2 or parents.shape[0] * parents.shape[1] != B:
-            raise AssertionError(f"parents shape {tuple(parents.shape)} does not hold {B} rows")
-        W = parents.shape[1]
-        if W > _lib.GLA_MOST_BEAMS:
-            raise AssertionError(f"{W} beams: at most {_lib.GLA_MOST_BEAMS} are built")
-        parents = _indices("parents", parents, tuple(parents.shape), states.device)
-    if B == 0 or H == 0 or states.shape[0] == 0:
-        return torch.zeros_like(value)
-    wide, (slots, parents) = _same_width(slots, parents)
-    v, k, q = (_rows(t, value.dtype) for t in (value, key, query))
-    a = log_decay.to(torch.float32).expand(B, H)
-    with torch.cuda.device(states.device):
-        out = torch.empty(B, H, DV, dtype=v.dtype, device=v.device)
-        rc = _lib.load().gla_decay_step(_stream(), states.shape[0], B, H, HK, DK, DV, W, _DT[v.dtype], _DT[states.dtype], wide,
-                                        _strides((a, 2), (v, 2), (k, 2), (q, 2)), _ptr(a), _ptr(v), _ptr(k), _ptr(q), _ptr(slots),
-                                        _ptr(parents), _ptr(states), _ptr(out))
-    _lib.check("gla_decay_step", rc)
-    torch.autograd.graph.increment_version(states)
-    return out
+    _refuse_gradients("decay_step", states, log_decay, value, key, query)
+    return _apply(_DecayStep, states, log_decay, value, key, query, slots, parents)
 
 
-for _cls in (_ChunkDecay, _ChunkDecayBwd):
+for _cls in (_ChunkDecay, _ChunkDecayBwd, _DecayStep):
     _cls._twin = _twin(_cls)

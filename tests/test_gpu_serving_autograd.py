@@ -79,3 +79,59 @@ def test_versions(name):
     update(want)
     update(want)
     assert torch.equal(made, want)
+
+
+def _serve(states, other, logits, scores, a, v, k, q):
+    """A step of a beam search: the candidates, and the states behind them in both ways."""
+    from gla_jax_amd import beam_select, decay_step, reorder_states
+    scores, parents, tokens = beam_select(logits, scores)
+    out = decay_step(states, a, v, k, q, parents=parents)
+    reorder_states(other, parents)
+    return scores, parents, tokens, out, other.sum(-1)
+
+
+def _search(seed):
+    g = torch.Generator().manual_seed(seed)
+    logits, scores = torch.randn(2, 4, 300, generator=g).cuda(), -torch.rand(2, 4, generator=g).cuda()
+    return [_states(seed), _states(seed + 1), logits, scores, *_token(seed)]
+
+
+def test_traced_calls_compute_on_new_inputs():
+    """torch.jit.trace records the calls themselves, not the buffers that they fill or the values that they found."""
+    traced = torch.jit.trace(_serve, tuple(_search(3)), check_trace=False)
+    for seed in (5, 7, 9):
+        mine, want = _search(seed), _search(seed)
+        for _ in range(3):
+            for x, y in zip(traced(*mine), _serve(*want)):
+                assert torch.equal(x, y)
+            assert torch.equal(mine[0], want[0]) and torch.equal(mine[1], want[1])
+
+
+@pytest.mark.parametrize("pooled", [False, True])
+def test_traced_steps_update_their_states(pooled):
+    from gla_jax_amd import decay_step
+    slots = torch.tensor([3, -1, 0, 7, 1, 2, 6, 4], device="cuda") if pooled else None
+    fn = lambda s, *rows: decay_step(s, *rows, slots)  # noqa: E731
+    traced = torch.jit.trace(fn, (_states(1), *_token(1)), check_trace=False)
+    mine, want = _states(2), _states(2)
+    for seed in (2, 3, 4, 5):
+        a, v, k, q = _token(seed)
+        # rows in another layout than the traced ones
+        spread = torch.stack((v, v), -1)[..., 0]
+        assert torch.equal(traced(mine, a, spread, k, q), fn(want, a, v, k, q)) and torch.equal(mine, want)
+
+
+def test_traced_calls_check_what_they_are_given():
+    """States of another shape or layout than the traced ones are refused, as in a plain call."""
+    from gla_jax_amd import decay_step, reorder_states
+    traced = torch.jit.trace(decay_step, (_states(1), *_token(1)), check_trace=False)
+    for other in (_states(1)[:4], _states(1)[:, :, :16].contiguous(), _states(1).transpose(2, 3), _states(1).double()):
+        before = other.clone()
+        with pytest.raises(Exception, match="states"):
+            traced(other, *_token(1))
+        assert torch.equal(other, before)
+    parents = torch.tensor(PARENTS, device="cuda")
+    traced = torch.jit.trace(lambda s, p: reorder_states(s, p), (_states(1), parents), check_trace=False)
+    for other in (_states(1)[:4], _states(1).transpose(2, 3)):
+        with pytest.raises(Exception, match="states"):
+            traced(other, parents)
