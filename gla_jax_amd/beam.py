@@ -5,7 +5,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .decay import _check, _indices, _no_gradient, _refuse_gradients, _same_width
+from .decay import _check, _indices, _no_gradient, _refuse_gradients, _refuse_tangents, _same_width
 from .gla import _DT, _apply, _native, _ptr, _stream, _twin
 
 
@@ -81,6 +81,7 @@ def beam_select(logits, scores, num=None, finished=None, eos=0):
     done = _native("beam_select", (logits, scores), num, finished, eos)
     if done is not None:
         return tuple(done)
+    _refuse_tangents("beam_select", logits, scores)
     logits, scores = (t.detach() if isinstance(t, torch.Tensor) else t for t in (logits, scores))
     return _apply(_BeamSelect, logits, scores, num, finished, eos)
 
@@ -131,6 +132,7 @@ def reorder_states(states, parents, slots=None):
     if _native("reorder", (states, parents), slots):
         return states
     _refuse_gradients("reorder_states", states)
+    _refuse_tangents("reorder_states", states)
     _apply(_ReorderStates, states, parents, slots)
     return states
 

@@ -542,11 +542,17 @@ at::ScalarType index_type(const std::optional<Tensor> &x, const std::optional<Te
     const at::ScalarType t = x ? x->scalar_type() : y ? y->scalar_type() : at::kLong;
     return t == at::kInt ? at::kInt : at::kLong;
 }
+bool has_tangent(at::ArrayRef<Tensor> arrays)
+{
+    for (const Tensor &t : arrays)
+        if (t._fw_grad(/*level=*/0).defined()) return true;
+    return false;
+}
 bool takes_gradient(at::ArrayRef<Tensor> arrays)
 {
     for (const Tensor &t : arrays)
-        if ((at::GradMode::is_enabled() && t.requires_grad()) || t._fw_grad(/*level=*/0).defined()) return true;
-    return false;
+        if (at::GradMode::is_enabled() && t.requires_grad()) return true;
+    return has_tangent(arrays);
 }
 
 // States that a call has updated in place count as a new version: autograd then refuses to use what it saved of the old one.  (What
@@ -592,7 +598,7 @@ Result beam_select(const Tensor &logits, const Tensor &scores, const std::option
 {
     const int64_t n = logits.dim();
     if (traced() || n < 2 || !logits.is_cuda() || logits.layout() != at::kStrided || logits.stride(-1) != 1 || !known(logits.scalar_type()) ||
-        !plain_f32(scores) || scores.dim() != n - 1 || scores.device() != logits.device())
+        !plain_f32(scores) || scores.dim() != n - 1 || scores.device() != logits.device() || has_tangent({logits, scores}))
         return std::nullopt;
     const int64_t W = logits.size(-2), V = logits.size(-1), row = W > 1 ? logits.stride(-2) : V;
     int64_t G = 1;

@@ -243,6 +243,13 @@ def _refuse_gradients(name, *arrays):
         _no_gradient(name)
 
 
+def _refuse_tangents(name, *arrays):
+    """There is no forward-mode rule, and a result without its tangent would be a wrong one.  (An autograd function refuses them as well, but
+    after its forward, which updates states in place.)"""
+    if any(isinstance(t, torch.Tensor) and torch.autograd.forward_ad.unpack_dual(t).tangent is not None for t in arrays):
+        raise RuntimeError(f"{name} has no forward-mode rule: an array carries a tangent")
+
+
 class _DecayStep(torch.autograd.Function):
     """decay_step for arrays that are not as the native host side takes them, and under a tracer, which records a Function as a call of
     it.  So all checks are here, where a recorded call makes them again.  There is no gradient."""
@@ -316,6 +323,7 @@ def decay_step(states, log_decay, value, key, query, slots=None, parents=None):
     if done is not None:
         return done
     _refuse_gradients("decay_step", states, log_decay, value, key, query)
+    _refuse_tangents("decay_step", states, log_decay, value, key, query)
     return _apply(_DecayStep, states, log_decay, value, key, query, slots, parents)
 
 

@@ -135,3 +135,32 @@ def test_traced_calls_check_what_they_are_given():
     for other in (_states(1)[:4], _states(1).transpose(2, 3)):
         with pytest.raises(Exception, match="states"):
             traced(other, parents)
+
+
+def test_forward_mode_tangents_are_refused():
+    """There is no forward-mode rule: a call on an array with a tangent raises before it updates anything, also where no gradient is
+    asked for, instead of returning results without one."""
+    import torch.autograd.forward_ad as fwAD
+    from gla_jax_amd import beam_select, decay_step, reorder_states
+    parents = torch.tensor(PARENTS, device="cuda")
+    logits, scores = torch.randn(2, 4, 50, device="cuda"), torch.zeros(2, 4, device="cuda")
+    arrays = [_states(1), *_token(1)]
+    calls = [(lambda *x: decay_step(*x), arrays), (lambda *x: decay_step(*x, parents=parents), arrays), (lambda s: reorder_states(s, parents), arrays[:1]),
+             (beam_select, [logits, scores])]
+    with fwAD.dual_level():
+        for fn, plain in calls:
+            for i, x in enumerate(plain):
+                dual = list(plain)
+                dual[i] = fwAD.make_dual(x.clone(), torch.ones_like(x))
+                before = [t.clone() for t in dual]
+                for mode in (torch.enable_grad, torch.no_grad):
+                    with mode(), pytest.raises(RuntimeError, match="forward-mode"):
+                        fn(*dual)
+                for t, y in zip(dual, before):
+                    assert torch.equal(t, y)
+    for fn, plain in calls:
+        before = [t.clone() for t in plain]
+        with pytest.raises(RuntimeError):
+            torch.func.jvp(fn, tuple(plain), tuple(torch.ones_like(t) for t in plain))
+        for t, y in zip(plain, before):
+            assert torch.equal(t, y)
