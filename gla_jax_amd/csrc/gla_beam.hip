@@ -27,6 +27,14 @@ __device__ __forceinline__ u64 key_of(float x, uint32_t place)
 {
     return ((u64)ordered(x + 0.f) << 32) | (uint32_t)~place;      // (-0 + 0 is 0: the two are equal)
 }
+// A logit; -inf where it is not a number.  The maximum of a signalling NaN and a number is a quiet NaN, only that of a quiet one the number, and the
+// compiler takes every float that comes from a bfloat16 for quiet: so the first instruction is written out.  (A comparison instead cost a
+// register too many where rows do not begin on 16 bytes: 16 searches of 8 beams over 131071 bfloat16 logits 32.3 us, this 29.9, and 30 with neither.)
+__device__ __forceinline__ float number(float x)
+{
+    asm("v_max_f32 %0, %0, %0\n\tv_max_f32 %0, 0xff800000, %0" : "+v"(x));
+    return x;
+}
 constexpr int kThreads = 256, kHeld = 4;
 
 struct SelectArgs {
@@ -108,7 +116,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(PIECES
     }
     float v[EACH];
 #pragma unroll
-    for (int i = 0; i < EACH; ++i) v[i] = fmaxf((float)raw[i], -INFINITY);      // (of a NaN and a number the number)
+    for (int i = 0; i < EACH; ++i) v[i] = number((float)raw[i]);
     if (there < kThreads * EACH)
 #pragma unroll
         for (int i = 0; i < EACH; ++i)
@@ -147,7 +155,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(PIECES
             const int bit = 31 - __clz((int)left), at = place((j + 1) * kWord - 1 - bit);
             left ^= 1u << bit;
             if (at >= there) continue;
-            const u64 key = key_of(fmaxf((float)x[at], -INFINITY), (uint32_t)(first + at));
+            const u64 key = key_of(number((float)x[at]), (uint32_t)(first + at));
             if (key >= bound) collected[atomicAdd(&lds.count, 1)] = key;
         }
 #pragma unroll
