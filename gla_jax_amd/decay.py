@@ -45,6 +45,11 @@ def _strides(*rows):
 def _decay_forward(h0, a, v, k, q, lengths, residual):
     B, T, H, DV = v.shape
     HK, DK = k.shape[2:]
+    # (chunk_decay has checked its own arguments; a call that a tracer has recorded may be given others)
+    if tuple(h0.shape) != (B, H, DK, DV) or tuple(k.shape[:2]) != (B, T) or q.shape != k.shape or k.dtype != v.dtype or q.dtype != v.dtype:
+        raise ValueError("chunk_decay: arrays that do not fit each other")
+    if lengths is not None and (tuple(lengths.shape) != (B,) or lengths.dtype != torch.int32 or not lengths.is_contiguous()):
+        raise ValueError("chunk_decay: lengths of another type or number than the sequences")
     lib, dt = _lib.load(), _DT[v.dtype]
     h0, v, k, q = _dense(h0), _rows(v, v.dtype), _rows(k, k.dtype), _rows(q, q.dtype)
     at = a.expand(B, T, H)

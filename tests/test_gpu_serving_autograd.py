@@ -164,3 +164,27 @@ def test_forward_mode_tangents_are_refused():
             torch.func.jvp(fn, tuple(plain), tuple(torch.ones_like(t) for t in plain))
         for t, y in zip(plain, before):
             assert torch.equal(t, y)
+
+
+@pytest.mark.parametrize("ragged", [False, True])
+def test_traced_sequences_check_what_they_are_given(ragged):
+    """A recorded chunk_decay computes on other lengths and refuses arrays that do not fit each other."""
+    from gla_jax_amd import chunk_decay
+    g = torch.Generator().manual_seed(4)
+    rows = lambda T, n=B: [torch.randn(n, T, H, D, generator=g).cuda() for _ in range(3)]  # noqa: E731
+    fn = lambda h0, a, v, k, q, *n: chunk_decay(h0, a, v, k, q, *n)  # noqa: E731
+    lengths = (torch.arange(B, device="cuda", dtype=torch.int32),) if ragged else ()
+    head = torch.full((H,), -0.1, device="cuda")
+    traced = torch.jit.trace(fn, (_states(1), head, *rows(20), *lengths), check_trace=False)
+    new = (_states(2), head, *rows(70), *lengths)
+    for x, y in zip(traced(*new), fn(*new)):
+        assert torch.equal(x, y)
+    h0, a, v, k, q = new[:5]
+    for other in ((h0[:4], a, v, k, q), (h0[..., :16].contiguous(), a, v, k, q), (h0, a, v, k[:, :30], q), (h0, a, v, k, q[:, :30]),
+                  (h0, a, v, k[:4], q[:4]), (h0, a, v, k.bfloat16(), q)):
+        with pytest.raises(Exception, match="chunk_decay"):
+            traced(*other, *lengths)
+    if ragged:
+        for n in (lengths[0][:4], lengths[0].long()):
+            with pytest.raises(Exception, match="chunk_decay"):
+                traced(*new[:5], n)
