@@ -69,7 +69,6 @@ DecayParts plan_parts(const DecaySizes &n)
     p.rows = (int)(vs * (n.H / n.HK));
     p.values = (int)ks;
     p.gates = (int)(ks * vs);
-    p.gate_step = (n.B * n.T * n.H + 3) / 4 * 4;
     return p;
 }
 // Assigns the parts' arrays behind `ws` (which may be NULL: for the size alone).
@@ -86,7 +85,7 @@ int64_t place_parts(const DecaySizes &n, const DecayPlan &plan, bool constant_ga
         p.dkey = reinterpret_cast<float *>(take(p.rows * n.B * n.T * n.HK * n.DK * 4));
     }
     if (p.values > 1) p.dvalue = reinterpret_cast<float *>(take(p.values * n.B * n.T * n.H * n.DV * 4));
-    if (p.gates > 1 && !constant_gates) p.dgate = reinterpret_cast<float *>(take(p.gates * p.gate_step * 4));
+    if (p.gates > 1 && !constant_gates) p.dgate = reinterpret_cast<float *>(take(p.gates * n.B * n.T * n.H * 4));
     if (constant_gates) p.gate_sums = reinterpret_cast<double *>(take(p.gates * n.H * n.B * plan.segments * 8));
     return at;
 }

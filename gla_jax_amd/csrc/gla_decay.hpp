@@ -407,11 +407,9 @@ int decay_forward(void *stream, const DecaySizes &n, const DecayPlan &plan, gla_
                   float *decays);
 
 // Results that several workgroups add to (the heads that share a key head; key and value features in slabs of 128) are
-// written as floats in so many parts and summed in order.  Every part begins on 16 bytes: those of dlog_decay, whose number may be odd, lie
-// `gate_step` floats apart.
+// written as floats in so many parts and summed in order.
 struct DecayParts {
     int rows, values, gates;
-    int64_t gate_step;
     float *dquery, *dkey, *dvalue, *dgate;
     double *gate_sums;
 };

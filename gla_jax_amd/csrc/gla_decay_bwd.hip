@@ -27,8 +27,7 @@ struct BackwardArgs {
     void *dhidden_init;
     // results: in their own type, or (more than one part) floats [part][...]
     void *dvalue, *dkey, *dquery;
-    float *dgate;                                // [part][B,T,H], parts gate_step apart, or NULL
-    int64_t gate_step;
+    float *dgate;                                // [part][B,T,H], or NULL
     double *dgate_sums;                          // [part][H][B][segments] where the gates are one constant a head, or NULL
     int row_parts, value_parts;                  // of dquery and dkey; of dvalue
 };
@@ -188,7 +187,7 @@ __global__ __launch_bounds__(((DKW > DVW ? DKW : DVW) + DKW) * 4) void decay_gra
         const int t = n * C + lane;
         const float d = t < len ? x + before + u : 0.f;
         if (lane < C && t < T_) {
-            if (a.dgate) a.dgate[blockIdx.y * a.gate_step + (b * a.n.T + t) * a.n.H + h] = d;
+            if (a.dgate) a.dgate[((blockIdx.y * a.n.B + b) * a.n.T + t) * a.n.H + h] = d;
             sGate[lane] += d;
         }
     };
@@ -476,7 +475,7 @@ __global__ __launch_bounds__(((DKW > DVW ? DKW : DVW) + DKW) * 4) void decay_gra
                 if (value_wave && there) dv.put_as<T>(t, r, c, zero);
             }
             if (a.dgate && w == 0 && lane < C && m * C + lane < T_)
-                a.dgate[blockIdx.y * a.gate_step + (b * a.n.T + m * C + lane) * a.n.H + h] = 0.f;
+                a.dgate[((blockIdx.y * a.n.B + b) * a.n.T + m * C + lane) * a.n.H + h] = 0.f;
             qk.p += (int64_t)C * qk.row;
             dv.p += (int64_t)C * dv.row;
         }
@@ -491,11 +490,11 @@ __global__ __launch_bounds__(((DKW > DVW ? DKW : DVW) + DKW) * 4) void decay_gra
     }
 }
 
-// An array as the sum of `parts` arrays of n floats, `step` apart and each on 16 bytes, rounded once; all of a call's in one launch.
+// An array as the sum of `parts` arrays of n floats behind each other, rounded once; all of a call's in one launch.
 struct PartSum {
     const float *src;
     void *dst;
-    int64_t n, step;
+    int64_t n;
     int parts;
     bool floats;                                 // dst is float, else T
 };
@@ -503,21 +502,23 @@ struct PartSums {
     PartSum of[4];
     int count;
 };
-template <typename T> __device__ void sum_parts_of(const float *__restrict__ src, int parts, int64_t n, int64_t step, T *__restrict__ dst)
+template <typename T> __device__ void sum_parts_of(const float *__restrict__ src, int parts, int64_t n, T *__restrict__ dst)
 {
+    // Rows come in multiples of 16 features, so their parts all begin on 16 bytes; those of dlog_decay, B T H floats each, need not.
+    const bool fours = n % 4 == 0;
     for (int64_t i = 4 * (blockIdx.x * (int64_t)256 + threadIdx.x); i < n; i += 1024 * (int64_t)gridDim.x) {
-        if (i + 4 <= n) {
+        if (fours) {
             float s[4] = {0.f, 0.f, 0.f, 0.f}, x[4];
             for (int p = 0; p < parts; ++p) {
-                load_vec<float, 4>(src + p * step + i, x);
+                load_vec<float, 4>(src + p * n + i, x);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) s[e] += x[e];
             }
             store_vec<T, 4>(dst + i, s);
         } else {
-            for (int64_t j = i; j < n; ++j) {
+            for (int64_t j = i; j < min(i + 4, n); ++j) {
                 float s = 0.f;
-                for (int p = 0; p < parts; ++p) s += src[p * step + j];
+                for (int p = 0; p < parts; ++p) s += src[p * n + j];
                 Elem<T>::store(dst + j, s);
             }
         }
@@ -526,8 +527,8 @@ template <typename T> __device__ void sum_parts_of(const float *__restrict__ src
 template <typename T> __global__ __launch_bounds__(256) void decay_sum_parts_kernel(const PartSums a)
 {
     const PartSum &s = a.of[blockIdx.y];
-    if (s.floats) sum_parts_of(s.src, s.parts, s.n, s.step, static_cast<float *>(s.dst));
-    else sum_parts_of(s.src, s.parts, s.n, s.step, static_cast<T *>(s.dst));
+    if (s.floats) sum_parts_of(s.src, s.parts, s.n, static_cast<float *>(s.dst));
+    else sum_parts_of(s.src, s.parts, s.n, static_cast<T *>(s.dst));
 }
 
 // The gradient of one constant a head: the sum over parts, batch and segments, by one wave a head.
@@ -593,21 +594,20 @@ int decay_backward(void *stream, const DecaySizes &n, const DecayPlan &plan, gla
     a.dkey = parts.rows > 1 ? parts.dkey : dkey;
     a.dvalue = parts.values > 1 ? parts.dvalue : dvalue;
     a.dgate = constant_gates ? nullptr : parts.gates > 1 ? parts.dgate : dlog_decay;
-    a.gate_step = parts.gate_step;
     a.dgate_sums = constant_gates ? parts.gate_sums : nullptr;
     e = dtype == GLA_BF16 ? dispatch_gradient<__bf16>(s, a) : dispatch_gradient<float>(s, a);
     const int64_t nk = n.B * n.T * n.HK * n.DK, nv = n.B * n.T * n.H * n.DV;
     PartSums sums{};
     int64_t most = 0;
-    auto sum = [&](const float *src, int count, int64_t m, int64_t step, void *dst, bool floats) {
+    auto sum = [&](const float *src, int count, int64_t m, void *dst, bool floats) {
         if (count < 2 || m < 1) return;
-        sums.of[sums.count++] = PartSum{src, dst, m, step, count, floats};
+        sums.of[sums.count++] = PartSum{src, dst, m, count, floats};
         most = most < m ? m : most;
     };
-    sum(parts.dquery, parts.rows, nk, nk, dquery, false);
-    sum(parts.dkey, parts.rows, nk, nk, dkey, false);
-    sum(parts.dvalue, parts.values, nv, nv, dvalue, false);
-    if (!constant_gates) sum(parts.dgate, parts.gates, n.B * n.T * n.H, parts.gate_step, dlog_decay, true);
+    sum(parts.dquery, parts.rows, nk, dquery, false);
+    sum(parts.dkey, parts.rows, nk, dkey, false);
+    sum(parts.dvalue, parts.values, nv, dvalue, false);
+    if (!constant_gates) sum(parts.dgate, parts.gates, n.B * n.T * n.H, dlog_decay, true);
     if (!e && sums.count) {
         const int64_t blocks = (most + 1023) / 1024;
         const dim3 grid((unsigned)(blocks < 4096 ? blocks : 4096), sums.count);
