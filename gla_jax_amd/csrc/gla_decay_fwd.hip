@@ -600,7 +600,9 @@ __global__ __launch_bounds__(NW * 64 + 64) __attribute__((amdgpu_waves_per_eu(DK
 
 // The states that enter segments 2, 3, ... from what each segment adds, in place: slot s holds the state after segment s (of cotangents,
 // after the s-th from the sequence's end).
-// One value a thread: four would make wider accesses of it and a quarter of the workgroups (B1 T32768 H8 D128, 32 segments: 12.5 us).
+// One value a thread, all slots one after the other: for all that the compiler knows a store may change the next slot, so every load waits for the store
+// before it.  A chain of as many memory latencies as there are segments bounds it (B1 T32768 H8 D128, 32 segments: 12.5 us for 31 MB, of
+// which a copy of as much takes 6).
 __global__ __launch_bounds__(256) void decay_scan_kernel(float *__restrict__ entering, const float *__restrict__ decays,
                                                          const int32_t *__restrict__ lengths, DecaySizes n, DecayPlan plan, int C,
                                                          int64_t count)
@@ -611,7 +613,6 @@ __global__ __launch_bounds__(256) void decay_scan_kernel(float *__restrict__ ent
     float *p = entering + bh * segments * count + at;
     const float *d = decays + bh * segments;
     float s = p[0];
-#pragma unroll 16
     for (int64_t i = 1; i < tail; ++i) {
         s = d[i] * s + p[i * count];
         p[i * count] = s;
