@@ -15,7 +15,8 @@ int64_t pad256(int64_t x) { return (x + 255) & ~(int64_t)255; }
 // workgroup's start, and what segments cost besides: the pass that finds the states entering them (`pass` of the work, on half of the rows)
 // and a state for each to write, scan and read.  A whole number of rounds leaves no compute unit idle, so only the counts that just fill some are looked
 // at; a segment has two chunks at least.  Ragged sequences count as half full, their longest segment as what the others wait for: B16 T1337
-// H16 D128 of lengths 0 to 1337 takes 75 us whole, 111 in two segments and 121 in four.
+// H16 D128 of lengths 0 to 1337 takes 77 us whole; in two segments 103 by decay_pass_kernel, which 512 workgroups take, and 100 by
+// decay_forward_kernel, made to take them; in four 121 and 122.
 DecayPlan plan_segments(const DecaySizes &n, gla_dtype dtype, int64_t workgroups, int64_t slots, double pass, bool ragged)
 {
     const int64_t C = dtype == GLA_BF16 ? DecayChunk<__bf16>::C : DecayChunk<float>::C;

@@ -4,7 +4,7 @@
 // A wave takes 32 value columns of one state: a lane holds a piece of 16 bytes of each of DKP / (rows side by side) rows, all
 // of them requested before the first is used.  A lane's rows follow each other, so that it reads its keys and queries in
 // whole pieces; the lanes that hold the same columns are summed at the end.  Nothing goes through LDS.  128 rows of 16 heads of 128 x 128
-// float states: 51 us for 270 MB, 5.3 TB/s.
+// float states, none idle: 51.4 us for 270 MB, 5.25 TB/s.
 #include "gla_common.hpp"
 
 namespace gla {
@@ -281,7 +281,8 @@ extern "C" int gla_decay_step(void *stream, int64_t pool, int64_t B, int64_t H, 
         (reinterpret_cast<uintptr_t>(log_decay) & 3))
         return GLA_ERR_ALIGN;
     if (beams > waves_of_beams((int)DK)) {
-        // more beams than a workgroup has waves for take the reordering as a pass of its own
+        // more beams than a workgroup has waves for take the reordering as a pass of its own, in pieces of 4 bytes (128 rows of 16 heads of 64 x 64
+        // bfloat16: 25 us in searches of 32 beams, 8.4 of 16)
         const int rc = gla_reorder_states(stream, pool, B / beams, beams, H * DK * DV * bytes_of(state_dtype), wide_indices, parents,
                                           slots, states);
         if (rc) return rc;
