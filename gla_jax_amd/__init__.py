@@ -5,14 +5,16 @@ Public surface, mirroring the reference's modules:
     ops.py : cumsum_recursive, rnn_recursive
 and, for models whose heads have one decay each and for serving them:
     decay.py : chunk_decay (prompts, training), decay_step (single tokens)
+    delta.py : chunk_delta (prompts, training), delta_step (single tokens), by the gated delta rule
     beam.py : beam_select, reorder_states (beam search)
 All of them run hand-written HIP kernels from libgla_hip.so; there is no CPU or eager fallback.
 """
 from . import _lib
 from .beam import beam_select, reorder_states
 from .decay import chunk_decay, decay_step
+from .delta import chunk_delta, delta_step
 from .gla import chunk_gla, recurrent_gla, recurrent_gla_naive
 from .ops import cumsum_recursive, rnn_recursive
 
 __all__ = ["chunk_gla", "recurrent_gla", "recurrent_gla_naive", "cumsum_recursive", "rnn_recursive",
-           "chunk_decay", "decay_step", "beam_select", "reorder_states"]
+           "chunk_decay", "decay_step", "chunk_delta", "delta_step", "beam_select", "reorder_states"]

@@ -14,6 +14,7 @@ LIB_PATH = os.path.join(_HERE, "libgla_hip.so")
 GLA_F32, GLA_BF16 = 0, 1
 ABI_VERSION = 3                             # GLA_HIP_ABI_VERSION of include/gla_hip.h
 GLA_MOST_BEAMS = GLA_MOST_CANDIDATES = 64
+GLA_MOST_DELTA_KEYS = 128
 GLA_CHUNK_FWD_STATIC_BYTES = 80 << 20      # capacity of gla_chunk_fwd_static's workspace (gla_hip.h)
 
 _i64, _int, _vp, _sz = ctypes.c_int64, ctypes.c_int, ctypes.c_void_p, ctypes.c_size_t
@@ -49,6 +50,12 @@ SIGNATURES = {
     "gla_decay_fwd": (_int, [_vp] + [_i64] * 6 + [_int, _int] + [_vp] * 11 + [_sz]),
     "gla_decay_bwd": (_int, [_vp] + [_i64] * 6 + [_int] * 3 + [_vp] * 15 + [_sz]),
     "gla_decay_step": (_int, [_vp] + [_i64] * 7 + [_int] * 3 + [_vp] * 9),
+    "gla_delta_states_bytes": (_sz, [_i64] * 6 + [_int]),
+    "gla_delta_fwd_workspace_bytes": (_sz, [_i64] * 6 + [_int]),
+    "gla_delta_bwd_workspace_bytes": (_sz, [_i64] * 6 + [_int]),
+    "gla_delta_fwd": (_int, [_vp] + [_i64] * 6 + [_int, _int] + [_vp] * 12 + [_sz]),
+    "gla_delta_bwd": (_int, [_vp] + [_i64] * 6 + [_int, _int] + [_vp] * 17 + [_sz]),
+    "gla_delta_step": (_int, [_vp] + [_i64] * 7 + [_int] * 3 + [_vp] * 10),
     "gla_beam_select_workspace_bytes": (_sz, [_i64] * 4),
     "gla_beam_select": (_int, [_vp] + [_i64] * 4 + [_int, _i64] + [_vp] * 3 + [_i64] + [_vp] * 4 + [_sz]),
     "gla_reorder_states": (_int, [_vp] + [_i64] * 4 + [_int] + [_vp] * 3),

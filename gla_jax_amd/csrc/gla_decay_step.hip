@@ -1,10 +1,12 @@
-// Linear attention with one decay a head, one token for each row of a batch: the states lie in a pool and are updated where
-// they lie.  Bound by reading and writing every state once.
+// Linear attention with one decay a head, and by the gated delta rule, one token for each row of a batch: the states lie in a pool and are
+// updated where they lie.  Bound by reading and writing every state once.
 //
 // A wave takes 32 value columns of one state: a lane holds a piece of 16 bytes of each of DKP / (rows side by side) rows, all
 // of them requested before the first is used.  A lane's rows follow each other, so that it reads its keys and queries in
 // whole pieces; the lanes that hold the same columns are summed at the end.  Nothing goes through LDS.  128 rows of 16 heads of 128 x 128
 // float states, none idle: 51.4 us for 270 MB, 5.25 TB/s.
+//
+// The delta rule writes b (v - S^T k) instead of v, S being decayed already: one more sum over the key features, of what the registers hold.
 #include "gla_common.hpp"
 
 namespace gla {
@@ -23,8 +25,8 @@ struct Indices {
 struct StepArgs {
     int64_t pool, B, H, HK, DK, DV, beams;
     void *states;
-    const float *log_decay;
-    int64_t gates_b, gates_h;
+    const float *log_decay, *beta;               // beta: NULL where all of the value is written
+    int64_t gates_b, gates_h, beta_b, beta_h;
     const void *value, *key, *query;
     int64_t value_b, value_h, key_b, key_h, query_b, query_h;
     Indices slots, parents;
@@ -38,16 +40,17 @@ __device__ __forceinline__ int64_t slot_of(const StepArgs &a, int64_t i)
     return s >= 0 && s < a.pool ? s : -1;
 }
 
-template <typename T, typename HT, int DKP> struct StepState {
+template <typename T, typename HT, int DKP, bool DELTA> struct StepState {
     static constexpr int VEC = 16 / sizeof(HT), LPR = 32 / VEC, SIDE = 64 / LPR, PER = DKP / SIDE;
     typedef HT Piece __attribute__((ext_vector_type(VEC)));
     typedef T Four __attribute__((ext_vector_type(4)));
     Piece x[PER];
     Four k[PER / 4], q[PER / 4], v[VEC / 4];
-    float log_decay;
+    float log_decay, beta;
     // The token's rows, before the state: it takes longer, and in the beams' case it is not yet known where it lies.  No load is under a
     // condition, after which memory would be waited for; what does not exist reads what does, and counts as zero later.
-    __device__ __forceinline__ void load_rows(const T *key, const T *query, const T *value, const float *gate, int DK, int DV, int row0, int col)
+    __device__ __forceinline__ void load_rows(const T *key, const T *query, const T *value, const float *gate, const float *rate, int DK,
+                                              int DV, int row0, int col)
     {
 #pragma unroll
         for (int i = 0; i < PER; i += 4) {
@@ -58,6 +61,7 @@ template <typename T, typename HT, int DKP> struct StepState {
 #pragma unroll
         for (int e = 0; e < VEC; e += 4) v[e / 4] = *reinterpret_cast<const Four *>(value + (col < DV ? col : 0) + e);
         log_decay = *gate;
+        if constexpr (DELTA) beta = *rate;
     }
     __device__ __forceinline__ void load(const HT *state, int DK, int DV, int row0, int col)
     {
@@ -66,6 +70,14 @@ template <typename T, typename HT, int DKP> struct StepState {
             x[i] = Piece{};
             if (row0 + i < DK && col < DV) x[i] = *reinterpret_cast<const Piece *>(state + (int64_t)(row0 + i) * DV + col);
         }
+    }
+    // over the lanes that hold the same columns
+    static __device__ __forceinline__ void sum_rows(float (&o)[VEC])
+    {
+#pragma unroll
+        for (int m = LPR; m < 64; m *= 2)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) o[e] += shfl_xor_f32(o[e], m);
     }
     // The token's update, and its output for the lane's columns (zeros outside): the sum runs over the key features in 32 bits
     // from the state before it is rounded.
@@ -77,6 +89,21 @@ template <typename T, typename HT, int DKP> struct StepState {
         for (int e = 0; e < VEC; ++e) {
             vv[e] = (float)v[e / 4][e % 4];
             o[e] = 0.f;
+        }
+        if constexpr (DELTA) {
+            // what the state answers the key with
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                const float ki = row0 + i < DK ? (float)k[i / 4][i % 4] : 0.f;
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) o[e] += ki * (decay * (float)x[i][e]);
+            }
+            sum_rows(o);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                vv[e] = beta * (vv[e] - o[e]);
+                o[e] = 0.f;
+            }
         }
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
@@ -90,18 +117,15 @@ template <typename T, typename HT, int DKP> struct StepState {
             }
             if (row0 + i < DK && col < DV) store_vec<HT, VEC>(state + (int64_t)(row0 + i) * DV + col, s);
         }
-#pragma unroll
-        for (int m = LPR; m < 64; m *= 2)
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) o[e] += shfl_xor_f32(o[e], m);
+        sum_rows(o);
         if ((threadIdx.x & 63) < LPR && col < DV) store_vec<T, VEC>(out + col, o);
     }
 };
 
-template <typename T, typename HT, int DKP>
+template <typename T, typename HT, int DKP, bool DELTA>
 __global__ __launch_bounds__(256) void decay_step_kernel(const StepArgs a)
 {
-    typedef StepState<T, HT, DKP> State;
+    typedef StepState<T, HT, DKP, DELTA> State;
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, waves = blockDim.x >> 6;
     const unsigned H = (unsigned)a.H;
     const int64_t b = blockIdx.x / H, h = blockIdx.x % H, hk = blockIdx.x % H / (H / (unsigned)a.HK);
@@ -109,7 +133,8 @@ __global__ __launch_bounds__(256) void decay_step_kernel(const StepArgs a)
               row0 = State::PER * (lane / State::LPR);
     State s;
     s.load_rows(static_cast<const T *>(a.key) + b * a.key_b + hk * a.key_h, static_cast<const T *>(a.query) + b * a.query_b + hk * a.query_h,
-                static_cast<const T *>(a.value) + b * a.value_b + h * a.value_h, a.log_decay + b * a.gates_b + h * a.gates_h, DK, DV, row0, col);
+                static_cast<const T *>(a.value) + b * a.value_b + h * a.value_h, a.log_decay + b * a.gates_b + h * a.gates_h,
+                a.beta + b * a.beta_b + h * a.beta_h, DK, DV, row0, col);
     const int64_t slot = slot_of(a, b);
     T *out = static_cast<T *>(a.out) + (b * a.H + h) * DV;
     if (slot < 0) {                               // a row without a state
@@ -128,10 +153,10 @@ constexpr int waves_of_beams(int DK) { return DK <= 128 ? 16 : 8; }
 // The same for a group of beams, each from the state of the beam that it continues: a wave a beam, all of a group in one
 // workgroup, which has read every state (of these columns) before it writes the first.  16 groups of 8 beams, 16 heads of 64 x 64 bfloat16:
 // 7.7 us for 35 MB, 4.5 TB/s.
-template <typename T, typename HT, int DKP>
+template <typename T, typename HT, int DKP, bool DELTA>
 __global__ __launch_bounds__(64 * waves_of_beams(DKP)) void decay_step_beams_kernel(const StepArgs a)
 {
-    typedef StepState<T, HT, DKP> State;
+    typedef StepState<T, HT, DKP, DELTA> State;
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     const unsigned H = (unsigned)a.H;
     const int64_t group = blockIdx.x / H, h = blockIdx.x % H, hk = blockIdx.x % H / (H / (unsigned)a.HK), b = group * a.beams + w;
@@ -139,7 +164,8 @@ __global__ __launch_bounds__(64 * waves_of_beams(DKP)) void decay_step_beams_ker
               row0 = State::PER * (lane / State::LPR);
     State s;
     s.load_rows(static_cast<const T *>(a.key) + b * a.key_b + hk * a.key_h, static_cast<const T *>(a.query) + b * a.query_b + hk * a.query_h,
-                static_cast<const T *>(a.value) + b * a.value_b + h * a.value_h, a.log_decay + b * a.gates_b + h * a.gates_h, DK, DV, row0, col);
+                static_cast<const T *>(a.value) + b * a.value_b + h * a.value_h, a.log_decay + b * a.gates_b + h * a.gates_h,
+                a.beta + b * a.beta_b + h * a.beta_h, DK, DV, row0, col);
     const int64_t parent = a.parents.at(b), source = parent >= 0 && parent < a.beams ? group * a.beams + parent : b;
     const int64_t slot = slot_of(a, b);
     int64_t from = slot_of(a, source);
@@ -157,22 +183,23 @@ __global__ __launch_bounds__(64 * waves_of_beams(DKP)) void decay_step_beams_ker
     s.step(static_cast<HT *>(a.states) + (slot * a.H + h) * DK * DV, out, DK, DV, row0, col);
 }
 
-template <typename T, typename HT, int DKP> int launch_step(hipStream_t stream, const StepArgs &a)
+template <typename T, typename HT, int DKP, bool DELTA> int launch_step(hipStream_t stream, const StepArgs &a)
 {
     const int64_t cols = (a.DV + 31) / 32;
     if (a.beams) {
-        decay_step_beams_kernel<T, HT, DKP><<<dim3(a.B / a.beams * a.H, cols), a.beams * 64, 0, stream>>>(a);
+        decay_step_beams_kernel<T, HT, DKP, DELTA><<<dim3(a.B / a.beams * a.H, cols), a.beams * 64, 0, stream>>>(a);
     } else {
         // Four waves side by side share the lines of a row (128 rows of 16 heads of 128 x 128: 51 us, each in a workgroup of its own 57); where there
         // are few, each has a compute unit of its own (4 rows: 4.3 us against 4.5; 16 rows take 8.0 either way).
         const int waves = a.B * a.H * cols >= 1024 ? (cols < 4 ? (int)cols : 4) : 1;
-        decay_step_kernel<T, HT, DKP><<<dim3(a.B * a.H, (cols + waves - 1) / waves), waves * 64, 0, stream>>>(a);
+        decay_step_kernel<T, HT, DKP, DELTA><<<dim3(a.B * a.H, (cols + waves - 1) / waves), waves * 64, 0, stream>>>(a);
     }
     return launch_status();
 }
-template <typename T, typename HT> int dispatch_step(hipStream_t stream, const StepArgs &a)
+template <typename T, typename HT, bool DELTA> int dispatch_step(hipStream_t stream, const StepArgs &a)
 {
-    return a.DK <= 64 ? launch_step<T, HT, 64>(stream, a) : a.DK <= 128 ? launch_step<T, HT, 128>(stream, a) : launch_step<T, HT, 256>(stream, a);
+    return a.DK <= 64 ? launch_step<T, HT, 64, DELTA>(stream, a) : a.DK <= 128 ? launch_step<T, HT, 128, DELTA>(stream, a)
+                                                                               : launch_step<T, HT, 256, DELTA>(stream, a);
 }
 
 // ---- states in another order ------------------------------------------------------------------
@@ -255,21 +282,26 @@ extern "C" int gla_reorder_states(void *stream, int64_t pool, int64_t groups, in
     return piece == 16 ? launch_reorder<u32x4>(s, a, groups) : piece == 4 ? launch_reorder<uint32_t>(s, a, groups) : launch_reorder<uint8_t>(s, a, groups);
 }
 
-extern "C" int gla_decay_step(void *stream, int64_t pool, int64_t B, int64_t H, int64_t HK, int64_t DK, int64_t DV, int64_t beams,
-                              gla_dtype dtype, gla_dtype state_dtype, int wide_indices, const int64_t *strides, const float *log_decay,
-                              const void *value, const void *key, const void *query, const void *slots, const void *parents,
-                              void *states, void *out)
+namespace gla {
+namespace {
+
+// Strides: batch and head strides of log_decay, beta (delta), value, key and query.
+template <bool DELTA>
+int step(void *stream, int64_t pool, int64_t B, int64_t H, int64_t HK, int64_t DK, int64_t DV, int64_t beams, gla_dtype dtype,
+         gla_dtype state_dtype, int wide_indices, const int64_t *strides, const float *log_decay, const float *beta, const void *value,
+         const void *key, const void *query, const void *slots, const void *parents, void *states, void *out)
 {
-    if (!log_decay || !value || !key || !query || !states || !out || (beams > 0 && !parents)) return GLA_ERR_NULL;
+    if (!log_decay || (DELTA && !beta) || !value || !key || !query || !states || !out || (beams > 0 && !parents)) return GLA_ERR_NULL;
     if (pool < 1 || B < 1 || H < 1 || HK < 1 || DK < 1 || DV < 1 || beams < 0 || H % HK || DK % 16 || DV % 16 || DK > 256 || DV > 256)
         return GLA_ERR_SHAPE;
     if (B * H >= ((int64_t)1 << 31) || (!slots && B > pool) || (beams > 0 && (B % beams || beams > GLA_MOST_BEAMS))) return GLA_ERR_SHAPE;
     if (!dtype_ok(dtype) || !dtype_ok(state_dtype)) return GLA_ERR_DTYPE;
-    StepArgs a{pool, B, H, HK, DK, DV, beams, states, log_decay, H, 1, value, key, query,
+    StepArgs a{pool, B, H, HK, DK, DV, beams, states, log_decay, beta, H, 1, H, 1, value, key, query,
                H * DV, DV, HK * DK, DK, HK * DK, DK, {slots, wide_indices}, {parents, wide_indices}, out};
     if (strides) {
-        int64_t *all[8] = {&a.gates_b, &a.gates_h, &a.value_b, &a.value_h, &a.key_b, &a.key_h, &a.query_b, &a.query_h};
-        for (int i = 0; i < 8; ++i) *all[i] = strides[i];
+        int64_t *all[10] = {&a.gates_b, &a.gates_h, &a.beta_b, &a.beta_h, &a.value_b, &a.value_h, &a.key_b, &a.key_h, &a.query_b, &a.query_h};
+        for (int i = 0, from = 0; i < 10; ++i)
+            if (DELTA || (i != 2 && i != 3)) *all[i] = strides[from++];
     }
     const int64_t piece = 16 / bytes_of(dtype);
     for (int64_t x : {a.value_b, a.value_h, a.key_b, a.key_h, a.query_b, a.query_h})
@@ -278,7 +310,7 @@ extern "C" int gla_decay_step(void *stream, int64_t pool, int64_t B, int64_t H, 
         if (!aligned16(x)) return GLA_ERR_ALIGN;
     const uintptr_t index = wide_indices ? 7 : 3;
     if ((reinterpret_cast<uintptr_t>(slots) & index) || (reinterpret_cast<uintptr_t>(parents) & index) ||
-        (reinterpret_cast<uintptr_t>(log_decay) & 3))
+        (reinterpret_cast<uintptr_t>(log_decay) & 3) || (reinterpret_cast<uintptr_t>(beta) & 3))
         return GLA_ERR_ALIGN;
     if (beams > waves_of_beams((int)DK)) {
         // more beams than a workgroup has waves for take the reordering as a pass of its own, in pieces of 4 bytes (128 rows of 16 heads of 64 x 64
@@ -289,6 +321,27 @@ extern "C" int gla_decay_step(void *stream, int64_t pool, int64_t B, int64_t H, 
         a.beams = 0;
     }
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    if (dtype == GLA_BF16) return state_dtype == GLA_BF16 ? dispatch_step<__bf16, __bf16>(s, a) : dispatch_step<__bf16, float>(s, a);
-    return state_dtype == GLA_BF16 ? dispatch_step<float, __bf16>(s, a) : dispatch_step<float, float>(s, a);
+    if (dtype == GLA_BF16) return state_dtype == GLA_BF16 ? dispatch_step<__bf16, __bf16, DELTA>(s, a) : dispatch_step<__bf16, float, DELTA>(s, a);
+    return state_dtype == GLA_BF16 ? dispatch_step<float, __bf16, DELTA>(s, a) : dispatch_step<float, float, DELTA>(s, a);
+}
+
+}  // namespace
+}  // namespace gla
+
+extern "C" int gla_decay_step(void *stream, int64_t pool, int64_t B, int64_t H, int64_t HK, int64_t DK, int64_t DV, int64_t beams,
+                              gla_dtype dtype, gla_dtype state_dtype, int wide_indices, const int64_t *strides, const float *log_decay,
+                              const void *value, const void *key, const void *query, const void *slots, const void *parents,
+                              void *states, void *out)
+{
+    return step<false>(stream, pool, B, H, HK, DK, DV, beams, dtype, state_dtype, wide_indices, strides, log_decay, nullptr, value, key, query,
+                       slots, parents, states, out);
+}
+
+extern "C" int gla_delta_step(void *stream, int64_t pool, int64_t B, int64_t H, int64_t HK, int64_t DK, int64_t DV, int64_t beams,
+                              gla_dtype dtype, gla_dtype state_dtype, int wide_indices, const int64_t *strides, const float *log_decay,
+                              const float *beta, const void *value, const void *key, const void *query, const void *slots,
+                              const void *parents, void *states, void *out)
+{
+    return step<true>(stream, pool, B, H, HK, DK, DV, beams, dtype, state_dtype, wide_indices, strides, log_decay, beta, value, key, query,
+                      slots, parents, states, out);
 }

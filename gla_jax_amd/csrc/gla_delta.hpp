@@ -1,0 +1,120 @@
+// Building blocks of linear attention by the gated delta rule (gfx950):
+//       S_t = (1 - b_t k_t k_t^T) e^{a_t} S_{t-1} + b_t k_t v_t^T,   o_t = S_t^T q_t,   a_t and b_t one number a head and token.
+//
+// In chunks of C tokens, with L_i the sum of a up to and with token i of a chunk and S the state before it, what the tokens write is
+// the solution of a triangular system whose matrix does not depend on the state:
+//       M_ij = e^{L_i - L_j} k_i.k_j for j < i,   r_i = v_i - e^{L_i} S^T k_i,   x = (1 + M b)^{-1} r,   u_i = b_i x_i
+//       o_i = e^{L_i} S^T q_i + sum_{j<=i} P_ij u_j,   P_ij = e^{L_i - L_j} q_i.k_j,     S' = e^{L_C} S + sum_j e^{L_C - L_j} k_j u_j^T.
+// So the work is in two kinds of kernels.  delta_prepare_kernel, all chunks at once, forms the inverses and the scores.  The walks go
+// through a sequence's chunks with the state in the accumulators of their matrix instructions, and need nothing but products.
+//
+// A wave walks alone: it holds 16 or 32 value columns of the state, and all that it multiplies by comes from memory as operands of its matrix
+// instructions, keys and queries as they lie and the rest in the order in which delta_prepare_kernel's lanes held it.  No LDS, no
+// barrier, and where there are few sequences their columns are spread over the compute units.
+//
+// Precision.  Keys, queries and values are 16-bit numbers as they come.  What a 32-bit result (states, gradients of the gates) depends on
+// and is formed in between, i.e. the state, the inverse, r and u, enters a product as two or three bf16 parts (Split): two are off by 2^-18 of a
+// value at most.  What only a 16-bit result depends on is rounded to 16 bits once.  float data take the matrix cores' float products.
+//
+// Operand layouts: gla_decay.hpp.  Rows of the state are the features pi(t, m) of gla_chunk_common.hpp, so that two accumulators above each
+// other (tiles 2p and 2p + 1) are features 32p + 8c .. + 7: an operand of the contraction with keys in their natural order.
+#pragma once
+
+#include "gla_decay.hpp"
+
+namespace gla {
+
+template <typename T> struct DeltaChunk {
+    static constexpr int C = DecayChunk<T>::C, CT = C / 16, CS = C / 32;
+    static constexpr int kParts = sizeof(T) == 2 ? 2 : 1;      // of an operand that is a 32-bit number
+    // steps of 32 tokens of a triangle's rows of tiles, 512 values each: lower ones have step ks <= t / 2, upper ones ks >= t / 2
+    static constexpr int kSteps = CS == 1 ? CT : 6;
+    static constexpr int lower(int t, int ks) { return t < 2 ? t : 2 * t - 2 + ks; }
+    static constexpr int upper(int t, int ks) { return CS == 1 ? t : t < 2 ? 2 * t + ks : t + 2; }
+    static constexpr int kGates = 4 * C;                        // floats of a chunk: e^{L_i}, e^{L_C - L_i}, b_i, and e^{L_C} in the last
+};
+
+// Where the prepared operands of a call lie.
+struct DeltaPrepared {
+    void *inverse;      // [pairs, chunks][steps][parts][64][8]
+    void *scores;       // [pairs, chunks][steps][parts, of the backward walk][64][8]
+    void *keys;         // [B, HK, chunks][features / 16][C / 32][64][8]: keys with tokens as the contracted index
+    void *queries;      // the same, of the backward walk
+    float *gates;       // [pairs, chunks][kGates]
+};
+
+struct DeltaArgs {
+    DecaySizes n;
+    int64_t chunks, pairs;
+    DecayRows gates, betas, keys, values, queries, dout;
+    const int32_t *lengths;
+    DeltaPrepared to;
+    const void *hidden;             // hidden_init; backward: dhidden_final
+    int hidden_dtype;
+    void *hidden_out;               // hidden_final; dhidden_init
+    void *out;
+    // what the forward pass leaves for the backward: of each pair the states before its chunks and at its end, [chunks + 1][DV][DK], and x,
+    // [chunks][DV / 16][C / 16][4][16][4], floats
+    float *kept;
+    // what the backward walk leaves for the gradients: the same of the cotangent of u (all parts of it), and the cotangents of the states behind the
+    // chunks, [chunks][DV][DK] in T, and <state, its cotangent> there, [pairs, chunks][value columns / columns of a wave]
+    float *du;
+    void *dstates;
+    float *dots;
+    int dot_slabs;
+    void *dvalue, *dkey, *dquery;   // dkey, dquery: in their own type, or (more than one part) floats [part][...]
+    float *dgate, *dbeta;
+    int row_parts;
+};
+inline __host__ __device__ int64_t delta_states_floats(const DecaySizes &n, int64_t chunks) { return (chunks + 1) * n.DK * n.DV; }
+inline __host__ __device__ int64_t delta_written_floats(const DecaySizes &n, int64_t chunks, int C) { return chunks * C * n.DV; }
+
+inline __host__ __device__ int64_t delta_key_width(int64_t DK) { return DK <= 64 ? 64 : 128; }
+
+// Features pi(t, r) as the operand's rows, rows 32 * ks .. as the contracted index, in two halves: LdsTile::columns with another
+// order of the features.
+template <int F> __device__ __forceinline__ bf16x8 feature_columns(const __bf16 *p, int ks, int t)
+{
+    const int lane = threadIdx.x & 63, r = lane & 15, c = lane >> 4, row = 4 * c + (r >> 2);
+    const unsigned at = (2 * row * F + (((r & 3) ^ LdsTile<__bf16, F>::permuted(row)) << 4)) ^ (64 * (t >> 1) + 8 * (t & 1));
+    return lds_tr4x2(at_bytes(p + 32 * ks * F, at), 16 * F);
+}
+template <int F> __device__ __forceinline__ f32x8 feature_columns(const float *p, int ks, int t)
+{
+    constexpr int kRow = LdsTile<float, F>::kRow;
+    const int lane = threadIdx.x & 63, r = lane & 15, c = lane >> 4;
+    p += (32 * ks + 4 * c) * kRow + 32 * (t >> 1) + 8 * (r >> 2) + 4 * (t & 1) + (r & 3);
+    f32x8 x;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x.v[e] = p[((e & 3) + 16 * (e >> 2)) * kRow];
+    return x;
+}
+
+// A product of two operands in two parts each, without the product of the small ones (2^-18 of it).
+__device__ __forceinline__ f32x4 mma_parts(const bf16x8 (&a)[2], const bf16x8 (&b)[2], f32x4 c)
+{
+    return mma_d(a[0], b[0], mma_d(a[0], b[1], mma_d(a[1], b[0], c)));
+}
+__device__ __forceinline__ f32x4 mma_parts(const f32x8 (&a)[1], const f32x8 (&b)[1], f32x4 c) { return mma_d(a[0], b[0], c); }
+// and of one in parts with one that is whole
+template <typename D8, int N> __device__ __forceinline__ f32x4 mma_whole(const D8 &a, const D8 (&b)[N], f32x4 c)
+{
+#pragma unroll
+    for (int i = N - 1; i >= 0; --i) c = mma_d(a, b[i], c);
+    return c;
+}
+template <typename D8, int N> __device__ __forceinline__ f32x4 mma_whole(const D8 (&a)[N], const D8 &b, f32x4 c)
+{
+#pragma unroll
+    for (int i = N - 1; i >= 0; --i) c = mma_d(a[i], b, c);
+    return c;
+}
+
+int delta_prepare(void *stream, const DeltaArgs &a, gla_dtype dtype, bool backward);
+int delta_walk(void *stream, const DeltaArgs &a, gla_dtype dtype, bool backward);
+int delta_gradients(void *stream, const DeltaArgs &a, gla_dtype dtype);
+// dst <- the sum over the heads of a key head of parts [H / HK][B,T,HK,DK], in order
+int delta_sum_heads(void *stream, const DecaySizes &n, gla_dtype dtype, const float *parts, void *dst);
+int64_t delta_wave_columns(const DecaySizes &n);
+
+}  // namespace gla

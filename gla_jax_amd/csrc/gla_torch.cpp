@@ -451,6 +451,107 @@ struct Decay : torch::autograd::Function<Decay> {
     }
 };
 
+// ---- linear attention by the gated delta rule -----------------------------------------------------
+bool gates_on_gpu(const Tensor &b, const Tensor &v)
+{
+    return b.defined() && b.is_cuda() && b.layout() == at::kStrided && b.scalar_type() == at::kFloat && b.dim() == v.dim() - 1 &&
+           b.device() == v.device() && b.size(-1) == v.size(-2) && b.size(-2) == v.size(-3) && (v.dim() == 3 || b.size(0) == v.size(0));
+}
+bool delta_rows(const Tensor &a, const Tensor &b, const Tensor &v, const Tensor &k, const Tensor &q, const std::optional<Tensor> &lengths)
+{
+    return decay_rows(a, v, k, q, lengths) && k.size(-1) <= GLA_MOST_DELTA_KEYS && gates_on_gpu(a, v) && gates_on_gpu(b, v);
+}
+std::array<int64_t, 15> delta_strides(const Tensor &a, const Tensor &b, const Tensor &v, const Tensor &k, const Tensor &q)
+{
+    const auto rows = decay_strides(a, v, k, q);
+    std::array<int64_t, 15> s{rows[0], rows[1], rows[2], b.dim() == 3 ? b.stride(0) : 0, b.stride(-2), b.stride(-1)};
+    for (size_t i = 3; i < 12; ++i) s[i + 3] = rows[i];
+    return s;
+}
+
+ChunkOut delta_forward(const Tensor &h0, const Tensor &a, const Tensor &b, const Tensor &v, const Tensor &k, const Tensor &q,
+                       const std::optional<Tensor> &lengths, bool residual)
+{
+    const c10::DeviceGuard guard(v.device());
+    const DecayDims n = decay_dims(v, k);
+    const gla_dtype dt = code(v);
+    const size_t nws = gla_delta_fwd_workspace_bytes(n.B, n.T, n.H, n.HK, n.DK, n.DV, dt);
+    const size_t nst = residual ? gla_delta_states_bytes(n.B, n.T, n.H, n.HK, n.DK, n.DV, dt) : 0;
+    ChunkOut r{at::empty_like(h0), dense_like(v), Tensor()};
+    if (residual) r.states = at::empty({n.B, (int64_t)nst / n.B}, v.options().dtype(at::kByte));
+    Tensor ws;
+    if (nws) ws = bytes_like(nws, v);
+    const auto strides = delta_strides(a, b, v, k, q);
+    check("gla_delta_fwd",
+          gla_delta_fwd(stream_of(v), n.B, n.T, n.H, n.HK, n.DK, n.DV, dt, code(h0), strides.data(), h0.data_ptr(),
+                        (const float *)a.data_ptr(), (const float *)b.data_ptr(), v.data_ptr(), k.data_ptr(), q.data_ptr(), lengths_of(lengths),
+                        r.hT.data_ptr(), r.out.data_ptr(), nst ? r.states.data_ptr() : nullptr, nws ? ws.data_ptr() : nullptr, nws));
+    return r;
+}
+
+variable_list delta_backward(const Tensor &states, const Tensor &a, const Tensor &b, const Tensor &v, const Tensor &k, const Tensor &q,
+                             const std::optional<Tensor> &lengths, const Tensor &dhT, const Tensor &dout)
+{
+    const c10::DeviceGuard guard(v.device());
+    const DecayDims n = decay_dims(v, k);
+    const gla_dtype dt = code(v);
+    const size_t nws = gla_delta_bwd_workspace_bytes(n.B, n.T, n.H, n.HK, n.DK, n.DV, dt);
+    Tensor ws;
+    if (nws) ws = bytes_like(nws, v);
+    Tensor dh0 = at::empty_like(dhT), da = dense_like(a), db = dense_like(b), dv = dense_like(v), dk = dense_like(k), dq = dense_like(q);
+    const auto strides = delta_strides(a, b, v, k, q);
+    check("gla_delta_bwd",
+          gla_delta_bwd(stream_of(v), n.B, n.T, n.H, n.HK, n.DK, n.DV, dt, code(dhT), strides.data(), (const float *)a.data_ptr(),
+                        (const float *)b.data_ptr(), v.data_ptr(), k.data_ptr(), q.data_ptr(), lengths_of(lengths), states.data_ptr(),
+                        dhT.data_ptr(), dout.data_ptr(), dh0.data_ptr(), (float *)da.data_ptr(), (float *)db.data_ptr(), dv.data_ptr(),
+                        dk.data_ptr(), dq.data_ptr(), nws ? ws.data_ptr() : nullptr, nws));
+    return {dh0, da, db, dv, dk, dq};
+}
+
+struct DeltaBackward : torch::autograd::Function<DeltaBackward> {
+    static variable_list forward(AutogradContext *, const Tensor &states, const Tensor &a, const Tensor &b, const Tensor &v, const Tensor &k,
+                                 const Tensor &q, const std::optional<Tensor> &lengths, const Tensor &dhT, const Tensor &dout)
+    {
+        return delta_backward(states, a, b, v, k, q, lengths, dhT, dout);
+    }
+    static variable_list backward(AutogradContext *, variable_list) { no_double_backward("chunk_delta"); }
+};
+
+struct Delta : torch::autograd::Function<Delta> {
+    static variable_list forward(AutogradContext *ctx, const Tensor &h0, const Tensor &a, const Tensor &b, const Tensor &v, const Tensor &k,
+                                 const Tensor &q, const std::optional<Tensor> &lengths)
+    {
+        ChunkOut r = delta_forward(h0, a, b, v, k, q, lengths, true);
+        ctx->save_for_backward({r.states, a, b, v, k, q, lengths.value_or(Tensor())});
+        ctx->saved_data["hidden"] = (int64_t)h0.scalar_type();
+        ctx->set_materialize_grads(false);
+        return {r.hT, r.out};
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list d)
+    {
+        variable_list s = ctx->get_saved_variables();
+        for (size_t i = 3; i < 6; ++i)
+            if (s[i].defined() && !rows_on_gpu(s[i])) s[i] = s[i].clone(at::MemoryFormat::Contiguous);
+        if (!s[0].is_contiguous() || !on_16_bytes(s[0])) s[0] = s[0].clone(at::MemoryFormat::Contiguous);
+        if (s[6].defined() && !s[6].is_contiguous()) s[6] = s[6].contiguous();
+        const std::optional<Tensor> lengths = s[6].defined() ? std::optional<Tensor>(s[6]) : std::nullopt;
+        check_saved(delta_rows(s[1], s[2], s[3], s[4], s[5], lengths));
+        const DecayDims n = decay_dims(s[3], s[4]);
+        check_saved(holds(s[0], gla_delta_states_bytes(n.B, n.T, n.H, n.HK, n.DK, n.DV, code(s[3])), s[3]));
+        Tensor dhT = cotangent(d[0], decay_state_sizes(s[3], s[4]), (at::ScalarType)ctx->saved_data["hidden"].toInt(), s[3]);
+        Tensor dout = cotangent(d[1], s[3].sizes(), s[3].scalar_type(), s[3]);
+        if (!transforms_active())
+            for (Tensor *t : {&dhT, &dout})
+                if (!on_16_bytes(*t)) *t = t->clone();
+        variable_list r =
+            transforms_active() ? python_rule("gla_jax_amd.delta", "_ChunkDeltaBwd", s[0], s[1], s[2], s[3], s[4], s[5], lengths, dhT, dout)
+            : at::GradMode::is_enabled() ? DeltaBackward::apply(s[0], s[1], s[2], s[3], s[4], s[5], lengths, dhT, dout)
+                                         : delta_backward(s[0], s[1], s[2], s[3], s[4], s[5], lengths, dhT, dout);
+        r.emplace_back();
+        return r;
+    }
+};
+
 // ---- module -------------------------------------------------------------------------------------
 typedef std::optional<std::vector<Tensor>> Result;       // none: not for this path
 
@@ -533,6 +634,17 @@ Result decay(const Tensor &h0, const Tensor &a, const Tensor &v, const Tensor &k
     return std::vector<Tensor>{r.hT, r.out};
 }
 
+Result delta(const Tensor &h0, const Tensor &a, const Tensor &b, const Tensor &v, const Tensor &k, const Tensor &q,
+             const std::optional<Tensor> &lengths)
+{
+    if (traced() || !delta_rows(a, b, v, k, q, lengths) || !dense_on_gpu(h0) || !on_16_bytes(h0) || h0.device() != v.device() ||
+        !known(h0.scalar_type()) || h0.sizes() != at::IntArrayRef(decay_state_sizes(v, k)))
+        return std::nullopt;
+    if (wants_grad(h0, a, v, k, q) || wants_grad(b, b, b, b, b)) return Delta::apply(h0, a, b, v, k, q, lengths);
+    ChunkOut r = delta_forward(h0, a, b, v, k, q, lengths, false);
+    return std::vector<Tensor>{r.hT, r.out};
+}
+
 bool index_array(const std::optional<Tensor> &t, at::IntArrayRef sizes, const Tensor &like, at::ScalarType type)
 {
     return !t || (dense_on_gpu(*t) && t->sizes() == sizes && t->device() == like.device() && t->scalar_type() == type);
@@ -562,19 +674,24 @@ void updated(const Tensor &states)
     if (!states.is_inference()) states.unsafeGetTensorImpl()->bump_version();
 }
 
-std::optional<Tensor> decay_step(const Tensor &states, const Tensor &a, const Tensor &v, const Tensor &k, const Tensor &q,
-                                 const std::optional<Tensor> &slots, const std::optional<Tensor> &parents)
+// decay_step and, with `beta`, delta_step
+std::optional<Tensor> one_step(const Tensor &states, const Tensor &a, const Tensor *beta, const Tensor &v, const Tensor &k, const Tensor &q,
+                               const std::optional<Tensor> &slots, const std::optional<Tensor> &parents)
 {
-    if (traced() || !dense_on_gpu(states) || states.dim() != 4 || !known(states.scalar_type()) || takes_gradient({states, a, v, k, q}))
+    if (traced() || !dense_on_gpu(states) || states.dim() != 4 || !known(states.scalar_type()) || takes_gradient({states, a, v, k, q}) ||
+        (beta && takes_gradient({*beta})))
         return std::nullopt;
     if (!rows_on_gpu(v) || !rows_on_gpu(k) || !rows_on_gpu(q) || v.dim() != 3 || k.dim() != 3 || q.sizes() != k.sizes()) return std::nullopt;
     const int64_t B = v.size(0), H = v.size(1), DV = v.size(2), HK = k.size(1), DK = k.size(2), N = states.size(0);
     if (B < 1 || H < 1 || N < 1 || HK < 1 || H % HK || k.size(0) != B || states.size(1) != H || states.size(2) != DK || states.size(3) != DV)
         return std::nullopt;
     if (!known(v.scalar_type()) || k.scalar_type() != v.scalar_type() || q.scalar_type() != v.scalar_type()) return std::nullopt;
-    if (!a.is_cuda() || a.layout() != at::kStrided || a.scalar_type() != at::kFloat || a.size(-1) != H || a.dim() > 2 || (a.dim() == 2 && a.size(0) != B))
-        return std::nullopt;
-    for (const Tensor *t : {&a, &v, &k, &q})
+    const Tensor &b = beta ? *beta : a;
+    for (const Tensor *t : {&a, &b})
+        if (!t->is_cuda() || t->layout() != at::kStrided || t->scalar_type() != at::kFloat || t->dim() < 1 || t->size(-1) != H || t->dim() > 2 ||
+            (t->dim() == 2 && t->size(0) != B))
+            return std::nullopt;
+    for (const Tensor *t : {&a, &b, &v, &k, &q})
         if (t->device() != states.device()) return std::nullopt;
     const at::ScalarType type = index_type(slots, parents);
     const int64_t W = parents && parents->dim() == 2 ? parents->size(1) : 0;
@@ -583,14 +700,39 @@ std::optional<Tensor> decay_step(const Tensor &states, const Tensor &a, const Te
         return std::nullopt;
     const c10::DeviceGuard guard(states.device());
     Tensor out = dense_like(v);
-    const int64_t strides[8] = {a.dim() == 2 ? a.stride(0) : 0, a.stride(-1), B > 1 ? v.stride(0) : 0, H > 1 ? v.stride(1) : 0,
-                                B > 1 ? k.stride(0) : 0, HK > 1 ? k.stride(1) : 0, B > 1 ? q.stride(0) : 0, HK > 1 ? q.stride(1) : 0};
-    const int rc = gla_decay_step(stream_of(states), N, B, H, HK, DK, DV, W, code(v), code(states), type == at::kLong, strides,
-                                  (const float *)a.data_ptr(), v.data_ptr(), k.data_ptr(), q.data_ptr(), slots ? slots->data_ptr() : nullptr,
-                                  parents ? parents->data_ptr() : nullptr, states.data_ptr(), out.data_ptr());
-    check("gla_decay_step", rc);
+    std::array<int64_t, 10> strides{};
+    int64_t i = 0;
+    for (const Tensor *t : {&a, &b}) {
+        if (i && !beta) break;
+        strides[i++] = t->dim() == 2 ? t->stride(0) : 0;
+        strides[i++] = t->stride(-1);
+    }
+    for (const Tensor *t : {&v, &k, &q}) {
+        strides[i++] = B > 1 ? t->stride(0) : 0;
+        strides[i++] = t->size(1) > 1 ? t->stride(1) : 0;
+    }
+    const void *at_slots = slots ? slots->data_ptr() : nullptr, *at_parents = parents ? parents->data_ptr() : nullptr;
+    const float *decays = (const float *)a.data_ptr();
+    if (beta)
+        check("gla_delta_step", gla_delta_step(stream_of(states), N, B, H, HK, DK, DV, W, code(v), code(states), type == at::kLong, strides.data(),
+                                               decays, (const float *)b.data_ptr(), v.data_ptr(), k.data_ptr(), q.data_ptr(), at_slots,
+                                               at_parents, states.data_ptr(), out.data_ptr()));
+    else
+        check("gla_decay_step", gla_decay_step(stream_of(states), N, B, H, HK, DK, DV, W, code(v), code(states), type == at::kLong, strides.data(),
+                                               decays, v.data_ptr(), k.data_ptr(), q.data_ptr(), at_slots, at_parents, states.data_ptr(),
+                                               out.data_ptr()));
     updated(states);
     return out;
+}
+std::optional<Tensor> decay_step(const Tensor &states, const Tensor &a, const Tensor &v, const Tensor &k, const Tensor &q,
+                                 const std::optional<Tensor> &slots, const std::optional<Tensor> &parents)
+{
+    return one_step(states, a, nullptr, v, k, q, slots, parents);
+}
+std::optional<Tensor> delta_step(const Tensor &states, const Tensor &a, const Tensor &b, const Tensor &v, const Tensor &k, const Tensor &q,
+                                 const std::optional<Tensor> &slots, const std::optional<Tensor> &parents)
+{
+    return one_step(states, a, &b, v, k, q, slots, parents);
 }
 
 // ---- beam search ----------------------------------------------------------------------------------
@@ -660,6 +802,8 @@ PYBIND11_MODULE(_gla_torch, m)
     m.def("rnn", &rnn, NoGil());
     m.def("decay", &decay, NoGil());
     m.def("decay_step", &decay_step, NoGil());
+    m.def("delta", &delta, NoGil());
+    m.def("delta_step", &delta_step, NoGil());
     m.def("beam_select", &beam_select, NoGil());
     m.def("reorder", &reorder, NoGil());
 }

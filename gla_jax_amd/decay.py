@@ -255,52 +255,58 @@ def _refuse_tangents(name, *arrays):
         raise RuntimeError(f"{name} has no forward-mode rule: an array carries a tangent")
 
 
+def _step(entry, states, gates, value, key, query, slots, parents):
+    """One launch of `entry` with all of its checks; `gates`: pairs of a name and an array [B,H] or [H]."""
+    _check((("states", states), *gates, ("value", value), ("key", key), ("query", query)),
+           states.device if isinstance(states, torch.Tensor) else None)
+    if value.ndim != 3 or key.ndim != 3 or query.shape != key.shape or key.shape[0] != value.shape[0]:
+        raise AssertionError("value must be [B, H, DV], key and query [B, HK, DK]")
+    B, H, DV = value.shape
+    HK, DK = key.shape[1:]
+    _check_heads(value, key, query, HK, H)
+    if states.ndim != 4 or tuple(states.shape[1:]) != (H, DK, DV):
+        raise AssertionError(f"states shape {tuple(states.shape)} != {('N', H, DK, DV)}")
+    if states.dtype not in _DT:
+        raise TypeError("states must be float32 or bfloat16")
+    if not states.is_contiguous() or states.data_ptr() % 16 or DK % 16 or DV % 16:
+        raise AssertionError("states are updated where they lie: dense, on 16 bytes, DK and DV multiples of 16")
+    for name, t in gates:
+        if tuple(t.shape) not in ((B, H), (H,)):
+            raise AssertionError(f"{name} shape {tuple(t.shape)} is neither {(B, H)} nor {(H,)}")
+    if slots is None and states.shape[0] < B:
+        raise AssertionError(f"{states.shape[0]} states for {B} rows")
+    if slots is not None:
+        slots = _indices("slots", slots, (B,), states.device)
+    W = 0
+    if parents is not None:
+        if parents.ndim != 2 or parents.shape[0] * parents.shape[1] != B:
+            raise AssertionError(f"parents shape {tuple(parents.shape)} does not hold {B} rows")
+        W = parents.shape[1]
+        if W > _lib.GLA_MOST_BEAMS:
+            raise AssertionError(f"{W} beams: at most {_lib.GLA_MOST_BEAMS} are built")
+        parents = _indices("parents", parents, tuple(parents.shape), states.device)
+    if B == 0 or H == 0 or states.shape[0] == 0:
+        return torch.zeros_like(value)
+    wide, (slots, parents) = _same_width(slots, parents)
+    v, k, q = (_rows(t, value.dtype) for t in (value, key, query))
+    gates = [t.to(torch.float32).expand(B, H) for _, t in gates]
+    with torch.cuda.device(states.device):
+        out = torch.empty(B, H, DV, dtype=v.dtype, device=v.device)
+        rc = getattr(_lib.load(), entry)(_stream(), states.shape[0], B, H, HK, DK, DV, W, _DT[v.dtype], _DT[states.dtype], wide,
+                                         _strides(*((t, 2) for t in (*gates, v, k, q))), *(_ptr(t) for t in gates), _ptr(v), _ptr(k),
+                                         _ptr(q), _ptr(slots), _ptr(parents), _ptr(states), _ptr(out))
+    _lib.check(entry, rc)
+    torch.autograd.graph.increment_version(states)
+    return out
+
+
 class _DecayStep(torch.autograd.Function):
     """decay_step for arrays that are not as the native host side takes them, and under a tracer, which records a Function as a call of
     it.  So all checks are here, where a recorded call makes them again.  There is no gradient."""
 
     @staticmethod
     def forward(states, log_decay, value, key, query, slots, parents):
-        arrays = (("states", states), ("log_decay", log_decay), ("value", value), ("key", key), ("query", query))
-        _check(arrays, states.device if isinstance(states, torch.Tensor) else None)
-        if value.ndim != 3 or key.ndim != 3 or query.shape != key.shape or key.shape[0] != value.shape[0]:
-            raise AssertionError("value must be [B, H, DV], key and query [B, HK, DK]")
-        B, H, DV = value.shape
-        HK, DK = key.shape[1:]
-        _check_heads(value, key, query, HK, H)
-        if states.ndim != 4 or tuple(states.shape[1:]) != (H, DK, DV):
-            raise AssertionError(f"states shape {tuple(states.shape)} != {('N', H, DK, DV)}")
-        if states.dtype not in _DT:
-            raise TypeError("states must be float32 or bfloat16")
-        if not states.is_contiguous() or states.data_ptr() % 16 or DK % 16 or DV % 16:
-            raise AssertionError("states are updated where they lie: dense, on 16 bytes, DK and DV multiples of 16")
-        if tuple(log_decay.shape) not in ((B, H), (H,)):
-            raise AssertionError(f"log_decay shape {tuple(log_decay.shape)} is neither {(B, H)} nor {(H,)}")
-        if slots is None and states.shape[0] < B:
-            raise AssertionError(f"{states.shape[0]} states for {B} rows")
-        if slots is not None:
-            slots = _indices("slots", slots, (B,), states.device)
-        W = 0
-        if parents is not None:
-            if parents.ndim != 2 or parents.shape[0] * parents.shape[1] != B:
-                raise AssertionError(f"parents shape {tuple(parents.shape)} does not hold {B} rows")
-            W = parents.shape[1]
-            if W > _lib.GLA_MOST_BEAMS:
-                raise AssertionError(f"{W} beams: at most {_lib.GLA_MOST_BEAMS} are built")
-            parents = _indices("parents", parents, tuple(parents.shape), states.device)
-        if B == 0 or H == 0 or states.shape[0] == 0:
-            return torch.zeros_like(value)
-        wide, (slots, parents) = _same_width(slots, parents)
-        v, k, q = (_rows(t, value.dtype) for t in (value, key, query))
-        a = log_decay.to(torch.float32).expand(B, H)
-        with torch.cuda.device(states.device):
-            out = torch.empty(B, H, DV, dtype=v.dtype, device=v.device)
-            rc = _lib.load().gla_decay_step(_stream(), states.shape[0], B, H, HK, DK, DV, W, _DT[v.dtype], _DT[states.dtype], wide,
-                                            _strides((a, 2), (v, 2), (k, 2), (q, 2)), _ptr(a), _ptr(v), _ptr(k), _ptr(q), _ptr(slots),
-                                            _ptr(parents), _ptr(states), _ptr(out))
-        _lib.check("gla_decay_step", rc)
-        torch.autograd.graph.increment_version(states)
-        return out
+        return _step("gla_decay_step", states, (("log_decay", log_decay),), value, key, query, slots, parents)
 
     @staticmethod
     def setup_context(ctx, inputs, output):

@@ -296,6 +296,42 @@ int gla_decay_step(void *stream, int64_t pool, int64_t B, int64_t H, int64_t HK,
                    const void *value, const void *key, const void *query, const void *slots, const void *parents, void *states,
                    void *out);
 
+/* ---- linear attention by the gated delta rule ----------------------------------------------------- */
+
+/* S_t = (1 - b_t k_t k_t^T) exp(a_t) S_{t-1} + b_t k_t v_t^T,  o_t = S_t^T q_t: the state forgets by one number a head and token, and then
+ * writes only what it does not answer the key with yet, a share b_t of it.  No counterpart in the reference.  Arrays, strides, lengths
+ * and the rules for them are those of gla_decay_fwd and gla_decay_bwd, with
+ *   beta [B,T,H] float32 (any strides)
+ * and DK at most GLA_MOST_DELTA_KEYS.  `strides` holds batch, token and head strides of log_decay, beta, value, key and query: 15 numbers.  Keys of a length of at
+ * most sqrt(2 / beta) keep the states bounded; others are taken as they are. */
+
+#define GLA_MOST_DELTA_KEYS 128
+
+/* Bytes of the `states` that gla_delta_fwd leaves for gla_delta_bwd: the states before every chunk (of 64 tokens, float32 data: 32) and at the
+ * end, and what every token wrote, in float32. */
+size_t gla_delta_states_bytes(int64_t B, int64_t T, int64_t H, int64_t HK, int64_t DK, int64_t DV, gla_dtype dtype);
+/* Bytes of scratch (0: none is needed and it may be NULL). */
+size_t gla_delta_fwd_workspace_bytes(int64_t B, int64_t T, int64_t H, int64_t HK, int64_t DK, int64_t DV, gla_dtype dtype);
+size_t gla_delta_bwd_workspace_bytes(int64_t B, int64_t T, int64_t H, int64_t HK, int64_t DK, int64_t DV, gla_dtype dtype);
+/* `states` may be NULL when no gradient will be taken. */
+int gla_delta_fwd(void *stream, int64_t B, int64_t T, int64_t H, int64_t HK, int64_t DK, int64_t DV, gla_dtype dtype,
+                  gla_dtype hidden_dtype, const int64_t *strides, const void *hidden_init, const float *log_decay, const float *beta,
+                  const void *value, const void *key, const void *query, const int32_t *lengths, void *hidden_final, void *out,
+                  void *states, void *workspace, size_t workspace_bytes);
+/* Gradients, dense, in the types of their arrays.  dout is dense. */
+int gla_delta_bwd(void *stream, int64_t B, int64_t T, int64_t H, int64_t HK, int64_t DK, int64_t DV, gla_dtype dtype,
+                  gla_dtype hidden_dtype, const int64_t *strides, const float *log_decay, const float *beta, const void *value,
+                  const void *key, const void *query, const int32_t *lengths, const void *states, const void *dhidden_final,
+                  const void *dout, void *dhidden_init, float *dlog_decay, float *dbeta, void *dvalue, void *dkey, void *dquery,
+                  void *workspace, size_t workspace_bytes);
+
+/* gla_decay_step by the gated delta rule: beta [B,H] float32; `strides` holds the batch and head strides of log_decay, beta, value, key and
+ * query, 10 numbers.  DK up to 256. */
+int gla_delta_step(void *stream, int64_t pool, int64_t B, int64_t H, int64_t HK, int64_t DK, int64_t DV, int64_t beams,
+                   gla_dtype dtype, gla_dtype state_dtype, int wide_indices, const int64_t *strides, const float *log_decay,
+                   const float *beta, const void *value, const void *key, const void *query, const void *slots, const void *parents,
+                   void *states, void *out);
+
 /* ---- beam search --------------------------------------------------------------------------------- */
 
 /* The `num` (at most 64) best continuations of every group's beams: logits [groups,beams,vocab] with `row` elements from one
