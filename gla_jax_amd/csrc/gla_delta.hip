@@ -28,7 +28,7 @@ int check_sizes(const DecaySizes &n, gla_dtype dtype)
 // Assigns the places of a call's scratch behind `ws` (which may be NULL: for the size alone); what the backward pass takes more of.
 int64_t lay_out(DeltaArgs &a, gla_dtype dtype, bool backward, char *ws, float **dquery, float **dkey)
 {
-    const int64_t C = chunk_of(dtype), e = bytes_of(dtype), parts = dtype == GLA_BF16 ? 2 : 1, chunk_pairs = a.pairs * a.chunks;
+    const int64_t C = chunk_of(dtype), e = bytes_of(dtype), parts = dtype == GLA_BF16 ? DeltaChunk<__bf16>::kParts : 1, chunk_pairs = a.pairs * a.chunks;
     const int64_t steps = dtype == GLA_BF16 ? DeltaChunk<__bf16>::kSteps : DeltaChunk<float>::kSteps;
     int64_t at = 0;
     auto take = [&](int64_t bytes) {
@@ -43,10 +43,9 @@ int64_t lay_out(DeltaArgs &a, gla_dtype dtype, bool backward, char *ws, float **
     a.to.queries = backward ? take(columns) : nullptr;
     a.to.gates = reinterpret_cast<float *>(take(chunk_pairs * 4 * C * 4));
     if (!backward) return at;
-    a.dot_slabs = (int)((a.n.DV + delta_wave_columns(a.n) - 1) / delta_wave_columns(a.n));
     a.du = reinterpret_cast<float *>(take(a.pairs * delta_written_floats(a.n, a.chunks, (int)C) * 4));
     a.dstates = take(chunk_pairs * a.n.DK * a.n.DV * e);
-    a.dots = reinterpret_cast<float *>(take(chunk_pairs * a.dot_slabs * 4));
+    a.dots = reinterpret_cast<float *>(take(chunk_pairs * (a.n.DV / 16) * 4 * 4));
     a.row_parts = (int)(a.n.H / a.n.HK);
     if (a.row_parts > 1) {
         const int64_t rows = a.row_parts * a.n.B * a.n.T * a.n.HK * a.n.DK * 4;

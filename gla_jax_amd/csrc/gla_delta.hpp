@@ -8,13 +8,16 @@
 // So the work is in two kinds of kernels.  delta_prepare_kernel, all chunks at once, forms the inverses and the scores.  The walks go
 // through a sequence's chunks with the state in the accumulators of their matrix instructions, and need nothing but products.
 //
-// A wave walks alone: it holds 16 or 32 value columns of the state, and all that it multiplies by comes from memory as operands of its matrix
-// instructions, keys and queries as they lie and the rest in the order in which delta_prepare_kernel's lanes held it.  No LDS, no
-// barrier, and where there are few sequences their columns are spread over the compute units.
+// A workgroup of four waves walks: it holds 16 to 64 value columns of the state, each wave a quarter of the features and, of a chunk's
+// products, 16 tokens.  Three times a chunk they hand each other operands through LDS: the state, r, and u.  Everything else comes from memory in the
+// order of the matrix instructions' operands, keys and queries as they lie and the rest as delta_prepare_kernel's lanes held it,
+// requested a chunk ahead.  Where there are few sequences their columns are spread over the compute units.
 //
 // Precision.  Keys, queries and values are 16-bit numbers as they come.  What a 32-bit result (states, gradients of the gates) depends on
-// and is formed in between, i.e. the state, the inverse, r and u, enters a product as two or three bf16 parts (Split): two are off by 2^-18 of a
-// value at most.  What only a 16-bit result depends on is rounded to 16 bits once.  float data take the matrix cores' float products.
+// and is formed in between enters a product as bf16 parts (Split): the inverse, r, u and the scores of the backward walk in three, 2^-25 of a value, the
+// state where keys meet it in two, 2^-18 (against values that it is subtracted from; three changed no digit).  What only a 16-bit
+// result depends on is rounded to 16 bits once, but for the state in out, in two parts that are there.  float data take the matrix cores'
+// float products.
 //
 // Operand layouts: gla_decay.hpp.  Rows of the state are the features pi(t, m) of gla_chunk_common.hpp, so that two accumulators above each
 // other (tiles 2p and 2p + 1) are features 32p + 8c .. + 7: an operand of the contraction with keys in their natural order.
@@ -26,7 +29,8 @@ namespace gla {
 
 template <typename T> struct DeltaChunk {
     static constexpr int C = DecayChunk<T>::C, CT = C / 16, CS = C / 32;
-    static constexpr int kParts = sizeof(T) == 2 ? 2 : 1;      // of an operand that is a 32-bit number
+    static constexpr int kParts = sizeof(T) == 2 ? 3 : 1;      // of an operand that is a 32-bit number
+    static constexpr int kFew = sizeof(T) == 2 ? 2 : 1;        // of the state where keys or queries meet it
     // steps of 32 tokens of a triangle's rows of tiles, 512 values each: lower ones have step ks <= t / 2, upper ones ks >= t / 2
     static constexpr int kSteps = CS == 1 ? CT : 6;
     static constexpr int lower(int t, int ks) { return t < 2 ? t : 2 * t - 2 + ks; }
@@ -56,12 +60,11 @@ struct DeltaArgs {
     // what the forward pass leaves for the backward: of each pair the states before its chunks and at its end, [chunks + 1][DV][DK], and x,
     // [chunks][DV / 16][C / 16][4][16][4], floats
     float *kept;
-    // what the backward walk leaves for the gradients: the same of the cotangent of u (all parts of it), and the cotangents of the states behind the
-    // chunks, [chunks][DV][DK] in T, and <state, its cotangent> there, [pairs, chunks][value columns / columns of a wave]
+    // what the backward walk leaves for the gradients: the cotangents of u in the order of x, the cotangents of the states behind the
+    // chunks, [chunks][DV][DK] in T, and <state, its cotangent> there, [pairs, chunks][columns / 16][4]
     float *du;
     void *dstates;
     float *dots;
-    int dot_slabs;
     void *dvalue, *dkey, *dquery;   // dkey, dquery: in their own type, or (more than one part) floats [part][...]
     float *dgate, *dbeta;
     int row_parts;
@@ -90,12 +93,15 @@ template <int F> __device__ __forceinline__ f32x8 feature_columns(const float *p
     return x;
 }
 
-// A product of two operands in two parts each, without the product of the small ones (2^-18 of it).
-__device__ __forceinline__ f32x4 mma_parts(const bf16x8 (&a)[2], const bf16x8 (&b)[2], f32x4 c)
+// A product of two operands in N parts each, without the products below 2^-9N of it; the small ones first.
+template <typename D8, int N> __device__ __forceinline__ f32x4 mma_parts(const D8 (&a)[N], const D8 (&b)[N], f32x4 c)
 {
-    return mma_d(a[0], b[0], mma_d(a[0], b[1], mma_d(a[1], b[0], c)));
+#pragma unroll
+    for (int s = N - 1; s >= 0; --s)
+#pragma unroll
+        for (int i = 0; i <= s; ++i) c = mma_d(a[i], b[s - i], c);
+    return c;
 }
-__device__ __forceinline__ f32x4 mma_parts(const f32x8 (&a)[1], const f32x8 (&b)[1], f32x4 c) { return mma_d(a[0], b[0], c); }
 // and of one in parts with one that is whole
 template <typename D8, int N> __device__ __forceinline__ f32x4 mma_whole(const D8 &a, const D8 (&b)[N], f32x4 c)
 {
@@ -115,6 +121,5 @@ int delta_walk(void *stream, const DeltaArgs &a, gla_dtype dtype, bool backward)
 int delta_gradients(void *stream, const DeltaArgs &a, gla_dtype dtype);
 // dst <- the sum over the heads of a key head of parts [H / HK][B,T,HK,DK], in order
 int delta_sum_heads(void *stream, const DecaySizes &n, gla_dtype dtype, const float *parts, void *dst);
-int64_t delta_wave_columns(const DecaySizes &n);
 
 }  // namespace gla

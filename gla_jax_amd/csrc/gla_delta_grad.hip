@@ -23,7 +23,7 @@ template <typename T, int F> __device__ __forceinline__ int place_in(int row, in
 template <typename T, int DKP> __global__ __launch_bounds__(DKP * 4) void delta_gradient_kernel(const DeltaArgs a)
 {
     typedef DeltaChunk<T> DC;
-    constexpr int C = DC::C, CT = DC::CT, CS = DC::CS, KS = DKP / 32, NW = DKP / 16, NT = 64 * NW, VS = kSlice / 32, kParts = DC::kParts;
+    constexpr int C = DC::C, CT = DC::CT, CS = DC::CS, KS = DKP / 32, NW = DKP / 16, NT = 64 * NW, VS = kSlice / 32, kParts = DC::kFew;
     constexpr int kTriangle = CT * (CT + 1) / 2, kUnits = (2 * kTriangle + NW - 1) / NW, kShare = NW / CT;
     typedef typename FragTypes<T>::d8 D8;
     typedef typename Packed4<T>::t Four;
@@ -269,7 +269,7 @@ template <typename T, int DKP> __global__ __launch_bounds__(DKP * 4) void delta_
             if (lane >= there) x = 0.0;
         }
         double behind = 0.0;
-        for (int i = 0; i < a.dot_slabs; ++i) behind += a.dots[(pair * chunks + n) * a.dot_slabs + i];
+        for (int i = 0; i < DV / 4; ++i) behind += a.dots[(pair * chunks + n) * (DV / 4) + i];
         const double before = prefix_sum_wave(x), all = __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(before), 63),
                                                                          __builtin_amdgcn_readlane(__double2loint(before), 63));
         if (lane < C && first + lane < T_) {
@@ -315,7 +315,7 @@ template <typename T, int DKP> int launch_gradient(hipStream_t stream, const Del
 {
     typedef DeltaChunk<T> DC;
     static LdsGrant grant;
-    constexpr int C = DC::C, NW = DKP / 16, kParts = DC::kParts;
+    constexpr int C = DC::C, NW = DKP / 16, kParts = DC::kFew;
     constexpr size_t lds = sizeof(T) * ((2 * C + (kParts + 1) * kSlice) * LdsTile<T, DKP>::kRow + C * LdsTile<T, kSlice>::kRow +
                                         ((kParts + 1) * kSlice + 2 * C) * LdsTile<T, C>::kRow) +
                            sizeof(ChunkGates<C>) + sizeof(float) * C * (1 + DC::CT + NW + 2 * (NW / DC::CT));
