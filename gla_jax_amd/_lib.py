@@ -15,6 +15,7 @@ GLA_F32, GLA_BF16 = 0, 1
 ABI_VERSION = 3                             # GLA_HIP_ABI_VERSION of include/gla_hip.h
 GLA_MOST_BEAMS = GLA_MOST_CANDIDATES = 64
 GLA_MOST_DELTA_KEYS = 128
+GLA_MOST_ALTERNATIVES = 64
 GLA_CHUNK_FWD_STATIC_BYTES = 80 << 20      # capacity of gla_chunk_fwd_static's workspace (gla_hip.h)
 
 _i64, _int, _vp, _sz = ctypes.c_int64, ctypes.c_int, ctypes.c_void_p, ctypes.c_size_t
@@ -58,6 +59,8 @@ SIGNATURES = {
     "gla_delta_step": (_int, [_vp] + [_i64] * 7 + [_int] * 3 + [_vp] * 10),
     "gla_beam_select_workspace_bytes": (_sz, [_i64] * 4),
     "gla_beam_select": (_int, [_vp] + [_i64] * 4 + [_int, _i64] + [_vp] * 3 + [_i64] + [_vp] * 4 + [_sz]),
+    "gla_token_logprobs": (_int, [_vp] + [_i64] * 3 + [_int, _i64, _int] + [_vp] * 7),
+    "gla_token_logprobs_bwd": (_int, [_vp] + [_i64] * 2 + [_int] + [_i64] * 2 + [_int] + [_vp] * 7),
     "gla_reorder_states": (_int, [_vp] + [_i64] * 4 + [_int] + [_vp] * 3),
 }
 

@@ -790,6 +790,131 @@ bool reorder(const Tensor &states, const Tensor &parents, const std::optional<Te
     return true;
 }
 
+// ---- log probabilities ----------------------------------------------------------------------------
+// Rows of logits one distance apart from each other, whatever axes lie in front.
+struct LogitRows {
+    int64_t rows, vocab, row;
+};
+std::optional<LogitRows> logit_rows(const Tensor &x)
+{
+    const int64_t n = x.dim();
+    if (!x.defined() || !x.is_cuda() || x.layout() != at::kStrided || n < 1 || !known(x.scalar_type()) || x.size(-1) < 1 ||
+        (x.size(-1) > 1 && x.stride(-1) != 1))
+        return std::nullopt;
+    LogitRows r{1, x.size(-1), 0};
+    int64_t step = 0;
+    for (int64_t i = n - 2; i >= 0; --i) {
+        const int64_t m = x.size(i);
+        if (m > 1) {
+            if (r.rows == 1) step = r.row = x.stride(i);
+            else if (x.stride(i) != step) return std::nullopt;
+        }
+        r.rows *= m;
+        step *= m;
+    }
+    if (r.rows <= 1) r.row = r.vocab;
+    if (r.rows < 1 || r.row < r.vocab) return std::nullopt;
+    return r;
+}
+bool logprob_arrays(const Tensor &logits, const Tensor &tokens)
+{
+    return dense_on_gpu(tokens) && (tokens.scalar_type() == at::kInt || tokens.scalar_type() == at::kLong) && tokens.device() == logits.device() &&
+           tokens.dim() == logits.dim() - 1 && tokens.sizes() == logits.sizes().slice(0, logits.dim() - 1);
+}
+
+struct Logprobs {
+    Tensor given, entropy, near, index, stats;
+};
+Logprobs logprobs_forward(const Tensor &logits, const Tensor &tokens, int64_t top, bool residual)
+{
+    const c10::DeviceGuard guard(logits.device());
+    const LogitRows n = *logit_rows(logits);
+    const auto floats = logits.options().dtype(at::kFloat);
+    Logprobs r{at::empty(tokens.sizes(), floats), at::empty(tokens.sizes(), floats), Tensor(), Tensor(), Tensor()};
+    if (top) {
+        std::vector<int64_t> sizes = tokens.sizes().vec();
+        sizes.push_back(top);
+        r.near = at::empty(sizes, floats);
+        r.index = at::empty(sizes, floats.dtype(at::kLong));
+    }
+    if (residual) r.stats = at::empty({n.rows, 2}, floats);
+    check("gla_token_logprobs",
+          gla_token_logprobs(stream_of(logits), n.rows, n.vocab, top, code(logits), n.row, tokens.scalar_type() == at::kLong, logits.data_ptr(),
+                             tokens.data_ptr(), (float *)r.given.data_ptr(), (float *)r.entropy.data_ptr(),
+                             residual ? (float *)r.stats.data_ptr() : nullptr, top ? (float *)r.near.data_ptr() : nullptr,
+                             top ? (int64_t *)r.index.data_ptr() : nullptr));
+    return r;
+}
+Tensor logprobs_backward(const Tensor &logits, const Tensor &tokens, const Tensor &stats, const Tensor &entropy, const Tensor &dgiven,
+                         const Tensor &dentropy)
+{
+    const c10::DeviceGuard guard(logits.device());
+    const LogitRows n = *logit_rows(logits);
+    // rows that begin at the same place within 16 bytes as those of the logits: as long, or as those are where they lie apart
+    const int64_t piece = 16 / (int64_t)logits.element_size(), odd = (n.row - n.vocab) % piece;
+    const int64_t row = n.rows > 1 ? n.vocab + odd : n.vocab;
+    const int64_t ahead = (int64_t)(reinterpret_cast<uintptr_t>(logits.data_ptr()) % 16) / (int64_t)logits.element_size();
+    Tensor d = at::empty({ahead + n.rows * row}, logits.options());
+    TORCH_CHECK(reinterpret_cast<uintptr_t>(d.data_ptr()) % 16 == 0, "an allocation that does not begin on 16 bytes");
+    check("gla_token_logprobs_bwd",
+          gla_token_logprobs_bwd(stream_of(logits), n.rows, n.vocab, code(logits), n.row, row, tokens.scalar_type() == at::kLong, logits.data_ptr(),
+                                 tokens.data_ptr(), (const float *)stats.data_ptr(), (const float *)entropy.data_ptr(),
+                                 dgiven.defined() ? (const float *)dgiven.data_ptr() : nullptr,
+                                 dentropy.defined() ? (const float *)dentropy.data_ptr() : nullptr,
+                                 (char *)d.data_ptr() + ahead * logits.element_size()));
+    std::vector<int64_t> strides(logits.dim());
+    int64_t step = row;
+    strides.back() = 1;
+    for (int64_t i = logits.dim() - 2; i >= 0; --i) {
+        strides[i] = step;
+        step *= logits.size(i);
+    }
+    return d.as_strided(logits.sizes(), strides, ahead);
+}
+struct LogprobsBackward : torch::autograd::Function<LogprobsBackward> {
+    static variable_list forward(AutogradContext *, const Tensor &logits, const Tensor &tokens, const Tensor &stats, const Tensor &entropy,
+                                 const Tensor &dgiven, const Tensor &dentropy)
+    {
+        return {logprobs_backward(logits, tokens, stats, entropy, dgiven, dentropy)};
+    }
+    static variable_list backward(AutogradContext *, variable_list) { no_double_backward("token_logprobs"); }
+};
+struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
+    static variable_list forward(AutogradContext *ctx, const Tensor &logits, const Tensor &tokens, int64_t top)
+    {
+        Logprobs r = logprobs_forward(logits, tokens, top, true);
+        ctx->save_for_backward({logits, tokens, r.stats, r.entropy});
+        ctx->set_materialize_grads(false);
+        if (!top) return {r.given, r.entropy};
+        ctx->mark_non_differentiable({r.near, r.index});
+        return {r.given, r.entropy, r.near, r.index};
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list d)
+    {
+        variable_list s = ctx->get_saved_variables();
+        check_saved(s[0].is_cuda() && known(s[0].scalar_type()));
+        if (!logit_rows(s[0])) s[0] = s[0].contiguous();
+        s[1] = s[1].contiguous();
+        check_saved(logprob_arrays(s[0], s[1]) && s[2].is_contiguous() && s[3].is_contiguous() && s[2].numel() == 2 * s[1].numel() &&
+                    s[3].numel() == s[1].numel() && s[2].scalar_type() == at::kFloat && s[3].scalar_type() == at::kFloat &&
+                    s[2].device() == s[0].device() && s[3].device() == s[0].device());
+        const Tensor dgiven = cotangent(d[0], s[1].sizes(), at::kFloat, s[0]), dentropy = cotangent(d[1], s[1].sizes(), at::kFloat, s[0]);
+        const variable_list r = transforms_active() ? python_rule("gla_jax_amd.logprobs", "_TokenLogprobsBwd", s[0], s[1], s[2], s[3], dgiven, dentropy)
+                                : at::GradMode::is_enabled() ? LogprobsBackward::apply(s[0], s[1], s[2], s[3], dgiven, dentropy)
+                                                             : variable_list{logprobs_backward(s[0], s[1], s[2], s[3], dgiven, dentropy)};
+        return {r[0], Tensor(), Tensor()};
+    }
+};
+Result token_logprobs(const Tensor &logits, const Tensor &tokens, int64_t top)
+{
+    if (traced() || !logit_rows(logits) || !logprob_arrays(logits, tokens) || top < 0 || top > GLA_MOST_ALTERNATIVES || top > logits.size(-1))
+        return std::nullopt;
+    if (takes_gradient({logits})) return TokenLogprobs::apply(logits, tokens, top);
+    Logprobs r = logprobs_forward(logits, tokens, top, false);
+    if (!top) return std::vector<Tensor>{r.given, r.entropy};
+    return std::vector<Tensor>{r.given, r.entropy, r.near, r.index};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_gla_torch, m)
@@ -806,4 +931,5 @@ PYBIND11_MODULE(_gla_torch, m)
     m.def("delta_step", &delta_step, NoGil());
     m.def("beam_select", &beam_select, NoGil());
     m.def("reorder", &reorder, NoGil());
+    m.def("token_logprobs", &token_logprobs, NoGil());
 }

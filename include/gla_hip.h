@@ -351,6 +351,25 @@ int gla_beam_select(void *stream, int64_t groups, int64_t beams, int64_t vocab, 
 int gla_reorder_states(void *stream, int64_t pool, int64_t groups, int64_t beams, int64_t row_bytes, int wide_indices,
                        const void *parents, const void *slots, void *states);
 
+/* ---- log probabilities ---------------------------------------------------------------------------- */
+
+#define GLA_MOST_ALTERNATIVES 64
+
+/* Of every row of logits [rows,vocab], `row` elements from one to the next: the log softmax of its given token, the entropy of its distribution
+ * (in nats), and the `top` (at most 64) largest log probabilities with their tokens, largest first, of equal ones the lower token.  `tokens`
+ * (int32, or int64 with wide_indices != 0): one outside 0..vocab-1 marks a row that does not count, whose logits are not read: logprobs and
+ * entropy are 0, its alternatives -inf and -1.  Logits of -inf have probability 0; a row with a logit that is not a number, or of +inf, or with
+ * none above -inf, has results that are not numbers (such logits count as -inf in the order of the alternatives).
+ * `stats` [rows,2] is what the backward needs, or NULL.  Any alignment of the rows. */
+int gla_token_logprobs(void *stream, int64_t rows, int64_t vocab, int64_t top, gla_dtype dtype, int64_t row, int wide_indices,
+                       const void *logits, const void *tokens, float *logprobs, float *entropy, float *stats, float *top_logprobs,
+                       int64_t *top_tokens);
+/* The gradient of the logits from the cotangents of logprobs and entropy [rows] (NULL: zero).  dlogits has `grad_row` elements from one row to the next,
+ * and its rows begin at the same place within 16 bytes as those of logits.  Rows that do not count get zeros. */
+int gla_token_logprobs_bwd(void *stream, int64_t rows, int64_t vocab, gla_dtype dtype, int64_t row, int64_t grad_row, int wide_indices,
+                           const void *logits, const void *tokens, const float *stats, const float *entropy, const float *dlogprobs,
+                           const float *dentropy, void *dlogits);
+
 #ifdef __cplusplus
 }
 #endif
