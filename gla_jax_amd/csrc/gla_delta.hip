@@ -41,10 +41,12 @@ int64_t lay_out(DeltaArgs &a, gla_dtype dtype, bool backward, char *ws, float **
     a.to.scores = take(chunk_pairs * steps * (backward ? parts : 1) * 512 * e);
     a.to.keys = take(columns);
     a.to.queries = backward ? take(columns) : nullptr;
+    a.to.key_rows = take(columns);
+    a.to.query_rows = backward ? nullptr : take(columns);
     a.to.gates = reinterpret_cast<float *>(take(chunk_pairs * 4 * C * 4));
     if (!backward) return at;
     a.du = reinterpret_cast<float *>(take(a.pairs * delta_written_floats(a.n, a.chunks, (int)C) * 4));
-    a.dstates = take(chunk_pairs * a.n.DK * a.n.DV * e);
+    a.dstates = take(chunk_pairs * delta_state_floats(a.n) * e);
     a.dots = reinterpret_cast<float *>(take(chunk_pairs * (a.n.DV / 16) * 4 * 4));
     a.row_parts = (int)(a.n.H / a.n.HK);
     if (a.row_parts > 1) {

@@ -10,8 +10,9 @@
 //
 // A workgroup of four waves walks: it holds 16 to 64 value columns of the state, each wave a quarter of the features and, of a chunk's
 // products, 16 tokens.  Three times a chunk they hand each other operands through LDS: the state, r, and u.  Everything else comes from memory in the
-// order of the matrix instructions' operands, keys and queries as they lie and the rest as delta_prepare_kernel's lanes held it,
-// requested a chunk ahead.  Where there are few sequences their columns are spread over the compute units.
+// order of the matrix instructions' operands, as delta_prepare_kernel's lanes held it, requested a chunk ahead: a wave's load is then 1 KB
+// in one piece.  (Keys and queries as they lie are 64 pieces of 16 bytes a load, each a cycle of the cache's: of a chunk's 4900 cycles a wave
+// spent 900 to 1500 on issuing them.)  Where there are few sequences their columns are spread over the compute units.
 //
 // Precision.  Keys, queries and values are 16-bit numbers as they come.  What a 32-bit result (states, gradients of the gates) depends on
 // and is formed in between enters a product as bf16 parts (Split): the inverse, r, u and the scores of the backward walk in three, 2^-25 of a value, the
@@ -44,6 +45,8 @@ struct DeltaPrepared {
     void *scores;       // [pairs, chunks][steps][parts, of the backward walk][64][8]
     void *keys;         // [B, HK, chunks][features / 16][C / 32][64][8]: keys with tokens as the contracted index
     void *queries;      // the same, of the backward walk
+    void *key_rows;     // [B, HK, chunks][C / 16][features / 32][64][8]: keys with features as the contracted index
+    void *query_rows;   // the same, of the forward walk
     float *gates;       // [pairs, chunks][kGates]
 };
 
@@ -57,11 +60,12 @@ struct DeltaArgs {
     int hidden_dtype;
     void *hidden_out;               // hidden_final; dhidden_init
     void *out;
-    // what the forward pass leaves for the backward: of each pair the states before its chunks and at its end, [chunks + 1][DV][DK], and x,
-    // [chunks][DV / 16][C / 16][4][16][4], floats
+    // what the forward pass leaves for the backward, floats in the order of accumulators, four features or tokens of a column together: of
+    // each pair the states before its chunks and at its end, [chunks + 1][DV / 16][tiles of features][4][16][4], and x,
+    // [chunks][DV / 16][C / 16][4][16][4]
     float *kept;
-    // what the backward walk leaves for the gradients: the cotangents of u in the order of x, the cotangents of the states behind the
-    // chunks, [chunks][DV][DK] in T, and <state, its cotangent> there, [pairs, chunks][columns / 16][4]
+    // what the backward walk leaves for the gradients: the cotangents of u in the order of x, those of the states behind the chunks
+    // in the states' order, in T, and <state, its cotangent> there, [pairs, chunks][columns / 16][4]
     float *du;
     void *dstates;
     float *dots;
@@ -69,7 +73,10 @@ struct DeltaArgs {
     float *dgate, *dbeta;
     int row_parts;
 };
-inline __host__ __device__ int64_t delta_states_floats(const DecaySizes &n, int64_t chunks) { return (chunks + 1) * n.DK * n.DV; }
+// (features pi come in pairs of tiles)
+inline __host__ __device__ int delta_state_tiles(int64_t DK) { return (int)((DK + 31) / 32 * 2); }
+inline __host__ __device__ int64_t delta_state_floats(const DecaySizes &n) { return 16 * delta_state_tiles(n.DK) * n.DV; }
+inline __host__ __device__ int64_t delta_states_floats(const DecaySizes &n, int64_t chunks) { return (chunks + 1) * delta_state_floats(n); }
 inline __host__ __device__ int64_t delta_written_floats(const DecaySizes &n, int64_t chunks, int C) { return chunks * C * n.DV; }
 
 inline __host__ __device__ int64_t delta_key_width(int64_t DK) { return DK <= 64 ? 64 : 128; }

@@ -71,7 +71,7 @@ template <typename T, int DKP> __global__ __launch_bounds__(DKP * 4) void delta_
     const T *V = static_cast<const T *>(a.values.p) + b * a.values.sb + h * a.values.sh + first * a.values.st;
     const T *O = static_cast<const T *>(a.dout.p) + b * a.dout.sb + h * a.dout.sh + first * a.dout.st;
     const float *G = static_cast<const float *>(a.gates.p) + b * a.gates.sb + h * a.gates.sh + first * a.gates.st;
-    const int64_t floats = delta_written_floats(a.n, a.chunks, C), state = (int64_t)DK * DV;
+    const int64_t floats = delta_written_floats(a.n, a.chunks, C), state = delta_state_floats(a.n);
     const float *kept = a.kept + pair * (delta_states_floats(a.n, a.chunks) + floats), *xs = kept + delta_states_floats(a.n, a.chunks) + n * C * DV;
     const float *dus = a.du + pair * floats + n * C * DV;
     const T *dS = static_cast<const T *>(a.dstates) + (pair * chunks + n) * state;
@@ -105,21 +105,23 @@ template <typename T, int DKP> __global__ __launch_bounds__(DKP * 4) void delta_
         {
             RowsInFlight<T, C, kSlice, NT> o;
             o.load(tid, O + dv0, (int)a.dout.st, there, DV - dv0);
-            // states: a thread's pieces of 8 features
+            // states: four features of a value feature a lane
 #pragma unroll
-            for (int i = tid; i < kSlice * (DKP / 8); i += NT) {
-                const int row = i / (DKP / 8), col = 8 * (i % (DKP / 8)), at = TileK::piece(row, col);
-                const bool is = dv0 + row < DV && col < DK;
-                float s[8] = {};
-                D8 d{};
-                if (is) {
-                    load_vec<float, 8>(kept + (int64_t)(dv0 + row) * DK + col, s);
-                    d = ld8(dS + (int64_t)(dv0 + row) * DK + col);
+            for (int i = w; i < kSlice / 16 * (DKP / 16); i += NW) {
+                const int m = i / (DKP / 16), t = i % (DKP / 16), col = 32 * (t >> 1) + 8 * c + 4 * (t & 1), at = place_in<T, DKP>(16 * m + r, col);
+                const bool is = dv0 + 16 * m < DV && col < DK;
+                const unsigned from = is ? (((dv0 >> 4) + m) * delta_state_tiles(DK) + t) * 256 + lane * 4 : 0;
+                f32x4 s = *reinterpret_cast<const f32x4 *>(kept + from);
+                Four d = *reinterpret_cast<const Four *>(dS + from);
+                if (!is) s = f32x4{0.f, 0.f, 0.f, 0.f}, d = Four{};
+#pragma unroll
+                for (int p = 0; p < kParts; ++p) {
+                    const Four f = pack_results<T>(s);
+                    *reinterpret_cast<Four *>(sS + p * kS + at) = f;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[e] -= (float)f[e];
                 }
-                const Split<T, kParts> split(s);
-#pragma unroll
-                for (int p = 0; p < kParts; ++p) st8(sS + p * kS + at, split.part[p]);
-                st8(sD + at, d);
+                *reinterpret_cast<Four *>(sD + at) = d;
             }
             const int ti = w % CT, token = 16 * ti + 4 * c;
             const f32x4 beta = *reinterpret_cast<const f32x4 *>(sums.beta + token);

@@ -94,6 +94,13 @@ template <typename T, int DKP, bool BACK> __global__ __launch_bounds__(256) void
             st8(reinterpret_cast<T *>(keys + m * 64 + lane), feature_columns<DKP>(sK, ks, t));
             if (BACK) st8(reinterpret_cast<T *>(queries + m * 64 + lane), feature_columns<DKP>(sQ, ks, t));
         }
+        D8 *key_rows = static_cast<D8 *>(a.to.key_rows) + kc * (CT * KS * 64), *query_rows = static_cast<D8 *>(a.to.query_rows) + kc * (CT * KS * 64);
+#pragma unroll
+        for (int m = w; m < CT * KS; m += NW) {
+            const int t = m / KS, ks = m % KS;
+            st8(reinterpret_cast<T *>(key_rows + m * 64 + lane), tile.rows(sK, t, ks));
+            if (!BACK) st8(reinterpret_cast<T *>(query_rows + m * 64 + lane), tile.rows(sQ, t, ks));
+        }
     }
     if (tid < C) {
         float *to = a.to.gates + pc * DC::kGates;

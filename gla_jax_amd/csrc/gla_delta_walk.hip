@@ -4,12 +4,31 @@
 namespace gla {
 namespace {
 
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 template <typename T, int N> struct Columns { typedef T t __attribute__((ext_vector_type(N))); };
 template <typename T> struct Columns<T, 1> { typedef T t; };
 template <typename T, int N> __device__ __forceinline__ float column_of(typename Columns<T, N>::t v, int q)
 {
     if constexpr (N == 1) return (float)v;
     else return (float)v[q];
+}
+
+// Of packed results the values that they stand for, without the conversions done again.
+__device__ __forceinline__ f32x4 unpack_results(bf16x4 v)
+{
+    const auto u = __builtin_bit_cast(u32x2, v);
+    return {__uint_as_float(u[0] << 16), __uint_as_float(u[0] & 0xffff0000u), __uint_as_float(u[1] << 16), __uint_as_float(u[1] & 0xffff0000u)};
+}
+__device__ __forceinline__ f32x4 unpack_results(f32x4 v) { return v; }
+
+// Rows of a chunk as the load instructions see them: what lies behind the last row reads as zero, and a lane keeps one 32-bit place for
+// the whole walk.
+constexpr unsigned kNowhere = 0x7fffff00u;       // (rows of a chunk take at most 2^30 bytes)
+template <typename Cols> __device__ __forceinline__ Cols load_columns(__amdgpu_buffer_rsrc_t rows, unsigned at)
+{
+    if constexpr (sizeof(Cols) == 2) return __builtin_bit_cast(Cols, __builtin_amdgcn_raw_buffer_load_b16(rows, at, 0, 0));
+    else if constexpr (sizeof(Cols) == 4) return __builtin_bit_cast(Cols, __builtin_amdgcn_raw_buffer_load_b32(rows, at, 0, 0));
+    else return __builtin_bit_cast(Cols, __builtin_amdgcn_raw_buffer_load_b64(rows, at, 0, 0));
 }
 
 // What both walks share.  A workgroup of kWaves waves holds NG times 16 value columns of one (batch, head) pair's state; wave w its features
@@ -26,6 +45,12 @@ template <typename T, int DKP, int NG> struct Walk {
     unsigned pair;
     int64_t b, h, hk;
     f32x4 S[NG][PER];
+    // an array's rows: its first one, and a lane's place in a chunk's
+    struct Rows {
+        const T *p;
+        int st;
+        unsigned at[4];
+    };
     // true: there is nothing to do
     __device__ __forceinline__ bool place(const DeltaArgs &a)
     {
@@ -34,10 +59,11 @@ template <typename T, int DKP, int NG> struct Walk {
         lane = tid & 63;
         r = lane & 15;
         c = lane >> 4;
-        pair = blockIdx.x;
-        col0 = (int)blockIdx.y * 16 * NG;
         DK = (int)a.n.DK;
         DV = (int)a.n.DV;
+        const unsigned groups = ((unsigned)DV + 16 * NG - 1) / (16 * NG), turn = blockIdx.x / 8;
+        pair = turn / groups * 8 + blockIdx.x % 8;
+        col0 = (int)(turn % groups) * 16 * NG;
         if (pair >= (unsigned)a.pairs) return true;
         const unsigned H = (unsigned)a.n.H;
         b = pair / H;
@@ -57,17 +83,23 @@ template <typename T, int DKP, int NG> struct Walk {
     }
     __device__ __forceinline__ void load_state(const void *from, int dtype)
     {
+        auto load = [&](auto *rows) {            // (every lane loads, so that no load waits for another)
+            typedef std::remove_const_t<std::remove_pointer_t<decltype(rows)>> H;
 #pragma unroll
-        for (int g = 0; g < NG; g += NC)
+            for (int g = 0; g < NG; g += NC)
 #pragma unroll
-            for (int p = 0; p < PER; ++p)
+                for (int p = 0; p < PER; ++p)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float x[NC] = {};
-                    if (mine(g) && feature(p) < DK) load_hidden<NC>(from, dtype, ((int64_t)pair * DK + feature(p) + e) * DV + column(g), x);
+                    for (int e = 0; e < 4; ++e) {
+                        const bool is = mine(g) && feature(p) < DK;
+                        float x[NC];
+                        load_vec<H, NC>(rows + ((int64_t)pair * DK + (is ? feature(p) + e : 0)) * DV + (is ? column(g) : 0), x);
 #pragma unroll
-                    for (int q = 0; q < NC; ++q) S[g + q][p][e] = x[q];
-                }
+                        for (int q = 0; q < NC; ++q) S[g + q][p][e] = is ? x[q] : 0.f;
+                    }
+        };
+        if (dtype == GLA_BF16) load(static_cast<const __bf16 *>(from));
+        else load(static_cast<const float *>(from));
     }
     __device__ __forceinline__ void store_state(void *to, int dtype) const
     {
@@ -83,67 +115,72 @@ template <typename T, int DKP, int NG> struct Walk {
                     if (mine(g) && feature(p) < DK) store_hidden<NC>(to, dtype, ((int64_t)pair * DK + feature(p) + e) * DV + column(g), x);
                 }
     }
-    // the wave's tokens of keys or queries, features as the contracted index in their order; tokens behind the end read the last one
-    __device__ __forceinline__ void load_rows(const DecayRows &x, int n, D8 (&to)[KS]) const
+    // the wave's tokens of keys or queries, features as the contracted index in their order
+    __device__ __forceinline__ void load_rows(const void *from, const DeltaArgs &a, int n, D8 (&to)[KS]) const
     {
-        const T *row = static_cast<const T *>(x.p) + b * x.sb + hk * x.sh + (int64_t)min(n * C + 16 * w + r, len - 1) * x.st;
+        const T *p = static_cast<const T *>(from) + ((b * a.n.HK + hk) * a.chunks + n) * (CT * KS * 512) + min(w, CT - 1) * KS * 512;
+        const unsigned at = lane * 8 * (unsigned)sizeof(T);
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) to[ks] = ld8(row + (32 * ks + 8 * c < DK ? 32 * ks + 8 * c : 0));
+        for (int ks = 0; ks < KS; ++ks) to[ks] = ld8(at_bytes(p + ks * 512, at));
     }
     // the wave's features of keys or queries, tokens as the contracted index
     __device__ __forceinline__ void load_features(const void *from, const DeltaArgs &a, int n, D8 (&to)[PER][CS]) const
     {
-        const T *p = static_cast<const T *>(from) + ((b * a.n.HK + hk) * a.chunks + n) * (TILES * CS * 512) + w * PER * CS * 512 + lane * 8;
+        const T *p = static_cast<const T *>(from) + ((b * a.n.HK + hk) * a.chunks + n) * (TILES * CS * 512) + w * PER * CS * 512;
+        const unsigned at = lane * 8 * (unsigned)sizeof(T);
 #pragma unroll
         for (int t = 0; t < PER; ++t)
 #pragma unroll
-            for (int ks = 0; ks < CS; ++ks) to[t][ks] = ld8(p + (t * CS + ks) * 512);
+            for (int ks = 0; ks < CS; ++ks) to[t][ks] = ld8(at_bytes(p + (t * CS + ks) * 512, at));
     }
     // the wave's tokens of a lower (upper) triangle: steps 0 .. w / 2 (w / 2 ..), the last one twice where there is one alone
     template <bool UPPER, int N> __device__ __forceinline__ void load_steps(const void *from, const DeltaArgs &a, int n, D8 (&to)[CS][N]) const
     {
-        const T *p = static_cast<const T *>(from) + ((int64_t)pair * a.chunks + n) * (DC::kSteps * N * 512) + lane * 8;
+        const T *p = static_cast<const T *>(from) + ((int64_t)pair * a.chunks + n) * (DC::kSteps * N * 512);
+        const unsigned at = lane * 8 * (unsigned)sizeof(T);
 #pragma unroll
         for (int ks = 0; ks < CS; ++ks) {
             const int t = CS == 1 ? min(w, CT - 1) : w, step = UPPER ? DC::upper(t, max(ks, t / 2)) : DC::lower(t, min(ks, t / 2));
 #pragma unroll
-            for (int i = 0; i < N; ++i) to[ks][i] = ld8(p + (step * N + i) * 512);
+            for (int i = 0; i < N; ++i) to[ks][i] = ld8(at_bytes(p + (step * N + i) * 512, at));
         }
     }
-    // the lane's columns of values or their cotangents, tokens 16w + 4c + e
-    __device__ __forceinline__ void load_values(const DecayRows &x, int n, Cols (&to)[NG / NC][4]) const
+    // the lane's columns of values or their cotangents, tokens 16w + 4c + e; columns behind the last are whatever is there, and stay by themselves
+    __device__ __forceinline__ Rows value_rows(const DecayRows &x) const
     {
-        const T *p = static_cast<const T *>(x.p) + b * x.sb + h * x.sh;
+        Rows y{static_cast<const T *>(x.p) + b * x.sb + h * x.sh, (int)x.st, {}};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const T *row = p + (int64_t)min(n * C + 16 * w + 4 * c + e, len - 1) * x.st;
+        for (int e = 0; e < 4; ++e) y.at[e] = (unsigned)((16 * min(w, CT - 1) + 4 * c + e) * y.st + column(0)) * (unsigned)sizeof(T);
+        return y;
+    }
+    __device__ __forceinline__ void load_values(const Rows &x, int n, Cols (&to)[NG / NC][4]) const
+    {
+        // (at most 2^30 bytes)
+        const auto rows = __builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(x.p + (int64_t)n * C * x.st), 0,
+                                                            ((min(C, len - n * C) - 1) * x.st + DV) * (int)sizeof(T), 0x00027000);
 #pragma unroll
-            for (int g = 0; g < NG; g += NC) to[g / NC][e] = *reinterpret_cast<const Cols *>(row + (mine(g) ? column(g) : 0));
-        }
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int g = 0; g < NG; g += NC) to[g / NC][e] = load_columns<Cols>(rows, x.at[e] + 16 * g * (unsigned)sizeof(T));
     }
-    __device__ __forceinline__ float value(const Cols (&v)[NG / NC][4], int n, int g, int e) const
+    static __device__ __forceinline__ float value(const Cols (&v)[NG / NC][4], int g, int e) { return column_of<T, NC>(v[g / NC][e], g % NC); }
+    // of the chunk's gates: e^{L_i} (0), e^{L_C - L_i} (1) or b_i (2) of the wave's tokens 4c .., e^{L_i} of token r, e^{L_C}
+    __device__ __forceinline__ const float *gates(const DeltaArgs &a, int n) const { return a.to.gates + ((int64_t)pair * a.chunks + n) * DC::kGates; }
+    __device__ __forceinline__ f32x4 gate(const DeltaArgs &a, int n, int kind) const
     {
-        return mine(g) && n * C + 16 * w + 4 * c + e < len ? column_of<T, NC>(v[g / NC][e], g % NC) : 0.f;
+        return *reinterpret_cast<const f32x4 *>(at_bytes(gates(a, n) + kind * C + 16 * min(w, CT - 1), 16u * c));
     }
-    // e^{L_i}, e^{L_C - L_i} and b_i of the wave's tokens
-    struct Gates {
-        f32x4 start, end, beta;
-        float at_start, whole;                   // of token r
-    };
-    __device__ __forceinline__ void load_gates(const DeltaArgs &a, int n, Gates &to) const
-    {
-        const float *gate = a.to.gates + ((int64_t)pair * a.chunks + n) * DC::kGates;
-        const int t = 16 * min(w, CT - 1);
-        to.start = *reinterpret_cast<const f32x4 *>(gate + t + 4 * c);
-        to.end = *reinterpret_cast<const f32x4 *>(gate + C + t + 4 * c);
-        to.beta = *reinterpret_cast<const f32x4 *>(gate + 2 * C + t + 4 * c);
-        to.at_start = gate[t + r];
-        to.whole = gate[3 * C];
-    }
+    __device__ __forceinline__ float gate_r(const DeltaArgs &a, int n) const { return *at_bytes(gates(a, n) + 16 * min(w, CT - 1), 4u * r); }
+    __device__ __forceinline__ float gate_whole(const DeltaArgs &a, int n) const { return *at_bytes(gates(a, n) + 3 * C, again(0)); }
     // x or the cotangents of u: the four tokens of a column
     __device__ __forceinline__ int64_t written(int n, int g) const
     {
         return (((int64_t)n * (DV >> 4) + (column(g) >> 4)) * CT + w) * 256 + (c * 16 + (column(g) & 15)) * 4;
+    }
+    // states: the four features of a column
+    __device__ __forceinline__ int64_t state_place(int n, int g, int p) const
+    {
+        return (((int64_t)n * (DV >> 4) + (column(g) >> 4)) * delta_state_tiles(DK) + (w * PER + p)) * 256 + (c * 16 + (column(g) & 15)) * 4;
     }
     // ---- operands in LDS: [group][step][part][lane][8], a wave's accumulators being half of a step ----
     template <int STEPS, int N> static __device__ __forceinline__ void put(T *to, int g, int t, int lane, f32x4 v)
@@ -152,9 +189,11 @@ template <typename T, int DKP, int NG> struct Walk {
         for (int i = 0; i < N; ++i) {
             const Four f = pack_results<T>(v);
             *reinterpret_cast<Four *>(to + (((g * STEPS + (t >> 1)) * N + i) * 64 + lane) * 8 + 4 * (t & 1)) = f;
-            if (i + 1 < N)
+            if (i + 1 < N) {
+                const f32x4 taken = unpack_results(f);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] -= (float)f[e];
+                for (int e = 0; e < 4; ++e) v[e] -= taken[e];
+            }
         }
     }
     template <int STEPS, int N, int M> static __device__ __forceinline__ void get(const T *from, int g, int step, int lane, D8 (&to)[M])
@@ -184,7 +223,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void d
     W w;
     if (w.place(a)) return;
     const int r = w.r, c = w.c, lane = w.lane;
-    const bool tokens = w.w < CT;
+    const bool tokens = CT == W::kWaves || w.w < CT;
     w.load_state(a.hidden, a.hidden_dtype);
     float *kept = KEEP ? a.kept + w.pair * (delta_states_floats(a.n, a.chunks) + delta_written_floats(a.n, a.chunks, C)) : nullptr;
     float *xs = KEEP ? kept + delta_states_floats(a.n, a.chunks) : nullptr;
@@ -194,11 +233,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void d
 #pragma unroll
             for (int p = 0; p < PER; ++p)
                 if (w.mine(g) && w.feature(p) < w.DK)
-                    *reinterpret_cast<f32x4 *>(kept + ((int64_t)n * w.DV + w.column(g)) * w.DK + w.feature(p)) = w.S[g][p];
+                    *reinterpret_cast<f32x4 *>(kept + w.state_place(n, g, p)) = w.S[g][p];
     };
     D8 K[KS], Q[KS], KT[PER][CS], Z[CS][kParts], P[CS][1];
     typename W::Cols V[NG / NC][4];
-    typename W::Gates next_gates;
+    const typename W::Rows values = w.value_rows(a.values);
+    f32x4 start, end, beta;
+    float at_start, whole;
     T *out = static_cast<T *>(a.out) + (w.b * w.T_ * a.n.H + w.h) * w.DV;
     const int64_t row = a.n.H * w.DV;
     auto store = [&](int token, auto values) {   // the lane's columns of a token, 4 NC of each NC groups
@@ -212,10 +253,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void d
         }
     };
     if (w.live > 0) {
-        w.load_gates(a, 0, next_gates);
-        w.load_rows(a.keys, 0, K);
-        w.load_rows(a.queries, 0, Q);
-        w.load_values(a.values, 0, V);
+        w.load_rows(a.to.key_rows, a, 0, K);
+        w.load_rows(a.to.query_rows, a, 0, Q);
+        w.load_values(values, 0, V);
+        start = w.gate(a, 0, 0);
+        end = w.gate(a, 0, 1);
+        beta = w.gate(a, 0, 2);
+        whole = w.gate_whole(a, 0);
+        at_start = w.gate_r(a, 0);
         w.template load_steps<false>(a.to.inverse, a, 0, Z);
         w.template load_steps<false>(a.to.scores, a, 0, P);
         w.load_features(a.to.keys, a, 0, KT);
@@ -223,8 +268,6 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void d
     w.template put_state<kFew>(sS);
     for (int n = 0; n < w.live; ++n) {
         const int next = min(n + 1, w.live - 1);
-        const typename W::Gates gate = next_gates;
-        w.load_gates(a, next, next_gates);
         if constexpr (KEEP) keep(n);
         f32x4 x[NG], o[NG];
         lds_barrier();                           // the state's operands are there
@@ -244,13 +287,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void d
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) x[g][e] = w.value(V, n, g, e) - gate.start[e] * x[g][e];
+                for (int e = 0; e < 4; ++e) x[g][e] = W::value(V, g, e) - start[e] * x[g][e];
                 W::template put<CS, kParts>(sR, g, w.w, lane, x[g]);
             }
-            w.load_rows(a.keys, next, K);
-            w.load_rows(a.queries, next, Q);
-            w.load_values(a.values, next, V);
         }
+        w.load_rows(a.to.key_rows, a, next, K);
+        w.load_rows(a.to.query_rows, a, next, Q);
+        w.load_values(values, next, V);
+        start = w.gate(a, next, 0);
         lds_barrier();                           // r
         if (tokens) {
 #pragma unroll
@@ -269,16 +313,18 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void d
                 f32x4 u, weighted;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    u[e] = gate.beta[e] * x[g][e];
-                    weighted[e] = gate.end[e] * u[e];
+                    u[e] = beta[e] * x[g][e];
+                    weighted[e] = end[e] * u[e];
                 }
                 W::template put<CS, kParts>(sU, g, w.w, lane, weighted);
-                W::template put<CS, 1>(sO, g, w.w, lane, u);
+                W::template put<CS, kFew>(sO, g, w.w, lane, u);
                 if constexpr (KEEP)
                     if (w.mine(g)) *reinterpret_cast<f32x4 *>(xs + w.written(n, g)) = x[g];
             }
-            w.template load_steps<false>(a.to.inverse, a, next, Z);
         }
+        w.template load_steps<false>(a.to.inverse, a, next, Z);
+        end = w.gate(a, next, 1);
+        beta = w.gate(a, next, 2);
         lds_barrier();                           // u
         // the state behind the chunk
 #pragma unroll
@@ -286,7 +332,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void d
 #pragma unroll
             for (int p = 0; p < PER; ++p)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) w.S[g][p][e] *= gate.whole;
+                for (int e = 0; e < 4; ++e) w.S[g][p][e] *= whole;
 #pragma unroll
         for (int ks = 0; ks < CS; ++ks)
 #pragma unroll
@@ -297,25 +343,27 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void d
                 for (int p = 0; p < PER; ++p) w.S[g][p] = mma_whole(KT[p][ks], u, w.S[g][p]);
             }
         w.load_features(a.to.keys, a, next, KT);
+        whole = w.gate_whole(a, next);
         w.template put_state<kFew>(sS);
         if (tokens) {
 #pragma unroll
             for (int g = 0; g < NG; ++g)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) o[g][e] *= gate.at_start;
+                for (int e = 0; e < 4; ++e) o[g][e] *= at_start;
 #pragma unroll
             for (int ks = 0; ks < CS; ++ks)
                 if (ks <= w.w / 2)
 #pragma unroll
                     for (int g = 0; g < NG; ++g) {
-                        D8 u[1];
-                        W::template get<CS, 1>(sO, g, ks, lane, u);
-                        o[g] = mma_d(u[0], P[ks][0], o[g]);
+                        D8 u[kFew];
+                        W::template get<CS, kFew>(sO, g, ks, lane, u);
+                        o[g] = mma_whole(u, P[ks][0], o[g]);
                     }
-            w.template load_steps<false>(a.to.scores, a, next, P);
             const int token = n * C + 16 * w.w + r;
             store(token, [&](int g, int e) { return token < w.len ? o[g][e] : 0.f; });
         }
+        w.template load_steps<false>(a.to.scores, a, next, P);
+        at_start = w.gate_r(a, next);
     }
     // rows past the end of a shorter sequence
     for (int token = w.live * C + 16 * w.w + r; token < w.T_; token += 16 * W::kWaves) store(token, [](int, int) { return 0.f; });
@@ -340,14 +388,16 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void d
     W w;
     if (w.place(a)) return;
     const int lane = w.lane;
-    const bool tokens = w.w < CT;
+    const bool tokens = CT == W::kWaves || w.w < CT;
     w.load_state(a.hidden, a.hidden_dtype);
     const float *kept = a.kept + w.pair * (delta_states_floats(a.n, a.chunks) + delta_written_floats(a.n, a.chunks, C));
     float *dus = a.du + w.pair * delta_written_floats(a.n, a.chunks, C);
-    T *dstates = static_cast<T *>(a.dstates) + w.pair * a.chunks * a.n.DK * a.n.DV;
+    T *dstates = static_cast<T *>(a.dstates) + w.pair * a.chunks * delta_state_floats(a.n);
     D8 K[KS], KT[PER][CS], QT[PER][CS], Z[CS][kParts], P[CS][kParts];
     typename W::Cols O[NG / NC][4];
-    typename W::Gates next_gates;
+    const typename W::Rows douts = w.value_rows(a.dout);
+    f32x4 start, end, beta;
+    float whole;
     f32x4 S[NG][PER];
     auto load_kept = [&](int n) {
 #pragma unroll
@@ -355,15 +405,18 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void d
 #pragma unroll
             for (int p = 0; p < PER; ++p) {
                 const bool is = w.mine(g) && w.feature(p) < w.DK;
-                S[g][p] = *reinterpret_cast<const f32x4 *>(kept + ((int64_t)n * w.DV + (is ? w.column(g) : 0)) * w.DK + (is ? w.feature(p) : 0));
+                S[g][p] = *reinterpret_cast<const f32x4 *>(kept + (is ? w.state_place(n, g, p) : 0));
             }
     };
     if (w.live > 0) {
         const int n = w.live - 1;
-        w.load_gates(a, n, next_gates);
         load_kept(n + 1);
-        w.load_values(a.dout, n, O);
-        w.load_rows(a.keys, n, K);
+        w.load_values(douts, n, O);
+        w.load_rows(a.to.key_rows, a, n, K);
+        start = w.gate(a, n, 0);
+        end = w.gate(a, n, 1);
+        beta = w.gate(a, n, 2);
+        whole = w.gate_whole(a, n);
         w.template load_steps<true>(a.to.scores, a, n, P);
         w.template load_steps<true>(a.to.inverse, a, n, Z);
         w.load_features(a.to.queries, a, n, QT);
@@ -371,8 +424,6 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void d
     }
     for (int n = w.live - 1; n >= 0; --n) {
         const int next = max(n - 1, 0);
-        const typename W::Gates gate = next_gates;
-        w.load_gates(a, next, next_gates);
         // the cotangent of the state behind the chunk, for the gradients; its product with that state
         w.template put_state<kParts>(sS);
         float *dots = a.dots + (((int64_t)w.pair * a.chunks + n) * (w.DV >> 4) + (w.col0 >> 4)) * 4 + w.w;
@@ -386,7 +437,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void d
                     if (w.mine(q) && w.feature(p) < w.DK) {
 #pragma unroll
                         for (int e = 0; e < 4; ++e) dot += w.S[q][p][e] * S[q][p][e];
-                        *reinterpret_cast<typename W::Four *>(dstates + ((int64_t)n * w.DV + w.column(q)) * w.DK + w.feature(p)) = pack_results<T>(w.S[q][p]);
+                        *reinterpret_cast<typename W::Four *>(dstates + w.state_place(n, q, p)) = pack_results<T>(w.S[q][p]);
                     }
             dot = sum_over_c(sum_over_r(dot));
             if (lane == 0)
@@ -400,14 +451,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void d
                 f32x4 o, scaled;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    o[e] = w.value(O, n, g, e);
-                    scaled[e] = gate.start[e] * o[e];
+                    o[e] = W::value(O, g, e);
+                    scaled[e] = start[e] * o[e];
                 }
                 W::template put<CS, 1>(sD, g, w.w, lane, o);
                 W::template put<CS, kParts>(sO, g, w.w, lane, scaled);
             }
-            w.load_values(a.dout, next, O);
         }
+        w.load_values(douts, next, O);
         lds_barrier();                           // dS and do
         f32x4 du[NG];
         if (tokens) {
@@ -421,11 +472,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void d
                     W::template get<KS, kParts>(sS, g, ks, lane, s);
                     du[g] = mma_whole(K[ks], s, du[g]);
                 }
-            w.load_rows(a.keys, next, K);
 #pragma unroll
             for (int g = 0; g < NG; ++g)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) du[g][e] *= gate.end[e];
+                for (int e = 0; e < 4; ++e) du[g][e] *= end[e];
 #pragma unroll
             for (int ks = 0; ks < CS; ++ks)
                 if (ks >= w.w / 2 || CS == 1)
@@ -435,10 +485,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void d
                         W::template get<CS, 1>(sD, g, ks, lane, o);
                         du[g] = mma_whole(P[ks], o[0], du[g]);
                     }
-            w.template load_steps<true>(a.to.scores, a, next, P);
 #pragma unroll
             for (int g = 0; g < NG; ++g) W::template put<CS, kParts>(sU, g, w.w, lane, du[g]);
         }
+        w.load_rows(a.to.key_rows, a, next, K);
+        w.template load_steps<true>(a.to.scores, a, next, P);
+        end = w.gate(a, next, 1);
         lds_barrier();                           // du
         if (tokens) {
 #pragma unroll
@@ -452,23 +504,25 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void d
                         W::template get<CS, kParts>(sU, g, ks, lane, u);
                         du[g] = mma_parts(Z[ks], u, du[g]);
                     }
-            w.template load_steps<true>(a.to.inverse, a, next, Z);
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
                 f32x4 v;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = -gate.start[e] * (gate.beta[e] * du[g][e]);
+                for (int e = 0; e < 4; ++e) v[e] = -start[e] * (beta[e] * du[g][e]);
                 W::template put<CS, kParts>(sR, g, w.w, lane, v);
                 if (w.mine(g)) *reinterpret_cast<f32x4 *>(dus + w.written(n, g)) = du[g];
             }
         }
+        w.template load_steps<true>(a.to.inverse, a, next, Z);
+        start = w.gate(a, next, 0);
+        beta = w.gate(a, next, 2);
         lds_barrier();                           // dr
 #pragma unroll
         for (int g = 0; g < NG; ++g)
 #pragma unroll
             for (int p = 0; p < PER; ++p)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) w.S[g][p][e] *= gate.whole;
+                for (int e = 0; e < 4; ++e) w.S[g][p][e] *= whole;
 #pragma unroll
         for (int ks = 0; ks < CS; ++ks)
 #pragma unroll
@@ -483,6 +537,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void d
             }
         w.load_features(a.to.queries, a, next, QT);
         w.load_features(a.to.keys, a, next, KT);
+        whole = w.gate_whole(a, next);
         lds_barrier();                           // what the next chunk's operands take the place of is read
     }
     w.store_state(a.hidden_out, a.hidden_dtype);
@@ -492,9 +547,9 @@ template <typename T, int DKP, int NG> int launch_walk(hipStream_t stream, const
 {
     typedef Walk<T, DKP, NG> W;
     typedef DeltaChunk<T> DC;
-    // the columns of a pair share a die, to which workgroups are dealt in turn
-    const dim3 grid((unsigned)((a.pairs + 7) / 8 * 8), (unsigned)((a.n.DV + 16 * NG - 1) / (16 * NG)));
-    constexpr size_t lds = sizeof(T) * 512 * NG * (W::KS * DC::kFew + W::CS * (2 * DC::kParts + 1));
+    // the columns of a pair start next to each other on one die (workgroups are dealt to the eight in turn) and share what they read in its cache
+    const unsigned grid = (unsigned)((a.pairs + 7) / 8 * 8 * ((a.n.DV + 16 * NG - 1) / (16 * NG)));
+    constexpr size_t lds = sizeof(T) * 512 * NG * (W::KS * DC::kFew + W::CS * (2 * DC::kParts + DC::kFew));
     constexpr size_t lds_back = sizeof(T) * 512 * NG * (W::KS * DC::kParts + W::CS * (3 * DC::kParts + 1));
     static_assert(lds_back <= 160 * 1024, "");
     static LdsGrant grants[3];
