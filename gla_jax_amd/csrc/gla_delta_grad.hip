@@ -105,23 +105,21 @@ template <typename T, int DKP> __global__ __launch_bounds__(DKP * 4) void delta_
         {
             RowsInFlight<T, C, kSlice, NT> o;
             o.load(tid, O + dv0, (int)a.dout.st, there, DV - dv0);
-            // states: four features of a value feature a lane
+            // states: eight features of a value feature a lane
 #pragma unroll
-            for (int i = w; i < kSlice / 16 * (DKP / 16); i += NW) {
-                const int m = i / (DKP / 16), t = i % (DKP / 16), col = 32 * (t >> 1) + 8 * c + 4 * (t & 1), at = place_in<T, DKP>(16 * m + r, col);
+            for (int i = w; i < kSlice / 16 * KS; i += NW) {
+                const int m = i / KS, ks = i % KS, col = 32 * ks + 8 * c, at = TileK::piece(16 * m + r, col);
                 const bool is = dv0 + 16 * m < DV && col < DK;
-                const unsigned from = is ? (((dv0 >> 4) + m) * delta_state_tiles(DK) + t) * 256 + lane * 4 : 0;
-                f32x4 s = *reinterpret_cast<const f32x4 *>(kept + from);
-                Four d = *reinterpret_cast<const Four *>(dS + from);
-                if (!is) s = f32x4{0.f, 0.f, 0.f, 0.f}, d = Four{};
+                const unsigned from = is ? (((dv0 >> 4) + m) * (delta_state_tiles(DK) / 2) + ks) * 512 : 0;
+                const f32x4 low = *reinterpret_cast<const f32x4 *>(kept + from + lane * 4), high = *reinterpret_cast<const f32x4 *>(kept + from + 256 + lane * 4);
+                const D8 d = ld8(dS + from + lane * 8);
+                float s[8];
 #pragma unroll
-                for (int p = 0; p < kParts; ++p) {
-                    const Four f = pack_results<T>(s);
-                    *reinterpret_cast<Four *>(sS + p * kS + at) = f;
+                for (int e = 0; e < 4; ++e) s[e] = is ? low[e] : 0.f, s[4 + e] = is ? high[e] : 0.f;
+                const Split<T, kParts> split(s);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) s[e] -= (float)f[e];
-                }
-                *reinterpret_cast<Four *>(sD + at) = d;
+                for (int p = 0; p < kParts; ++p) st8(sS + p * kS + at, split.part[p]);
+                st8(sD + at, is ? d : D8{});
             }
             const int ti = w % CT, token = 16 * ti + 4 * c;
             const f32x4 beta = *reinterpret_cast<const f32x4 *>(sums.beta + token);
