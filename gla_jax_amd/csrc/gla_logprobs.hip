@@ -5,9 +5,10 @@
 //       log p_i = (x_i - m) - log s,    H = log s - t / s.
 // Bound by the read; what comes near it are the exponentials (four issue slots of a value's eleven).
 //
-// The alternatives need no second pass over the row.  `top` threads have a largest value that reaches the top-th largest of all threads' largest
-// values, and what else reaches it lies in those threads' stretches: they alone are read again, by whole waves.  Equal values
-// are common in 16 bits, and all of them are taken along; if they are more than there is room for, the row is searched once for each alternative.
+// The alternatives need no second pass over the row.  The threads are 64 groups, each with a largest value; the top-th largest of the 64
+// is reached by `top` values at least, and whatever reaches it lies in the stretches of threads whose own largest value does: they alone are read
+// again, by whole waves (24 threads at 20 alternatives of a row in no order: 64 ln(64 / 44)).  Equal values are common in 16 bits, and all of them are
+// taken along; if they are more than there is room for, the row is searched once for each alternative.
 #include "gla_common.hpp"
 
 namespace gla {
@@ -134,6 +135,7 @@ __global__ __launch_bounds__(THREADS) void token_logprobs_kernel(const LogprobAr
         return;
     }
     const Row x(static_cast<const T *>(a.logits) + row * a.row, a.vocab);
+    const float given = tid == 0 ? (float)x.x[token] : 0.f;      // (on its way beside the row)
     Softmax mine;
     int64_t p = tid;
     auto chunk = [&](auto whole) {
@@ -178,7 +180,7 @@ __global__ __launch_bounds__(THREADS) void token_logprobs_kernel(const LogprobAr
     for (int i = 1; i < kWaves; ++i) joined.join(parts[i][0], parts[i][1], parts[i][2]);
     const float most = joined.most, log_sum = most == -INFINITY ? NAN : logf(joined.sum);
     if (tid == 0) {
-        a.given[row] = ((float)x.x[token] - most) - log_sum;
+        a.given[row] = (given - most) - log_sum;
         a.entropy[row] = log_sum - joined.weighted / joined.sum;
         if (a.stats) {
             a.stats[2 * row] = most;
@@ -186,56 +188,46 @@ __global__ __launch_bounds__(THREADS) void token_logprobs_kernel(const LogprobAr
         }
     }
     if constexpr (TOP) {
-        __shared__ float names[THREADS];
-        __shared__ float bounds[kWaves];
+        __shared__ float names[THREADS], peaks[64];
         __shared__ u64 collected[kRoom];
-        __shared__ int listed[kRoom];
+        __shared__ int listed[THREADS];
         __shared__ int threads, values;
         __shared__ float bound_of_all;
         const int top = a.top;
-        // a wave's top-th largest name is reached by as many; the highest of the waves' is a first bound
         const bool numbers = joined.sum == joined.sum;       // (where one is none, the largest of the others may have been lost beside it)
         names[tid] = own_most;
+        float peak = own_most;
+#pragma unroll
+        for (int m = 1; m < THREADS / 64; m *= 2) peak = fmaxf(peak, shfl_xor_f32(peak, m));
+        if (tid % (THREADS / 64) == 0) peaks[tid / (THREADS / 64)] = peak;
         if (tid == 0) threads = values = 0;
         __syncthreads();
-        int above = 0;
+        if (w == 0) {
+            const float mine_of_64 = peaks[lane];
+            int above = 0;
 #pragma unroll 16
-        for (int i = 0; i < 64; ++i) {
-            const float other = names[64 * w + i];
-            above += other > own_most || (other == own_most && i < lane);
+            for (int i = 0; i < 64; ++i) {
+                const float other = peaks[i];
+                above += other > mine_of_64 || (other == mine_of_64 && i < lane);
+            }
+            if (above == top - 1) bound_of_all = mine_of_64;
         }
-        if (above == top - 1) bounds[w] = own_most;      // (in every wave, if all names are numbers)
         __syncthreads();
-        float bound = bounds[0];
-#pragma unroll 1
-        for (int i = 1; i < kWaves; ++i) bound = fmaxf(bound, bounds[i]);
+        // where fewer than `top` of the 64 have anything above -inf: all that is above
+        const float bound = fmaxf(bound_of_all, -3.4028235e38f);
         if (own_most >= bound) listed[atomicAdd(&threads, 1)] = tid;
         __syncthreads();
-        // and the top-th largest name of all the second
         const int names_there = threads;
-        for (int i = tid; i < names_there; i += THREADS) {
-            const int id = listed[i];
-            const float name = names[id];
-            int over = 0;
-            for (int j = 0; j < names_there; ++j) {
-                const float other = names[listed[j]];
-                over += other > name || (other == name && listed[j] < id);
-            }
-            if (over == top - 1) bound_of_all = name;
-        }
-        __syncthreads();
-        bound = bound_of_all;
         auto collect = [&](float v, int64_t place) {
-            if (!(v >= bound) && !(bound == -INFINITY)) return;
+            if (!(v >= bound)) return;
             const int at = atomicAdd(&values, 1);
             if (at < kRoom) collected[at] = key_of(v, place);
         };
         // A wave reads the pieces of as many threads as it has lanes for.
         const int64_t each = (x.pieces + THREADS - 1) / THREADS;     // pieces of a thread, at most
-        const int lanes = each >= 64 ? 64 : each > 32 ? 64 : each > 16 ? 32 : each > 8 ? 16 : each > 4 ? 8 : 4, side = 64 / lanes;
+        const int lanes = each > 32 ? 64 : each > 16 ? 32 : each > 8 ? 16 : each > 4 ? 8 : 4, side = 64 / lanes;
         for (int i = w * side + lane / lanes; i < names_there; i += kWaves * side) {
             const int id = listed[i];
-            if (names[id] < bound) continue;
             for (int64_t q = id + (int64_t)(lane % lanes) * THREADS; q < x.pieces; q += (int64_t)lanes * THREADS) {
                 const typename Row::Piece piece = *x.at(q);
 #pragma unroll
@@ -251,12 +243,23 @@ __global__ __launch_bounds__(THREADS) void token_logprobs_kernel(const LogprobAr
             near[n] = (value_of(key) - most) - log_sum;
             index[n] = (uint32_t)~(uint32_t)key;
         };
-        if (numbers && count <= kRoom && count >= top) {
+        if (numbers && count <= kRoom) {
             for (int i = tid; i < count; i += THREADS) {
                 const u64 key = collected[i];
                 int over = 0;
                 for (int j = 0; j < count; ++j) over += collected[j] > key;
                 if (over < top) put(over, key);
+            }
+            // the rest are the first tokens of -inf, which lie among the first `top`, of all and more as are above
+            if (w == 0 && count < top) {
+                int found = count;
+                for (int64_t i = lane; i - lane < a.vocab && found < top; i += 64) {
+                    const bool is = i < a.vocab && !((float)x.x[i] >= bound);
+                    const u64 all = __ballot(is);
+                    const int n = found + __popcll(all & (((u64)1 << lane) - 1));
+                    if (is && n < top) put(n, key_of(-INFINITY, i));
+                    found += __popcll(all);
+                }
             }
             return;
         }
@@ -351,9 +354,11 @@ template <typename T, int THREADS> int launch_logprobs(hipStream_t stream, const
     else token_logprobs_kernel<T, THREADS, false><<<rows, THREADS, 0, stream>>>(a);
     return launch_status();
 }
+// A compute unit holds 2048 threads: rows are taken by as many as let all of them begin at once.
 template <typename T> int dispatch_logprobs(hipStream_t stream, const LogprobArgs &a, int64_t rows)
 {
-    return rows < 1024 ? launch_logprobs<T, 1024>(stream, a, rows) : launch_logprobs<T, 256>(stream, a, rows);
+    if (rows <= 512) return launch_logprobs<T, 1024>(stream, a, rows);
+    return rows <= 1024 ? launch_logprobs<T, 512>(stream, a, rows) : launch_logprobs<T, 256>(stream, a, rows);
 }
 
 }  // namespace
