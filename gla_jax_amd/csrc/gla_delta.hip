@@ -36,13 +36,8 @@ int64_t lay_out(DeltaArgs &a, gla_dtype dtype, bool backward, char *ws, float **
         at += pad256(bytes);
         return x;
     };
-    const int64_t columns = a.n.B * a.n.HK * a.chunks * delta_key_width(a.n.DK) * C * e;
     a.to.inverse = take(chunk_pairs * steps * parts * 512 * e);
     a.to.scores = take(chunk_pairs * steps * (backward ? parts : 1) * 512 * e);
-    a.to.keys = take(columns);
-    a.to.queries = backward ? take(columns) : nullptr;
-    a.to.key_rows = take(columns);
-    a.to.query_rows = backward ? nullptr : take(columns);
     a.to.gates = reinterpret_cast<float *>(take(chunk_pairs * 4 * C * 4));
     if (!backward) return at;
     a.du = reinterpret_cast<float *>(take(a.pairs * delta_written_floats(a.n, a.chunks, (int)C) * 4));

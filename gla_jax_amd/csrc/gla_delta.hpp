@@ -8,11 +8,11 @@
 // So the work is in two kinds of kernels.  delta_prepare_kernel, all chunks at once, forms the inverses and the scores.  The walks go
 // through a sequence's chunks with the state in the accumulators of their matrix instructions, and need nothing but products.
 //
-// A workgroup of four waves walks: it holds 16 to 64 value columns of the state, each wave a quarter of the features and, of a chunk's
-// products, 16 tokens.  Three times a chunk they hand each other operands through LDS: the state, r, and u.  Everything else comes from memory in the
-// order of the matrix instructions' operands, as delta_prepare_kernel's lanes held it, requested a chunk ahead: a wave's load is then 1 KB
-// in one piece.  (Keys and queries as they lie are 64 pieces of 16 bytes a load, each a cycle of the cache's: of a chunk's 4900 cycles a wave
-// spent 900 to 1500 on issuing them.)  Where there are few sequences their columns are spread over the compute units.
+// A workgroup walks with 16 to 64 value columns of the state: four waves each hold a quarter of the features and make, of a chunk's products, 16
+// tokens; three times a chunk they hand each other operands through LDS: the state, r, and u.  Four more bring keys and queries and do what
+// the next state does not wait for.  The inverses and scores come from memory as delta_prepare_kernel's lanes held them.  All of it is requested two chunks
+// ahead: a chunk takes 2300 cycles, and memory's answer now and then longer.  Where there are few sequences their columns are spread over the
+// compute units.
 //
 // Precision.  Keys, queries and values are 16-bit numbers as they come.  What a 32-bit result (states, gradients of the gates) depends on
 // and is formed in between enters a product as bf16 parts (Split): the inverse, r, u and the scores of the backward walk in three, 2^-25 of a value, the
@@ -43,10 +43,6 @@ template <typename T> struct DeltaChunk {
 struct DeltaPrepared {
     void *inverse;      // [pairs, chunks][steps][parts][64][8]
     void *scores;       // [pairs, chunks][steps][parts, of the backward walk][64][8]
-    void *keys;         // [B, HK, chunks][features / 16][C / 32][64][8]: keys with tokens as the contracted index
-    void *queries;      // the same, of the backward walk
-    void *key_rows;     // [B, HK, chunks][C / 16][features / 32][64][8]: keys with features as the contracted index
-    void *query_rows;   // the same, of the forward walk
     float *gates;       // [pairs, chunks][kGates]
 };
 
@@ -78,8 +74,6 @@ inline __host__ __device__ int delta_state_tiles(int64_t DK) { return (int)((DK 
 inline __host__ __device__ int64_t delta_state_floats(const DecaySizes &n) { return 16 * delta_state_tiles(n.DK) * n.DV; }
 inline __host__ __device__ int64_t delta_states_floats(const DecaySizes &n, int64_t chunks) { return (chunks + 1) * delta_state_floats(n); }
 inline __host__ __device__ int64_t delta_written_floats(const DecaySizes &n, int64_t chunks, int C) { return chunks * C * n.DV; }
-
-inline __host__ __device__ int64_t delta_key_width(int64_t DK) { return DK <= 64 ? 64 : 128; }
 
 // Features pi(t, r) as the operand's rows, rows 32 * ks .. as the contracted index, in two halves: LdsTile::columns with another
 // order of the features.

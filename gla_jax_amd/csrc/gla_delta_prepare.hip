@@ -5,7 +5,7 @@ namespace gla {
 namespace {
 
 // One workgroup: a chunk of a (batch, head) pair.  Forward it leaves (1 + M b)^{-1} and P with rows i as the operands' rows, backward
-// the transposes of (1 + b M)^{-1} and P, with rows j; and keys (backward: and queries) with tokens as the contracted index.
+// the transposes of (1 + b M)^{-1} and P, with rows j.
 //
 // The inverse, in 32 bits throughout: each wave solves for one block of 16 rows on the diagonal by substitution, a column a lane, and then
 // goes down (forward, for the transposed matrix: up) its own column of blocks, X_ij = -X_ii sum_k N_ik X_kj, by float products whose accumulators are
@@ -13,9 +13,8 @@ namespace {
 template <typename T, int DKP, bool BACK> __global__ __launch_bounds__(256) void delta_prepare_kernel(const DeltaArgs a)
 {
     typedef DeltaChunk<T> DC;
-    constexpr int C = DC::C, CT = DC::CT, CS = DC::CS, KS = DKP / 32, TILES = DKP / 16, NW = 4, NT = 256, kTriangle = CT * (CT + 1) / 2;
+    constexpr int C = DC::C, CT = DC::CT, KS = DKP / 32, NW = 4, NT = 256, kTriangle = CT * (CT + 1) / 2;
     constexpr int kRow = C + 4, kBlock = 16 * 20, kParts = DC::kParts, kScoreParts = BACK ? kParts : 1;
-    typedef typename FragTypes<T>::d8 D8;
     typedef typename Packed4<T>::t Four;
     typedef LdsTile<T, DKP> Tile;
     extern __shared__ char smem[];
@@ -84,23 +83,6 @@ template <typename T, int DKP, bool BACK> __global__ __launch_bounds__(256) void
         if (keys) *reinterpret_cast<f32x4 *>(sN + (rows ? j0 * kRow + i0 : i0 * kRow + j0)) = v;
         else if (BACK) put(scores, std::integral_constant<int, kScoreParts>{}, tj, ti, v);
         else put(scores, std::integral_constant<int, kScoreParts>{}, ti, tj, v);
-    }
-    if (blockIdx.x % H % group == 0) {
-        const int64_t kc = (b * a.n.HK + hk) * chunks + n;
-        D8 *keys = static_cast<D8 *>(a.to.keys) + kc * (TILES * CS * 64), *queries = static_cast<D8 *>(a.to.queries) + kc * (TILES * CS * 64);
-#pragma unroll
-        for (int m = w; m < TILES * CS; m += NW) {
-            const int t = m / CS, ks = m % CS;
-            st8(reinterpret_cast<T *>(keys + m * 64 + lane), feature_columns<DKP>(sK, ks, t));
-            if (BACK) st8(reinterpret_cast<T *>(queries + m * 64 + lane), feature_columns<DKP>(sQ, ks, t));
-        }
-        D8 *key_rows = static_cast<D8 *>(a.to.key_rows) + kc * (CT * KS * 64), *query_rows = static_cast<D8 *>(a.to.query_rows) + kc * (CT * KS * 64);
-#pragma unroll
-        for (int m = w; m < CT * KS; m += NW) {
-            const int t = m / KS, ks = m % KS;
-            st8(reinterpret_cast<T *>(key_rows + m * 64 + lane), tile.rows(sK, t, ks));
-            if (!BACK) st8(reinterpret_cast<T *>(query_rows + m * 64 + lane), tile.rows(sQ, t, ks));
-        }
     }
     if (tid < C) {
         float *to = a.to.gates + pc * DC::kGates;

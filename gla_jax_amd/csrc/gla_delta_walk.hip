@@ -5,6 +5,8 @@ namespace gla {
 namespace {
 
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+constexpr unsigned kNowhere = 0x7fffff00u;       // a place behind any chunk's rows
 template <typename T, int N> struct Columns { typedef T t __attribute__((ext_vector_type(N))); };
 template <typename T> struct Columns<T, 1> { typedef T t; };
 template <typename T, int N> __device__ __forceinline__ float column_of(typename Columns<T, N>::t v, int q)
@@ -23,7 +25,6 @@ __device__ __forceinline__ f32x4 unpack_results(f32x4 v) { return v; }
 
 // Rows of a chunk as the load instructions see them: what lies behind the last row reads as zero, and a lane keeps one 32-bit place for
 // the whole walk.
-constexpr unsigned kNowhere = 0x7fffff00u;       // (rows of a chunk take at most 2^30 bytes)
 template <typename Cols> __device__ __forceinline__ Cols load_columns(__amdgpu_buffer_rsrc_t rows, unsigned at)
 {
     if constexpr (sizeof(Cols) == 2) return __builtin_bit_cast(Cols, __builtin_amdgcn_raw_buffer_load_b16(rows, at, 0, 0));
@@ -53,6 +54,11 @@ template <typename T, int DKP, int NG> struct Walk {
         int st;
         unsigned at[4];
     };
+    __device__ __forceinline__ __amdgpu_buffer_rsrc_t chunk_rows(const Rows &x, int n, int width) const      // (at most 2^30 bytes)
+    {
+        return __builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(x.p + (int64_t)n * C * x.st), 0, ((min(C, len - n * C) - 1) * x.st + width) * (int)sizeof(T),
+                                                 0x00027000);
+    }
     // true: there is nothing to do
     __device__ __forceinline__ bool place(const DeltaArgs &a)
     {
@@ -119,29 +125,52 @@ template <typename T, int DKP, int NG> struct Walk {
                     if (mine(g) && feature(p) < DK) store_hidden<NC>(to, dtype, ((int64_t)pair * DK + feature(p) + e) * DV + column(g), x);
                 }
     }
-    // a prepared array's chunk: for each pair, or for each key head
+    // a prepared array's chunk
     template <int SIZE> __device__ __forceinline__ const T *of_pair(const void *from, const DeltaArgs &a, int n) const
     {
         return static_cast<const T *>(from) + ((int64_t)pair * a.chunks + n) * SIZE;
     }
-    template <int SIZE> __device__ __forceinline__ const T *of_key_head(const void *from, const DeltaArgs &a, int n) const
-    {
-        return static_cast<const T *>(from) + ((b * a.n.HK + hk) * a.chunks + n) * SIZE;
-    }
     __device__ __forceinline__ D8 load_operand(const T *p) const { return ld8(at_bytes(p, lane * 8 * (unsigned)sizeof(T))); }
-    // the wave's tokens of keys or queries, features as the contracted index in their order, step ks
-    __device__ __forceinline__ D8 load_row(const void *from, const DeltaArgs &a, int n, int ks) const
+    // the wave's tokens of keys or queries on their way from memory to a tile in LDS: 1 KB of neighbouring pieces a load
+    static constexpr int kPieces = DKP * (int)sizeof(T) / 16, kPer = 16 / (int)sizeof(T), kAtOnce = 64 / kPieces, kLoads = 16 / kAtOnce;
+    typedef u32x4 Stage[kLoads];
+    __device__ __forceinline__ Rows key_rows(const DecayRows &x) const
     {
-        return load_operand(of_key_head<CT * KS * 512>(from, a, n) + (min(w, CT - 1) * KS + ks) * 512);
+        Rows y{static_cast<const T *>(x.p) + b * x.sb + hk * x.sh, (int)x.st, {}};
+        const int col = lane % kPieces * kPer;
+        y.at[0] = col < DK ? (unsigned)((16 * min(w, CT - 1) + lane / kPieces) * y.st + col) * (unsigned)sizeof(T) : kNowhere;
+        return y;
     }
-    // the wave's features of keys or queries, tokens as the contracted index
-    __device__ __forceinline__ void load_features(const void *from, const DeltaArgs &a, int n, D8 (&to)[PER][CS]) const
+    __device__ __forceinline__ void load_stage(const Rows &x, int n, Stage &to) const
     {
-        const T *p = of_key_head<TILES * CS * 512>(from, a, n) + w * PER * CS * 512;
+        const auto rows = chunk_rows(x, n, DK);
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i)
+            to[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rows, x.at[0] + (unsigned)(i * kAtOnce * x.st) * (unsigned)sizeof(T), 0, 0));
+    }
+    __device__ __forceinline__ void put_stage(T *tile, const Stage &from) const
+    {
+        if (tokens())
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                const int col = lane % kPieces * kPer, at = LdsTile<T, DKP>::piece(16 * w + lane / kPieces + i * kAtOnce, col & ~7) + (col & 7);
+                *reinterpret_cast<u32x4 *>(tile + at) = from[i];
+            }
+    }
+    // the wave's tokens, features as the contracted index in their order
+    __device__ __forceinline__ void get_rows(const T *tile, D8 (&to)[KS]) const
+    {
+        if (tokens())
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) to[ks] = LdsTile<T, DKP>().rows(tile, w, ks);
+    }
+    // the wave's features, tokens as the contracted index
+    __device__ __forceinline__ void get_features(const T *tile, D8 (&to)[PER][CS]) const
+    {
 #pragma unroll
         for (int t = 0; t < PER; ++t)
 #pragma unroll
-            for (int ks = 0; ks < CS; ++ks) to[t][ks] = load_operand(p + (t * CS + ks) * 512);
+            for (int ks = 0; ks < CS; ++ks) to[t][ks] = feature_columns<DKP>(tile, ks, w * PER + t);
     }
     // the wave's tokens of a lower (upper) triangle: steps 0 .. w / 2 (w / 2 ..), the last one twice where there is one alone
     template <bool UPPER, int N> __device__ __forceinline__ void load_steps(const void *from, const DeltaArgs &a, int n, D8 (&to)[CS][N]) const
@@ -166,23 +195,70 @@ template <typename T, int DKP, int NG> struct Walk {
     }
     __device__ __forceinline__ void load_values(const Rows &x, int n, Cols (&to)[NG / NC][4]) const
     {
-        // (at most 2^30 bytes)
-        const auto rows = __builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(x.p + (int64_t)n * C * x.st), 0,
-                                                            ((min(C, len - n * C) - 1) * x.st + DV) * (int)sizeof(T), 0x00027000);
+        const auto rows = chunk_rows(x, n, DV);
 #pragma unroll
         for (int e = 0; e < 4; ++e)
 #pragma unroll
             for (int g = 0; g < NG; g += NC) to[g / NC][e] = load_columns<Cols>(rows, x.at[e] + 16 * g * (unsigned)sizeof(T));
     }
     static __device__ __forceinline__ float value(const Cols (&v)[NG / NC][4], int g, int e) { return column_of<T, NC>(v[g / NC][e], g % NC); }
-    // of the chunk's gates: e^{L_i} (0), e^{L_C - L_i} (1) or b_i (2) of the wave's tokens 4c .., e^{L_i} of token r, e^{L_C}
-    __device__ __forceinline__ const float *gates(const DeltaArgs &a, int n) const { return a.to.gates + ((int64_t)pair * a.chunks + n) * DC::kGates; }
-    __device__ __forceinline__ f32x4 gate(const DeltaArgs &a, int n, int kind) const
+    // A chunk's gates: e^{L_i} (0), e^{L_C - L_i} (1), b_i (2), and e^{L_C}.  Each helper brings a kind.
+    __device__ __forceinline__ float load_gate(const DeltaArgs &a, int n) const
     {
-        return *reinterpret_cast<const f32x4 *>(at_bytes(gates(a, n) + kind * C + 16 * min(w, CT - 1), 16u * c));
+        return *at_bytes(a.to.gates + ((int64_t)pair * a.chunks + n) * DC::kGates + w * C, 4u * (lane & (C - 1)));
     }
-    __device__ __forceinline__ float gate_r(const DeltaArgs &a, int n) const { return *at_bytes(gates(a, n) + 16 * min(w, CT - 1), 4u * r); }
-    __device__ __forceinline__ float gate_whole(const DeltaArgs &a, int n) const { return *at_bytes(gates(a, n) + 3 * C, again(0)); }
+    __device__ __forceinline__ f32x4 load_start(const DeltaArgs &a, int n) const
+    {
+        return *reinterpret_cast<const f32x4 *>(at_bytes(a.to.gates + ((int64_t)pair * a.chunks + n) * DC::kGates + 16 * min(w, CT - 1), 16u * c));
+    }
+    __device__ __forceinline__ void put_gate(float *gates, float x) const
+    {
+        if (lane < C) gates[w * C + lane] = x;
+    }
+    __device__ __forceinline__ f32x4 gate(const float *gates, int kind) const
+    {
+        return *reinterpret_cast<const f32x4 *>(gates + kind * C + 16 * min(w, CT - 1) + 4 * c);
+    }
+    // What brings chunks into the die's cache before the loads above ask for them.  A compute unit has only so many requests on their way to
+    // memory: the 80 KB of a chunk, two chunks ahead, kept it at 1.6 us a chunk, whatever the loop did meanwhile.  The workgroups of a pair's columns want
+    // the same, so each helper touches a part, one value of each 128 bytes: keys, queries, inverse, scores (in this order, 64 lines a
+    // wave, as far as there are waves), and of its own columns the values.
+    static constexpr int kAhead = 6;
+    struct Ahead {
+        const char *p;
+        int64_t step;                            // bytes from chunk to chunk
+        int st, size;                            // of rows: their distance; or the bytes of a chunk
+        unsigned at;
+    };
+    template <int SCORE_PARTS> __device__ __forceinline__ Ahead ahead(const DeltaArgs &a, const Rows &keys, const Rows &queries) const
+    {
+        constexpr int e = (int)sizeof(T), kLines = DKP * e / 128, kOfRows = C * kLines / 64, kInverse = DC::kSteps * DC::kParts * 512 * e,
+                      kScores = DC::kSteps * SCORE_PARTS * 512 * e, kOfInverse = (kInverse + 8191) / 8192, kOfScores = (kScores + 8191) / 8192;
+        int job = col0 / (16 * NG) * kWaves + w;
+        if (job < 2 * kOfRows) {
+            const Rows &x = job < kOfRows ? keys : queries;
+            const int line = lane % kLines * 128;
+            return {reinterpret_cast<const char *>(x.p), (int64_t)C * x.st * e, x.st, 0,
+                    line < DK * e ? (unsigned)((job % kOfRows * (64 / kLines) + lane / kLines) * x.st * e + line) : kNowhere};
+        }
+        job -= 2 * kOfRows;
+        const bool inverse = job < kOfInverse;
+        const int size = inverse ? kInverse : kScores;
+        if (!inverse) job -= kOfInverse;
+        return {static_cast<const char *>(inverse ? a.to.inverse : a.to.scores) + (int64_t)pair * a.chunks * size, size, 0, size,
+                inverse || job < kOfScores ? 8192u * job + 128u * lane : kNowhere};
+    }
+    __device__ __forceinline__ uint32_t touch(const Ahead &x, int n) const
+    {
+        const int size = x.size ? x.size : ((min(C, len - n * C) - 1) * x.st + DK) * (int)sizeof(T);
+        const auto chunk = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(x.p + n * x.step), 0, size, 0x00027000);
+        return __builtin_amdgcn_raw_buffer_load_b32(chunk, x.at, 0, 0);
+    }
+    __device__ __forceinline__ uint32_t touch_values(const Rows &x, int n) const
+    {
+        return __builtin_amdgcn_raw_buffer_load_b32(chunk_rows(x, n, DV), lane < 16 ? (unsigned)((16 * min(w, CT - 1) + r) * x.st + col0) * (unsigned)sizeof(T) : kNowhere,
+                                                    0, 0);
+    }
     // x or the cotangents of u: the four tokens of a column
     __device__ __forceinline__ int64_t written(int n, int g) const
     {
@@ -225,66 +301,62 @@ template <typename T, int DKP, int NG> struct Walk {
             for (int p = 0; p < PER; ++p) put<KS, N>(to, g, w * PER + p, lane, S[g][p]);
     }
     // ---- the three products of a walker's chunk ----
-    // K S: the small parts' sum apart, so that products need not wait for each other; keys are loaded again as soon as they are used
-    template <int N> __device__ __forceinline__ void keys_times_state(const DeltaArgs &a, int next, const T *state, D8 (&K)[KS], f32x4 (&x)[NG]) const
+    // K S: the small parts' sum apart, so that products need not wait for each other
+    template <int N> __device__ __forceinline__ void keys_times_state(const T *state, const D8 (&K)[KS], f32x4 (&x)[NG]) const
     {
+        if (!tokens()) return;
         f32x4 low[NG];
 #pragma unroll
         for (int g = 0; g < NG; ++g) x[g] = low[g] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-            if (tokens())
+        for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-                for (int g = 0; g < NG; ++g) {
-                    D8 s[N];
-                    get<KS, N>(state, g, ks, lane, s);
+            for (int g = 0; g < NG; ++g) {
+                D8 s[N];
+                get<KS, N>(state, g, ks, lane, s);
 #pragma unroll
-                    for (int i = N - 1; i >= 0; --i) {
-                        f32x4 &to = i ? low[g] : x[g];
-                        to = mma_d(K[ks], s[i], to);
-                    }
+                for (int i = N - 1; i >= 0; --i) {
+                    f32x4 &to = i ? low[g] : x[g];
+                    to = mma_d(K[ks], s[i], to);
                 }
-            K[ks] = load_row(a.to.key_rows, a, next, ks);
-        }
+            }
         if constexpr (N > 1)
 #pragma unroll
             for (int g = 0; g < NG; ++g)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) x[g][e] += low[g][e];
     }
-    template <bool UPPER> __device__ __forceinline__ void solve(const DeltaArgs &a, int next, const T *rows, D8 (&Z)[CS][DC::kParts], f32x4 (&x)[NG]) const
+    template <bool UPPER> __device__ __forceinline__ void solve(const T *rows, const D8 (&Z)[CS][DC::kParts], f32x4 (&x)[NG]) const
     {
         constexpr int N = DC::kParts;
-        if (tokens()) {
-            f32x4 sum[NG][N];
+        if (!tokens()) return;
+        f32x4 sum[NG][N];
 #pragma unroll
-            for (int g = 0; g < NG; ++g)
+        for (int g = 0; g < NG; ++g)
 #pragma unroll
-                for (int i = 0; i < N; ++i) sum[g][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int i = 0; i < N; ++i) sum[g][i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int ks = 0; ks < CS; ++ks)
-                if (step<UPPER>(ks))
+        for (int ks = 0; ks < CS; ++ks)
+            if (step<UPPER>(ks))
 #pragma unroll
-                    for (int g = 0; g < NG; ++g) {
-                        D8 v[N];
-                        get<CS, N>(rows, g, ks, lane, v);
+                for (int g = 0; g < NG; ++g) {
+                    D8 v[N];
+                    get<CS, N>(rows, g, ks, lane, v);
 #pragma unroll
-                        for (int i = 0; i < N; ++i)
+                    for (int i = 0; i < N; ++i)
 #pragma unroll
-                            for (int s = i; s < N; ++s) sum[g][s] = mma_d(Z[ks][i], v[s - i], sum[g][s]);
-                    }
+                        for (int s = i; s < N; ++s) sum[g][s] = mma_d(Z[ks][i], v[s - i], sum[g][s]);
+                }
 #pragma unroll
-            for (int g = 0; g < NG; ++g) {
-                x[g] = sum[g][N - 1];
+        for (int g = 0; g < NG; ++g) {
+            x[g] = sum[g][N - 1];
 #pragma unroll
-                for (int i = N - 2; i >= 0; --i)
+            for (int i = N - 2; i >= 0; --i)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) x[g][e] += sum[g][i][e];
-            }
+                for (int e = 0; e < 4; ++e) x[g][e] += sum[g][i][e];
         }
-        load_steps<UPPER>(a.to.inverse, a, next, Z);
     }
-    __device__ __forceinline__ void add_keys(const DeltaArgs &a, int next, const T *written, D8 (&KT)[PER][CS], f32x4 (&S)[NG][PER]) const
+    __device__ __forceinline__ void add_keys(const T *written, const D8 (&KT)[PER][CS], f32x4 (&S)[NG][PER]) const
     {
 #pragma unroll
         for (int ks = 0; ks < CS; ++ks)
@@ -297,9 +369,21 @@ template <typename T, int DKP, int NG> struct Walk {
 #pragma unroll
                     for (int p = 0; p < PER; ++p) S[g][p] = mma_d(KT[p][ks], u[i], S[g][p]);
             }
-        load_features(a.to.keys, a, next, KT);
     }
 };
+// step(n, x, y) for n = 0 .. live - 1, x and y taking turns.  The compiler's waits for a load count the loads behind it, the fewest on any way
+// there: so what was requested before the loop has to be there first, and the loop has no way out in its middle.
+template <typename Set, typename F> __device__ __forceinline__ void in_turns(int live, Set &x, Set &y, F step)
+{
+    wait_for_memory();
+    int n = 0;
+    for (; n + 1 < live; n += 2) {
+        step(n, x, y);
+        step(n + 1, y, x);
+    }
+    if (n < live) step(n, x, y);
+}
+template <typename T, int DKP> constexpr int kTile = DeltaChunk<T>::C * LdsTile<T, DKP>::kRow;
 
 // Forward.  Three times a chunk the waves wait for each other: for the state's operands, r and u.
 template <typename T, int DKP, int NG, bool KEEP> __global__ __launch_bounds__(512) void delta_walk_kernel(const DeltaArgs a)
@@ -307,12 +391,16 @@ template <typename T, int DKP, int NG, bool KEEP> __global__ __launch_bounds__(5
     typedef Walk<T, DKP, NG> W;
     typedef typename W::DC DC;
     typedef typename W::D8 D8;
-    constexpr int C = W::C, CS = W::CS, KS = W::KS, PER = W::PER, NC = W::NC, kParts = DC::kParts, kFew = DC::kFew;
+    constexpr int C = W::C, CT = W::CT, CS = W::CS, KS = W::KS, PER = W::PER, NC = W::NC, kParts = DC::kParts, kFew = DC::kFew;
     extern __shared__ char smem[];
-    T *sS = reinterpret_cast<T *>(smem), *sR = sS + NG * KS * kFew * 512, *sU = sR + NG * CS * kParts * 512, *sO = sU + NG * CS * kParts * 512;
+    // keys of two chunks and queries of one; the state, r, u (for the state, scaled) and u (for out); values, and gates of two chunks
+    T *sK[2] = {reinterpret_cast<T *>(smem), reinterpret_cast<T *>(smem) + kTile<T, DKP>}, *sQ = sK[1] + kTile<T, DKP>, *sS = sQ + kTile<T, DKP>,
+      *sR = sS + NG * KS * kFew * 512, *sU = sR + NG * CS * kParts * 512, *sO = sU + NG * CS * kParts * 512;
+    float *sV = reinterpret_cast<float *>(sO + NG * CS * kFew * 512), *sG[2] = {sV + NG * CT * 256, sV + NG * CT * 256 + DC::kGates};
     W w;
     if (w.place(a)) return;
     const int lane = w.lane, last = w.live - 1;
+    auto four = [&](float *p, int i) -> f32x4 & { return *reinterpret_cast<f32x4 *>(p + i * 256 + lane * 4); };
     if (w.helper) {
         const int64_t row = a.n.H * w.DV;
         const unsigned places = (unsigned)((16 * w.w + w.r) * row);
@@ -328,38 +416,74 @@ template <typename T, int DKP, int NG, bool KEEP> __global__ __launch_bounds__(5
                 if (at < w.DV && from + 16 * w.w + w.r < w.T_) store_vec<T, 4 * NC>(to + at, v);
             }
         };
-        D8 Q[KS], P[CS][1];
-        float at_start;
-        if (w.live > 0) {
+        struct Set {
+            typename W::Stage key, query;
+            typename W::Cols V[NG / NC][4];
+            float gate;
+            D8 P[CS][1];
+            uint32_t touched[2];
+        } x, y;
+        const typename W::Rows keys = w.key_rows(a.keys), queries = w.key_rows(a.queries), values = w.value_rows(a.values);
+        D8 Q[KS];
+        auto load_rows = [&](int n, Set &to) {
+            n = min(n, last);
+            w.load_stage(keys, n, to.key);
+            w.load_stage(queries, n, to.query);
+            w.load_values(values, n, to.V);
+            to.gate = w.load_gate(a, n);
+        };
+        auto load_scores = [&](int n, Set &to) { w.template load_steps<false>(a.to.scores, a, min(n, last), to.P); };
+        const typename W::Ahead ahead = w.template ahead<1>(a, keys, queries);
+        auto touch = [&](int n, Set &to) {
+            n = min(n, last);
+            to.touched[0] = w.touch(ahead, n);
+            to.touched[1] = w.touch_values(values, n);
+        };
+        auto put_rows = [&](int n, const Set &from) {
+            w.put_stage(sK[n & 1], from.key);
+            w.put_stage(sQ, from.query);
+            if (w.tokens())
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) Q[ks] = w.load_row(a.to.query_rows, a, 0, ks);
-            w.template load_steps<false>(a.to.scores, a, 0, P);
-            at_start = w.gate_r(a, 0);
+                for (int g = 0; g < NG; ++g)
+                    four(sV, g * CT + w.w) = f32x4{W::value(from.V, g, 0), W::value(from.V, g, 1), W::value(from.V, g, 2), W::value(from.V, g, 3)};
+            w.put_gate(sG[n & 1], from.gate);
+            w.get_rows(sQ, Q);                   // (the wave's own)
+        };
+        if (w.live > 0) {
+            load_rows(0, x);
+            load_scores(0, x);
+            load_rows(1, y);
+            load_scores(1, y);
+            put_rows(0, x);
+            load_rows(2, x);
+            touch(W::kAhead - 2, x);
+            touch(W::kAhead - 1, y);
+            lds_barrier();                       // the first rows
         }
-        for (int n = 0; n < w.live; ++n) {
-            const int next = min(n + 1, last);
+        in_turns(w.live, x, y, [&](int n, Set &mine, Set &next) {
             f32x4 o[NG];
             lds_barrier();                       // the state's operands are there
 #pragma unroll
             for (int g = 0; g < NG; ++g) o[g] = f32x4{0.f, 0.f, 0.f, 0.f};
+            if (w.tokens())
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                if (w.tokens())
+                for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
                     for (int g = 0; g < NG; ++g) {
                         D8 s[kFew];
                         W::template get<KS, kFew>(sS, g, ks, lane, s);
                         o[g] = mma_whole(s, Q[ks], o[g]);
                     }
-                Q[ks] = w.load_row(a.to.query_rows, a, next, ks);
-            }
             lds_barrier();                       // r
+            put_rows(n + 1, next);
+            load_rows(n + 3, next);
             lds_barrier();                       // u
             if (w.tokens()) {
+                const float start = sG[n & 1][16 * w.w + w.r];
 #pragma unroll
                 for (int g = 0; g < NG; ++g)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) o[g][e] *= at_start;
+                    for (int e = 0; e < 4; ++e) o[g][e] *= start;
 #pragma unroll
                 for (int ks = 0; ks < CS; ++ks)
                     if (w.template step<false>(ks))
@@ -367,14 +491,15 @@ template <typename T, int DKP, int NG, bool KEEP> __global__ __launch_bounds__(5
                         for (int g = 0; g < NG; ++g) {
                             D8 u[kFew];
                             W::template get<CS, kFew>(sO, g, ks, lane, u);
-                            o[g] = mma_whole(u, P[ks][0], o[g]);
+                            o[g] = mma_whole(u, mine.P[ks][0], o[g]);
                         }
                 const bool is = n * C + 16 * w.w + w.r < w.len;
                 store(n * C, [&](int g, int e) { return is ? o[g][e] : 0.f; });
             }
-            w.template load_steps<false>(a.to.scores, a, next, P);
-            at_start = w.gate_r(a, next);
-        }
+            load_scores(n + 2, mine);
+            asm volatile("" ::"v"(mine.touched[0]), "v"(mine.touched[1]));       // (asked for two chunks ago)
+            touch(n + W::kAhead, mine);
+        });
         // rows past the end of a shorter sequence
         for (int from = w.live * C; from < w.T_; from += 16 * W::kWaves) store(from, [](int, int) { return 0.f; });
         return;
@@ -390,68 +515,66 @@ template <typename T, int DKP, int NG, bool KEEP> __global__ __launch_bounds__(5
             for (int p = 0; p < PER; ++p)
                 if (w.mine(g) && w.feature(p) < w.DK) *reinterpret_cast<f32x4 *>(kept + w.state_place(n, g, w.w * PER + p)) = S[g][p];
     };
-    D8 K[KS], KT[PER][CS], Z[CS][kParts];
-    typename W::Cols V[NG / NC][4];
-    const typename W::Rows values = w.value_rows(a.values);
-    f32x4 start, end, beta;
-    float whole;
+    struct Set {
+        D8 Z[CS][kParts];
+    } x, y;
+    auto load = [&](int n, Set &to) { w.template load_steps<false>(a.to.inverse, a, min(n, last), to.Z); };
+    D8 K[KS], KT[PER][CS];
     if (w.live > 0) {
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) K[ks] = w.load_row(a.to.key_rows, a, 0, ks);
-        w.load_values(values, 0, V);
-        start = w.gate(a, 0, 0);
-        w.template load_steps<false>(a.to.inverse, a, 0, Z);
-        end = w.gate(a, 0, 1);
-        beta = w.gate(a, 0, 2);
-        w.load_features(a.to.keys, a, 0, KT);
-        whole = w.gate_whole(a, 0);
+        load(0, x);
+        load(1, y);
+        w.template put_state<kFew>(sS, S);
+        lds_barrier();                           // the first rows
+        w.get_rows(sK[0], K);
     }
-    w.template put_state<kFew>(sS, S);
-    for (int n = 0; n < w.live; ++n) {
-        const int next = min(n + 1, last);
+    in_turns(w.live, x, y, [&](int n, Set &mine, Set &) {
+        const float *gates = sG[n & 1];
         if constexpr (KEEP) keep(n);
-        f32x4 x[NG];
+        f32x4 v[NG];
         lds_barrier();                           // the state's operands are there
-        w.template keys_times_state<kFew>(a, next, sS, K, x);
-        if (w.tokens())
+        w.template keys_times_state<kFew>(sS, K, v);
+        if (w.tokens()) {
+            const f32x4 start = w.gate(gates, 0);
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
+                const f32x4 value = four(sV, g * CT + w.w);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) x[g][e] = W::value(V, g, e) - start[e] * x[g][e];
-                W::template put<CS, kParts>(sR, g, w.w, lane, x[g]);
+                for (int e = 0; e < 4; ++e) v[g][e] = value[e] - start[e] * v[g][e];
+                W::template put<CS, kParts>(sR, g, w.w, lane, v[g]);
             }
-        w.load_values(values, next, V);
-        start = w.gate(a, next, 0);
+        }
         lds_barrier();                           // r
-        w.template solve<false>(a, next, sR, Z, x);
-        if (w.tokens())
+        w.template solve<false>(sR, mine.Z, v);
+        if (w.tokens()) {
+            const f32x4 end = w.gate(gates, 1), beta = w.gate(gates, 2);
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
                 f32x4 u, weighted;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    u[e] = beta[e] * x[g][e];
+                    u[e] = beta[e] * v[g][e];
                     weighted[e] = end[e] * u[e];
                 }
                 W::template put<CS, kParts>(sU, g, w.w, lane, weighted);
                 W::template put<CS, kFew>(sO, g, w.w, lane, u);
                 if constexpr (KEEP)
-                    if (w.mine(g)) *reinterpret_cast<f32x4 *>(xs + w.written(n, g)) = x[g];
+                    if (w.mine(g)) *reinterpret_cast<f32x4 *>(xs + w.written(n, g)) = v[g];
             }
-        end = w.gate(a, next, 1);
-        beta = w.gate(a, next, 2);
-        lds_barrier();                           // u
-        // the state behind the chunk
+        }
+        w.get_features(sK[n & 1], KT);
+        const float whole = gates[3 * C];
 #pragma unroll
         for (int g = 0; g < NG; ++g)
 #pragma unroll
             for (int p = 0; p < PER; ++p)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) S[g][p][e] *= whole;
-        w.add_keys(a, next, sU, KT, S);
-        whole = w.gate_whole(a, next);
+        load(n + 2, mine);
+        lds_barrier();                           // u
+        w.add_keys(sU, KT, S);                   // the state behind the chunk
+        w.get_rows(sK[(n + 1) & 1], K);
         w.template put_state<kFew>(sS, S);
-    }
+    });
     if constexpr (KEEP) keep(w.live);
     w.store_state(a.hidden_out, a.hidden_dtype, S);
 }
@@ -468,46 +591,75 @@ template <typename T, int DKP, int NG> __global__ __launch_bounds__(512) void de
     constexpr int C = W::C, CT = W::CT, CS = W::CS, KS = W::KS, PER = W::PER, TILES = W::TILES, NC = W::NC, kParts = DC::kParts;
     constexpr int kRows = NG * CS * kParts * 512;
     extern __shared__ char smem[];
-    // the cotangents of the state, of u before the system is solved, of r and of out (scaled), of out as it is; the helpers' sums, in floats
-    T *sS = reinterpret_cast<T *>(smem), *sU = sS + NG * KS * kParts * 512, *sR = sU + kRows, *sO = sR + kRows, *sD = sO + kRows;
+    // keys of two chunks and queries of one; the cotangents of the state, of u before the system is solved, of r and of out (scaled), of out as
+    // it is; the helpers' sums, in floats; gates of two chunks
+    T *sK[2] = {reinterpret_cast<T *>(smem), reinterpret_cast<T *>(smem) + kTile<T, DKP>}, *sQ = sK[1] + kTile<T, DKP>, *sS = sQ + kTile<T, DKP>,
+      *sU = sS + NG * KS * kParts * 512, *sR = sU + kRows, *sO = sR + kRows, *sD = sO + kRows;
     float *sWritten = reinterpret_cast<float *>(sD + NG * CS * 512), *sState = sWritten + NG * CT * 256;
+    float *sG[2] = {sState + NG * TILES * 256, sState + NG * TILES * 256 + DC::kGates};
     W w;
     if (w.place(a)) return;
     const int lane = w.lane;
+    auto chunk_of = [&](int step) { return max(w.live - 1 - step, 0); };
     auto four = [&](float *p, int i) -> f32x4 & { return *reinterpret_cast<f32x4 *>(p + i * 256 + lane * 4); };
     if (w.helper) {
         if (w.live == 0) return;
         const float *kept = a.kept + w.pair * (delta_states_floats(a.n, a.chunks) + delta_written_floats(a.n, a.chunks, C));
         T *dstates = static_cast<T *>(a.dstates) + w.pair * a.chunks * delta_state_floats(a.n);
-        const typename W::Rows douts = w.value_rows(a.dout);
-        D8 QT[PER][CS], P[CS][kParts];
-        typename W::Cols O[NG / NC][4];
-        f32x4 start, S[NG][2], written[NG], state[NG][PER];
+        const typename W::Rows douts = w.value_rows(a.dout), keys = w.key_rows(a.keys), queries = w.key_rows(a.queries);
         const bool features = w.w < KS && 32 * w.w + 8 * w.c < w.DK;     // of a state: the eight 32w + 8c ..
-        auto load_kept = [&](int n) {
+        struct Set {
+            typename W::Stage key, query;
+            typename W::Cols O[NG / NC][4];
+            float gate;
+            f32x4 start, S[NG][2];                      // the state behind the chunk
+            D8 P[CS][kParts];
+            uint32_t touched[3];
+        } x, y;
+        const typename W::Ahead ahead = w.template ahead<kParts>(a, keys, queries);
+        auto touch = [&](int step, Set &to) {
+            const int n = chunk_of(step);
+            to.touched[0] = w.touch(ahead, n);
+            to.touched[1] = w.touch_values(douts, n);
+            // the states' tiles of a group of columns: 16 lines a wave (as many as there are)
+            const int64_t line = w.state_place(n + 1, 0, 0) - (w.c * 16 + w.r) * 4 + 512 * w.w + 32 * w.r;
+            to.touched[2] = __float_as_uint(kept[w.w < delta_state_tiles(w.DK) / 2 ? line : 0]);
+        };
+        auto load_rows = [&](int step, Set &to) {
+            const int n = chunk_of(step);
+            w.load_stage(keys, n, to.key);
+            w.load_stage(queries, n, to.query);
+            w.load_values(douts, n, to.O);
+            to.gate = w.load_gate(a, n);
+            to.start = w.load_start(a, n);
+        };
+        auto load_kept = [&](int step, Set &to) {
 #pragma unroll
             for (int g = 0; g < NG; ++g)
 #pragma unroll
                 for (int t = 0; t < 2; ++t)
-                    S[g][t] = *reinterpret_cast<const f32x4 *>(kept + (features && w.mine(g) ? w.state_place(n, g, 2 * w.w + t) : 0));
+                    to.S[g][t] = *reinterpret_cast<const f32x4 *>(kept + (features && w.mine(g) ? w.state_place(chunk_of(step) + 1, g, 2 * w.w + t) : 0));
         };
-        auto put_out = [&](int next) {           // the cotangents of out of one chunk as operands; `next`: what is loaded then
+        auto load_scores = [&](int step, Set &to) { w.template load_steps<true>(a.to.scores, a, chunk_of(step), to.P); };
+        auto put_rows = [&](int step, const Set &from) {
+            w.put_stage(sK[step & 1], from.key);
+            w.put_stage(sQ, from.query);
+            w.put_gate(sG[step & 1], from.gate);
             if (w.tokens())
 #pragma unroll
                 for (int g = 0; g < NG; ++g) {
                     f32x4 o, scaled;
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        o[e] = W::value(O, g, e);
-                        scaled[e] = start[e] * o[e];
+                        o[e] = W::value(from.O, g, e);
+                        scaled[e] = from.start[e] * o[e];
                     }
                     W::template put<CS, 1>(sD, g, w.w, lane, o);
                     W::template put<CS, kParts>(sO, g, w.w, lane, scaled);
                 }
-            w.load_values(douts, next, O);
-            start = w.gate(a, next, 0);
         };
-        auto sums = [&](int next) {
+        f32x4 written[NG], state[NG][PER];
+        auto sums = [&](const Set &of) {
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
                 written[g] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -522,45 +674,41 @@ template <typename T, int DKP, int NG> __global__ __launch_bounds__(512) void de
                         for (int g = 0; g < NG; ++g) {
                             D8 o[1];
                             W::template get<CS, 1>(sD, g, ks, lane, o);
-                            written[g] = mma_whole(P[ks], o[0], written[g]);
+                            written[g] = mma_whole(of.P[ks], o[0], written[g]);
                         }
-            w.template load_steps<true>(a.to.scores, a, next, P);
-#pragma unroll
-            for (int ks = 0; ks < CS; ++ks)
-#pragma unroll
-                for (int g = 0; g < NG; ++g) {
-                    D8 o[kParts];
-                    W::template get<CS, kParts>(sO, g, ks, lane, o);
-#pragma unroll
-                    for (int i = kParts - 1; i >= 0; --i)
-#pragma unroll
-                        for (int p = 0; p < PER; ++p) state[g][p] = mma_d(QT[p][ks], o[i], state[g][p]);
-                }
-            w.load_features(a.to.queries, a, next, QT);
+            D8 QT[PER][CS];
+            w.get_features(sQ, QT);
+            w.add_keys(sO, QT, state);
         };
         auto hand_written = [&] {
             if (w.tokens())
 #pragma unroll
                 for (int g = 0; g < NG; ++g) four(sWritten, g * CT + w.w) = written[g];
         };
-        const int n0 = w.live - 1;
-        load_kept(n0 + 1);
-        w.load_values(douts, n0, O);
-        start = w.gate(a, n0, 0);
-        w.template load_steps<true>(a.to.scores, a, n0, P);
-        w.load_features(a.to.queries, a, n0, QT);
-        put_out(max(n0 - 1, 0));
-        lds_barrier();                           // the operands of the first chunk's sums
-        sums(max(n0 - 1, 0));
+        load_rows(0, x);
+        load_scores(0, x);
+        load_kept(0, x);
+        load_rows(1, y);
+        load_scores(1, y);
+        load_kept(1, y);
+        put_rows(0, x);
+        load_rows(2, x);
+        touch(W::kAhead - 2, x);
+        touch(W::kAhead - 1, y);
+        lds_barrier();                           // the first keys, and the operands of the first sums
+        sums(x);
+        load_scores(2, x);
         hand_written();
-        for (int n = n0; n >= 0; --n) {
-            const int next = max(n - 2, 0);
+        in_turns(w.live, x, y, [&](int step, Set &mine, Set &next) {
+            const int n = w.live - 1 - step;
             lds_barrier();                       // dS, and what the helpers add to du
 #pragma unroll
             for (int g = 0; g < NG; ++g)
 #pragma unroll
                 for (int p = 0; p < PER; ++p) four(sState, g * TILES + w.w * PER + p) = state[g][p];
-            put_out(next);
+            put_rows(step + 1, next);
+            lds_barrier();                       // du
+            sums(next);
             // the cotangent of the state behind the chunk, for the gradients; its product with that state
             float *dots = a.dots + (((int64_t)w.pair * a.chunks + n) * (w.DV >> 4) + (w.col0 >> 4)) * 4 + w.w;
 #pragma unroll
@@ -571,16 +719,16 @@ template <typename T, int DKP, int NG> __global__ __launch_bounds__(512) void de
                     if (features && w.mine(q)) {
                         D8 parts[kParts];
                         W::template get<KS, kParts>(sS, q, w.w, lane, parts);
-                        float d[8], x[8];
+                        float d[8], z[8];
                         unpack8(parts[kParts - 1], d);
 #pragma unroll
                         for (int i = kParts - 2; i >= 0; --i) {
-                            unpack8(parts[i], x);
+                            unpack8(parts[i], z);
 #pragma unroll
-                            for (int e = 0; e < 8; ++e) d[e] += x[e];
+                            for (int e = 0; e < 8; ++e) d[e] += z[e];
                         }
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) dot += d[e] * S[q][e >> 2][e & 3];
+                        for (int e = 0; e < 8; ++e) dot += d[e] * mine.S[q][e >> 2][e & 3];
                         st8(dstates + w.cotangent_place(n, q, w.w), parts[0]);
                     }
                 dot = sum_over_c(sum_over_r(dot));
@@ -588,35 +736,38 @@ template <typename T, int DKP, int NG> __global__ __launch_bounds__(512) void de
                     for (int q = 0; q < NC; ++q)
                         if (w.col0 + 16 * (g + q) < w.DV) dots[4 * (g + q)] = q ? 0.f : dot;
             }
-            load_kept(n);
-            lds_barrier();                       // du
-            sums(next);
             lds_barrier();                       // dr
             hand_written();
-        }
+            load_kept(step + 2, mine);
+            load_rows(step + 3, next);
+            load_scores(step + 3, next);
+            asm volatile("" ::"v"(mine.touched[0]), "v"(mine.touched[1]), "v"(mine.touched[2]));
+            touch(step + W::kAhead, mine);
+        });
         return;
     }
     f32x4 S[NG][PER];
     w.load_state(a.hidden, a.hidden_dtype, S);
     if (w.live > 0) {
         float *dus = a.du + w.pair * delta_written_floats(a.n, a.chunks, C);
-        D8 K[KS], KT[PER][CS], Z[CS][kParts];
-        const int n0 = w.live - 1;
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) K[ks] = w.load_row(a.to.key_rows, a, n0, ks);
-        f32x4 end = w.gate(a, n0, 1);
-        w.template load_steps<true>(a.to.inverse, a, n0, Z);
-        f32x4 start = w.gate(a, n0, 0), beta = w.gate(a, n0, 2);
-        w.load_features(a.to.keys, a, n0, KT);
-        float whole = w.gate_whole(a, n0);
+        struct Set {
+            D8 Z[CS][kParts];
+        } x, y;
+        auto load = [&](int step, Set &to) { w.template load_steps<true>(a.to.inverse, a, chunk_of(step), to.Z); };
+        load(0, x);
+        load(1, y);
+        D8 K[KS], KT[PER][CS];
         w.template put_state<kParts>(sS, S);
-        lds_barrier();                           // (the helpers')
-        for (int n = n0; n >= 0; --n) {
-            const int next = max(n - 1, 0);
+        lds_barrier();                           // the first keys
+        w.get_rows(sK[0], K);
+        in_turns(w.live, x, y, [&](int step, Set &mine, Set &) {
+            const int n = w.live - 1 - step;
+            const float *gates = sG[step & 1];
             f32x4 du[NG];
             lds_barrier();                       // dS, and what the helpers add to du
-            w.template keys_times_state<kParts>(a, next, sS, K, du);
-            if (w.tokens())
+            w.template keys_times_state<kParts>(sS, K, du);
+            if (w.tokens()) {
+                const f32x4 end = w.gate(gates, 1);
 #pragma unroll
                 for (int g = 0; g < NG; ++g) {
                     const f32x4 scores = four(sWritten, g * CT + w.w);
@@ -624,10 +775,11 @@ template <typename T, int DKP, int NG> __global__ __launch_bounds__(512) void de
                     for (int e = 0; e < 4; ++e) du[g][e] = end[e] * du[g][e] + scores[e];
                     W::template put<CS, kParts>(sU, g, w.w, lane, du[g]);
                 }
-            end = w.gate(a, next, 1);
+            }
             lds_barrier();                       // du
-            w.template solve<true>(a, next, sU, Z, du);
-            if (w.tokens())
+            w.template solve<true>(sU, mine.Z, du);
+            if (w.tokens()) {
+                const f32x4 start = w.gate(gates, 0), beta = w.gate(gates, 2);
 #pragma unroll
                 for (int g = 0; g < NG; ++g) {
                     f32x4 v;
@@ -636,8 +788,10 @@ template <typename T, int DKP, int NG> __global__ __launch_bounds__(512) void de
                     W::template put<CS, kParts>(sR, g, w.w, lane, v);
                     if (w.mine(g)) *reinterpret_cast<f32x4 *>(dus + w.written(n, g)) = du[g];
                 }
-            start = w.gate(a, next, 0);
-            beta = w.gate(a, next, 2);
+            }
+            w.get_features(sK[step & 1], KT);
+            const float whole = gates[3 * C];
+            load(step + 2, mine);
             lds_barrier();                       // dr
 #pragma unroll
             for (int g = 0; g < NG; ++g)
@@ -647,10 +801,10 @@ template <typename T, int DKP, int NG> __global__ __launch_bounds__(512) void de
 #pragma unroll
                     for (int e = 0; e < 4; ++e) S[g][p][e] = S[g][p][e] * whole + out[e];
                 }
-            w.add_keys(a, next, sR, KT, S);
-            whole = w.gate_whole(a, next);
+            w.add_keys(sR, KT, S);
+            w.get_rows(sK[(step + 1) & 1], K);
             w.template put_state<kParts>(sS, S);
-        }
+        });
     }
     w.store_state(a.hidden_out, a.hidden_dtype, S);
 }
@@ -660,8 +814,10 @@ template <typename T, int DKP, int NG, bool BACK> constexpr size_t walk_lds()
 {
     typedef Walk<T, DKP, NG> W;
     typedef DeltaChunk<T> DC;
-    return BACK ? sizeof(T) * 512 * NG * (W::KS * DC::kParts + W::CS * (3 * DC::kParts + 1)) + sizeof(float) * 256 * NG * (W::CT + W::TILES)
-                : sizeof(T) * 512 * NG * (W::KS * DC::kFew + W::CS * (2 * DC::kParts + DC::kFew));
+    constexpr size_t tiles = sizeof(T) * 3 * kTile<T, DKP>;
+    return tiles + sizeof(float) * 2 * DC::kGates +
+           (BACK ? sizeof(T) * 512 * NG * (W::KS * DC::kParts + W::CS * (3 * DC::kParts + 1)) + sizeof(float) * 256 * NG * (W::CT + W::TILES)
+                         : sizeof(T) * 512 * NG * (W::KS * DC::kFew + W::CS * (2 * DC::kParts + DC::kFew)) + sizeof(float) * 256 * NG * W::CT);
 }
 template <typename T, int DKP, int NG, bool BACK> int launch_walk(hipStream_t stream, const DeltaArgs &a)
 {
@@ -678,13 +834,11 @@ template <typename T, int DKP, int NG, bool BACK> int launch_walk(hipStream_t st
     if constexpr (BACK) return launch(grants[0], delta_walk_back_kernel<T, DKP, NG>);
     else return a.kept ? launch(grants[0], delta_walk_kernel<T, DKP, NG, true>) : launch(grants[1], delta_walk_kernel<T, DKP, NG, false>);
 }
-// Value columns of a workgroup: 64 share the operands' way from memory, 16 make four times the workgroups.
+// Value columns of a workgroup: 32 share the operands' way from memory, 16 make twice the workgroups.
 template <typename T, int DKP, bool BACK> int choose_walk(hipStream_t stream, const DeltaArgs &a)
 {
     const int64_t groups = a.pairs * ((a.n.DV + 15) / 16);
-    if constexpr (walk_lds<T, DKP, 4, BACK>() <= 160 * 1024)
-        if (a.n.DV > 32 && groups >= 8 * kComputeUnits) return launch_walk<T, DKP, 4, BACK>(stream, a);
-    if (a.n.DV > 16 && groups >= 4 * kComputeUnits) return launch_walk<T, DKP, 2, BACK>(stream, a);
+    if (a.n.DV > 16 && groups > kComputeUnits) return launch_walk<T, DKP, 2, BACK>(stream, a);
     return launch_walk<T, DKP, 1, BACK>(stream, a);
 }
 template <typename T, bool BACK> int dispatch_walk(hipStream_t stream, const DeltaArgs &a)
