@@ -23,7 +23,7 @@ template <typename T, int F> __device__ __forceinline__ int place_in(int row, in
 template <typename T, int DKP> __global__ __launch_bounds__(DKP * 4) void delta_gradient_kernel(const DeltaArgs a)
 {
     typedef DeltaChunk<T> DC;
-    constexpr int C = DC::C, CT = DC::CT, CS = DC::CS, KS = DKP / 32, NW = DKP / 16, NT = 64 * NW, VS = kSlice / 32, kParts = DC::kFew;
+    constexpr int C = DC::C, CT = DC::CT, CS = DC::CS, KS = DKP / 32, NW = DKP / 16, NT = 64 * NW, VS = kSlice / 32, kParts = DC::kParts, kFew = DC::kFew;
     constexpr int kTriangle = CT * (CT + 1) / 2, kUnits = (2 * kTriangle + NW - 1) / NW, kShare = NW / CT;
     typedef typename FragTypes<T>::d8 D8;
     typedef typename Packed4<T>::t Four;
@@ -33,8 +33,9 @@ template <typename T, int DKP> __global__ __launch_bounds__(DKP * 4) void delta_
     constexpr int kK = C * TileK::kRow, kS = kSlice * TileK::kRow, kU = kSlice * TileU::kRow, kP = C * TileU::kRow;
     extern __shared__ char smem[];
     T *sQ = reinterpret_cast<T *>(smem), *sK = sQ + kK, *sS = sK + kK, *sD = sS + kParts * kS, *sO = sD + kS, *sU = sO + C * TileO::kRow,
-      *sX = sU + kParts * kU, *sP = sX + kU, *sE = sP + kP;
-    ChunkGates<C> *gate = reinterpret_cast<ChunkGates<C> *>(sE + kP);
+      *sX = sU + kParts * kU, *sP = sS, *sE = sP + kP;     // (the scores take the states' place)
+    static_assert(2 * kP <= kParts * kS, "");
+    ChunkGates<C> *gate = reinterpret_cast<ChunkGates<C> *>(sX + kU);
     struct Sums {
         float beta[C];
         float pairs[CT][C];                      // row sums of P (do.u), one column of tiles each
@@ -76,6 +77,35 @@ template <typename T, int DKP> __global__ __launch_bounds__(DKP * 4) void delta_
     const float *dus = a.du + pair * floats + n * C * DV;
     const T *dS = static_cast<const T *>(a.dstates) + (pair * chunks + n) * state;
     kept += n * state;
+    // A slice of values on its way: no load is under a branch, for then each waits for the one before, and the next slice's are issued before the
+    // products of one.  (One after the other they took 25000 of a chunk's 46000 cycles at 128 x 128 features.)
+    constexpr int kStates = kSlice / 16 * KS / NW, kTiles = kSlice / 16 / kShare;
+    static_assert(kSlice / 16 * KS % NW == 0 && kSlice / 16 % kShare == 0, "");
+    RowsInFlight<T, C, kSlice, NT> o;
+    f32x4 low[kStates], high[kStates], written[kTiles], dwritten[kTiles];
+    D8 dstate[kStates];
+    T value[kTiles][4];
+    const int own = w % CT, token = 16 * own + 4 * c;       // of what was written
+    auto load_slice = [&](int dv0) {
+        o.load(tid, O + dv0, (int)a.dout.st, there, DV - dv0);
+#pragma unroll
+        for (int i = 0; i < kStates; ++i) {
+            const int m = (w + i * NW) / KS, ks = (w + i * NW) % KS;
+            const unsigned from = dv0 + 16 * m < DV && 32 * ks < DK ? (((dv0 >> 4) + m) * (delta_state_tiles(DK) / 2) + ks) * 512 : 0;
+            low[i] = *reinterpret_cast<const f32x4 *>(kept + from + lane * 4);
+            high[i] = *reinterpret_cast<const f32x4 *>(kept + from + 256 + lane * 4);
+            dstate[i] = ld8(dS + from + lane * 8);
+        }
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i) {
+            const int m = w / CT + i * kShare, at = dv0 + 16 * m < DV ? dv0 + 16 * m : 0;
+            const unsigned from = (at / 16 * CT + own) * 256 + lane * 4;
+            written[i] = *reinterpret_cast<const f32x4 *>(xs + from);
+            dwritten[i] = *reinterpret_cast<const f32x4 *>(dus + from);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) value[i][e] = V[(int64_t)min(token + e, there - 1) * a.values.st + at + r];
+        }
+    };
     float log_decay = 0.f;
     {
         RowsInFlight<T, C, DKP, NT> x, q;
@@ -86,7 +116,7 @@ template <typename T, int DKP> __global__ __launch_bounds__(DKP * 4) void delta_
             chunk_gates<C>(*gate, log_decay);
         }
         if (w == 1 && lane < C) sums.beta[lane] = a.to.gates[(pair * chunks + n) * DC::kGates + 2 * C + lane];
-        for (int i = tid; i < kP; i += NT) sP[i] = (T)0.f;
+        load_slice(0);
         x.store(tid, sK, there, DK);
         q.store(tid, sQ, there, DK);
     }
@@ -102,58 +132,43 @@ template <typename T, int DKP> __global__ __launch_bounds__(DKP * 4) void delta_
 
     for (int dv0 = 0; dv0 < DV; dv0 += kSlice) {
         lds_barrier();                           // beta is there; the last slice's tiles are read
-        {
-            RowsInFlight<T, C, kSlice, NT> o;
-            o.load(tid, O + dv0, (int)a.dout.st, there, DV - dv0);
-            // states: eight features of a value feature a lane
 #pragma unroll
-            for (int i = w; i < kSlice / 16 * KS; i += NW) {
-                const int m = i / KS, ks = i % KS, col = 32 * ks + 8 * c, at = TileK::piece(16 * m + r, col);
-                const bool is = dv0 + 16 * m < DV && col < DK;
-                const unsigned from = is ? (((dv0 >> 4) + m) * (delta_state_tiles(DK) / 2) + ks) * 512 : 0;
-                const f32x4 low = *reinterpret_cast<const f32x4 *>(kept + from + lane * 4), high = *reinterpret_cast<const f32x4 *>(kept + from + 256 + lane * 4);
-                const D8 d = ld8(dS + from + lane * 8);
-                float s[8];
+        for (int i = 0; i < kStates; ++i) {      // eight features of a value feature a lane
+            const int m = (w + i * NW) / KS, ks = (w + i * NW) % KS, col = 32 * ks + 8 * c, at = TileK::piece(16 * m + r, col);
+            const bool is = dv0 + 16 * m < DV && col < DK;
+            float x[8];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) s[e] = is ? low[e] : 0.f, s[4 + e] = is ? high[e] : 0.f;
-                const Split<T, kParts> split(s);
+            for (int e = 0; e < 4; ++e) x[e] = is ? low[i][e] : 0.f, x[4 + e] = is ? high[i][e] : 0.f;
+            const Split<T, kParts> split(x);
 #pragma unroll
-                for (int p = 0; p < kParts; ++p) st8(sS + p * kS + at, split.part[p]);
-                st8(sD + at, is ? d : D8{});
-            }
-            const int ti = w % CT, token = 16 * ti + 4 * c;
-            const f32x4 beta = *reinterpret_cast<const f32x4 *>(sums.beta + token);
-#pragma unroll
-            for (int m = w / CT; m < kSlice / 16; m += kShare) {
-                const int value = 16 * m + r;
-                const bool is = dv0 + 16 * m < DV;
-                f32x4 x = {0.f, 0.f, 0.f, 0.f}, du = {0.f, 0.f, 0.f, 0.f};
-                const int64_t from = ((int64_t)(dv0 / 16 + m) * CT + ti) * 256 + lane * 4;
-                if (is) {
-                    x = *reinterpret_cast<const f32x4 *>(xs + from);
-                    du = *reinterpret_cast<const f32x4 *>(dus + from);
-                }
-                f32x4 u, dx;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float v = is && token + e < there ? (float)V[(int64_t)min(token + e, there - 1) * a.values.st + (is ? dv0 + value : 0)] : 0.f;
-                    u[e] = beta[e] * x[e];
-                    dx[e] = beta[e] * du[e];
-                    db[e] += x[e] * du[e];
-                    vdv[e] += v * dx[e];
-                }
-                const int at = place_in<T, C>(value, token);
-                *reinterpret_cast<Four *>(sX + at) = pack_results<T>(dx);
-#pragma unroll
-                for (int p = 0; p < kParts; ++p) {
-                    const Four f = pack_results<T>(u);
-                    *reinterpret_cast<Four *>(sU + p * kU + at) = f;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) u[e] -= (float)f[e];
-                }
-            }
-            o.store(tid, sO, there, DV - dv0);
+            for (int p = 0; p < kParts; ++p) st8(sS + p * kS + at, split.part[p]);
+            st8(sD + at, is ? dstate[i] : D8{});
         }
+        const f32x4 beta = *reinterpret_cast<const f32x4 *>(sums.beta + token);
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i) {
+            const int m = w / CT + i * kShare, at = place_in<T, C>(16 * m + r, token);
+            const bool is = dv0 + 16 * m < DV;
+            f32x4 u, dx;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float x = is ? written[i][e] : 0.f, du = is ? dwritten[i][e] : 0.f, v = is && token + e < there ? (float)value[i][e] : 0.f;
+                u[e] = beta[e] * x;
+                dx[e] = beta[e] * du;
+                db[e] += x * du;
+                vdv[e] += v * dx[e];
+            }
+            *reinterpret_cast<Four *>(sX + at) = pack_results<T>(dx);
+#pragma unroll
+            for (int p = 0; p < kParts; ++p) {
+                const Four f = pack_results<T>(u);
+                *reinterpret_cast<Four *>(sU + p * kU + at) = f;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) u[e] -= (float)f[e];
+            }
+        }
+        o.store(tid, sO, there, DV - dv0);
+        if (dv0 + kSlice < DV) load_slice(dv0 + kSlice);
         lds_barrier();
         // dv, a token's 4 values twice
         for (int unit = w; unit < CT * VS; unit += NW) {
@@ -181,7 +196,9 @@ template <typename T, int DKP> __global__ __launch_bounds__(DKP * 4) void delta_
 #pragma unroll
                     for (int p = kParts - 1; p >= 0; --p) score[m] = mma_d(tu.columns(sU + p * kU, ks, tj), o, score[m]);
                 } else {
-                    score[m] = mma_d(tu.columns(sU, ks, tj), tu.columns(sX, ks, ti), score[m]);
+                    const D8 x = tu.columns(sX, ks, ti);
+#pragma unroll
+                    for (int p = kFew - 1; p >= 0; --p) score[m] = mma_d(tu.columns(sU + p * kU, ks, tj), x, score[m]);
                 }
             }
         }
@@ -194,11 +211,17 @@ template <typename T, int DKP> __global__ __launch_bounds__(DKP * 4) void delta_
 #pragma unroll
             for (int ti = 0; ti < CT; ++ti) {
                 fromO[ti] = mma_whole(s, to.halves(sO, ti, ks), fromO[ti]);
-                fromX[ti] = mma_d(s[0], tu.columns(sX, ks, ti), fromX[ti]);
-                fromU[ti] = mma_d(d, tu.columns(sU, ks, ti), fromU[ti]);
+                const D8 x = tu.columns(sX, ks, ti);
+#pragma unroll
+                for (int p = kFew - 1; p >= 0; --p) {
+                    fromX[ti] = mma_d(s[p], x, fromX[ti]);
+                    fromU[ti] = mma_d(d, tu.columns(sU + p * kU, ks, ti), fromU[ti]);
+                }
             }
         }
     }
+    lds_barrier();                               // the states are read
+    if (w < CT / 2) *reinterpret_cast<Four *>(tu.four(sP, 2 * w, 2 * w + 1)) = Four{};      // the tiles above the diagonal that operands reach into
 #pragma unroll
     for (int m = 0; m < kUnits; ++m) {
         const int unit = w + m * NW;
@@ -315,9 +338,9 @@ template <typename T, int DKP> int launch_gradient(hipStream_t stream, const Del
 {
     typedef DeltaChunk<T> DC;
     static LdsGrant grant;
-    constexpr int C = DC::C, NW = DKP / 16, kParts = DC::kFew;
+    constexpr int C = DC::C, NW = DKP / 16, kParts = DC::kParts;
     constexpr size_t lds = sizeof(T) * ((2 * C + (kParts + 1) * kSlice) * LdsTile<T, DKP>::kRow + C * LdsTile<T, kSlice>::kRow +
-                                        ((kParts + 1) * kSlice + 2 * C) * LdsTile<T, C>::kRow) +
+                                        (kParts + 1) * kSlice * LdsTile<T, C>::kRow) +
                            sizeof(ChunkGates<C>) + sizeof(float) * C * (1 + DC::CT + NW + 2 * (NW / DC::CT));
     static_assert(lds <= 160 * 1024 && NW % DC::CT == 0, "");
     if (int e = allow_lds(grant, reinterpret_cast<const void *>(delta_gradient_kernel<T, DKP>), lds)) return e;
