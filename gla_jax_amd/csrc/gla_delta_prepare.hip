@@ -15,11 +15,13 @@ template <typename T, int DKP, bool BACK> __global__ __launch_bounds__(256) void
     typedef DeltaChunk<T> DC;
     constexpr int C = DC::C, CT = DC::CT, KS = DKP / 32, NW = 4, NT = 256, kTriangle = CT * (CT + 1) / 2;
     constexpr int kRow = C + 4, kBlock = 16 * 20, kParts = DC::kParts, kScoreParts = BACK ? kParts : 1;
+    typedef typename FragTypes<T>::d8 D8;
     typedef typename Packed4<T>::t Four;
     typedef LdsTile<T, DKP> Tile;
     extern __shared__ char smem[];
     T *sK = reinterpret_cast<T *>(smem), *sQ = sK + C * Tile::kRow;
-    float *sN = reinterpret_cast<float *>(sQ + C * Tile::kRow), *sX = sN + C * kRow, *sB = sX + CT * kBlock;
+    float *sN = reinterpret_cast<float *>(sQ + C * Tile::kRow), *sB = sN + C * kRow, *sX = reinterpret_cast<float *>(sQ);      // (behind the scores the queries are not needed)
+    static_assert(CT * kBlock * sizeof(float) <= C * Tile::kRow * sizeof(T), "");
     ChunkGates<C> *gate = reinterpret_cast<ChunkGates<C> *>(sB + C);
 
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, r = lane & 15, c = lane >> 4;
@@ -61,28 +63,37 @@ template <typename T, int DKP, bool BACK> __global__ __launch_bounds__(256) void
             for (int e = 0; e < 4; ++e) v[e] -= (float)f[e];
         }
     };
+    // M and P tile by tile, both at a time: they have one operand and their weights in common.  Forward four neighbouring j of one i a lane,
+    // backward four i of one j.
     const Tile tile;
-#pragma unroll 1
-    for (int unit = w; unit < 2 * kTriangle; unit += NW) {
-        const bool keys = unit < kTriangle;
+#pragma unroll
+    for (int m = 0; m < (kTriangle + NW - 1) / NW; ++m) {
+        const int unit = w + m * NW;
+        if (unit >= kTriangle) break;
         int ti, tj;
-        triangle(keys ? unit : unit - kTriangle, ti, tj);
-        // four neighbouring i of one j a lane, or four j of one i
-        const bool rows = keys != BACK;
-        const T *mine = keys ? sK : sQ;
+        triangle(unit, ti, tj);
         const Tile L = tile.here();
-        const f32x4 s = rows ? tile_product<KS>(L, mine, ti, sK, tj) : tile_product<KS>(L, sK, tj, mine, ti);
-        const int i0 = 16 * ti + (rows ? 4 * c : r), j0 = 16 * tj + (rows ? r : 4 * c);
-        f32x4 v;
+        f32x4 kk = {0.f, 0.f, 0.f, 0.f}, qk = kk;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            const D8 kj = L.rows(sK, tj, ks), ki = L.rows(sK, ti, ks), qi = L.rows(sQ, ti, ks);
+            kk = BACK ? mma_d(ki, kj, kk) : mma_d(kj, ki, kk);
+            qk = BACK ? mma_d(qi, kj, qk) : mma_d(kj, qi, qk);
+        }
+        const int i0 = 16 * ti + (BACK ? 4 * c : r), j0 = 16 * tj + (BACK ? r : 4 * c), one = BACK ? j0 : i0, four = BACK ? i0 : j0;
+        const float sum1 = gate->sum[one], rest1 = gate->rest[one];
+        const f32x4 sum4 = *reinterpret_cast<const f32x4 *>(gate->sum + four), rest4 = *reinterpret_cast<const f32x4 *>(gate->rest + four),
+                    beta4 = *reinterpret_cast<const f32x4 *>(sB + four);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const int i = rows ? i0 + e : i0, j = rows ? j0 : j0 + e;
-            const float weight = ChunkGates<C>::weight(gate->sum[i], gate->rest[i], gate->sum[j], gate->rest[j]);
-            v[e] = keys ? (j < i ? s[e] * weight * sB[BACK ? i : j] : 0.f) : j <= i ? s[e] * weight : 0.f;
+            const int i = BACK ? i0 + e : i0, j = BACK ? j0 : j0 + e;
+            const float weight = BACK ? ChunkGates<C>::weight(sum4[e], rest4[e], sum1, rest1) : ChunkGates<C>::weight(sum1, rest1, sum4[e], rest4[e]);
+            // (the gate that N takes is b_j forward and b_i backward: of the four in both cases)
+            sN[(four + e) * kRow + one] = j < i ? kk[e] * weight * beta4[e] : 0.f;
+            qk[e] = j <= i ? qk[e] * weight : 0.f;
         }
-        if (keys) *reinterpret_cast<f32x4 *>(sN + (rows ? j0 * kRow + i0 : i0 * kRow + j0)) = v;
-        else if (BACK) put(scores, std::integral_constant<int, kScoreParts>{}, tj, ti, v);
-        else put(scores, std::integral_constant<int, kScoreParts>{}, ti, tj, v);
+        if (BACK) put(scores, std::integral_constant<int, kScoreParts>{}, tj, ti, qk);
+        else put(scores, std::integral_constant<int, kScoreParts>{}, ti, tj, qk);
     }
     if (tid < C) {
         float *to = a.to.gates + pc * DC::kGates;
@@ -97,21 +108,24 @@ template <typename T, int DKP, bool BACK> __global__ __launch_bounds__(256) void
     f32x4 X[CT];
     if (w < CT) {
         float x[16];
+        f32x4 rows[16][4];                       // (of the triangle: all on their way at once)
         const float *D = sN + 16 * w * kRow + 16 * w;
 #pragma unroll
         for (int m = 0; m < 16; ++m) {
             const int i = BACK ? m : 15 - m;
-            float row[16];
 #pragma unroll
-            for (int j = 0; j < 16; j += 4) {
-                const f32x4 t = *reinterpret_cast<const f32x4 *>(D + i * kRow + j);
+            for (int j = 0; j < 4; ++j)
+                if (BACK ? 4 * j < i : 4 * j + 3 > i) rows[i][j] = *reinterpret_cast<const f32x4 *>(D + i * kRow + 4 * j);
+        }
 #pragma unroll
-                for (int e = 0; e < 4; ++e) row[j + e] = t[e];
-            }
+        for (int m = 0; m < 16; ++m) {
+            const int i = BACK ? m : 15 - m;
             float s = i == r ? 1.f : 0.f;
 #pragma unroll
-            for (int j = 0; j < 16; ++j)
-                if (BACK ? j < i : j > i) s -= row[j] * x[j];
+            for (int k = 0; k < m; ++k) {        // the newest last
+                const int j = BACK ? k : 15 - k;
+                s -= rows[i][j >> 2][j & 3] * x[j];
+            }
             x[i] = s;
         }
 #pragma unroll
@@ -145,7 +159,7 @@ template <typename T, int DKP, bool BACK> int launch_prepare(hipStream_t stream,
 {
     typedef DeltaChunk<T> DC;
     constexpr size_t lds = sizeof(T) * 2 * DC::C * LdsTile<T, DKP>::kRow +
-                           sizeof(float) * (DC::C * (DC::C + 4) + DC::CT * 16 * 20 + DC::C) + sizeof(ChunkGates<DC::C>);
+                           sizeof(float) * (DC::C * (DC::C + 4) + DC::C) + sizeof(ChunkGates<DC::C>);
     static_assert(lds <= 64 * 1024, "");
     delta_prepare_kernel<T, DKP, BACK><<<a.pairs * a.chunks, 256, lds, stream>>>(a);
     return launch_status();
