@@ -39,6 +39,8 @@ int64_t lay_out(DeltaArgs &a, gla_dtype dtype, bool backward, char *ws, float **
     a.to.inverse = take(chunk_pairs * steps * parts * 512 * e);
     a.to.scores = take(chunk_pairs * steps * (backward ? parts : 1) * 512 * e);
     a.to.gates = reinterpret_cast<float *>(take(chunk_pairs * 4 * C * 4));
+    a.summary = reinterpret_cast<float *>(take(a.pairs * (a.segments - 1) * (a.n.DV + a.n.DK) * a.n.DK * 4));
+    a.starts = reinterpret_cast<float *>(take(a.pairs * (a.segments - 1) * a.n.DV * a.n.DK * 4));
     if (!backward) return at;
     a.du = reinterpret_cast<float *>(take(a.pairs * delta_written_floats(a.n, a.chunks, (int)C) * 4));
     a.dstates = take(chunk_pairs * delta_state_floats(a.n) * e);
@@ -57,6 +59,12 @@ DeltaArgs sizes_of(const DecaySizes &n, gla_dtype dtype)
     a.n = n;
     a.chunks = chunks_of(n, dtype);
     a.pairs = n.B * n.H;
+    a.segments = 1;
+    a.segment_chunks = (int)a.chunks;
+    if (a.chunks) {
+        a.segment_chunks = (int)((a.chunks + delta_segments(a) - 1) / delta_segments(a));
+        a.segments = (int)((a.chunks + a.segment_chunks - 1) / a.segment_chunks);
+    }
     return a;
 }
 int64_t workspace_bytes(const DecaySizes &n, gla_dtype dtype, bool backward)

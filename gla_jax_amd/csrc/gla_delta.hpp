@@ -65,6 +65,10 @@ struct DeltaArgs {
     float *du;
     void *dstates;
     float *dots;
+    // A long walk in segments of chunks at once (segments > 1): of each but the last, in the walk's order, what it leaves of a start from zero (of the
+    // first, of hidden) and of a basis, [pairs, segments - 1][DV + DK][DK] floats; and the states that the others start from, [pairs, segments - 1][DV][DK].
+    int segments, segment_chunks;
+    float *summary, *starts;
     void *dvalue, *dkey, *dquery;   // dkey, dquery: in their own type, or (more than one part) floats [part][...]
     float *dgate, *dbeta;
     int row_parts;
@@ -117,6 +121,8 @@ template <typename D8, int N> __device__ __forceinline__ f32x4 mma_whole(const D
     return c;
 }
 
+// How many segments a walk is cut into.
+int delta_segments(const DeltaArgs &a);
 int delta_prepare(void *stream, const DeltaArgs &a, gla_dtype dtype, bool backward);
 int delta_walk(void *stream, const DeltaArgs &a, gla_dtype dtype, bool backward);
 int delta_gradients(void *stream, const DeltaArgs &a, gla_dtype dtype);

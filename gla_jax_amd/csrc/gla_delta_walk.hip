@@ -45,6 +45,8 @@ template <typename T, int DKP, int NG> struct Walk {
     static constexpr int NC = NG > 1 ? 2 : 1;            // columns of a lane that lie next to each other
     typedef typename Columns<T, NC>::t Cols;
     int w, lane, r, c, DK, DV, T_, len, live, col0;
+    int order, segment, first, end;                      // the segment's chunks: first .. end - 1
+    bool basis;                                          // the columns are not the state's, but a basis of it
     unsigned pair;
     int64_t b, h, hk;
     bool helper;
@@ -60,7 +62,7 @@ template <typename T, int DKP, int NG> struct Walk {
                                                  0x00027000);
     }
     // true: there is nothing to do
-    __device__ __forceinline__ bool place(const DeltaArgs &a)
+    template <bool SUMMARY, bool BACK> __device__ __forceinline__ bool place(const DeltaArgs &a)
     {
         w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         helper = w >= kWaves;
@@ -70,9 +72,14 @@ template <typename T, int DKP, int NG> struct Walk {
         c = lane >> 4;
         DK = (int)a.n.DK;
         DV = (int)a.n.DV;
-        const unsigned groups = ((unsigned)DV + 16 * NG - 1) / (16 * NG), turn = blockIdx.x / 8;
-        pair = turn / groups * 8 + blockIdx.x % 8;
-        col0 = (int)(turn % groups) * 16 * NG;
+        const unsigned of_values = ((unsigned)DV + 16 * NG - 1) / (16 * NG), groups = of_values + (SUMMARY ? ((unsigned)DK + 16 * NG - 1) / (16 * NG) : 0);
+        const unsigned turn = blockIdx.x / 8, units = (a.segments - (SUMMARY ? 1 : 0)) * groups, group = turn % units % groups;
+        pair = turn / units * 8 + blockIdx.x % 8;
+        order = turn % units / groups;
+        segment = BACK ? a.segments - 1 - order : order;
+        basis = group >= of_values;
+        col0 = (int)(basis ? group - of_values : group) * 16 * NG;
+        if (SUMMARY && basis && order == 0) return true;         // (the first one's start is known)
         if (pair >= (unsigned)a.pairs) return true;
         const unsigned H = (unsigned)a.n.H;
         b = pair / H;
@@ -81,11 +88,13 @@ template <typename T, int DKP, int NG> struct Walk {
         T_ = (int)a.n.T;
         len = a.lengths ? min(max(a.lengths[b], 0), T_) : T_;
         live = (len + C - 1) / C;
+        first = min(segment * a.segment_chunks, live);
+        end = segment + 1 < a.segments ? min(first + a.segment_chunks, live) : live;
         return false;
     }
     __device__ __forceinline__ bool tokens() const { return CT == kWaves || w < CT; }
     __device__ __forceinline__ int column(int g) const { return col0 + (NC == 2 ? 32 * (g >> 1) + 2 * r + (g & 1) : r); }
-    __device__ __forceinline__ bool mine(int g) const { return column(g) < DV; }
+    __device__ __forceinline__ bool mine(int g) const { return column(g) < (basis ? DK : DV); }
     __device__ __forceinline__ int feature(int p) const      // of accumulator element 0
     {
         const int t = w * PER + p;
@@ -124,6 +133,38 @@ template <typename T, int DKP, int NG> struct Walk {
                     for (int q = 0; q < NC; ++q) x[q] = S[g + q][p][e];
                     if (mine(g) && feature(p) < DK) store_hidden<NC>(to, dtype, ((int64_t)pair * DK + feature(p) + e) * DV + column(g), x);
                 }
+    }
+    // The state that a segment starts from: zero or a basis for its summary, else what the segments before it leave.
+    template <bool SUMMARY> __device__ __forceinline__ void start_state(const DeltaArgs &a, f32x4 (&S)[NG][PER]) const
+    {
+        if (order == 0 && !basis) return load_state(a.hidden, a.hidden_dtype, S);
+#pragma unroll
+        for (int g = 0; g < NG; ++g)
+#pragma unroll
+            for (int p = 0; p < PER; ++p) {
+                const bool is = mine(g) && feature(p) < DK;
+                if constexpr (SUMMARY)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) S[g][p][e] = basis && feature(p) + e == column(g) ? 1.f : 0.f;
+                else {
+                    const float *from = a.starts + ((int64_t)pair * (a.segments - 1) + order - 1) * DV * DK;
+                    const f32x4 x = *reinterpret_cast<const f32x4 *>(from + (is ? column(g) * DK + feature(p) : 0));
+                    S[g][p] = is ? x : f32x4{0.f, 0.f, 0.f, 0.f};
+                }
+            }
+    }
+    template <bool SUMMARY> __device__ __forceinline__ void end_state(const DeltaArgs &a, const f32x4 (&S)[NG][PER]) const
+    {
+        if constexpr (SUMMARY) {
+            float *to = a.summary + (((int64_t)pair * (a.segments - 1) + order) * (DV + DK) + (basis ? DV : 0)) * DK;
+#pragma unroll
+            for (int g = 0; g < NG; ++g)
+#pragma unroll
+                for (int p = 0; p < PER; ++p)
+                    if (mine(g) && feature(p) < DK) *reinterpret_cast<f32x4 *>(to + column(g) * DK + feature(p)) = S[g][p];
+        } else if (order == a.segments - 1) {
+            store_state(a.hidden_out, a.hidden_dtype, S);
+        }
     }
     // a prepared array's chunk
     template <int SIZE> __device__ __forceinline__ const T *of_pair(const void *from, const DeltaArgs &a, int n) const
@@ -230,23 +271,24 @@ template <typename T, int DKP, int NG> struct Walk {
         int st, size;                            // of rows: their distance; or the bytes of a chunk
         unsigned at;
     };
-    template <int SCORE_PARTS> __device__ __forceinline__ Ahead ahead(const DeltaArgs &a, const Rows &keys, const Rows &queries) const
+    template <int SCORE_PARTS, bool QUERIES = true> __device__ __forceinline__ Ahead ahead(const DeltaArgs &a, const Rows &keys, const Rows &queries) const
     {
         constexpr int e = (int)sizeof(T), kLines = DKP * e / 128, kOfRows = C * kLines / 64, kInverse = DC::kSteps * DC::kParts * 512 * e,
                       kScores = DC::kSteps * SCORE_PARTS * 512 * e, kOfInverse = (kInverse + 8191) / 8192, kOfScores = (kScores + 8191) / 8192;
         int job = col0 / (16 * NG) * kWaves + w;
-        if (job < 2 * kOfRows) {
+        constexpr int kRowJobs = QUERIES ? 2 * kOfRows : kOfRows;
+        if (job < kRowJobs) {
             const Rows &x = job < kOfRows ? keys : queries;
             const int line = lane % kLines * 128;
             return {reinterpret_cast<const char *>(x.p), (int64_t)C * x.st * e, x.st, 0,
                     line < DK * e ? (unsigned)((job % kOfRows * (64 / kLines) + lane / kLines) * x.st * e + line) : kNowhere};
         }
-        job -= 2 * kOfRows;
+        job -= kRowJobs;
         const bool inverse = job < kOfInverse;
         const int size = inverse ? kInverse : kScores;
         if (!inverse) job -= kOfInverse;
         return {static_cast<const char *>(inverse ? a.to.inverse : a.to.scores) + (int64_t)pair * a.chunks * size, size, 0, size,
-                inverse || job < kOfScores ? 8192u * job + 128u * lane : kNowhere};
+                inverse || (QUERIES && job < kOfScores) ? 8192u * job + 128u * lane : kNowhere};
     }
     __device__ __forceinline__ uint32_t touch(const Ahead &x, int n) const
     {
@@ -386,7 +428,7 @@ template <typename Set, typename F> __device__ __forceinline__ void in_turns(int
 template <typename T, int DKP> constexpr int kTile = DeltaChunk<T>::C * LdsTile<T, DKP>::kRow;
 
 // Forward.  Three times a chunk the waves wait for each other: for the state's operands, r and u.
-template <typename T, int DKP, int NG, bool KEEP> __global__ __launch_bounds__(512) void delta_walk_kernel(const DeltaArgs a)
+template <typename T, int DKP, int NG, bool KEEP, bool SUMMARY> __global__ __launch_bounds__(512) void delta_walk_kernel(const DeltaArgs a)
 {
     typedef Walk<T, DKP, NG> W;
     typedef typename W::DC DC;
@@ -398,8 +440,8 @@ template <typename T, int DKP, int NG, bool KEEP> __global__ __launch_bounds__(5
       *sR = sS + NG * KS * kFew * 512, *sU = sR + NG * CS * kParts * 512, *sO = sU + NG * CS * kParts * 512;
     float *sV = reinterpret_cast<float *>(sO + NG * CS * kFew * 512), *sG[2] = {sV + NG * CT * 256, sV + NG * CT * 256 + DC::kGates};
     W w;
-    if (w.place(a)) return;
-    const int lane = w.lane, last = w.live - 1;
+    if (w.template place<SUMMARY, false>(a)) return;
+    const int lane = w.lane, count = w.end - w.first, last = w.end - 1;
     auto four = [&](float *p, int i) -> f32x4 & { return *reinterpret_cast<f32x4 *>(p + i * 256 + lane * 4); };
     if (w.helper) {
         const int64_t row = a.n.H * w.DV;
@@ -425,31 +467,34 @@ template <typename T, int DKP, int NG, bool KEEP> __global__ __launch_bounds__(5
         } x, y;
         const typename W::Rows keys = w.key_rows(a.keys), queries = w.key_rows(a.queries), values = w.value_rows(a.values);
         D8 Q[KS];
-        auto load_rows = [&](int n, Set &to) {
-            n = min(n, last);
+        auto load_rows = [&](int step, Set &to) {
+            const int n = min(w.first + step, last);
             w.load_stage(keys, n, to.key);
-            w.load_stage(queries, n, to.query);
+            if constexpr (!SUMMARY) w.load_stage(queries, n, to.query);
             w.load_values(values, n, to.V);
             to.gate = w.load_gate(a, n);
         };
-        auto load_scores = [&](int n, Set &to) { w.template load_steps<false>(a.to.scores, a, min(n, last), to.P); };
-        const typename W::Ahead ahead = w.template ahead<1>(a, keys, queries);
-        auto touch = [&](int n, Set &to) {
-            n = min(n, last);
+        auto load_scores = [&](int step, Set &to) {
+            if constexpr (!SUMMARY) w.template load_steps<false>(a.to.scores, a, min(w.first + step, last), to.P);
+        };
+        const typename W::Ahead ahead = w.template ahead<1, !SUMMARY>(a, keys, queries);
+        auto touch = [&](int step, Set &to) {
+            const int n = min(w.first + step, last);
             to.touched[0] = w.touch(ahead, n);
             to.touched[1] = w.touch_values(values, n);
         };
-        auto put_rows = [&](int n, const Set &from) {
-            w.put_stage(sK[n & 1], from.key);
-            w.put_stage(sQ, from.query);
+        auto put_rows = [&](int step, const Set &from) {
+            w.put_stage(sK[step & 1], from.key);
+            if constexpr (!SUMMARY) w.put_stage(sQ, from.query);
             if (w.tokens())
 #pragma unroll
                 for (int g = 0; g < NG; ++g)
-                    four(sV, g * CT + w.w) = f32x4{W::value(from.V, g, 0), W::value(from.V, g, 1), W::value(from.V, g, 2), W::value(from.V, g, 3)};
-            w.put_gate(sG[n & 1], from.gate);
-            w.get_rows(sQ, Q);                   // (the wave's own)
+                    four(sV, g * CT + w.w) = SUMMARY && w.basis ? f32x4{0.f, 0.f, 0.f, 0.f}
+                                                                : f32x4{W::value(from.V, g, 0), W::value(from.V, g, 1), W::value(from.V, g, 2), W::value(from.V, g, 3)};
+            w.put_gate(sG[step & 1], from.gate);
+            if constexpr (!SUMMARY) w.get_rows(sQ, Q);       // (the wave's own)
         };
-        if (w.live > 0) {
+        if (count > 0) {
             load_rows(0, x);
             load_scores(0, x);
             load_rows(1, y);
@@ -460,12 +505,12 @@ template <typename T, int DKP, int NG, bool KEEP> __global__ __launch_bounds__(5
             touch(W::kAhead - 1, y);
             lds_barrier();                       // the first rows
         }
-        in_turns(w.live, x, y, [&](int n, Set &mine, Set &next) {
+        in_turns(count, x, y, [&](int step, Set &mine, Set &next) {
             f32x4 o[NG];
             lds_barrier();                       // the state's operands are there
 #pragma unroll
             for (int g = 0; g < NG; ++g) o[g] = f32x4{0.f, 0.f, 0.f, 0.f};
-            if (w.tokens())
+            if (!SUMMARY && w.tokens())
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
@@ -475,11 +520,11 @@ template <typename T, int DKP, int NG, bool KEEP> __global__ __launch_bounds__(5
                         o[g] = mma_whole(s, Q[ks], o[g]);
                     }
             lds_barrier();                       // r
-            put_rows(n + 1, next);
-            load_rows(n + 3, next);
+            put_rows(step + 1, next);
+            load_rows(step + 3, next);
             lds_barrier();                       // u
-            if (w.tokens()) {
-                const float start = sG[n & 1][16 * w.w + w.r];
+            if (!SUMMARY && w.tokens()) {
+                const float start = sG[step & 1][16 * w.w + w.r];
 #pragma unroll
                 for (int g = 0; g < NG; ++g)
 #pragma unroll
@@ -493,19 +538,21 @@ template <typename T, int DKP, int NG, bool KEEP> __global__ __launch_bounds__(5
                             W::template get<CS, kFew>(sO, g, ks, lane, u);
                             o[g] = mma_whole(u, mine.P[ks][0], o[g]);
                         }
-                const bool is = n * C + 16 * w.w + w.r < w.len;
-                store(n * C, [&](int g, int e) { return is ? o[g][e] : 0.f; });
+                const int from = (w.first + step) * C;
+                const bool is = from + 16 * w.w + w.r < w.len;
+                store(from, [&](int g, int e) { return is ? o[g][e] : 0.f; });
             }
-            load_scores(n + 2, mine);
+            load_scores(step + 2, mine);
             asm volatile("" ::"v"(mine.touched[0]), "v"(mine.touched[1]));       // (asked for two chunks ago)
-            touch(n + W::kAhead, mine);
+            touch(step + W::kAhead, mine);
         });
         // rows past the end of a shorter sequence
-        for (int from = w.live * C; from < w.T_; from += 16 * W::kWaves) store(from, [](int, int) { return 0.f; });
+        if (!SUMMARY && w.segment == a.segments - 1)
+            for (int from = w.live * C; from < w.T_; from += 16 * W::kWaves) store(from, [](int, int) { return 0.f; });
         return;
     }
     f32x4 S[NG][PER];
-    w.load_state(a.hidden, a.hidden_dtype, S);
+    w.template start_state<SUMMARY>(a, S);
     float *kept = KEEP ? a.kept + w.pair * (delta_states_floats(a.n, a.chunks) + delta_written_floats(a.n, a.chunks, C)) : nullptr;
     float *xs = KEEP ? kept + delta_states_floats(a.n, a.chunks) : nullptr;
     auto keep = [&](int n) {
@@ -518,17 +565,18 @@ template <typename T, int DKP, int NG, bool KEEP> __global__ __launch_bounds__(5
     struct Set {
         D8 Z[CS][kParts];
     } x, y;
-    auto load = [&](int n, Set &to) { w.template load_steps<false>(a.to.inverse, a, min(n, last), to.Z); };
+    auto load = [&](int step, Set &to) { w.template load_steps<false>(a.to.inverse, a, min(w.first + step, last), to.Z); };
     D8 K[KS], KT[PER][CS];
-    if (w.live > 0) {
+    if (count > 0) {
         load(0, x);
         load(1, y);
         w.template put_state<kFew>(sS, S);
         lds_barrier();                           // the first rows
         w.get_rows(sK[0], K);
     }
-    in_turns(w.live, x, y, [&](int n, Set &mine, Set &) {
-        const float *gates = sG[n & 1];
+    in_turns(count, x, y, [&](int step, Set &mine, Set &) {
+        const int n = w.first + step;
+        const float *gates = sG[step & 1];
         if constexpr (KEEP) keep(n);
         f32x4 v[NG];
         lds_barrier();                           // the state's operands are there
@@ -556,12 +604,12 @@ template <typename T, int DKP, int NG, bool KEEP> __global__ __launch_bounds__(5
                     weighted[e] = end[e] * u[e];
                 }
                 W::template put<CS, kParts>(sU, g, w.w, lane, weighted);
-                W::template put<CS, kFew>(sO, g, w.w, lane, u);
+                if constexpr (!SUMMARY) W::template put<CS, kFew>(sO, g, w.w, lane, u);
                 if constexpr (KEEP)
                     if (w.mine(g)) *reinterpret_cast<f32x4 *>(xs + w.written(n, g)) = v[g];
             }
         }
-        w.get_features(sK[n & 1], KT);
+        w.get_features(sK[step & 1], KT);
         const float whole = gates[3 * C];
 #pragma unroll
         for (int g = 0; g < NG; ++g)
@@ -569,21 +617,22 @@ template <typename T, int DKP, int NG, bool KEEP> __global__ __launch_bounds__(5
             for (int p = 0; p < PER; ++p)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) S[g][p][e] *= whole;
-        load(n + 2, mine);
+        load(step + 2, mine);
         lds_barrier();                           // u
         w.add_keys(sU, KT, S);                   // the state behind the chunk
-        w.get_rows(sK[(n + 1) & 1], K);
+        w.get_rows(sK[(step + 1) & 1], K);
         w.template put_state<kFew>(sS, S);
     });
-    if constexpr (KEEP) keep(w.live);
-    w.store_state(a.hidden_out, a.hidden_dtype, S);
+    if constexpr (KEEP)
+        if (w.end == w.live && (count > 0 || w.segment == 0)) keep(w.live);
+    w.template end_state<SUMMARY>(a, S);
 }
 
 // Backward, from the last chunk to the first.  With dS the cotangent of the state behind a chunk and du that of u from what reads u,
 //       du_j = sum_{i>=j} P_ij do_i + e^{L_C - L_j} dS^T k_j,   du <- (1 + b M)^{-T} du,   dv = dr = b du,
 //       dS  <- e^{L_C} dS + sum_i e^{L_i} (q_i do_i^T - k_i dv_i^T).
 // The helpers make the first sum and sum_i e^{L_i} q_i do_i^T, a chunk ahead.
-template <typename T, int DKP, int NG> __global__ __launch_bounds__(512) void delta_walk_back_kernel(const DeltaArgs a)
+template <typename T, int DKP, int NG, bool SUMMARY> __global__ __launch_bounds__(512) void delta_walk_back_kernel(const DeltaArgs a)
 {
     typedef Walk<T, DKP, NG> W;
     typedef typename W::DC DC;
@@ -598,12 +647,12 @@ template <typename T, int DKP, int NG> __global__ __launch_bounds__(512) void de
     float *sWritten = reinterpret_cast<float *>(sD + NG * CS * 512), *sState = sWritten + NG * CT * 256;
     float *sG[2] = {sState + NG * TILES * 256, sState + NG * TILES * 256 + DC::kGates};
     W w;
-    if (w.place(a)) return;
-    const int lane = w.lane;
-    auto chunk_of = [&](int step) { return max(w.live - 1 - step, 0); };
+    if (w.template place<SUMMARY, true>(a)) return;
+    const int lane = w.lane, count = w.end - w.first;
+    auto chunk_of = [&](int step) { return max(w.end - 1 - step, w.first); };
     auto four = [&](float *p, int i) -> f32x4 & { return *reinterpret_cast<f32x4 *>(p + i * 256 + lane * 4); };
     if (w.helper) {
-        if (w.live == 0) return;
+        if (count == 0) return;
         const float *kept = a.kept + w.pair * (delta_states_floats(a.n, a.chunks) + delta_written_floats(a.n, a.chunks, C));
         T *dstates = static_cast<T *>(a.dstates) + w.pair * a.chunks * delta_state_floats(a.n);
         const typename W::Rows douts = w.value_rows(a.dout), keys = w.key_rows(a.keys), queries = w.key_rows(a.queries);
@@ -623,7 +672,7 @@ template <typename T, int DKP, int NG> __global__ __launch_bounds__(512) void de
             to.touched[1] = w.touch_values(douts, n);
             // the states' tiles of a group of columns: 16 lines a wave (as many as there are)
             const int64_t line = w.state_place(n + 1, 0, 0) - (w.c * 16 + w.r) * 4 + 512 * w.w + 32 * w.r;
-            to.touched[2] = __float_as_uint(kept[w.w < delta_state_tiles(w.DK) / 2 ? line : 0]);
+            to.touched[2] = SUMMARY ? 0 : __float_as_uint(kept[w.w < delta_state_tiles(w.DK) / 2 ? line : 0]);
         };
         auto load_rows = [&](int step, Set &to) {
             const int n = chunk_of(step);
@@ -634,6 +683,7 @@ template <typename T, int DKP, int NG> __global__ __launch_bounds__(512) void de
             to.start = w.load_start(a, n);
         };
         auto load_kept = [&](int step, Set &to) {
+            if constexpr (SUMMARY) return;
 #pragma unroll
             for (int g = 0; g < NG; ++g)
 #pragma unroll
@@ -651,7 +701,7 @@ template <typename T, int DKP, int NG> __global__ __launch_bounds__(512) void de
                     f32x4 o, scaled;
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        o[e] = W::value(from.O, g, e);
+                        o[e] = SUMMARY && w.basis ? 0.f : W::value(from.O, g, e);
                         scaled[e] = from.start[e] * o[e];
                     }
                     W::template put<CS, 1>(sD, g, w.w, lane, o);
@@ -699,8 +749,8 @@ template <typename T, int DKP, int NG> __global__ __launch_bounds__(512) void de
         sums(x);
         load_scores(2, x);
         hand_written();
-        in_turns(w.live, x, y, [&](int step, Set &mine, Set &next) {
-            const int n = w.live - 1 - step;
+        in_turns(count, x, y, [&](int step, Set &mine, Set &next) {
+            const int n = w.end - 1 - step;
             lds_barrier();                       // dS, and what the helpers add to du
 #pragma unroll
             for (int g = 0; g < NG; ++g)
@@ -710,6 +760,7 @@ template <typename T, int DKP, int NG> __global__ __launch_bounds__(512) void de
             lds_barrier();                       // du
             sums(next);
             // the cotangent of the state behind the chunk, for the gradients; its product with that state
+            if constexpr (!SUMMARY) {
             float *dots = a.dots + (((int64_t)w.pair * a.chunks + n) * (w.DV >> 4) + (w.col0 >> 4)) * 4 + w.w;
 #pragma unroll
             for (int g = 0; g < NG; g += NC) {
@@ -736,6 +787,7 @@ template <typename T, int DKP, int NG> __global__ __launch_bounds__(512) void de
                     for (int q = 0; q < NC; ++q)
                         if (w.col0 + 16 * (g + q) < w.DV) dots[4 * (g + q)] = q ? 0.f : dot;
             }
+            }
             lds_barrier();                       // dr
             hand_written();
             load_kept(step + 2, mine);
@@ -747,8 +799,8 @@ template <typename T, int DKP, int NG> __global__ __launch_bounds__(512) void de
         return;
     }
     f32x4 S[NG][PER];
-    w.load_state(a.hidden, a.hidden_dtype, S);
-    if (w.live > 0) {
+    w.template start_state<SUMMARY>(a, S);
+    if (count > 0) {
         float *dus = a.du + w.pair * delta_written_floats(a.n, a.chunks, C);
         struct Set {
             D8 Z[CS][kParts];
@@ -760,8 +812,8 @@ template <typename T, int DKP, int NG> __global__ __launch_bounds__(512) void de
         w.template put_state<kParts>(sS, S);
         lds_barrier();                           // the first keys
         w.get_rows(sK[0], K);
-        in_turns(w.live, x, y, [&](int step, Set &mine, Set &) {
-            const int n = w.live - 1 - step;
+        in_turns(count, x, y, [&](int step, Set &mine, Set &) {
+            const int n = w.end - 1 - step;
             const float *gates = sG[step & 1];
             f32x4 du[NG];
             lds_barrier();                       // dS, and what the helpers add to du
@@ -786,7 +838,7 @@ template <typename T, int DKP, int NG> __global__ __launch_bounds__(512) void de
 #pragma unroll
                     for (int e = 0; e < 4; ++e) v[e] = -start[e] * (beta[e] * du[g][e]);
                     W::template put<CS, kParts>(sR, g, w.w, lane, v);
-                    if (w.mine(g)) *reinterpret_cast<f32x4 *>(dus + w.written(n, g)) = du[g];
+                    if (!SUMMARY && w.mine(g)) *reinterpret_cast<f32x4 *>(dus + w.written(n, g)) = du[g];
                 }
             }
             w.get_features(sK[step & 1], KT);
@@ -806,7 +858,52 @@ template <typename T, int DKP, int NG> __global__ __launch_bounds__(512) void de
             w.template put_state<kParts>(sS, S);
         });
     }
-    w.store_state(a.hidden_out, a.hidden_dtype, S);
+    w.template end_state<SUMMARY>(a, S);
+}
+
+// From the segments' summaries the states that they start from: of the first, what it leaves; of each other, with A the basis' way through it,
+//       S' = A S + what it leaves of a start from zero,
+// in float products, a column of 16 values a workgroup.  Wave w makes features 32w .. of S', whose tiles are the next product's operand by way of LDS.
+__global__ __launch_bounds__(256) void delta_join_kernel(const DeltaArgs a)
+{
+    constexpr int kRow = 128 + 4;
+    __shared__ float state[2][16 * kRow];
+    const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, r = lane & 15, c = lane >> 4;
+    const int DK = (int)a.n.DK, DV = (int)a.n.DV, column = 16 * (int)blockIdx.y + r;
+    const int64_t pair = blockIdx.x, size = (int64_t)(DV + DK) * DK;
+    const float *summary = a.summary + pair * (a.segments - 1) * size;
+    float *starts = a.starts + pair * (a.segments - 1) * DV * DK;
+    f32x4 S[2];
+    for (int order = 0; order + 1 < a.segments; ++order, summary += size, starts += (int64_t)DV * DK) {
+        const float *before = state[order & 1];
+        float *behind = state[(order + 1) & 1];
+        f32x4 A[2][8];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {            // (places behind the last feature are the first one's again, and go nowhere)
+            const int tile = 32 * w + 16 * t < DK ? 32 * w + 16 * t : 0;
+            S[t] = *reinterpret_cast<const f32x4 *>(summary + (int64_t)column * DK + tile + 4 * c);
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) A[t][k][e] = order ? summary[(int64_t)(DV + (16 * k < DK ? 16 * k : 0) + 4 * c + e) * DK + tile + r] : 0.f;
+        }
+        if (order)
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (16 * k < DK) {
+                    const f32x4 s = *reinterpret_cast<const f32x4 *>(before + r * kRow + 16 * k + 4 * c);
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) S[t] = mma_t(A[t][k], s, S[t]);
+                }
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const int f = 32 * w + 16 * t + 4 * c;
+            if (f >= DK) continue;
+            *reinterpret_cast<f32x4 *>(starts + (int64_t)column * DK + f) = S[t];
+            *reinterpret_cast<f32x4 *>(behind + r * kRow + f) = S[t];
+        }
+        __syncthreads();
+    }
 }
 
 // bytes of shared memory
@@ -819,27 +916,38 @@ template <typename T, int DKP, int NG, bool BACK> constexpr size_t walk_lds()
            (BACK ? sizeof(T) * 512 * NG * (W::KS * DC::kParts + W::CS * (3 * DC::kParts + 1)) + sizeof(float) * 256 * NG * (W::CT + W::TILES)
                          : sizeof(T) * 512 * NG * (W::KS * DC::kFew + W::CS * (2 * DC::kParts + DC::kFew)) + sizeof(float) * 256 * NG * W::CT);
 }
-template <typename T, int DKP, int NG, bool BACK> int launch_walk(hipStream_t stream, const DeltaArgs &a)
+template <typename T, int DKP, int NG, bool BACK> int launch_walk(hipStream_t stream, const DeltaArgs &a, bool summary)
 {
     // the columns of a pair start next to each other on one die (workgroups are dealt to the eight in turn) and share what they read in its cache
-    const unsigned grid = (unsigned)((a.pairs + 7) / 8 * 8 * ((a.n.DV + 16 * NG - 1) / (16 * NG)));
+    const int64_t groups = (a.n.DV + 16 * NG - 1) / (16 * NG) + (summary ? (a.n.DK + 16 * NG - 1) / (16 * NG) : 0);
+    const unsigned grid = (unsigned)((a.pairs + 7) / 8 * 8 * groups * (a.segments - (summary ? 1 : 0)));
     constexpr size_t lds = walk_lds<T, DKP, NG, BACK>();
     static_assert(lds <= 160 * 1024, "");
-    static LdsGrant grants[2];
+    static LdsGrant grants[3];
     auto launch = [&](LdsGrant &grant, auto *kernel) {
         if (int e = allow_lds(grant, reinterpret_cast<const void *>(kernel), lds)) return e;
         kernel<<<grid, 512, lds, stream>>>(a);
         return launch_status();
     };
-    if constexpr (BACK) return launch(grants[0], delta_walk_back_kernel<T, DKP, NG>);
-    else return a.kept ? launch(grants[0], delta_walk_kernel<T, DKP, NG, true>) : launch(grants[1], delta_walk_kernel<T, DKP, NG, false>);
+    if constexpr (BACK) {
+        return summary ? launch(grants[0], delta_walk_back_kernel<T, DKP, NG, true>) : launch(grants[1], delta_walk_back_kernel<T, DKP, NG, false>);
+    } else {
+        if (summary) return launch(grants[0], delta_walk_kernel<T, DKP, NG, false, true>);
+        return a.kept ? launch(grants[1], delta_walk_kernel<T, DKP, NG, true, false>) : launch(grants[2], delta_walk_kernel<T, DKP, NG, false, false>);
+    }
 }
 // Value columns of a workgroup: 32 share the operands' way from memory, 16 make twice the workgroups.
 template <typename T, int DKP, bool BACK> int choose_walk(hipStream_t stream, const DeltaArgs &a)
 {
     const int64_t groups = a.pairs * ((a.n.DV + 15) / 16);
-    if (a.n.DV > 16 && groups > kComputeUnits) return launch_walk<T, DKP, 2, BACK>(stream, a);
-    return launch_walk<T, DKP, 1, BACK>(stream, a);
+    if (a.segments > 1) {
+        if (int e = launch_walk<T, DKP, 2, BACK>(stream, a, true)) return e;
+        delta_join_kernel<<<dim3((unsigned)a.pairs, (unsigned)((a.n.DV + 15) / 16)), 256, 0, stream>>>(a);
+        if (int e = launch_status()) return e;
+        return launch_walk<T, DKP, 2, BACK>(stream, a, false);
+    }
+    if (a.n.DV > 16 && groups > kComputeUnits) return launch_walk<T, DKP, 2, BACK>(stream, a, false);
+    return launch_walk<T, DKP, 1, BACK>(stream, a, false);
 }
 template <typename T, bool BACK> int dispatch_walk(hipStream_t stream, const DeltaArgs &a)
 {
@@ -847,6 +955,26 @@ template <typename T, bool BACK> int dispatch_walk(hipStream_t stream, const Del
 }
 
 }  // namespace
+
+// Segments are worth their summaries (a walk for the values and one for the basis) where one walk leaves compute units idle.  The number with the
+// least time by what was measured at 128 x 128 features: 1.6 us a chunk for a workgroup of 16 columns, 2.45 for one of 32, 2.1 in a summary, 1.5 a
+// step of the join, and 12 for the two launches more and their beginnings.
+// (B1 T32768 H8: 803 us in one piece, 8 segments 265 + 20 + 157.)
+int delta_segments(const DeltaArgs &a)
+{
+    const int64_t of_pair = (a.n.DV + 31) / 32, wide = a.pairs * of_pair, basis = a.pairs * ((a.n.DK + 31) / 32);
+    auto rounds = [](int64_t groups) { return (double)((groups + kComputeUnits - 1) / kComputeUnits); };
+    int best = 1;
+    double least = a.pairs * ((a.n.DV + 15) / 16) <= kComputeUnits ? 1.6 * a.chunks : 2.45 * a.chunks * rounds(wide);
+    for (int64_t n = 2; a.n.DV > 16 && n <= 64 && 8 * n <= a.chunks && n * wide <= kComputeUnits; ++n) {
+        const double time = (a.chunks + n - 1) / n * (2.45 + 2.1 * rounds((n - 1) * (wide + basis))) + 1.5 * n + 12.0;
+        if (time < least) {
+            least = time;
+            best = (int)n;
+        }
+    }
+    return best;
+}
 
 int delta_walk(void *stream, const DeltaArgs &a, gla_dtype dtype, bool backward)
 {
