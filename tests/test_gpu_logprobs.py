@@ -225,3 +225,27 @@ def test_rows_that_do_not_count_are_not_read():
     assert not given[::2].any() and not entropy[::2].any() and not d[::2].any()
     assert bool((near[::2] == -math.inf).all()) and bool((index[::2] == -1).all())
     assert torch.isfinite(given[1::2]).all() and torch.isfinite(d[1::2]).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("V", [70, 1000, 40001])
+def test_rows_that_allow_few_tokens(V, dtype):
+    """Fewer above -inf than alternatives are asked for, none to 63 of them: the rest are the first tokens of -inf."""
+    rows, top = 66, 64
+    g = torch.Generator(device="cuda").manual_seed(10)
+    x = torch.full((rows, V), -math.inf, device="cuda", dtype=dtype)
+    for i in range(rows - 1):
+        at = torch.randperm(V, device="cuda", generator=g)[:i]
+        x[i, at] = torch.randn(i, device="cuda", generator=g).to(dtype)
+    x[rows - 1] = -3e38                            # the type's lowest (nearly) is above -inf
+    t = torch.randint(V, (rows,), device="cuda", generator=g)
+    given, entropy, near, index = token_logprobs(x, t, top)
+    assert torch.equal(index, x.float().sort(dim=-1, descending=True, stable=True)[1][:, :top])
+    p = torch.log_softmax(x.double(), -1)
+    assert torch.isnan(given[0]) and torch.isnan(entropy[0]) and torch.isnan(near[0]).all()
+    want = p.gather(-1, index)[1:]
+    assert torch.equal(near[1:] == -math.inf, want == -math.inf)
+    want = want.masked_fill(want == -math.inf, 0)
+    close(near[1:].masked_fill(near[1:] == -math.inf, 0), want, off(want, V))
+    want = torch.special.entr(p[1:].exp()).sum(-1)
+    close(entropy[1:], want, 2 * off(want, V))
