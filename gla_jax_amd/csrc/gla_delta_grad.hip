@@ -19,12 +19,21 @@ constexpr int kSlice = 64;                       // value features at a time
 
 template <typename T, int F> __device__ __forceinline__ int place_in(int row, int col) { return LdsTile<T, F>::piece(row, col & ~7) + (col & 7); }
 
-// One workgroup: a chunk of a (batch, head) pair; wave w makes key features 16w .. 16w + 15 of dq and dk.
-template <typename T, int DKP> __global__ __launch_bounds__(DKP * 4) void delta_gradient_kernel(const DeltaArgs a)
+// values of the states' place in LDS
+template <typename T, int DKP> constexpr int state_place()
 {
     typedef DeltaChunk<T> DC;
-    constexpr int C = DC::C, CT = DC::CT, CS = DC::CS, KS = DKP / 32, NW = DKP / 16, NT = 64 * NW, VS = kSlice / 32, kParts = DC::kParts, kFew = DC::kFew;
+    constexpr int states = (DC::kParts + 1) * kSlice * LdsTile<T, DKP>::kRow, scores = 2 * DC::C * (LdsTile<T, DC::C>::kRow + LdsTile<T, DKP>::kRow);
+    return states > scores ? states : scores;
+}
+
+// One workgroup: a chunk of a (batch, head) pair; a wave makes 16 key features of dq and dk, at 64 features of every second tile of tokens.
+template <typename T, int DKP> __global__ __launch_bounds__(512) void delta_gradient_kernel(const DeltaArgs a)
+{
+    typedef DeltaChunk<T> DC;
+    constexpr int C = DC::C, CT = DC::CT, CS = DC::CS, KS = DKP / 32, NW = 8, NT = 64 * NW, VS = kSlice / 32, kParts = DC::kParts, kFew = DC::kFew;
     constexpr int kTriangle = CT * (CT + 1) / 2, kUnits = (2 * kTriangle + NW - 1) / NW, kShare = NW / CT;
+    constexpr int FT = DKP / 16, SHARES = NW / FT, OWN = CT / SHARES;      // tiles of features; waves to each; its tiles of tokens
     typedef typename FragTypes<T>::d8 D8;
     typedef typename Packed4<T>::t Four;
     typedef LdsTile<T, DKP> TileK;
@@ -32,19 +41,20 @@ template <typename T, int DKP> __global__ __launch_bounds__(DKP * 4) void delta_
     typedef LdsTile<T, C> TileU;
     constexpr int kK = C * TileK::kRow, kS = kSlice * TileK::kRow, kU = kSlice * TileU::kRow, kP = C * TileU::kRow;
     extern __shared__ char smem[];
-    T *sQ = reinterpret_cast<T *>(smem), *sK = sQ + kK, *sS = sK + kK, *sD = sS + kParts * kS, *sO = sD + kS, *sU = sO + C * TileO::kRow,
-      *sX = sU + kParts * kU, *sP = sS, *sE = sP + kP;     // (the scores take the states' place)
-    static_assert(2 * kP <= kParts * kS, "");
+    // the scores, keys and queries take the states' place (two workgroups of 64 features a compute unit)
+    T *sS = reinterpret_cast<T *>(smem), *sD = sS + kParts * kS, *sO = sS + state_place<T, DKP>(), *sU = sO + C * TileO::kRow, *sX = sU + kParts * kU,
+      *sP = sS, *sE = sP + kP, *sK = sE + kP, *sQ = sK + kK;
     ChunkGates<C> *gate = reinterpret_cast<ChunkGates<C> *>(sX + kU);
     struct Sums {
         float beta[C];
         float pairs[CT][C];                      // row sums of P (do.u), one column of tiles each
-        float state[NW][C];                      // e^{L_i} q_i.(S do_i), 16 features each
+        float state[FT][C];                      // e^{L_i} q_i.(S do_i), 16 features each
         float db[kShare][C], vdv[kShare][C];
     };
     Sums &sums = *reinterpret_cast<Sums *>(gate + 1);
 
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, r = lane & 15, c = lane >> 4;
+    const int wf = w % FT, wt = w / FT;          // the wave's features 16 wf .. and tiles of tokens wt + SHARES t
     const unsigned H = (unsigned)a.n.H, group = H / (unsigned)a.n.HK, rest = blockIdx.x / H, chunks = (unsigned)a.chunks;
     const int64_t h = blockIdx.x % H, n = rest % chunks, b = rest / chunks, hk = blockIdx.x % H / group, pair = b * H + h;
     const int T_ = (int)a.n.T, len = a.lengths ? min(max(a.lengths[b], 0), T_) : T_, first = (int)n * C, there = len - first;
@@ -53,14 +63,14 @@ template <typename T, int DKP> __global__ __launch_bounds__(DKP * 4) void delta_
     const int64_t key_row = a.n.HK * DK, key_at = (((parts ? blockIdx.x % H % group : 0) * a.n.B + b) * T_ + first) * key_row + hk * DK;
     T *dV = static_cast<T *>(a.dvalue) + ((b * T_ + first) * H + h) * DV;
     auto put_keys = [&](void *array, int ti, f32x4 v) {       // four features of a token
-        const int64_t at = key_at + (16 * ti + r) * key_row + 16 * w + 4 * c;
-        if (16 * w >= DK || first + 16 * ti + r >= T_) return;
+        const int64_t at = key_at + (16 * ti + r) * key_row + 16 * wf + 4 * c;
+        if (16 * wf >= DK || first + 16 * ti + r >= T_) return;
         if (parts) *reinterpret_cast<f32x4 *>(static_cast<float *>(array) + at) = v;
         else *reinterpret_cast<Four *>(static_cast<T *>(array) + at) = pack_results<T>(v);
     };
     const int64_t gate_at = (b * T_ + first + lane) * H + h;
     if (there <= 0) {                            // behind the end: zeros
-        for (int ti = 0; ti < CT; ++ti) {
+        for (int ti = wt; ti < CT; ti += SHARES) {
             put_keys(a.dquery, ti, f32x4{0.f, 0.f, 0.f, 0.f});
             put_keys(a.dkey, ti, f32x4{0.f, 0.f, 0.f, 0.f});
         }
@@ -106,29 +116,25 @@ template <typename T, int DKP> __global__ __launch_bounds__(DKP * 4) void delta_
             for (int e = 0; e < 4; ++e) value[i][e] = V[(int64_t)min(token + e, there - 1) * a.values.st + at + r];
         }
     };
+    RowsInFlight<T, C, DKP, NT> key, query;
+    load_slice(0);
     float log_decay = 0.f;
     {
-        RowsInFlight<T, C, DKP, NT> x, q;
-        x.load(tid, static_cast<const T *>(a.keys.p) + b * a.keys.sb + hk * a.keys.sh + first * a.keys.st, (int)a.keys.st, there, DK);
-        q.load(tid, static_cast<const T *>(a.queries.p) + b * a.queries.sb + hk * a.queries.sh + first * a.queries.st, (int)a.queries.st, there, DK);
         if (w == 0) {
             log_decay = lane < C && lane < there ? G[lane * a.gates.st] : 0.f;
             chunk_gates<C>(*gate, log_decay);
         }
         if (w == 1 && lane < C) sums.beta[lane] = a.to.gates[(pair * chunks + n) * DC::kGates + 2 * C + lane];
-        load_slice(0);
-        x.store(tid, sK, there, DK);
-        q.store(tid, sQ, there, DK);
     }
     const TileK tk;
     const TileO to;
     const TileU tu;
-    f32x4 score[kUnits], fromO[CT], fromX[CT], fromU[CT];
+    f32x4 score[kUnits], fromO[OWN], fromX[OWN], fromU[OWN];
     float db[4] = {}, vdv[4] = {};               // of the tokens 16 (w % CT) + 4c + e
 #pragma unroll
     for (int m = 0; m < kUnits; ++m) score[m] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int ti = 0; ti < CT; ++ti) fromO[ti] = fromX[ti] = fromU[ti] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int t = 0; t < OWN; ++t) fromO[t] = fromX[t] = fromU[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 
     for (int dv0 = 0; dv0 < DV; dv0 += kSlice) {
         lds_barrier();                           // beta is there; the last slice's tiles are read
@@ -168,7 +174,12 @@ template <typename T, int DKP> __global__ __launch_bounds__(DKP * 4) void delta_
             }
         }
         o.store(tid, sO, there, DV - dv0);
-        if (dv0 + kSlice < DV) load_slice(dv0 + kSlice);
+        if (dv0 + kSlice < DV) {
+            load_slice(dv0 + kSlice);
+        } else {
+            key.load(tid, static_cast<const T *>(a.keys.p) + b * a.keys.sb + hk * a.keys.sh + first * a.keys.st, (int)a.keys.st, there, DK);
+            query.load(tid, static_cast<const T *>(a.queries.p) + b * a.queries.sb + hk * a.queries.sh + first * a.queries.st, (int)a.queries.st, there, DK);
+        }
         lds_barrier();
         // dv, a token's 4 values twice
         for (int unit = w; unit < CT * VS; unit += NW) {
@@ -206,22 +217,26 @@ template <typename T, int DKP> __global__ __launch_bounds__(DKP * 4) void delta_
         for (int ks = 0; ks < VS; ++ks) {
             D8 s[kParts];
 #pragma unroll
-            for (int p = 0; p < kParts; ++p) s[p] = tk.columns(sS + p * kS, ks, w);
-            const D8 d = tk.columns(sD, ks, w);
+            for (int p = 0; p < kParts; ++p) s[p] = tk.columns(sS + p * kS, ks, wf);
+            const D8 d = tk.columns(sD, ks, wf);
 #pragma unroll
-            for (int ti = 0; ti < CT; ++ti) {
-                fromO[ti] = mma_whole(s, to.halves(sO, ti, ks), fromO[ti]);
+            for (int t = 0; t < OWN; ++t) {
+                const int ti = wt + SHARES * t;
+                fromO[t] = mma_whole(s, to.halves(sO, ti, ks), fromO[t]);
                 const D8 x = tu.columns(sX, ks, ti);
 #pragma unroll
                 for (int p = kFew - 1; p >= 0; --p) {
-                    fromX[ti] = mma_d(s[p], x, fromX[ti]);
-                    fromU[ti] = mma_d(d, tu.columns(sU + p * kU, ks, ti), fromU[ti]);
+                    fromX[t] = mma_d(s[p], x, fromX[t]);
+                    fromU[t] = mma_d(d, tu.columns(sU + p * kU, ks, ti), fromU[t]);
                 }
             }
         }
     }
     lds_barrier();                               // the states are read
+    key.store(tid, sK, there, DK);
+    query.store(tid, sQ, there, DK);
     if (w < CT / 2) *reinterpret_cast<Four *>(tu.four(sP, 2 * w, 2 * w + 1)) = Four{};      // the tiles above the diagonal that operands reach into
+    lds_barrier();
 #pragma unroll
     for (int m = 0; m < kUnits; ++m) {
         const int unit = w + m * NW;
@@ -256,18 +271,19 @@ template <typename T, int DKP> __global__ __launch_bounds__(DKP * 4) void delta_
         }
     }
 #pragma unroll
-    for (int ti = 0; ti < CT; ++ti) {
+    for (int t = 0; t < OWN; ++t) {
+        const int ti = wt + SHARES * t;
         const float start = gate->from_start[16 * ti + r], end = gate->to_end[16 * ti + r];
-        const Four q = *reinterpret_cast<const Four *>(tk.four(sQ, ti, w));
+        const Four q = *reinterpret_cast<const Four *>(tk.four(sQ, ti, wf));
         float sum = 0.f;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            fromO[ti][e] *= start;
-            sum += fromO[ti][e] * (float)q[e];
-            fromX[ti][e] = end * fromU[ti][e] - start * fromX[ti][e];
+            fromO[t][e] *= start;
+            sum += fromO[t][e] * (float)q[e];
+            fromX[t][e] = end * fromU[t][e] - start * fromX[t][e];
         }
         sum = sum_over_c(sum);
-        if (c == 0) sums.state[w][16 * ti + r] = sum;
+        if (c == 0) sums.state[wf][16 * ti + r] = sum;
     }
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -284,7 +300,7 @@ template <typename T, int DKP> __global__ __launch_bounds__(DKP * 4) void delta_
         float beta = 0.f;
         if (lane < C) {
             for (int tj = 0; tj <= lane / 16; ++tj) x += sums.pairs[tj][lane];
-            for (int i = 0; i < NW; ++i) x += sums.state[i][lane];
+            for (int i = 0; i < FT; ++i) x += sums.state[i][lane];
             for (int i = 0; i < kShare; ++i) {
                 x -= sums.vdv[i][lane];
                 beta += sums.db[i][lane];
@@ -304,19 +320,20 @@ template <typename T, int DKP> __global__ __launch_bounds__(DKP * 4) void delta_
     D8 kc[CS], qc[CS];
 #pragma unroll
     for (int ks = 0; ks < CS; ++ks) {
-        kc[ks] = tk.columns(sK, ks, w);
-        qc[ks] = tk.columns(sQ, ks, w);
+        kc[ks] = tk.columns(sK, ks, wf);
+        qc[ks] = tk.columns(sQ, ks, wf);
     }
 #pragma unroll
-    for (int ti = 0; ti < CT; ++ti) {
+    for (int t = 0; t < OWN; ++t) {
+        const int ti = wt + SHARES * t;
 #pragma unroll
         for (int ks = 0; ks < CS; ++ks) {
-            if (ks <= ti / 2) fromO[ti] = mma_d(kc[ks], tu.halves(sP, ti, ks), fromO[ti]);
-            if (ks >= ti / 2) fromX[ti] = mma_d(qc[ks], tu.columns(sP, ks, ti), fromX[ti]);
-            fromX[ti] = mma_d(kc[ks], tu.halves(sE, ti, ks), fromX[ti]);
+            if (ks <= ti / 2) fromO[t] = mma_d(kc[ks], tu.halves(sP, ti, ks), fromO[t]);
+            if (ks >= ti / 2) fromX[t] = mma_d(qc[ks], tu.columns(sP, ks, ti), fromX[t]);
+            fromX[t] = mma_d(kc[ks], tu.halves(sE, ti, ks), fromX[t]);
         }
-        put_keys(a.dquery, ti, fromO[ti]);
-        put_keys(a.dkey, ti, fromX[ti]);
+        put_keys(a.dquery, ti, fromO[t]);
+        put_keys(a.dkey, ti, fromX[t]);
     }
 }
 
@@ -338,13 +355,12 @@ template <typename T, int DKP> int launch_gradient(hipStream_t stream, const Del
 {
     typedef DeltaChunk<T> DC;
     static LdsGrant grant;
-    constexpr int C = DC::C, NW = DKP / 16, kParts = DC::kParts;
-    constexpr size_t lds = sizeof(T) * ((2 * C + (kParts + 1) * kSlice) * LdsTile<T, DKP>::kRow + C * LdsTile<T, kSlice>::kRow +
-                                        (kParts + 1) * kSlice * LdsTile<T, C>::kRow) +
-                           sizeof(ChunkGates<C>) + sizeof(float) * C * (1 + DC::CT + NW + 2 * (NW / DC::CT));
+    constexpr int C = DC::C, NW = 8, kParts = DC::kParts;
+    constexpr size_t lds = sizeof(T) * (state_place<T, DKP>() + C * LdsTile<T, kSlice>::kRow + (kParts + 1) * kSlice * LdsTile<T, C>::kRow) +
+                           sizeof(ChunkGates<C>) + sizeof(float) * C * (1 + DC::CT + DKP / 16 + 2 * (NW / DC::CT));
     static_assert(lds <= 160 * 1024 && NW % DC::CT == 0, "");
     if (int e = allow_lds(grant, reinterpret_cast<const void *>(delta_gradient_kernel<T, DKP>), lds)) return e;
-    delta_gradient_kernel<T, DKP><<<a.pairs * a.chunks, DKP * 4, lds, stream>>>(a);
+    delta_gradient_kernel<T, DKP><<<a.pairs * a.chunks, 64 * NW, lds, stream>>>(a);
     return launch_status();
 }
 
