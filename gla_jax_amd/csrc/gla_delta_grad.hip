@@ -23,7 +23,7 @@ template <typename T, int F> __device__ __forceinline__ int place_in(int row, in
 template <typename T, int DKP> constexpr int state_place()
 {
     typedef DeltaChunk<T> DC;
-    constexpr int states = (DC::kParts + 1) * kSlice * LdsTile<T, DKP>::kRow, scores = 2 * DC::C * (LdsTile<T, DC::C>::kRow + LdsTile<T, DKP>::kRow);
+    constexpr int states = (DC::kParts + 1) * kSlice * LdsTile<T, DKP>::kRow, scores = 2 * DC::C * (DC::kFew * LdsTile<T, DC::C>::kRow + LdsTile<T, DKP>::kRow);
     return states > scores ? states : scores;
 }
 
@@ -43,8 +43,8 @@ template <typename T, int DKP> __global__ __launch_bounds__(512) void delta_grad
     extern __shared__ char smem[];
     // the scores, keys and queries take the states' place (two workgroups of 64 features a compute unit)
     T *sS = reinterpret_cast<T *>(smem), *sD = sS + kParts * kS, *sO = sS + state_place<T, DKP>(), *sU = sO + C * TileO::kRow, *sX = sU + kParts * kU,
-      *sP = sS, *sE = sP + kP, *sK = sE + kP, *sQ = sK + kK;
-    ChunkGates<C> *gate = reinterpret_cast<ChunkGates<C> *>(sX + kU);
+      *sP = sS, *sE = sP + kFew * kP, *sK = sE + kFew * kP, *sQ = sK + kK;
+    ChunkGates<C> *gate = reinterpret_cast<ChunkGates<C> *>(sX + kFew * kU);
     struct Sums {
         float beta[C];
         float pairs[CT][C];                      // row sums of P (do.u), one column of tiles each
@@ -164,7 +164,13 @@ template <typename T, int DKP> __global__ __launch_bounds__(512) void delta_grad
                 db[e] += x * du;
                 vdv[e] += v * dx[e];
             }
-            *reinterpret_cast<Four *>(sX + at) = pack_results<T>(dx);
+#pragma unroll
+            for (int p = 0; p < kFew; ++p) {
+                const Four f = pack_results<T>(dx);
+                *reinterpret_cast<Four *>(sX + p * kU + at) = f;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) dx[e] -= (float)f[e];
+            }
 #pragma unroll
             for (int p = 0; p < kParts; ++p) {
                 const Four f = pack_results<T>(u);
@@ -207,9 +213,13 @@ template <typename T, int DKP> __global__ __launch_bounds__(512) void delta_grad
 #pragma unroll
                     for (int p = kParts - 1; p >= 0; --p) score[m] = mma_d(tu.columns(sU + p * kU, ks, tj), o, score[m]);
                 } else {
-                    const D8 x = tu.columns(sX, ks, ti);
+                    D8 x[kFew], u[kFew];
 #pragma unroll
-                    for (int p = kFew - 1; p >= 0; --p) score[m] = mma_d(tu.columns(sU + p * kU, ks, tj), x, score[m]);
+                    for (int p = 0; p < kFew; ++p) {
+                        x[p] = tu.columns(sX + p * kU, ks, ti);
+                        u[p] = tu.columns(sU + p * kU, ks, tj);
+                    }
+                    score[m] = mma_parts(u, x, score[m]);
                 }
             }
         }
@@ -223,19 +233,21 @@ template <typename T, int DKP> __global__ __launch_bounds__(512) void delta_grad
             for (int t = 0; t < OWN; ++t) {
                 const int ti = wt + SHARES * t;
                 fromO[t] = mma_whole(s, to.halves(sO, ti, ks), fromO[t]);
-                const D8 x = tu.columns(sX, ks, ti);
+                D8 x[kFew], few[kFew];
 #pragma unroll
                 for (int p = kFew - 1; p >= 0; --p) {
-                    fromX[t] = mma_d(s[p], x, fromX[t]);
+                    x[p] = tu.columns(sX + p * kU, ks, ti);
+                    few[p] = s[p];
                     fromU[t] = mma_d(d, tu.columns(sU + p * kU, ks, ti), fromU[t]);
                 }
+                fromX[t] = mma_parts(few, x, fromX[t]);
             }
         }
     }
     lds_barrier();                               // the states are read
     key.store(tid, sK, there, DK);
     query.store(tid, sQ, there, DK);
-    if (w < CT / 2) *reinterpret_cast<Four *>(tu.four(sP, 2 * w, 2 * w + 1)) = Four{};      // the tiles above the diagonal that operands reach into
+    if (w < CT / 2 * kFew) *reinterpret_cast<Four *>(tu.four(sP + w % kFew * kP, w / kFew * 2, w / kFew * 2 + 1)) = Four{};      // the tiles above the diagonal that operands reach into
     lds_barrier();
 #pragma unroll
     for (int m = 0; m < kUnits; ++m) {
@@ -258,16 +270,27 @@ template <typename T, int DKP> __global__ __launch_bounds__(512) void delta_grad
             }
             sum = sum_over_c(sum);
             if (c == 0) sums.pairs[tj][i] = sum;
-            *reinterpret_cast<Four *>(tu.four(sP, ti, tj)) = pack_results<T>(d);
+#pragma unroll
+            for (int p = 0; p < kFew; ++p) {
+                const Four f = pack_results<T>(d);
+                *reinterpret_cast<Four *>(tu.four(sP + p * kP, ti, tj)) = f;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) d[e] -= (float)f[e];
+            }
         } else {
             f32x4 d;
 #pragma unroll
             for (int e = 0; e < 4; ++e) d[e] = j + e < i ? -weight[e] * score[m][e] : 0.f;
-            const Four f = pack_results<T>(d);
-            *reinterpret_cast<Four *>(tu.four(sE, ti, tj)) = f;
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (j + e < i) sE[place_in<T, C>(j + e, i)] = f[e];
+            for (int p = 0; p < kFew; ++p) {
+                const Four f = pack_results<T>(d);
+                *reinterpret_cast<Four *>(tu.four(sE + p * kP, ti, tj)) = f;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if (j + e < i) sE[p * kP + place_in<T, C>(j + e, i)] = f[e];
+                    d[e] -= (float)f[e];
+                }
+            }
         }
     }
 #pragma unroll
@@ -328,9 +351,12 @@ template <typename T, int DKP> __global__ __launch_bounds__(512) void delta_grad
         const int ti = wt + SHARES * t;
 #pragma unroll
         for (int ks = 0; ks < CS; ++ks) {
-            if (ks <= ti / 2) fromO[t] = mma_d(kc[ks], tu.halves(sP, ti, ks), fromO[t]);
-            if (ks >= ti / 2) fromX[t] = mma_d(qc[ks], tu.columns(sP, ks, ti), fromX[t]);
-            fromX[t] = mma_d(kc[ks], tu.halves(sE, ti, ks), fromX[t]);
+#pragma unroll
+            for (int p = kFew - 1; p >= 0; --p) {
+                if (ks <= ti / 2) fromO[t] = mma_d(kc[ks], tu.halves(sP + p * kP, ti, ks), fromO[t]);
+                if (ks >= ti / 2) fromX[t] = mma_d(qc[ks], tu.columns(sP + p * kP, ks, ti), fromX[t]);
+                fromX[t] = mma_d(kc[ks], tu.halves(sE + p * kP, ti, ks), fromX[t]);
+            }
         }
         put_keys(a.dquery, ti, fromO[t]);
         put_keys(a.dkey, ti, fromX[t]);
@@ -356,7 +382,7 @@ template <typename T, int DKP> int launch_gradient(hipStream_t stream, const Del
     typedef DeltaChunk<T> DC;
     static LdsGrant grant;
     constexpr int C = DC::C, NW = 8, kParts = DC::kParts;
-    constexpr size_t lds = sizeof(T) * (state_place<T, DKP>() + C * LdsTile<T, kSlice>::kRow + (kParts + 1) * kSlice * LdsTile<T, C>::kRow) +
+    constexpr size_t lds = sizeof(T) * (state_place<T, DKP>() + C * LdsTile<T, kSlice>::kRow + (kParts + DC::kFew) * kSlice * LdsTile<T, C>::kRow) +
                            sizeof(ChunkGates<C>) + sizeof(float) * C * (1 + DC::CT + DKP / 16 + 2 * (NW / DC::CT));
     static_assert(lds <= 160 * 1024 && NW % DC::CT == 0, "");
     if (int e = allow_lds(grant, reinterpret_cast<const void *>(delta_gradient_kernel<T, DKP>), lds)) return e;

@@ -437,7 +437,7 @@ template <typename T, int DKP, int NG, bool KEEP, bool SUMMARY> __global__ __lau
     extern __shared__ char smem[];
     // keys of two chunks and queries of one; the state, r, u (for the state, scaled) and u (for out); values, and gates of two chunks
     T *sK[2] = {reinterpret_cast<T *>(smem), reinterpret_cast<T *>(smem) + kTile<T, DKP>}, *sQ = sK[1] + kTile<T, DKP>, *sS = sQ + kTile<T, DKP>,
-      *sR = sS + NG * KS * kFew * 512, *sU = sR + NG * CS * kParts * 512, *sO = sU + NG * CS * kParts * 512;
+      *sR = sS + NG * KS * kParts * 512, *sU = sR + NG * CS * kParts * 512, *sO = sU + NG * CS * kParts * 512;
     float *sV = reinterpret_cast<float *>(sO + NG * CS * kFew * 512), *sG[2] = {sV + NG * CT * 256, sV + NG * CT * 256 + DC::kGates};
     W w;
     if (w.template place<SUMMARY, false>(a)) return;
@@ -516,7 +516,7 @@ template <typename T, int DKP, int NG, bool KEEP, bool SUMMARY> __global__ __lau
 #pragma unroll
                     for (int g = 0; g < NG; ++g) {
                         D8 s[kFew];
-                        W::template get<KS, kFew>(sS, g, ks, lane, s);
+                        W::template get<KS, kParts>(sS, g, ks, lane, s);
                         o[g] = mma_whole(s, Q[ks], o[g]);
                     }
             lds_barrier();                       // r
@@ -570,7 +570,7 @@ template <typename T, int DKP, int NG, bool KEEP, bool SUMMARY> __global__ __lau
     if (count > 0) {
         load(0, x);
         load(1, y);
-        w.template put_state<kFew>(sS, S);
+        w.template put_state<kParts>(sS, S);
         lds_barrier();                           // the first rows
         w.get_rows(sK[0], K);
     }
@@ -580,7 +580,7 @@ template <typename T, int DKP, int NG, bool KEEP, bool SUMMARY> __global__ __lau
         if constexpr (KEEP) keep(n);
         f32x4 v[NG];
         lds_barrier();                           // the state's operands are there
-        w.template keys_times_state<kFew>(sS, K, v);
+        w.template keys_times_state<kParts>(sS, K, v);
         if (w.tokens()) {
             const f32x4 start = w.gate(gates, 0);
 #pragma unroll
@@ -621,7 +621,7 @@ template <typename T, int DKP, int NG, bool KEEP, bool SUMMARY> __global__ __lau
         lds_barrier();                           // u
         w.add_keys(sU, KT, S);                   // the state behind the chunk
         w.get_rows(sK[(step + 1) & 1], K);
-        w.template put_state<kFew>(sS, S);
+        w.template put_state<kParts>(sS, S);
     });
     if constexpr (KEEP)
         if (w.end == w.live && (count > 0 || w.segment == 0)) keep(w.live);
@@ -914,7 +914,7 @@ template <typename T, int DKP, int NG, bool BACK> constexpr size_t walk_lds()
     constexpr size_t tiles = sizeof(T) * 3 * kTile<T, DKP>;
     return tiles + sizeof(float) * 2 * DC::kGates +
            (BACK ? sizeof(T) * 512 * NG * (W::KS * DC::kParts + W::CS * (3 * DC::kParts + 1)) + sizeof(float) * 256 * NG * (W::CT + W::TILES)
-                         : sizeof(T) * 512 * NG * (W::KS * DC::kFew + W::CS * (2 * DC::kParts + DC::kFew)) + sizeof(float) * 256 * NG * W::CT);
+                         : sizeof(T) * 512 * NG * (W::KS * DC::kParts + W::CS * (2 * DC::kParts + DC::kFew)) + sizeof(float) * 256 * NG * W::CT);
 }
 template <typename T, int DKP, int NG, bool BACK> int launch_walk(hipStream_t stream, const DeltaArgs &a, bool summary)
 {

@@ -196,7 +196,8 @@ def delta_step(states, log_decay, beta, value, key, query, slots=None, parents=N
     updated in place, with `slots` and `parents` as in `decay_step`: row b's state is states[slots[b]], and with `parents` [G,W] it continues from
     the state that its parent beam had before the call.
 
-    log_decay, beta [B,H] or [H];  value [B,H,DV];  key, query [B,HK,DK], HK divides H, DK up to 256.  Returns out [B,H,DV] in value.dtype.
+    log_decay, beta [B,H] or [H];  value [B,H,DV];  key, query [B,HK,DK], HK divides H, DK and DV multiples of 16 up to 256
+    (chunk_delta pads others; states are updated where they lie).  Returns out [B,H,DV] in value.dtype.
 
     States are updated in place: nothing here is differentiable, and arrays that require a gradient are refused.  The update counts as a
     new version of `states`."""
