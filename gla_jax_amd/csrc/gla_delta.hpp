@@ -51,6 +51,7 @@ struct DeltaArgs {
     int64_t chunks, pairs;
     DecayRows gates, betas, keys, values, queries, dout;
     const int32_t *lengths;
+    bool by_length;                 // walks: longest sequences first (at most 64)
     DeltaPrepared to;
     const void *hidden;             // hidden_init; backward: dhidden_final
     int hidden_dtype;
