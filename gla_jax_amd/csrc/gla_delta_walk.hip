@@ -274,6 +274,47 @@ template <typename T, int DKP, int NG> struct Walk {
     {
         return *reinterpret_cast<const f32x4 *>(gates + kind * C + 16 * min(w, CT - 1) + 4 * c);
     }
+    // What brings chunks into the die's cache before the loads above ask for them.  A compute unit has only so many requests on their way to
+    // memory, and a chunk takes 80 KB.  The workgroups of a pair's columns want the same, so each helper touches a part, one value of each 128
+    // bytes: keys, queries, inverse, scores (in this order, 64 lines a wave, as far as there are waves), and of its own columns the values.
+    // (Training step of B4 T4096 H6 D128 on data that no cache holds: walks 142 and 153 us without, 129 and 148 with; on data in the last-level
+    // cache no difference.  At 64 features, with half as much to bring, 59 us without and 62 with, and summaries 283 and 296: those do without.)
+    static constexpr int kAhead = 6;
+    struct Ahead {
+        const char *p;
+        int64_t step;                            // bytes from chunk to chunk
+        int st, size;                            // of rows: their distance; or the bytes of a chunk
+        unsigned at;
+    };
+    template <int SCORE_PARTS> __device__ __forceinline__ Ahead ahead(const DeltaArgs &a, const Rows &keys, const Rows &queries) const
+    {
+        constexpr int e = (int)sizeof(T), kLines = DKP * e / 128, kOfRows = C * kLines / 64, kInverse = DC::kSteps * DC::kParts * 512 * e,
+                      kScores = DC::kSteps * SCORE_PARTS * 512 * e, kOfInverse = (kInverse + 8191) / 8192, kOfScores = (kScores + 8191) / 8192;
+        int job = col0 / (16 * NG) * kWaves + w;
+        if (job < 2 * kOfRows) {
+            const Rows &x = job < kOfRows ? keys : queries;
+            const int line = lane % kLines * 128;
+            return {reinterpret_cast<const char *>(x.p), (int64_t)C * x.st * e, x.st, 0,
+                    line < DK * e ? (unsigned)((job % kOfRows * (64 / kLines) + lane / kLines) * x.st * e + line) : kNowhere};
+        }
+        job -= 2 * kOfRows;
+        const bool inverse = job < kOfInverse;
+        const int size = inverse ? kInverse : kScores;
+        if (!inverse) job -= kOfInverse;
+        return {static_cast<const char *>(inverse ? a.to.inverse : a.to.scores) + (int64_t)pair * a.chunks * size, size, 0, size,
+                inverse || job < kOfScores ? 8192u * job + 128u * lane : kNowhere};
+    }
+    __device__ __forceinline__ uint32_t touch(const Ahead &x, int n) const
+    {
+        const int size = x.size ? x.size : ((min(C, len - n * C) - 1) * x.st + DK) * (int)sizeof(T);
+        const auto chunk = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(x.p + n * x.step), 0, size, 0x00027000);
+        return __builtin_amdgcn_raw_buffer_load_b32(chunk, x.at, 0, 0);
+    }
+    __device__ __forceinline__ uint32_t touch_values(const Rows &x, int n) const
+    {
+        return __builtin_amdgcn_raw_buffer_load_b32(chunk_rows(x, n, DV), lane < 16 ? (unsigned)((16 * min(w, CT - 1) + r) * x.st + col0) * (unsigned)sizeof(T) : kNowhere,
+                                                    0, 0);
+    }
     // x or the cotangents of u: the four tokens of a column
     __device__ __forceinline__ int64_t written(int n, int g) const
     {
@@ -407,6 +448,7 @@ template <typename T, int DKP, int NG, bool KEEP, bool SUMMARY> __global__ __lau
     typedef typename W::DC DC;
     typedef typename W::D8 D8;
     constexpr int C = W::C, CT = W::CT, CS = W::CS, KS = W::KS, PER = W::PER, NC = W::NC, kParts = DC::kParts, kFew = DC::kFew;
+    constexpr bool kTouch = DKP > 64 && !SUMMARY;
     extern __shared__ char smem[];
     // keys of two chunks and queries of one; the state, r, u (for the state, scaled) and u (for out); values, and gates of two chunks
     T *sK[2] = {reinterpret_cast<T *>(smem), reinterpret_cast<T *>(smem) + kTile<T, DKP>}, *sQ = sK[1] + kTile<T, DKP>, *sS = sQ + kTile<T, DKP>,
@@ -436,6 +478,7 @@ template <typename T, int DKP, int NG, bool KEEP, bool SUMMARY> __global__ __lau
             typename W::Cols V[NG / NC][4];
             float gate;
             D8 P[CS][1];
+            uint32_t touched[2];
         } x, y;
         const typename W::Rows keys = w.key_rows(a.keys), queries = w.key_rows(a.queries), values = w.value_rows(a.values);
         D8 Q[KS];
@@ -448,6 +491,13 @@ template <typename T, int DKP, int NG, bool KEEP, bool SUMMARY> __global__ __lau
         };
         auto load_scores = [&](int step, Set &to) {
             if constexpr (!SUMMARY) w.template load_steps<false>(a.to.scores, a, min(w.first + step, last), to.P);
+        };
+        const typename W::Ahead ahead = w.template ahead<1>(a, keys, queries);
+        auto touch = [&](int step, Set &to) {
+            if constexpr (!kTouch) return;
+            const int n = min(w.first + step, last);
+            to.touched[0] = w.touch(ahead, n);
+            to.touched[1] = w.touch_values(values, n);
         };
         auto put_rows = [&](int step, const Set &from) {
             w.put_stage(sK[step & 1], from.key);
@@ -467,6 +517,8 @@ template <typename T, int DKP, int NG, bool KEEP, bool SUMMARY> __global__ __lau
             load_scores(1, y);
             put_rows(0, x);
             load_rows(2, x);
+            touch(W::kAhead - 2, x);
+            touch(W::kAhead - 1, y);
             lds_barrier();                       // the first rows
         }
         in_turns(count, x, y, [&](int step, Set &mine, Set &next) {
@@ -507,6 +559,8 @@ template <typename T, int DKP, int NG, bool KEEP, bool SUMMARY> __global__ __lau
                 store(from, [&](int g, int e) { return is ? o[g][e] : 0.f; });
             }
             load_scores(step + 2, mine);
+            if constexpr (kTouch) asm volatile("" ::"v"(mine.touched[0]), "v"(mine.touched[1]));       // (asked for two chunks ago)
+            touch(step + W::kAhead, mine);
         });
         // rows past the end of a shorter sequence
         if (!SUMMARY && w.segment == a.segments - 1)
@@ -601,6 +655,7 @@ template <typename T, int DKP, int NG, bool SUMMARY> __global__ __launch_bounds_
     typedef typename W::D8 D8;
     constexpr int C = W::C, CT = W::CT, CS = W::CS, KS = W::KS, PER = W::PER, TILES = W::TILES, NC = W::NC, kParts = DC::kParts;
     constexpr int kRows = NG * CS * kParts * 512;
+    constexpr bool kTouch = DKP > 64 && !SUMMARY;
     extern __shared__ char smem[];
     // keys of two chunks and queries of one; the cotangents of the state, of u before the system is solved, of r and of out (scaled), of out as
     // it is; the helpers' sums, in floats; gates of two chunks
@@ -625,7 +680,18 @@ template <typename T, int DKP, int NG, bool SUMMARY> __global__ __launch_bounds_
             float gate;
             f32x4 start, S[NG][2];                      // the state behind the chunk
             D8 P[CS][kParts];
+            uint32_t touched[3];
         } x, y;
+        const typename W::Ahead ahead = w.template ahead<kParts>(a, keys, queries);
+        auto touch = [&](int step, Set &to) {
+            if constexpr (!kTouch) return;
+            const int n = chunk_of(step);
+            to.touched[0] = w.touch(ahead, n);
+            to.touched[1] = w.touch_values(douts, n);
+            // the states' tiles of a group of columns: 16 lines a wave (as many as there are)
+            const int64_t line = w.state_place(n + 1, 0, 0) - (w.c * 16 + w.r) * 4 + 512 * w.w + 32 * w.r;
+            to.touched[2] = __float_as_uint(kept[w.w < delta_state_tiles(w.DK) / 2 ? line : 0]);
+        };
         auto load_rows = [&](int step, Set &to) {
             const int n = chunk_of(step);
             w.load_stage(keys, n, to.key);
@@ -695,6 +761,8 @@ template <typename T, int DKP, int NG, bool SUMMARY> __global__ __launch_bounds_
         load_kept(1, y);
         put_rows(0, x);
         load_rows(2, x);
+        touch(W::kAhead - 2, x);
+        touch(W::kAhead - 1, y);
         lds_barrier();                           // the first keys, and the operands of the first sums
         sums(x);
         load_scores(2, x);
@@ -743,6 +811,8 @@ template <typename T, int DKP, int NG, bool SUMMARY> __global__ __launch_bounds_
             load_kept(step + 2, mine);
             load_rows(step + 3, next);
             load_scores(step + 3, next);
+            if constexpr (kTouch) asm volatile("" ::"v"(mine.touched[0]), "v"(mine.touched[1]), "v"(mine.touched[2]));
+            touch(step + W::kAhead, mine);
         });
         return;
     }
