@@ -21,7 +21,9 @@ int check_sizes(const DecaySizes &n, gla_dtype dtype)
     if (n.B >= limit || n.H >= limit || n.T >= limit || n.B * n.H >= limit) return GLA_ERR_SHAPE;
     if (n.H * n.DV >= kMostRow || n.HK * n.DK >= kMostRow) return GLA_ERR_SHAPE;
     if (!dtype_ok(dtype)) return GLA_ERR_DTYPE;
-    if (n.B * n.H * (chunks_of(n, dtype) + 1) >= limit) return GLA_ERR_SHAPE;      // workgroups of a launch
+    // (workgroups of 512 threads, which a launch counts in 32 bits)
+    const int64_t most = (int64_t)1 << 23, pairs = (n.B * n.H + 7) / 8 * 8;
+    if (pairs * chunks_of(n, dtype) >= most || pairs * ((n.DV + 31) / 32) >= most) return GLA_ERR_SHAPE;
     return GLA_OK;
 }
 

@@ -8,11 +8,14 @@
 // So the work is in two kinds of kernels.  delta_prepare_kernel, all chunks at once, forms the inverses and the scores.  The walks go
 // through a sequence's chunks with the state in the accumulators of their matrix instructions, and need nothing but products.
 //
-// A workgroup walks with 16 to 64 value columns of the state: four waves each hold a quarter of the features and make, of a chunk's products, 16
-// tokens; three times a chunk they hand each other operands through LDS: the state, r, and u.  Four more bring keys and queries and do what
+// A workgroup walks with 16 or 32 value columns of the state: four waves each hold a quarter of the features and make, of a chunk's products, 16
+// tokens; three times a chunk they hand each other operands through LDS: the state, r, and u.  Four more bring keys, queries and values and do what
 // the next state does not wait for.  The inverses and scores come from memory as delta_prepare_kernel's lanes held them.  All of it is requested two chunks
-// ahead: a chunk takes 2300 cycles, and memory's answer now and then longer.  Where there are few sequences their columns are spread over the
-// compute units.
+// ahead.  Where there are few sequences their columns are spread over the compute units, and long ones go in segments.
+//
+// What bounds the walks (128 x 128 features): the chain of a chunk.  Its three exchanges with their products take 2300 cycles where nothing is loaded
+// (1.0 us); with a chunk's 80 KB, of which every column's workgroup needs all, 1.6 us for 16 columns where few workgroups run and 2.0 where they
+// fill the GPU, 2.5 to 3.2 for 32.  Of that the matrix cores work 17 %, LDS and the path from the caches 40 % each.
 //
 // Precision.  Keys, queries and values are 16-bit numbers as they come.  What a 32-bit result (states, gradients of the gates) depends on
 // and is formed in between enters a product as bf16 parts (Split): the state, the inverse, r, u and the scores of the backward walk in three, 2^-25 of a
@@ -31,7 +34,7 @@ namespace gla {
 template <typename T> struct DeltaChunk {
     static constexpr int C = DecayChunk<T>::C, CT = C / 16, CS = C / 32;
     static constexpr int kParts = sizeof(T) == 2 ? 3 : 1;      // of an operand that is a 32-bit number
-    static constexpr int kFew = sizeof(T) == 2 ? 2 : 1;        // of the state where keys or queries meet it
+    static constexpr int kFew = sizeof(T) == 2 ? 2 : 1;        // of one that only a 16-bit result depends on
     // steps of 32 tokens of a triangle's rows of tiles, 512 values each: lower ones have step ks <= t / 2, upper ones ks >= t / 2
     static constexpr int kSteps = CS == 1 ? CT : 6;
     static constexpr int lower(int t, int ks) { return t < 2 ? t : 2 * t - 2 + ks; }

@@ -303,12 +303,13 @@ int gla_decay_step(void *stream, int64_t pool, int64_t B, int64_t H, int64_t HK,
  * and the rules for them are those of gla_decay_fwd and gla_decay_bwd, with
  *   beta [B,T,H] float32 (any strides)
  * and DK at most GLA_MOST_DELTA_KEYS.  `strides` holds batch, token and head strides of log_decay, beta, value, key and query: 15 numbers.  Keys of a length of at
- * most sqrt(2 / beta) keep the states bounded; others are taken as they are. */
+ * most sqrt(2 / beta) keep the states bounded; others are taken as they are.  Fewer than 2^23 chunks (of 64 tokens, float32 data: 32) of all
+ * (batch, head) pairs, and pairs of 32 value columns. */
 
 #define GLA_MOST_DELTA_KEYS 128
 
 /* Bytes of the `states` that gla_delta_fwd leaves for gla_delta_bwd: the states before every chunk (of 64 tokens, float32 data: 32) and at the
- * end, and what every token wrote, in float32. */
+ * end, and what of every token's value they missed, in float32. */
 size_t gla_delta_states_bytes(int64_t B, int64_t T, int64_t H, int64_t HK, int64_t DK, int64_t DV, gla_dtype dtype);
 /* Bytes of scratch (0: none is needed and it may be NULL). */
 size_t gla_delta_fwd_workspace_bytes(int64_t B, int64_t T, int64_t H, int64_t HK, int64_t DK, int64_t DV, gla_dtype dtype);

@@ -96,7 +96,8 @@ def test_entry_points_reject_bad_arguments_without_touching_the_gpu():
         return lib.gla_delta_fwd(None, B, T, H, HK, DK, DV, dt, hd, st, h0, g, b, v, a, a, n, a, a, states, ws, size)
 
     assert fwd(h0=None) == -1 and fwd(v=None) == -1 and fwd(g=None) == -1 and fwd(b=None) == -1
-    for bad in ({"B": 0}, {"T": -1}, {"H": 0}, {"HK": 3}, {"HK": 0}, {"DK": 40}, {"DK": 144}, {"DV": 8}, {"DV": 272}, {"T": 1 << 31}, {"H": 1 << 20, "HK": 1 << 20}):
+    for bad in ({"B": 0}, {"T": -1}, {"H": 0}, {"HK": 3}, {"HK": 0}, {"DK": 40}, {"DK": 144}, {"DV": 8}, {"DV": 272}, {"T": 1 << 31}, {"H": 1 << 20, "HK": 1 << 20}, {"B": 1 << 21, "DV": 256},
+                {"B": 1 << 12, "T": 1 << 16}):
         assert fwd(**bad) == -2, bad
     assert fwd(dt=7) == -3 and fwd(hd=7) == -3
     assert fwd(h0=a + 8) == -6 and fwd(v=a + 2) == -6 and fwd(g=a + 2) == -6 and fwd(b=a + 2) == -6 and fwd(n=a + 1) == -6 and fwd(states=a + 8) == -6

@@ -249,3 +249,23 @@ def test_rows_that_allow_few_tokens(V, dtype):
     close(near[1:].masked_fill(near[1:] == -math.inf, 0), want, off(want, V))
     want = torch.special.entr(p[1:].exp()).sum(-1)
     close(entropy[1:], want, 2 * off(want, V))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_more_rows_than_a_launch_holds(dtype):
+    N = (1 << 22) + 3
+    x = torch.randint(-3, 4, (N, 3), device="cuda", generator=torch.Generator(device="cuda").manual_seed(11)).to(dtype)
+    t = torch.arange(N, device="cuda") % 4 - 1                 # every fourth does not count
+    leaf = x.detach().requires_grad_()
+    found = token_logprobs(leaf, t, 2)
+    g, h = torch.linspace(-1, 1, N, device="cuda"), torch.linspace(0, 1, N, device="cuda")
+    d, = torch.autograd.grad(found[:2], [leaf], (g, h))
+    at = torch.cat([torch.arange(5), torch.arange(N - 9, N)]).cuda()
+    want = exact(x[at], t[at], g[at], h[at])
+    close(found[0][at], want[0], off(want[0], 3))
+    close(found[1][at], want[1], 2 * off(want[1], 3))
+    close(d[at], want[2], 2 ** -7 * want[2].abs() + 2.0 ** -18 if dtype == BF16 else torch.full_like(want[2], 2.0 ** -18))
+    counts = (t >= 0) & (t < 3)
+    order = x.float().sort(dim=-1, descending=True, stable=True)[1][:, :2]
+    assert torch.equal(found[3], order.masked_fill(~counts[:, None], -1))
+    assert not found[0][~counts].any() and not d[~counts].any()
