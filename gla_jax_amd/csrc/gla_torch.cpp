@@ -12,10 +12,14 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/engine.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
+#include <torch/csrc/autograd/graph_task.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <array>
 #include <optional>
+#include <unordered_set>
 
 #include "../../include/gla_hip.h"
 
@@ -508,6 +512,41 @@ variable_list delta_backward(const Tensor &states, const Tensor &a, const Tensor
     return {dh0, da, db, dv, dk, dq};
 }
 
+// A leaf's gradient is accumulated on the stream of the first graph that holds the leaf, for as long as any graph holds it.  Is that the default
+// stream and this backward pass is captured on another, then the default stream would be made to wait for the capture, which HIP forbids and the
+// process does not outlive.  Called by a backward before it launches anything: looks through the graph behind it for such a leaf that the pass reaches.
+void refuse_capture_for_eager_leaves(const char *name, const Tensor &t)
+{
+    const auto stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.device().index());
+    const c10::Stream usual = c10::hip::getDefaultHIPStreamMasqueradingAsCUDA(t.device().index()).unwrap();
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    if (stream.unwrap() == usual) return;      // (which cannot be captured)
+    if (hipStreamIsCapturing(stream.stream(), &status) != hipSuccess || status == hipStreamCaptureStatusNone) return;
+    const auto here = torch::autograd::get_current_node();
+    if (!here) return;
+    const auto *reached = torch::autograd::get_current_graph_task_exec_info();
+    std::vector<torch::autograd::Node *> open{here.get()};
+    std::unordered_set<torch::autograd::Node *> seen{here.get()};
+    while (!open.empty()) {
+        torch::autograd::Node *node = open.back();
+        open.pop_back();
+        if (dynamic_cast<torch::autograd::AccumulateGrad *>(node)) {
+            const auto of = node->stream();
+            TORCH_CHECK(!of || *of != usual, name, ": a backward pass is captured while a graph of the same leaves from outside of the capture is alive: "
+                        "drop its results (or make them on another stream than the default one) first");
+        }
+        for (const auto &edge : node->next_edges()) {
+            torch::autograd::Node *next = edge.function.get();
+            if (!next || !seen.insert(next).second) continue;
+            if (reached && !reached->empty()) {
+                const auto it = reached->find(next);
+                if (it == reached->end() || !it->second.should_execute()) continue;
+            }
+            open.push_back(next);
+        }
+    }
+}
+
 struct DeltaBackward : torch::autograd::Function<DeltaBackward> {
     static variable_list forward(AutogradContext *, const Tensor &states, const Tensor &a, const Tensor &b, const Tensor &v, const Tensor &k,
                                  const Tensor &q, const std::optional<Tensor> &lengths, const Tensor &dhT, const Tensor &dout)
@@ -530,6 +569,7 @@ struct Delta : torch::autograd::Function<Delta> {
     static variable_list backward(AutogradContext *ctx, variable_list d)
     {
         variable_list s = ctx->get_saved_variables();
+        if (s[0].is_cuda()) refuse_capture_for_eager_leaves("chunk_delta", s[0]);
         for (size_t i = 3; i < 6; ++i)
             if (s[i].defined() && !rows_on_gpu(s[i])) s[i] = s[i].clone(at::MemoryFormat::Contiguous);
         if (!s[0].is_contiguous() || !on_16_bytes(s[0])) s[0] = s[0].clone(at::MemoryFormat::Contiguous);
@@ -893,6 +933,7 @@ struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
     {
         variable_list s = ctx->get_saved_variables();
         check_saved(s[0].is_cuda() && known(s[0].scalar_type()));
+        refuse_capture_for_eager_leaves("token_logprobs", s[0]);
         if (!logit_rows(s[0])) s[0] = s[0].contiguous();
         s[1] = s[1].contiguous();
         check_saved(logprob_arrays(s[0], s[1]) && s[2].is_contiguous() && s[3].is_contiguous() && s[2].numel() == 2 * s[1].numel() &&

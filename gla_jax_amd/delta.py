@@ -125,7 +125,8 @@ def chunk_delta(hidden_init, log_decay, beta, value, key, query, lengths=None):
     axes) ends sequences early: what lies behind is not read (it may be NaN), `out` is zero there and hidden_final is the state at the end.
 
     Returns (hidden_final [..,H,DK,DV] in hidden_init.dtype, out [..,T,H,DV] in value.dtype).  Differentiable in all six arrays; heads that
-    share a key head add up to its gradient."""
+    share a key head add up to its gradient.  A backward pass is captured into a graph only while no graph of the same leaves from the default
+    stream is alive (RuntimeError)."""
     done = _native("delta", (hidden_init, log_decay, beta, value, key, query), lengths)
     if done is not None:
         return tuple(done)

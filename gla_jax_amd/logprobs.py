@@ -109,7 +109,8 @@ def token_logprobs(logits, tokens, top=0):
     alternatives -inf and -1.  A logit of -inf has probability 0; a row with a NaN, or a +inf, or nothing above -inf, has NaN results, and such
     logits count as -inf in the order of the alternatives.
 
-    Differentiable in logits through logprobs and entropy: -logprobs.sum() is the cross entropy.  Positions that do not count get a gradient of 0."""
+    Differentiable in logits through logprobs and entropy: -logprobs.sum() is the cross entropy.  Positions that do not count get a gradient of 0.
+    A backward pass is captured into a graph only while no graph of the same leaves from the default stream is alive (RuntimeError)."""
     top = int(top)
     done = _native("token_logprobs", (logits, tokens), top)
     if done is None:

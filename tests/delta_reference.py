@@ -19,6 +19,7 @@ sum by at most sqrt(n) times one, and a single value by at most n times one of |
     close to 1 where nothing decays: a result behind m chunks has m times as many roundings, independent of each other.  (Without m,
     the cotangent of the first state behind three chunks of reflections, b = 2, with decays above 0.999 was held to 2 2^-18 = 7.6e-6 of
     its norm and off by 8.6e-6.)
+    (The kernels hold what 32-bit results depend on in three parts, which is off by less; the bounds count two.)
   * 32-bit data: products of floats, as for chunk_decay: 1e-5 (sqrt(2^14) 2^-24 = 2^-17, and room for the exponentials), and for dlog_decay by the same terms.
 """
 import numpy as np

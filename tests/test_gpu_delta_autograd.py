@@ -1,4 +1,5 @@
-"""chunk_delta, delta_step and token_logprobs recorded by a tracer, given arrays with tangents, and after their saved arrays were changed."""
+"""chunk_delta, delta_step and token_logprobs recorded by a tracer, given arrays with tangents,
+after their saved arrays were changed, and captured beside eager graphs."""
 import pytest
 import torch
 import torch.autograd.forward_ad as fwAD
@@ -108,3 +109,36 @@ def test_calls_under_inference_mode():
     plain = torch.zeros(3, 4, 32, 32, device="cuda")
     delta_step(plain, a, b, v, k, q)
     assert torch.equal(plain, made)
+
+
+@pytest.mark.parametrize("projected", [False, True])
+@pytest.mark.parametrize("op", ["chunk_delta", "token_logprobs"])
+def test_a_captured_backward_is_refused_while_an_eager_graph_of_its_leaves_lives(op, projected):
+    """(The default stream accumulates their gradients then, and cannot wait for a capture.)  Without that graph it is captured."""
+    if op == "chunk_delta":
+        arrays = rows(40, 31)
+        leaf = arrays[4].detach().clone().requires_grad_()
+        call = lambda k: chunk_delta(*arrays[:4], k, arrays[5])[1]  # noqa: E731
+    else:
+        x, tokens = logits(32)
+        leaf = x.detach().clone().requires_grad_()
+        call = lambda x: token_logprobs(x, tokens)[0]  # noqa: E731
+
+    def gradient():
+        out = call(2 * leaf if projected else leaf)
+        return torch.autograd.grad(out, [leaf], torch.ones_like(out))[0]
+    want = gradient()
+    alive = call(leaf)
+    with pytest.raises(RuntimeError, match="graph of the same leaves"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            gradient()
+    torch.cuda.synchronize()
+    del alive
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = gradient()
+    for _ in range(3):
+        got.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
