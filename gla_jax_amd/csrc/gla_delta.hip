@@ -30,7 +30,8 @@ int check_sizes(const DecaySizes &n, gla_dtype dtype)
 // Assigns the places of a call's scratch behind `ws` (which may be NULL: for the size alone); what the backward pass takes more of.
 int64_t lay_out(DeltaArgs &a, gla_dtype dtype, bool backward, char *ws, float **dquery, float **dkey)
 {
-    const int64_t C = chunk_of(dtype), e = bytes_of(dtype), parts = dtype == GLA_BF16 ? DeltaChunk<__bf16>::kParts : 1, chunk_pairs = a.pairs * a.chunks;
+    const int64_t C = chunk_of(dtype), e = bytes_of(dtype), chunk_pairs = a.pairs * a.chunks;
+    const int64_t parts = dtype == GLA_BF16 ? DeltaChunk<__bf16>::kParts : 1, few = dtype == GLA_BF16 ? DeltaChunk<__bf16>::kFew : 1;
     const int64_t steps = dtype == GLA_BF16 ? DeltaChunk<__bf16>::kSteps : DeltaChunk<float>::kSteps;
     int64_t at = 0;
     auto take = [&](int64_t bytes) {
@@ -39,7 +40,7 @@ int64_t lay_out(DeltaArgs &a, gla_dtype dtype, bool backward, char *ws, float **
         return x;
     };
     a.to.inverse = take(chunk_pairs * steps * parts * 512 * e);
-    a.to.scores = take(chunk_pairs * steps * (backward ? parts : 1) * 512 * e);
+    a.to.scores = take(chunk_pairs * steps * (backward ? parts : few) * 512 * e);
     a.to.gates = reinterpret_cast<float *>(take(chunk_pairs * 4 * C * 4));
     a.summary = reinterpret_cast<float *>(take(a.pairs * (a.segments - 1) * (a.n.DV + a.n.DK) * a.n.DK * 4));
     a.starts = reinterpret_cast<float *>(take(a.pairs * (a.segments - 1) * a.n.DV * a.n.DK * 4));

@@ -17,7 +17,7 @@ template <typename T, int DKP, bool BACK> __global__ __launch_bounds__(256) void
 {
     typedef DeltaChunk<T> DC;
     constexpr int C = DC::C, CT = DC::CT, KS = DKP / 32, NW = 4, NT = 256, kTriangle = CT * (CT + 1) / 2;
-    constexpr int kRow = C + 4, kBlock = 16 * 20, kParts = DC::kParts, kScoreParts = BACK ? kParts : 1;
+    constexpr int kRow = C + 4, kBlock = 16 * 20, kParts = DC::kParts, kScoreParts = BACK ? kParts : DC::kFew;
     typedef typename FragTypes<T>::d8 D8;
     typedef typename Packed4<T>::t Four;
     typedef LdsTile<T, DKP> Tile;

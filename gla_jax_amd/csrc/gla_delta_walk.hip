@@ -477,7 +477,7 @@ template <typename T, int DKP, int NG, bool KEEP, bool SUMMARY> __global__ __lau
             typename W::Stage key, query;
             typename W::Cols V[NG / NC][4];
             float gate;
-            D8 P[CS][1];
+            D8 P[CS][kFew];
             uint32_t touched[2];
         } x, y;
         const typename W::Rows keys = w.key_rows(a.keys), queries = w.key_rows(a.queries), values = w.value_rows(a.values);
@@ -492,7 +492,7 @@ template <typename T, int DKP, int NG, bool KEEP, bool SUMMARY> __global__ __lau
         auto load_scores = [&](int step, Set &to) {
             if constexpr (!SUMMARY) w.template load_steps<false>(a.to.scores, a, min(w.first + step, last), to.P);
         };
-        const typename W::Ahead ahead = w.template ahead<1>(a, keys, queries);
+        const typename W::Ahead ahead = w.template ahead<kFew>(a, keys, queries);
         auto touch = [&](int step, Set &to) {
             if constexpr (!kTouch) return;
             const int n = min(w.first + step, last);
@@ -552,7 +552,7 @@ template <typename T, int DKP, int NG, bool KEEP, bool SUMMARY> __global__ __lau
                         for (int g = 0; g < NG; ++g) {
                             D8 u[kFew];
                             W::template get<CS, kFew>(sO, g, ks, lane, u);
-                            o[g] = mma_whole(u, mine.P[ks][0], o[g]);
+                            o[g] = mma_parts(u, mine.P[ks], o[g]);
                         }
                 const int from = (w.first + step) * C;
                 const bool is = from + 16 * w.w + w.r < w.len;
