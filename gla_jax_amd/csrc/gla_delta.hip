@@ -46,7 +46,7 @@ int64_t lay_out(DeltaArgs &a, gla_dtype dtype, bool backward, char *ws, float **
     a.starts = reinterpret_cast<float *>(take(a.pairs * (a.segments - 1) * a.n.DV * a.n.DK * 4));
     if (!backward) return at;
     a.du = reinterpret_cast<float *>(take(a.pairs * delta_written_floats(a.n, a.chunks, (int)C) * 4));
-    a.dstates = take(chunk_pairs * delta_state_floats(a.n) * e);
+    a.dstates = take(chunk_pairs * delta_state_floats(a.n) * few * e);
     a.dots = reinterpret_cast<float *>(take(chunk_pairs * (a.n.DV / 16) * 4 * 4));
     a.row_parts = (int)(a.n.H / a.n.HK);
     if (a.row_parts > 1) {

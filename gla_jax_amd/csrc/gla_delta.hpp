@@ -21,10 +21,9 @@
 // and is formed in between enters a product as bf16 parts (Split): the state, the inverse, r, u and the scores of the backward walk in three, 2^-25 of a
 // value.  (The state where keys meet it in two, 2^-18: walks 4 to 8 % shorter, and a gradient of beta off by more than 1e-6 of its norm where
 // short sequences start from large states.)  What only 16-bit results depend on is in two, 2^-18, so that nothing but a result's own rounding is seen in it:
-// the state that queries read, u and the scores of out, dv and the scores of dkey and dquery.  (With the scores of out rounded to 16 bits once, out was off by 2.3e-3 of
-// its norm where its own rounding is 1.7e-3, and calls took 1 to 3 % less: B4 T4096 H6 D128 455 instead of 459 us for a training step, 16 prompts of 0 to
-// 1337 tokens 164 instead of 168.)  The cotangent of a state in dkey is rounded to 16 bits once.
-// float data take the matrix cores' float products.
+// the state that queries read, u and the scores of out, dv, the cotangents of states and the scores of dkey and dquery.  (With the scores of out and the cotangents
+// of states rounded to 16 bits once, out and dkey were off by 2.3e-3 of their norm where their own rounding is 1.7e-3; 16 prompts of 0 to 1337 tokens took 164 us
+// instead of 168, a training step of B4 T4096 H6 D128 455 instead of 493.)  float data take the matrix cores' float products.
 //
 // Operand layouts: gla_decay.hpp.  Rows of the state are the features pi(t, m) of gla_chunk_common.hpp, so that two accumulators above each
 // other (tiles 2p and 2p + 1) are features 32p + 8c .. + 7: an operand of the contraction with keys in their natural order.
@@ -68,7 +67,7 @@ struct DeltaArgs {
     // [chunks][DV / 16][C / 16][4][16][4]
     float *kept;
     // what the backward walk leaves for the gradients: the cotangents of u in the order of x, those of the states behind the chunks
-    // in the states' order, in T, and <state, its cotangent> there, [pairs, chunks][columns / 16][4]
+    // in the states' order, eight features of a column in T, part after part (kFew), and <state, its cotangent> there, [pairs, chunks][columns / 16][4]
     float *du;
     void *dstates;
     float *dots;

@@ -23,12 +23,12 @@ template <typename T, int F> __device__ __forceinline__ int place_in(int row, in
 template <typename T, int DKP> constexpr int state_place()
 {
     typedef DeltaChunk<T> DC;
-    constexpr int states = (DC::kParts + 1) * kSlice * LdsTile<T, DKP>::kRow, scores = 2 * DC::C * (DC::kFew * LdsTile<T, DC::C>::kRow + LdsTile<T, DKP>::kRow);
+    constexpr int states = (DC::kParts + DC::kFew) * kSlice * LdsTile<T, DKP>::kRow, scores = 2 * DC::C * (DC::kFew * LdsTile<T, DC::C>::kRow + LdsTile<T, DKP>::kRow);
     return states > scores ? states : scores;
 }
 
-// 150 us for the 1536 chunks of B4 T4096 H6 D128, 85 for the 1056 of B2 T2050 H16 64x128: 422 MB and 2.8 TB/s at 128 x 128, of which the states before the
-// chunks are 100 (32 bits), their cotangents 50, what was written and its cotangents 50 each.  LDS and registers leave one workgroup a compute unit, whose
+// 175 us for the 1536 chunks of B4 T4096 H6 D128, 87 for the 1056 of B2 T2050 H16 64x128: 472 MB and 2.7 TB/s at 128 x 128, of which the states before the
+// chunks are 100 (32 bits), their cotangents 100 (in two parts; in one, 154 and 85 us), what was written and its cotangents 50 each.  LDS and registers leave one workgroup a compute unit, whose
 // phases (a slice's rows arrive, its products, the scores) do not overlap; chunk after chunk in one workgroup, the next one's first rows on
 // their way, it needs 90 to 180 registers more than there are.
 // One workgroup: a chunk of a (batch, head) pair; a wave makes 16 key features of dq and dk, at 64 features of every second tile of tokens.
@@ -89,7 +89,7 @@ template <typename T, int DKP> __global__ __launch_bounds__(512) void delta_grad
     const int64_t floats = delta_written_floats(a.n, a.chunks, C), state = delta_state_floats(a.n);
     const float *kept = a.kept + pair * (delta_states_floats(a.n, a.chunks) + floats), *xs = kept + delta_states_floats(a.n, a.chunks) + n * C * DV;
     const float *dus = a.du + pair * floats + n * C * DV;
-    const T *dS = static_cast<const T *>(a.dstates) + (pair * chunks + n) * state;
+    const T *dS = static_cast<const T *>(a.dstates) + (pair * chunks + n) * state * kFew;
     kept += n * state;
     // A slice of values on its way: no load is under a branch, for then each waits for the one before, and the next slice's are issued before the
     // products of one.  (One after the other they took 25000 of a chunk's 46000 cycles at 128 x 128 features.)
@@ -97,7 +97,7 @@ template <typename T, int DKP> __global__ __launch_bounds__(512) void delta_grad
     static_assert(kSlice / 16 * KS % NW == 0 && kSlice / 16 % kShare == 0, "");
     RowsInFlight<T, C, kSlice, NT> o;
     f32x4 low[kStates], high[kStates], written[kTiles], dwritten[kTiles];
-    D8 dstate[kStates];
+    D8 dstate[kStates][kFew];
     T value[kTiles][4];
     const int own = w % CT, token = 16 * own + 4 * c;       // of what was written
     auto load_slice = [&](int dv0) {
@@ -108,7 +108,8 @@ template <typename T, int DKP> __global__ __launch_bounds__(512) void delta_grad
             const unsigned from = dv0 + 16 * m < DV && 32 * ks < DK ? (((dv0 >> 4) + m) * (delta_state_tiles(DK) / 2) + ks) * 512 : 0;
             low[i] = *reinterpret_cast<const f32x4 *>(kept + from + lane * 4);
             high[i] = *reinterpret_cast<const f32x4 *>(kept + from + 256 + lane * 4);
-            dstate[i] = ld8(dS + from + lane * 8);
+#pragma unroll
+            for (int p = 0; p < kFew; ++p) dstate[i][p] = ld8(dS + from * kFew + p * 512 + lane * 8);
         }
 #pragma unroll
         for (int i = 0; i < kTiles; ++i) {
@@ -152,7 +153,8 @@ template <typename T, int DKP> __global__ __launch_bounds__(512) void delta_grad
             const Split<T, kParts> split(x);
 #pragma unroll
             for (int p = 0; p < kParts; ++p) st8(sS + p * kS + at, split.part[p]);
-            st8(sD + at, is ? dstate[i] : D8{});
+#pragma unroll
+            for (int p = 0; p < kFew; ++p) st8(sD + p * kS + at, is ? dstate[i][p] : D8{});
         }
         const f32x4 beta = *reinterpret_cast<const f32x4 *>(sums.beta + token);
 #pragma unroll
@@ -232,19 +234,32 @@ template <typename T, int DKP> __global__ __launch_bounds__(512) void delta_grad
             D8 s[kParts];
 #pragma unroll
             for (int p = 0; p < kParts; ++p) s[p] = tk.columns(sS + p * kS, ks, wf);
-            const D8 d = tk.columns(sD, ks, wf);
 #pragma unroll
             for (int t = 0; t < OWN; ++t) {
                 const int ti = wt + SHARES * t;
                 fromO[t] = mma_whole(s, to.halves(sO, ti, ks), fromO[t]);
                 D8 x[kFew], few[kFew];
 #pragma unroll
-                for (int p = kFew - 1; p >= 0; --p) {
+                for (int p = 0; p < kFew; ++p) {
                     x[p] = tu.columns(sX + p * kU, ks, ti);
                     few[p] = s[p];
-                    fromU[t] = mma_d(d, tu.columns(sU + p * kU, ks, ti), fromU[t]);
                 }
                 fromX[t] = mma_parts(few, x, fromX[t]);
+            }
+        }
+        // (in a loop of its own, without the states' parts beside: 175 us, together 181)
+#pragma unroll
+        for (int ks = 0; ks < VS; ++ks) {
+            D8 d[kFew];
+#pragma unroll
+            for (int p = 0; p < kFew; ++p) d[p] = tk.columns(sD + p * kS, ks, wf);
+#pragma unroll
+            for (int t = 0; t < OWN; ++t) {
+                const int ti = wt + SHARES * t;
+                D8 u[kFew];
+#pragma unroll
+                for (int p = 0; p < kFew; ++p) u[p] = tu.columns(sU + p * kU, ks, ti);
+                fromU[t] = mma_parts(d, u, fromU[t]);
             }
         }
     }

@@ -325,10 +325,10 @@ template <typename T, int DKP, int NG> struct Walk {
     {
         return (((int64_t)n * (DV >> 4) + (column(g) >> 4)) * delta_state_tiles(DK) + t) * 256 + (c * 16 + (column(g) & 15)) * 4;
     }
-    // cotangents of states: the eight features 8c .. of tiles 2 ks and 2 ks + 1, a column
+    // cotangents of states: the eight features 8c .. of tiles 2 ks and 2 ks + 1, a column, the first part
     __device__ __forceinline__ int64_t cotangent_place(int n, int g, int ks) const
     {
-        return (((int64_t)n * (DV >> 4) + (column(g) >> 4)) * (delta_state_tiles(DK) / 2) + ks) * 512 + (c * 16 + (column(g) & 15)) * 8;
+        return (((int64_t)n * (DV >> 4) + (column(g) >> 4)) * (delta_state_tiles(DK) / 2) + ks) * (DC::kFew * 512) + (c * 16 + (column(g) & 15)) * 8;
     }
     // ---- operands in LDS: [group][step][part][lane][8], a wave's accumulators being half of a step ----
     template <int STEPS, int N> static __device__ __forceinline__ void put(T *to, int g, int t, int lane, f32x4 v)
@@ -671,7 +671,7 @@ template <typename T, int DKP, int NG, bool SUMMARY> __global__ __launch_bounds_
     if (w.helper) {
         if (count == 0) return;
         const float *kept = a.kept + w.pair * (delta_states_floats(a.n, a.chunks) + delta_written_floats(a.n, a.chunks, C));
-        T *dstates = static_cast<T *>(a.dstates) + w.pair * a.chunks * delta_state_floats(a.n);
+        T *dstates = static_cast<T *>(a.dstates) + w.pair * a.chunks * delta_state_floats(a.n) * DC::kFew;
         const typename W::Rows douts = w.value_rows(a.dout), keys = w.key_rows(a.keys), queries = w.key_rows(a.queries);
         const bool features = w.w < KS && 32 * w.w + 8 * w.c < w.DK;     // of a state: the eight 32w + 8c ..
         struct Set {
@@ -798,7 +798,8 @@ template <typename T, int DKP, int NG, bool SUMMARY> __global__ __launch_bounds_
                         }
 #pragma unroll
                         for (int e = 0; e < 8; ++e) dot += d[e] * mine.S[q][e >> 2][e & 3];
-                        st8(dstates + w.cotangent_place(n, q, w.w), parts[0]);
+#pragma unroll
+                        for (int i = 0; i < DC::kFew; ++i) st8(dstates + w.cotangent_place(n, q, w.w) + i * 512, parts[i]);
                     }
                 dot = sum_over_c(sum_over_r(dot));
                 if (lane == 0)

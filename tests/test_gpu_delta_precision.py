@@ -33,3 +33,9 @@ def found(sizes, gates, dtype=BF16):
 def test_out(sizes, gates):
     share = changed(*found(sizes, gates)["out"][:2])
     assert share <= CHANGED
+
+
+@pytest.mark.parametrize("sizes, gates", CASES, ids=ids)
+def test_dkey(sizes, gates):
+    share = changed(*found(sizes, gates)["dkey"][:2])
+    assert share <= CHANGED
