@@ -30,6 +30,7 @@
 #pragma once
 
 #include "gla_decay.hpp"
+#include "gla_delta_places.hpp"
 
 namespace gla {
 
@@ -79,8 +80,6 @@ struct DeltaArgs {
     float *dgate, *dbeta;
     int row_parts;
 };
-// (features pi come in pairs of tiles)
-inline __host__ __device__ int delta_state_tiles(int64_t DK) { return (int)((DK + 31) / 32 * 2); }
 inline __host__ __device__ int64_t delta_state_floats(const DecaySizes &n) { return 16 * delta_state_tiles(n.DK) * n.DV; }
 inline __host__ __device__ int64_t delta_states_floats(const DecaySizes &n, int64_t chunks) { return (chunks + 1) * delta_state_floats(n); }
 inline __host__ __device__ int64_t delta_written_floats(const DecaySizes &n, int64_t chunks, int C) { return chunks * C * n.DV; }

@@ -277,8 +277,8 @@ template <typename T, int DKP, int NG> struct Walk {
     // What brings chunks into the die's cache before the loads above ask for them.  A compute unit has only so many requests on their way to
     // memory, and a chunk takes 80 KB.  The workgroups of a pair's columns want the same, so each helper touches a part, one value of each 128
     // bytes: keys, queries, inverse, scores (in this order, 64 lines a wave, as far as there are waves), and of its own columns the values.
-    // (Training step of B4 T4096 H6 D128 on data that no cache holds: walks 142 and 153 us without, 129 and 148 with; on data in the last-level
-    // cache no difference.  At 64 features, with half as much to bring, 59 us without and 62 with, and summaries 283 and 296: those do without.)
+    // (Training step of B4 T4096 H6 D128 on data that no cache holds: walks 142 and 153 us without, 129 and 148 with, while cotangents of states were left
+    // in one part; on data in the last-level cache no difference, nor in the states' part of it for 32 columns, B8 T2048 H16: 291 us back with half of its lines and with all.  At 64 features, with half as much to bring, 59 us without and 62 with, and summaries 283 and 296: those do without.)
     static constexpr int kAhead = 6;
     struct Ahead {
         const char *p;
@@ -683,14 +683,15 @@ template <typename T, int DKP, int NG, bool SUMMARY> __global__ __launch_bounds_
             uint32_t touched[3];
         } x, y;
         const typename W::Ahead ahead = w.template ahead<kParts>(a, keys, queries);
+        const int64_t state_floats = delta_state_floats(a.n);
+        const unsigned touched_line = delta_touched_line(w.DK, w.col0, 16 * NG, w.w, lane);
         auto touch = [&](int step, Set &to) {
             if constexpr (!kTouch) return;
             const int n = chunk_of(step);
             to.touched[0] = w.touch(ahead, n);
             to.touched[1] = w.touch_values(douts, n);
-            // the states' tiles of a group of columns: 16 lines a wave (as many as there are)
-            const int64_t line = w.state_place(n + 1, 0, 0) - (w.c * 16 + w.r) * 4 + 512 * w.w + 32 * w.r;
-            to.touched[2] = __float_as_uint(kept[w.w < delta_state_tiles(w.DK) / 2 ? line : 0]);
+            to.touched[2] = __builtin_amdgcn_raw_buffer_load_b32(
+                __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(kept + (n + 1) * state_floats), 0, 4 * (int)state_floats, 0x00027000), touched_line, 0, 0);
         };
         auto load_rows = [&](int step, Set &to) {
             const int n = chunk_of(step);
