@@ -278,7 +278,8 @@ template <typename T, int DKP, int NG> struct Walk {
     // memory, and a chunk takes 80 KB.  The workgroups of a pair's columns want the same, so each helper touches a part, one value of each 128
     // bytes: keys, queries, inverse, scores (in this order, 64 lines a wave, as far as there are waves), and of its own columns the values.
     // (Training step of B4 T4096 H6 D128 on data that no cache holds: walks 142 and 153 us without, 129 and 148 with, while cotangents of states were left
-    // in one part; on data in the last-level cache no difference, nor in the states' part of it for 32 columns, B8 T2048 H16: 291 us back with half of its lines and with all.  At 64 features, with half as much to bring, 59 us without and 62 with, and summaries 283 and 296: those do without.)
+    // in one part; on data in the last-level cache no difference, nor with 32 columns from the other half of the states' lines: 291 us back for B8 T2048 H16.
+    // At 64 features, with half as much to bring, 59 us without and 62 with, and summaries 283 and 296: those do without.)
     static constexpr int kAhead = 6;
     struct Ahead {
         const char *p;

@@ -514,8 +514,9 @@ variable_list delta_backward(const Tensor &states, const Tensor &a, const Tensor
 
 // A leaf's gradient is accumulated on the stream of the first graph that holds the leaf, for as long as any graph holds it.  Is that the default
 // stream and this backward pass is captured on another, then the default stream would be made to wait for the capture, which HIP forbids and the
-// process does not outlive.  Called by a backward before it launches anything: looks through the graph behind it for such a leaf that the pass reaches.
-void refuse_capture_for_eager_leaves(const char *name, const Tensor &t)
+// process does not outlive.  Called by a backward before it launches anything, by those of delta.py and logprobs.py too: looks through the graph behind it for
+// such a leaf that the pass reaches.
+void refuse_capture_for_eager_leaves(const std::string &name, const Tensor &t)
 {
     const auto stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.device().index());
     const c10::Stream usual = c10::hip::getDefaultHIPStreamMasqueradingAsCUDA(t.device().index()).unwrap();
@@ -973,4 +974,5 @@ PYBIND11_MODULE(_gla_torch, m)
     m.def("beam_select", &beam_select, NoGil());
     m.def("reorder", &reorder, NoGil());
     m.def("token_logprobs", &token_logprobs, NoGil());
+    m.def("refuse_capture_for_eager_leaves", &refuse_capture_for_eager_leaves, NoGil());
 }

@@ -61,6 +61,7 @@ class _ChunkDelta(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dhT, dout, dstates=None):
         states, a, b, v, k, q, lengths = ctx.saved_tensors
+        _lib.binding().refuse_capture_for_eager_leaves("chunk_delta", v)
         shape, dtype = ctx.hidden
         dhT = torch.zeros(shape, dtype=dtype, device=v.device) if dhT is None else dhT
         dout = torch.zeros(v.shape, dtype=v.dtype, device=v.device) if dout is None else dout

@@ -58,6 +58,7 @@ class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dgiven, dentropy, *others):
         logits, tokens, stats, entropy = ctx.saved_tensors
+        _lib.binding().refuse_capture_for_eager_leaves("token_logprobs", logits)
         zero = lambda d: torch.zeros_like(entropy) if d is None else d  # noqa: E731
         return _apply(_TokenLogprobsBwd, logits, tokens, stats, entropy, zero(dgiven), zero(dentropy))[0], None, None
 
