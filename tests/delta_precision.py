@@ -17,6 +17,9 @@ instructions an accumulator for 128 features and 64 tokens, each of which adds a
 the exponentials, two units each, as much again.  Chunks are independent of each other: sqrt(m) 2^-21 behind m of them.  The cotangent of the state goes
 the same way from the other end.  A gradient of a gate takes one number of each way, whose errors add in quadrature, and its terms may be twice as large
 as it: 2 sqrt(2 m) 2^-21.  Two parts instead of three are off by 2^-18 / sqrt(3) for each operand: 2^-18 and more with the three products of a chunk.
+
+32-bit data.  The operands are whole, and all results are float sums: those of 16-bit data's 32-bit results, with chunks of 32 tokens; out and the gradients of
+rows take a number of each way, or two of one, and their terms may be twice as large as they are: 2 sqrt(2 m) 2^-21.
 """
 import torch
 

@@ -23,7 +23,9 @@ def found(sizes, gates, dtype=BF16):
     key = (sizes, tuple(sorted(gates.items())), dtype)
     if key not in _found:
         x = inputs(*sizes, dtype=dtype, seed=40, **gates)
-        exact = reference(*x[:6], None, x[6], x[7], 64 if dtype == BF16 else 32)
+        exact = list(reference(*x[:6], None, x[6], x[7], 64 if dtype == BF16 else 32))
+        if gates["decay"] == "head":          # one number a head: the sum over all tokens, whose errors add in quadrature
+            exact[3], exact[8] = exact[3].sum((0, 1)), exact[8].square().sum((0, 1)).sqrt()
         got = [t.cpu() for t in step(chunk_delta, *x)]
         _found[key] = {n: (s, t, exact[8] if n == "dlog_decay" else None) for n, s, t in zip(RESULTS, got, exact)}
     return _found[key]
@@ -39,3 +41,25 @@ def test_out(sizes, gates):
 def test_dkey(sizes, gates):
     share = changed(*found(sizes, gates)["dkey"][:2])
     assert share <= CHANGED
+
+
+@pytest.mark.parametrize("name", ["dvalue", "dquery"])
+@pytest.mark.parametrize("sizes, gates", CASES, ids=ids)
+def test_other_16_bit_results(sizes, gates, name):
+    share = changed(*found(sizes, gates)[name][:2])
+    assert share <= CHANGED
+
+
+@pytest.mark.parametrize("name", ["hidden_final", "dhidden_init", "dlog_decay", "dbeta"])
+@pytest.mark.parametrize("sizes, gates", CASES, ids=ids)
+def test_32_bit_results(sizes, gates, name):
+    """A third part less is seen: test_delta_precision.py."""
+    share = off(*found(sizes, gates)[name])
+    assert share <= bound_of_floats(name, -(-sizes[1] // 64))
+
+
+@pytest.mark.parametrize("name", RESULTS)
+@pytest.mark.parametrize("sizes, gates", CASES[:2] + [((1, 2081, 2, 1, 64, 64), dict(decay="token"))] + CASES[3:4], ids=ids)
+def test_results_of_32_bit_data(sizes, gates, name):
+    share = off(*found(sizes, gates, F32)[name])
+    assert share <= bound_of_floats(name, -(-sizes[1] // 32))
