@@ -107,8 +107,8 @@ def token_logprobs(logits, tokens, top=0):
     Returns (logprobs [..], entropy [..]), float32: the log softmax at each token, and the entropy of each distribution in nats; with `top`
     (at most 64) also (top_logprobs [..,top], top_tokens [..,top] int64): the largest log probabilities, of equal ones the lower token first.  A token
     outside 0..V-1 (-100, say) marks a position that does not count: its logits are not read, logprobs and entropy are 0 there and its
-    alternatives -inf and -1.  A logit of -inf has probability 0; a row with a NaN, or a +inf, or nothing above -inf, has NaN results, and such
-    logits count as -inf in the order of the alternatives.
+    alternatives -inf and -1.  A logit of -inf has probability 0; a row with a NaN, or a +inf, or nothing above -inf, has NaN results.  In the order of the
+    alternatives NaN counts as -inf, and +inf comes first.
 
     Differentiable in logits through logprobs and entropy: -logprobs.sum() is the cross entropy.  Positions that do not count get a gradient of 0.
     A backward pass is captured into a graph only while no graph of the same leaves from the default stream is alive (RuntimeError)."""

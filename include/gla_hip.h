@@ -360,7 +360,7 @@ int gla_reorder_states(void *stream, int64_t pool, int64_t groups, int64_t beams
  * (in nats), and the `top` (at most 64) largest log probabilities with their tokens, largest first, of equal ones the lower token.  `tokens`
  * (int32, or int64 with wide_indices != 0): one outside 0..vocab-1 marks a row that does not count, whose logits are not read: logprobs and
  * entropy are 0, its alternatives -inf and -1.  Logits of -inf have probability 0; a row with a logit that is not a number, or of +inf, or with
- * none above -inf, has results that are not numbers (such logits count as -inf in the order of the alternatives).
+ * none above -inf, has results that are not numbers.  In the order of the alternatives what is not a number counts as -inf, and +inf comes first.
  * `stats` [rows,2] is what the backward needs, or NULL.  Any alignment of the rows. */
 int gla_token_logprobs(void *stream, int64_t rows, int64_t vocab, int64_t top, gla_dtype dtype, int64_t row, int wide_indices,
                        const void *logits, const void *tokens, float *logprobs, float *entropy, float *stats, float *top_logprobs,
