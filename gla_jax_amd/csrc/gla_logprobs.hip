@@ -190,14 +190,13 @@ __global__ __launch_bounds__(THREADS) void token_logprobs_kernel(const LogprobAr
         }
     }
     if constexpr (TOP) {
-        __shared__ float names[THREADS], peaks[64];
+        __shared__ float peaks[64];
         __shared__ u64 collected[kRoom];
         __shared__ int listed[THREADS];
         __shared__ int threads, values;
         __shared__ float bound_of_all;
         const int top = a.top;
         const bool numbers = joined.sum == joined.sum;       // (where one is none, the largest of the others may have been lost beside it)
-        names[tid] = own_most;
         float peak = own_most;
 #pragma unroll
         for (int m = 1; m < THREADS / 64; m *= 2) peak = fmaxf(peak, shfl_xor_f32(peak, m));
@@ -219,7 +218,7 @@ __global__ __launch_bounds__(THREADS) void token_logprobs_kernel(const LogprobAr
         const float bound = fmaxf(bound_of_all, -3.4028235e38f);
         if (own_most >= bound) listed[atomicAdd(&threads, 1)] = tid;
         __syncthreads();
-        const int names_there = threads;
+        const int threads_there = threads;
         auto collect = [&](float v, int64_t place) {
             if (!(v >= bound)) return;
             const int at = atomicAdd(&values, 1);
@@ -228,7 +227,7 @@ __global__ __launch_bounds__(THREADS) void token_logprobs_kernel(const LogprobAr
         // A wave reads the pieces of as many threads as it has lanes for.
         const int64_t each = (x.pieces + THREADS - 1) / THREADS;     // pieces of a thread, at most
         const int lanes = each > 32 ? 64 : each > 16 ? 32 : each > 8 ? 16 : each > 4 ? 8 : 4, side = 64 / lanes;
-        for (int i = w * side + lane / lanes; i < names_there; i += kWaves * side) {
+        for (int i = w * side + lane / lanes; i < threads_there; i += kWaves * side) {
             const int id = listed[i];
             for (int64_t q = id + (int64_t)(lane % lanes) * THREADS; q < x.pieces; q += (int64_t)lanes * THREADS) {
                 const typename Row::Piece piece = *x.at(q);
