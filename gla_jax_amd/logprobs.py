@@ -102,7 +102,11 @@ class _TokenLogprobsBwd(torch.autograd.Function):
 
 
 def token_logprobs(logits, tokens, top=0):
-    """What logits say of given tokens: logits [..,V] (float32 or bfloat16, any distance between rows), tokens [..] (int32 or int64).
+    """What logits say of given tokens: logits [..,V] (float32 or bfloat16), tokens [..] (int32 or int64).
+
+    Rows that are one distance apart, whatever axes lie in front, are read where they lie, at any distance and alignment.  Others are copied first, in the
+    forward and again in the backward pass: features that lie apart, and rows such as logits[:, :-1] of several sequences, which skip one at
+    each sequence's end.  (All positions at once, with -100 for the token behind the last, take no copy.)
 
     Returns (logprobs [..], entropy [..]), float32: the log softmax at each token, and the entropy of each distribution in nats; with `top`
     (at most 64) also (top_logprobs [..,top], top_tokens [..,top] int64): the largest log probabilities, of equal ones the lower token first.  A token
