@@ -27,8 +27,9 @@ template <typename T, int DKP> constexpr int state_place()
     return states > scores ? states : scores;
 }
 
-// 175 us for the 1536 chunks of B4 T4096 H6 D128, 87 for the 1056 of B2 T2050 H16 64x128: 472 MB and 2.7 TB/s at 128 x 128, of which the states before the
-// chunks are 100 (32 bits), their cotangents 100 (in two parts; in one, 154 and 85 us), what was written and its cotangents 50 each.  LDS and registers leave one workgroup a compute unit, whose
+// 175 us for the 1536 chunks of B4 T4096 H6 D128, 87 for the 1056 of B2 T2050 H16 64x128: 537 MB and 3.1 TB/s at 128 x 128, of which the states before the
+// chunks are 100 (32 bits), their cotangents 100 (in two parts; in one, 154 and 85 us), what was written and its cotangents 50 each, and registers that do not fit 30
+// each way.  LDS and registers leave one workgroup a compute unit, whose
 // phases (a slice's rows arrive, its products, the scores) do not overlap; chunk after chunk in one workgroup, the next one's first rows on
 // their way, it needs 90 to 180 registers more than there are.
 // One workgroup: a chunk of a (batch, head) pair; a wave makes 16 key features of dq and dk, at 64 features of every second tile of tokens.

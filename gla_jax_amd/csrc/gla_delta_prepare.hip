@@ -11,7 +11,7 @@ namespace {
 // goes down (forward, for the transposed matrix: up) its own column of blocks, X_ij = -X_ii sum_k N_ik X_kj, by float products whose accumulators are
 // the next product's operands as they are.  The waves wait for each other once.
 //
-// 26 us for the 1536 chunks of B4 T4096 H6 D128 (63 MB, 2.4 TB/s), 54 for the 4096 of B1 T32768 H8, 6.7 for one.  A workgroup takes 19000 cycles, of which it
+// 27 us for the 1536 chunks of B4 T4096 H6 D128 (101 MB, 3.7 TB/s), 58 for the 4096 of B1 T32768 H8, 6.9 for one.  A workgroup takes 19000 cycles, of which it
 // waits 8000 for its rows, makes scores for 3000 and solves for 5500, each a chain of dependent steps; three of them share a compute unit.
 template <typename T, int DKP, bool BACK> __global__ __launch_bounds__(256) void delta_prepare_kernel(const DeltaArgs a)
 {

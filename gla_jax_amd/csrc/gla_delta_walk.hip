@@ -982,7 +982,11 @@ template <typename T, bool BACK> int dispatch_walk(hipStream_t stream, const Del
 // Segments are worth their summaries (a walk for the values and one for the basis) where one walk leaves compute units idle.  The number with the
 // least time by what was measured at 128 x 128 features: 1.6 us a chunk for a workgroup of 16 columns, 2.45 for one of 32, 2.1 in a summary, 1.5 a
 // step of the join, and 12 for the two launches more and their beginnings.
-// (B1 T32768 H8: 803 us in one piece, 8 segments 265 + 20 + 157.)
+// (B1 T32768 H8: 803 us in one piece, 8 segments 280 + 20 + 164.)  Elsewhere it takes the costs for the same, and the padded T for every length; whole calls in us as it
+// chooses, and in one piece:
+//       bf16: 64 x 64, T32768 H8 207, 684;  T16384 H16 187, 372;  64 x 128, T8192 H8 100, 154;  training 64 x 64, T8192 H8 250, 435;  128 x 128, B2 T8192 H8 241, 243
+//       float32: 64 x 64, T8192 H8 122, 336;  training H4 313, 771;  128 x 128, T8192 H4 346, 602;  T4096 H8 181, 312
+// 16 value columns stay in one piece: segments walk with 32.
 int delta_segments(const DeltaArgs &a)
 {
     const int64_t of_pair = (a.n.DV + 31) / 32, wide = a.pairs * of_pair, basis = a.pairs * ((a.n.DK + 31) / 32);
