@@ -9,8 +9,7 @@
 // state, u_j.du_j (written) and dv_i.(v_i - x_i) (read) leave dv.v:
 //       da_t = <S', dS'> + sum_{i>=t} (o_i.do_i - v_i.dv_i)    over the chunk's tokens i,
 // with o_i.do_i = sum_j P_ij (do_i.u_j) + e^{L_i} q_i.(S do_i).  The first term starts the sum anew at every chunk, so no difference runs over a
-// whole sequence.  (Off by 5e-7 of its norm; the chunked form differentiated step by step in 32-bit operations
-// is off by 3e-7.)
+// whole sequence.  (Off by 5e-7 of its norm; the chunked form differentiated step by step in 32-bit operations is off by 3e-7.)
 #include "gla_delta.hpp"
 
 namespace gla {
@@ -30,9 +29,8 @@ template <typename T, int DKP> constexpr int state_place()
 
 // 175 us for the 1536 chunks of B4 T4096 H6 D128, 87 for the 1056 of B2 T2050 H16 64x128: 537 MB and 3.1 TB/s at 128 x 128, of which the states before the
 // chunks are 100 (32 bits), their cotangents 100 (in two parts; in one, 154 and 85 us), what was written and its cotangents 50 each, and registers that do not fit 30
-// each way.  LDS and registers leave one workgroup a compute unit, whose
-// phases (a slice's rows arrive, its products, the scores) do not overlap; chunk after chunk in one workgroup, the next one's first rows on
-// their way, it needs 90 to 180 registers more than there are.
+// each way.  LDS and registers leave one workgroup a compute unit, whose phases (a slice's rows arrive, its products, the scores) do not overlap; chunk after
+// chunk in one workgroup, the next one's first rows on their way, it needs 90 to 180 registers more than there are.
 // One workgroup: a chunk of a (batch, head) pair; a wave makes 16 key features of dq and dk, at 64 features of every second tile of tokens.
 template <typename T, int DKP> __global__ __launch_bounds__(512) void delta_gradient_kernel(const DeltaArgs a)
 {

@@ -354,8 +354,7 @@ bool sizes_ok(int64_t rows, int64_t vocab, int64_t top)
 // 42, 1024 45), one of 131072 floats 15 (20, 16).  Neither looks at the length of a row, and a thread goes through eight whole pieces at its end: 8192 rows of 1000
 // to 8000 take 37 to 40 us in 16 bits (the read alone 3 to 27), with 20 alternatives 144 to 151.  Rows so short that fewer than `top` of the 64 groups of threads hold
 // a value (up to 1216 tokens in 16 bits at 20, 4032 at 64) hand over all that they have, or are searched once for each
-// alternative: 8192 rows of 1000 with 20 683 us, of 4000 with 64 2020.  A row of
-// 131072 floats has one compute unit.
+// alternative: 8192 rows of 1000 with 20 683 us, of 4000 with 64 2020.  A row of 131072 floats has one compute unit.
 template <typename T> int dispatch_logprobs(hipStream_t stream, const LogprobArgs &a, int64_t rows)
 {
     if (a.top) token_logprobs_kernel<T, 512, true><<<rows, 512, 0, stream>>>(a);
